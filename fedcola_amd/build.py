@@ -8,7 +8,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libfedcola_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (the compiler forms them from ordinary float code, and some of their forms have given wrong
+# results now and then on MI355X); the arithmetic per element is the same.  The host pass does not know the feature and says so: harmless.
+FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HEADERS = glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(HERE, "..", "include", "fedcola_hip.h")]
 
 
