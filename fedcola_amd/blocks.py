@@ -1,0 +1,236 @@
+"""Operators of a transformer block beside those of ``ModalityAgnosticTransformer``'s own blocks (LayerNorm, GELU MLP):
+
+* ``gated_mlp``: the gated feed-forward block, y = (act(x Wg^T) * (x Wu^T)) Wo^T,
+* ``norm_gate_residual``: what stands between two branches in one pass -- the norm after a branch, its gate and drop-path multiplier, the
+  scaled residual, and the norm in front of the next branch.
+
+Each has a forward and a backward function for programs that run their own backward pass, an autograd form and a module.  They run in
+libfedcola_hip (``fc_gated_mlp_*``, ``fc_norm_gate_*``) on the current stream of their tensors' device; there is no CPU form."""
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from ._lib import as_rows, check, in_place, on_device, operand_type, ptr
+
+_ACTS = {"silu": 0, "gelu": 1}
+_NORMS = {"layer": 0, "rms": 1}
+
+
+# ------------------------------------------------------------------------------------------------ gated feed-forward
+def _mlp_operands(x, w_in, w_out, act):
+    if act not in _ACTS:
+        raise ValueError(f"gated_mlp: activation {act!r}: silu or gelu")
+    code, dev = operand_type("gated_mlp", x, w_in, w_out)
+    if w_in.dim() != 2 or w_out.dim() != 2 or x.dim() < 1 or x.shape[-1] != w_in.shape[1] or w_out.shape != (w_in.shape[1], w_in.shape[0] // 2) or \
+            w_in.shape[0] % 2 or w_in.numel() == 0:
+        raise ValueError(f"gated_mlp: x [..., D], w_in [2F, D], w_out [D, F] are expected, not {tuple(x.shape)}, {tuple(w_in.shape)}, {tuple(w_out.shape)}")
+    return code, dev, as_rows(x), as_rows(w_in), as_rows(w_out)
+
+
+def gated_mlp_forward(x, w_in, w_out, act="silu"):
+    """y = (act(x wg^T) * (x wu^T)) w_out^T.  x [..., D]; w_in [2F, D]: wg over wu; w_out [D, F]; one type, bf16 or fp32.  act: "silu", "gelu" (erf)."""
+    code, dev, (x2, ldx), (wi, ldi), (wo, ldo) = _mlp_operands(x, w_in, w_out, act)
+    T, D, F, L = x2.shape[0], wi.shape[1], wo.shape[1], _lib.lib()
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    packed = not (in_place(x2, ldx) and in_place(wi, ldi) and in_place(wo, ldo))
+    with on_device(dev) as stream:
+        ws = torch.empty(L.fc_gated_mlp_workspace_bytes(code, T, D, F, packed, 0), dtype=torch.uint8, device=dev)
+        check(L.fc_gated_mlp_fwd(code, _ACTS[act], x2.data_ptr(), ldx, wi.data_ptr(), ldi, wo.data_ptr(), ldo, T, D, F, y.data_ptr(), D, ws.data_ptr(),
+                                 ws.numel(), stream))
+    return y
+
+
+def gated_mlp_backward(dy, x, w_in, w_out, act="silu", need=(True, True, True)):
+    """Gradients ``(dx, dw_in, dw_out)`` for the gradient dy of y (None where not needed), from the inputs alone."""
+    code, dev, (x2, ldx), (wi, ldi), (wo, ldo) = _mlp_operands(x, w_in, w_out, act)
+    operand_type("gated_mlp", x, dy)
+    if dy.shape != x.shape:
+        raise ValueError(f"gated_mlp: dy {tuple(dy.shape)} is not of y's shape {tuple(x.shape)}")
+    dy2, ldy = as_rows(dy)
+    T, D, F, L = x2.shape[0], wi.shape[1], wo.shape[1], _lib.lib()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+    dwi = torch.empty(2 * F, D, dtype=x.dtype, device=dev) if need[1] else None
+    dwo = torch.empty(D, F, dtype=x.dtype, device=dev) if need[2] else None
+    packed = not (in_place(x2, ldx) and in_place(dy2, ldy) and in_place(wi, ldi) and in_place(wo, ldo))
+    with on_device(dev) as stream:
+        ws = torch.empty(L.fc_gated_mlp_workspace_bytes(code, T, D, F, packed, 1), dtype=torch.uint8, device=dev)
+        check(L.fc_gated_mlp_bwd(code, _ACTS[act], dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wi.data_ptr(), ldi, wo.data_ptr(), ldo, T, D, F, ptr(dx), D,
+                                 ptr(dwi), D, ptr(dwo), F, ws.data_ptr(), ws.numel(), stream))
+    return dx, dwi, dwo
+
+
+class _GatedMlpFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, w_out, act):
+        ctx.save_for_backward(x, w_in, w_out)
+        ctx.act = act
+        return gated_mlp_forward(x, w_in, w_out, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w_in, w_out = ctx.saved_tensors
+        return (*gated_mlp_backward(dy, x, w_in, w_out, ctx.act, ctx.needs_input_grad[:3]), None)
+
+
+def gated_mlp(x, w_in, w_out, act="silu"):
+    """``gated_mlp_forward`` with autograd."""
+    return _GatedMlpFn.apply(x, w_in, w_out, act)
+
+
+class GatedMlp(nn.Module):
+    """Gated feed-forward block of width ``dim``, ``hidden`` units (default: 2/3 of the 4 dim of a plain MLP, in whole 64s: the same parameters)."""
+
+    def __init__(self, dim, hidden=None, act="silu", device=None, dtype=None):
+        super().__init__()
+        hidden = hidden or max(64, round(8 * dim / 3 / 64) * 64)
+        if act not in _ACTS:
+            raise ValueError(f"gated_mlp: activation {act!r}: silu or gelu")
+        self.act = act
+        self.w_in = nn.Parameter(torch.empty(2 * hidden, dim, device=device, dtype=dtype))
+        self.w_out = nn.Parameter(torch.empty(dim, hidden, device=device, dtype=dtype))
+        for w in (self.w_in, self.w_out):
+            nn.init.kaiming_uniform_(w, a=math.sqrt(5))       # nn.Linear's
+
+    def forward(self, x):
+        return gated_mlp(x, self.w_in, self.w_out, self.act)
+
+
+# ------------------------------------------------------------------------------------------------ norm, gate, residual, norm
+_VECTORS = ("post_weight", "post_bias", "gate", "row_scale", "pre_weight", "pre_bias")
+
+
+def _norm_operands(branch, residual, norm, eps, residual_scale, vectors):
+    if norm not in _NORMS:
+        raise ValueError(f"norm_gate_residual: norm {norm!r}: layer or rms")
+    code, dev = operand_type("norm_gate_residual", branch, residual)
+    if branch.shape != residual.shape or branch.dim() < 1 or not 1 <= branch.shape[-1] <= 8192:
+        raise ValueError(f"norm_gate_residual: branch {tuple(branch.shape)} and residual {tuple(residual.shape)} of one shape [..., D], D <= 8192, are expected")
+    if not eps > 0:
+        raise ValueError(f"norm_gate_residual: eps {eps}")
+    D = branch.shape[-1]
+    T = branch.shape[:-1].numel()
+    for name, v in vectors.items():
+        if v is None:
+            continue
+        if v.dtype != torch.float32 or v.device != dev:
+            raise ValueError(f"norm_gate_residual: {name} is float32 on {dev}, not {v.dtype} on {v.device}")
+        if name == "gate":
+            ok = v.shape == (D,) or (v.dim() == 2 and v.shape[1] == D and v.shape[0] >= 1 and T % v.shape[0] == 0)
+        elif name == "row_scale":
+            ok = v.dim() == 1 and v.shape[0] >= 1 and T % v.shape[0] == 0
+        else:
+            ok = v.shape == (D,)
+        if not ok:
+            raise ValueError(f"norm_gate_residual: {name} {tuple(v.shape)} does not match {T} rows of {D}")
+    for part in ("post", "pre"):
+        if vectors[part + "_bias"] is not None and (vectors[part + "_weight"] is None or norm == "rms"):
+            raise ValueError(f"norm_gate_residual: {part}_bias goes with {part}_weight and norm='layer'")
+    v = {k: None if t is None else t.contiguous() for k, t in vectors.items()}
+    gate_rows = T // v["gate"].shape[0] if v["gate"] is not None and v["gate"].dim() == 2 else 0
+    scale_rows = T // v["row_scale"].shape[0] if v["row_scale"] is not None else 0
+    return code, dev, T, D, v, gate_rows, scale_rows
+
+
+def norm_gate_residual_forward(branch, residual, *, post_weight=None, post_bias=None, gate=None, row_scale=None, residual_scale=1.0, pre_weight=None,
+                               pre_bias=None, norm="layer", eps=1e-5):
+    """``r = residual_scale * residual + row_scale * gate * norm(branch)`` and ``h = norm(r)``: (r, h), h None without pre_weight.
+
+    branch, residual [..., D] in one type, bf16 or fp32; the vectors fp32.  post_weight / post_bias [D]: the norm after the branch (None: no
+    norm).  gate [D] for all rows or [S, D], one for each of S samples of equally many consecutive rows.  row_scale [S]: a sample's drop-path
+    multiplier; 0 drops the branch, whatever it holds.  pre_weight / pre_bias [D]: the norm in front of the next branch.  norm: "layer" or
+    "rms" (which has no bias)."""
+    vectors = dict(post_weight=post_weight, post_bias=post_bias, gate=gate, row_scale=row_scale, pre_weight=pre_weight, pre_bias=pre_bias)
+    code, dev, T, D, v, gate_rows, scale_rows = _norm_operands(branch, residual, norm, eps, residual_scale, vectors)
+    y, ldy = as_rows(branch)
+    x, ldx = as_rows(residual)
+    r = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
+    h = torch.empty(residual.shape, dtype=residual.dtype, device=dev) if pre_weight is not None else None
+    with on_device(dev) as stream:
+        check(_lib.lib().fc_norm_gate_fwd(code, _NORMS[norm], y.data_ptr(), ldy, x.data_ptr(), ldx, T, D, ptr(v["post_weight"]), ptr(v["post_bias"]), ptr(v["gate"]),
+                                          gate_rows, ptr(v["row_scale"]), scale_rows, residual_scale, ptr(v["pre_weight"]), ptr(v["pre_bias"]), eps,
+                                          r.data_ptr(), ptr(h), stream))
+    return r, h
+
+
+def norm_gate_residual_backward(d_residual, d_normed, branch, residual, *, post_weight=None, post_bias=None, gate=None, row_scale=None, residual_scale=1.0,
+                                pre_weight=None, pre_bias=None, norm="layer", eps=1e-5, weight_grads=True):
+    """Gradients for those of r (d_residual) and h (d_normed), either None: a dict of ``branch``, ``residual`` and, for each vector that was
+    given and with weight_grads, ``post_weight``, ``post_bias``, ``gate``, ``pre_weight``, ``pre_bias`` (fp32)."""
+    vectors = dict(post_weight=post_weight, post_bias=post_bias, gate=gate, row_scale=row_scale, pre_weight=pre_weight, pre_bias=pre_bias)
+    code, dev, T, D, v, gate_rows, scale_rows = _norm_operands(branch, residual, norm, eps, residual_scale, vectors)
+    for g in (d_residual, d_normed):
+        if g is not None:
+            operand_type("norm_gate_residual", branch, g)
+            if g.shape != branch.shape:
+                raise ValueError(f"norm_gate_residual: a gradient of shape {tuple(g.shape)} for rows of shape {tuple(branch.shape)}")
+    if d_normed is not None and pre_weight is None:
+        raise ValueError("norm_gate_residual: d_normed without pre_weight")
+    y, ldy = as_rows(branch)
+    x, ldx = as_rows(residual)
+    dr, lddr = as_rows(d_residual) if d_residual is not None else (None, 0)
+    dh, lddh = as_rows(d_normed) if d_normed is not None else (None, 0)
+    out = dict(branch=torch.empty(branch.shape, dtype=branch.dtype, device=dev), residual=torch.empty(branch.shape, dtype=branch.dtype, device=dev))
+    grads = {k: torch.empty(t.shape, device=dev) if t is not None and weight_grads and k != "row_scale" else None for k, t in v.items()}
+    L = _lib.lib()
+    with on_device(dev) as stream:
+        ws = torch.empty(L.fc_norm_gate_workspace_bytes(T, D, gate_rows), dtype=torch.uint8, device=dev) if any(t is not None for t in grads.values()) else None
+        check(L.fc_norm_gate_bwd(code, _NORMS[norm], ptr(dr), lddr, ptr(dh), lddh, y.data_ptr(), ldy, x.data_ptr(), ldx, T, D, ptr(v["post_weight"]),
+                                 ptr(v["post_bias"]), ptr(v["gate"]), gate_rows, ptr(v["row_scale"]), scale_rows, residual_scale, ptr(v["pre_weight"]),
+                                 eps, out["branch"].data_ptr(), out["residual"].data_ptr(), ptr(grads["post_weight"]), ptr(grads["post_bias"]),
+                                 ptr(grads["pre_weight"]), ptr(grads["pre_bias"]), ptr(grads["gate"]), ptr(ws), ws.numel() if ws is not None else 0, stream))
+    out.update((k, g) for k, g in grads.items() if g is not None)
+    return out
+
+
+class _NormGateFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, branch, residual, residual_scale, norm, eps, *vectors):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(branch, residual, *vectors)
+        ctx.how = dict(residual_scale=residual_scale, norm=norm, eps=eps)
+        return norm_gate_residual_forward(branch, residual, **ctx.how, **dict(zip(_VECTORS, vectors)))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dr, dh):
+        branch, residual, *vectors = ctx.saved_tensors
+        if dr is None and dh is None:
+            return (None,) * (5 + len(_VECTORS))
+        d = norm_gate_residual_backward(dr, dh, branch, residual, weight_grads=any(ctx.needs_input_grad[5:]), **ctx.how, **dict(zip(_VECTORS, vectors)))
+        return (d["branch"], d["residual"], None, None, None, *(d.get(k) for k in _VECTORS))
+
+
+def norm_gate_residual(branch, residual, *, post_weight=None, post_bias=None, gate=None, row_scale=None, residual_scale=1.0, pre_weight=None, pre_bias=None,
+                       norm="layer", eps=1e-5):
+    """``norm_gate_residual_forward`` with autograd (row_scale, drawn by the caller, gets no gradient)."""
+    if row_scale is not None and row_scale.requires_grad:
+        raise ValueError("norm_gate_residual: row_scale has no gradient")
+    return _NormGateFn.apply(branch, residual, residual_scale, norm, eps, post_weight, post_bias, gate, row_scale, pre_weight, pre_bias)
+
+
+class NormGateResidual(nn.Module):
+    """``norm_gate_residual`` with its own weights: the norm after a branch, a gate for each channel (initially ``gate_init``; None: none), the
+    residual, and the norm in front of the next branch.  forward(branch, residual, row_scale=None, gate=None): (residual, normed); a ``gate``
+    argument ([S, D], of a conditioning network, say) replaces the module's own."""
+
+    def __init__(self, dim, norm="layer", eps=1e-5, gate_init=None, residual_scale=1.0, post=True, pre=True, device=None):
+        super().__init__()
+        if norm not in _NORMS:
+            raise ValueError(f"norm_gate_residual: norm {norm!r}: layer or rms")
+        self.norm, self.eps, self.residual_scale = norm, eps, residual_scale
+
+        def vec(on, value):
+            return nn.Parameter(torch.full((dim,), float(value), device=device)) if on else None
+        self.post_weight, self.post_bias = vec(post, 1), vec(post and norm == "layer", 0)
+        self.pre_weight, self.pre_bias = vec(pre, 1), vec(pre and norm == "layer", 0)
+        self.gate = vec(gate_init is not None, gate_init or 0)
+
+    def forward(self, branch, residual, row_scale=None, gate=None):
+        return norm_gate_residual(branch, residual, post_weight=self.post_weight, post_bias=self.post_bias, gate=self.gate if gate is None else gate,
+                                  row_scale=row_scale, residual_scale=self.residual_scale, pre_weight=self.pre_weight, pre_bias=self.pre_bias,
+                                  norm=self.norm, eps=self.eps)

@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import check, ptr
+from ._lib import as_rows, check, in_place, on_device, operand_type, ptr
 
 
 def contrastive_tau() -> float:
@@ -72,6 +72,82 @@ class _CEFn(torch.autograd.Function):
 class CrossEntropyLoss(nn.Module):
     def forward(self, logits, targets):
         return _CEFn.apply(logits, targets)
+
+
+# ------------------------------------------------------------------------------------------------ a linear layer's loss over a vocabulary
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy_forward(hidden, weight, targets, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the logits ``hidden @ weight.T`` against ``targets`` without keeping the logits: ``(loss, saved)``, ``saved`` for
+    ``linear_cross_entropy_backward``.  hidden [..., D] and weight [V, D] in one type, bf16 or fp32; targets int64 of hidden's leading shape.
+    loss: fp32, a scalar ("mean" over the targets that are not ignore_index, "sum") or of the targets' shape ("none")."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction {reduction!r}: none, mean or sum")
+    code, dev = operand_type("linear_cross_entropy", hidden, weight)
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise ValueError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
+    if targets.shape != hidden.shape[:-1] or targets.dtype != torch.int64 or targets.device != dev:
+        raise ValueError(f"linear_cross_entropy: targets are int64 of shape {tuple(hidden.shape[:-1])} on {dev}, not {targets.dtype} {tuple(targets.shape)} on {targets.device}")
+    x, ldx = as_rows(hidden)
+    w, ldw = as_rows(weight)
+    y = targets.contiguous()
+    T, (V, D), L, red = x.shape[0], w.shape, _lib.lib(), _REDUCTIONS[reduction]
+    loss = torch.empty(targets.shape if red == 0 else (), device=dev)
+    with on_device(dev) as stream:
+        saved = torch.empty(L.fc_linear_ce_saved_bytes(code, T, D), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw), 0), dtype=torch.uint8, device=dev)
+        check(L.fc_linear_ce_fwd(code, x.data_ptr(), ldx, w.data_ptr(), ldw, y.data_ptr(), T, V, D, ignore_index, red, loss.data_ptr(), saved.data_ptr(),
+                                 saved.numel(), ws.data_ptr(), ws.numel(), stream))
+    return loss, (saved, hidden.shape, red)
+
+
+def linear_cross_entropy_backward(gloss, saved, weight, need_hidden=True, need_weight=True):
+    """Gradients ``(dhidden, dweight)`` for the gradient ``gloss`` of the loss (fp32, of its shape); None where not needed."""
+    saved, shape, red = saved
+    code, dev = operand_type("linear_cross_entropy", weight)
+    w, ldw = as_rows(weight)
+    T, (V, D), L = math.prod(shape[:-1]), w.shape, _lib.lib()
+    if gloss.shape != (shape[:-1] if red == 0 else ()) or gloss.device != dev or shape[-1] != D:
+        raise ValueError(f"linear_cross_entropy: a gradient of shape {tuple(gloss.shape)} on {gloss.device} is not that of the loss")
+    g = gloss.float().contiguous()
+    dx = torch.empty(shape, dtype=weight.dtype, device=dev) if need_hidden else None
+    dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if need_weight else None
+    with on_device(dev) as stream:
+        ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw), 1), dtype=torch.uint8, device=dev)
+        check(L.fc_linear_ce_bwd(code, w.data_ptr(), ldw, T, V, D, red, g.data_ptr(), saved.data_ptr(), saved.numel(), ptr(dx), D, ptr(dw), D,
+                                 ws.data_ptr(), ws.numel(), stream))
+    return dx, dw
+
+
+class _LinearCEFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+        loss, (saved, shape, red) = linear_cross_entropy_forward(hidden, weight, targets, ignore_index, reduction)
+        ctx.save_for_backward(saved, weight)
+        ctx.how = shape, red
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        saved, weight = ctx.saved_tensors
+        dx, dw = linear_cross_entropy_backward(g, (saved, *ctx.how), weight, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+class LinearCrossEntropyLoss(nn.Module):
+    """``CrossEntropyLoss`` of a linear layer over a large vocabulary: ``loss(hidden, weight, targets)`` = cross entropy of
+    ``hidden @ weight.T``, whose logits [rows, V] never exist (``linear_cross_entropy_forward``)."""
+
+    def __init__(self, ignore_index=-100, reduction="mean"):
+        super().__init__()
+        if reduction not in _REDUCTIONS:
+            raise ValueError(f"reduction {reduction!r}: none, mean or sum")
+        self.ignore_index, self.reduction = ignore_index, reduction
+
+    def forward(self, hidden, weight, targets):
+        return _LinearCEFn.apply(hidden, weight, targets, self.ignore_index, self.reduction)
 
 
 CRITERIA = {"ContrastiveLoss": ContrastiveLoss, "CrossEntropyLoss": CrossEntropyLoss}

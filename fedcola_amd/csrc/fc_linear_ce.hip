@@ -1,0 +1,465 @@
+// Softmax cross entropy of a linear layer over a large vocabulary, the logits never kept.
+//
+//   L[t, v] = x[t] . w[v];   lse[t] = log sum_v exp L[t, v];   row[t] = lse[t] - L[t, y[t]]      (0 where y[t] is the ignored index)
+//   dL[t, v] = (exp(L[t, v] - lse[t]) - [v = y[t]]) g[t];      dx = dL w;   dw = dL^T x
+//
+// Forward: rows that count are gathered once (aligned; three bf16 planes for fp32), so ignored rows cost no products and what they hold
+// touches nothing.  One tiled product; each tile leaves its columns' maximum and sum of exponentials per row, and the target's logit,
+// behind (8 bytes for TN logits); a second pass joins them.  Backward: the logits are formed again in pieces of the vocabulary, dL of a
+// piece goes to the workspace in the operands' precision, and two products read it.  That is 8 T V D operations for 6 T V D; keeping the
+// exponentials instead costs another rounding (their sum is not known yet when they are stored) or 8 bytes a logit of traffic, more than
+// the 2 D operations they save up to D of about 1500.  A piece's dL (<= 192 MB) is written once and read twice.
+// Everything is added in a fixed order; nothing is zero-filled by a memset.
+#include <math.h>
+
+#include "../../include/fedcola_hip.h"
+#include "fc_tiles.h"
+
+#define CE_LOG2E 1.4426950408889634f
+
+// ---- what the forward leaves for the backward, at the caller's address
+struct CeSaved {
+  int* n;          // rows that count
+  int *pos, *idx, *y;   // row -> place among them or -1; place -> row; place -> target, -1 for one outside of the vocabulary
+  float* lse;      // [place]
+  FtMat x;         // gathered rows
+  size_t bytes;
+};
+static CeSaved ce_saved(void* base, int dt, long T, long D) {
+  CeSaved s;
+  char* p = (char*)base;
+  const long ld = ft_up(D, 8), t4 = ft_up(T * 4, 256);
+  s.n = (int*)p;
+  s.pos = (int*)(p + 256);
+  s.idx = (int*)(p + 256 + t4);
+  s.y = (int*)(p + 256 + 2 * t4);
+  s.lse = (float*)(p + 256 + 3 * t4);
+  s.x.p = (bf16_t*)(p + 256 + 4 * t4);
+  s.x.ld = ld;
+  s.x.plane = T * ld;
+  s.bytes = 256 + 4 * t4 + (size_t)(dt ? 1 : 3) * T * ld * 2;
+  return s;
+}
+
+// ---- which rows count, and their copies.  Workgroup b takes rows [b R, (b + 1) R) after counting the targets before them.
+template <typename T, int PL>
+__global__ void __launch_bounds__(256) k_ce_rows(const T* x, long ldx, const int64_t* y, long T_, int R, int V, int64_t ignore, int D, bool vec, CeSaved s) {
+  __shared__ int red[4], src[64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const long r0 = (long)blockIdx.x * R, r1 = r0 + R < T_ ? r0 + R : T_;
+  int c = 0;
+  for (long i = tid; i < r0; i += 256) c += y[i] != ignore;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+  if (lane == 0) red[tid >> 6] = c;
+  __syncthreads();
+  int at = red[0] + red[1] + red[2] + red[3];
+  const int cw = (int)(s.x.ld / 8);
+  for (long b = r0; b < r1; b += 64) {
+    const long r = b + lane;
+    const int64_t t = r < r1 ? y[r] : ignore;
+    const bool on = r < r1 && t != ignore;
+    const unsigned long long m = __ballot(on);
+    const int k = __popcll(m & ((1ull << lane) - 1)), n = __popcll(m);
+    if (tid < 64) {
+      if (r < r1) s.pos[r] = on ? at + k : -1;
+      if (on) {
+        s.idx[at + k] = (int)r;
+        s.y[at + k] = t >= 0 && t < V ? (int)t : -1;
+        src[k] = (int)(r - b);
+      }
+    }
+    __syncthreads();
+    for (int e = tid; e < n * cw; e += 256) {
+      const int i = e / cw, c0 = (e - i * cw) * 8;
+      const T* p = x + (b + src[i]) * ldx + c0;
+      bf16_t* d = (bf16_t*)s.x.p + (long)(at + i) * s.x.ld + c0;
+      if (PL == 1 && vec) {
+        *(uint4*)d = *(const uint4*)p;
+        continue;
+      }
+      float h[3][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = c0 + j < D ? Io<T>::ld(p, j) : 0.f;
+        if (PL == 1) h[0][j] = v; else ft_split(v, h[0][j], h[1][j], h[2][j]);
+      }
+#pragma unroll
+      for (int q = 0; q < PL; ++q)
+        *(uint4*)(d + q * s.x.plane) = make_uint4(f2bf2(h[q][0], h[q][1]), f2bf2(h[q][2], h[q][3]), f2bf2(h[q][4], h[q][5]), f2bf2(h[q][6], h[q][7]));
+    }
+    at += n;
+    __syncthreads();
+  }
+  if (r1 == T_ && tid == 0) *s.n = at;
+}
+
+// exp(v - m): through v_exp_f32 for bf16 operands, whose logits carry 2^-9 each; expf for fp32
+template <int NPROD> __device__ __forceinline__ float ce_exp(float v, float m) {
+  return NPROD == 1 ? __builtin_amdgcn_exp2f((v - m) * CE_LOG2E) : expf(v - m);
+}
+struct CePart { float m, s; };   // maximum, and sum of exp(. - maximum)
+template <int NPROD> __device__ __forceinline__ CePart ce_join(CePart a, CePart b) {
+  CePart r;
+  r.m = fmaxf(a.m, b.m);
+  // a side without a finite or infinite maximum holds nothing, unless it holds NaN in its sum
+  const float x = a.m == r.m ? 1.f : ce_exp<NPROD>(a.m, r.m), y = b.m == r.m ? 1.f : ce_exp<NPROD>(b.m, r.m);
+  r.s = a.s * x + b.s * y;
+  return r;
+}
+
+struct CeArgs {
+  FtMat x, w;
+  int T, V, D, v0, nv;        // this launch's columns [v0, v0 + nv) of the vocabulary
+  const int *n, *y, *idx;
+  CePart* part;               // [tiles of columns][T]
+  float* tlogit;              // [T]
+  const float *lse, *g;
+  int reduction;
+  bf16_t* dl;                 // planes of [T][ldl]
+  long ldl, plane;
+};
+
+template <class S, int NPROD>
+__device__ __forceinline__ bool ce_product(const CeArgs& a, char* smem, ft_f4 (&acc)[S::NI][S::NJ], FtTile& t, int M, int wave, int lane) {
+  t = ft_tile((M + S::TM - 1) / S::TM, (a.nv + S::TN - 1) / S::TN, 1);
+  if (!t.any) return false;
+  const int wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = a.v0 + t.n * S::TN;
+  FtStager<TK, S::TM, S::NW> sa;
+  FtStager<TK, S::TN, S::NW> sb;
+  sa.init(a.x, m0, a.D, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
+  sb.init(a.w, n0, a.D, wave, lane, [&](int r) { return n0 + r < a.V ? (long)n0 + r : -1L; });
+#pragma unroll
+  for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
+  ft_loop<S, TK, TK, NPROD, S::NJ>(sa, sb, smem, 0, (a.D + 63) / 64, acc, wm, wn, wave, lane);
+  return true;
+}
+
+template <class S, int NPROD>
+__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_stats(CeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4, M = min(a.T, *a.n);
+  ft_f4 acc[S::NI][S::NJ];
+  FtTile t;
+  if (!ce_product<S, NPROD>(a, smem, acc, t, M, wave, lane)) return;
+  const int m0 = t.m * S::TM, n0 = t.n * S::TN + wn * S::NJ * 16;
+  CePart* red = (CePart*)smem;                           // [WN][TM]
+  const bool edge = n0 + S::NJ * 16 > a.V;
+#pragma unroll
+  for (int i = 0; i < S::NI; ++i) {
+    const int r = (wm * S::NI + i) * 16 + (lane & 15), m = m0 + r;
+    if (edge)
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (n0 + 16 * j + 4 * g + x >= a.V) acc[i][j][x] = -__builtin_inff();
+    CePart p;
+    p.m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) p.m = fmaxf(p.m, acc[i][j][x]);
+    p.m = fmaxf(p.m, __shfl_xor(p.m, 16, 64));
+    p.m = fmaxf(p.m, __shfl_xor(p.m, 32, 64));
+    p.s = 0.f;
+    // a maximum of -inf: columns past the vocabulary alone, logits of -inf, or NaN, which fmaxf leaves out and the sum must not
+    const float base = p.m == -__builtin_inff() ? 0.f : p.m;
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) p.s += ce_exp<NPROD>(acc[i][j][x], base);
+    p.s += __shfl_xor(p.s, 16, 64);
+    p.s += __shfl_xor(p.s, 32, 64);
+    if (g == 0) red[wn * S::TM + r] = p;
+    const int rel = (m < M ? a.y[m] : -1) - n0;          // the target's logit, where this wave holds it
+    if (rel >= 0 && rel < S::NJ * 16 && ((rel >> 2) & 3) == g) {
+      float v = 0.f;
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (16 * j + x == (rel & ~12)) v = acc[i][j][x];
+      a.tlogit[m] = v;
+    }
+  }
+  ft_barrier();
+  for (int r = threadIdx.x; r < S::TM; r += S::NT)
+    if (m0 + r < M) {
+      CePart p = red[r];
+#pragma unroll
+      for (int q = 1; q < S::WN; ++q) p = ce_join<NPROD>(p, red[q * S::TM + r]);
+      a.part[(long)t.n * a.T + m0 + r] = p;
+    }
+}
+
+// joins the tiles' partial sums of 16 rows a workgroup, 16 lanes a row
+template <int NPROD>
+__global__ void __launch_bounds__(256) k_ce_join(const CePart* part, int tiles, const float* tlogit, CeSaved s, float* rows, long T) {
+  __shared__ CePart red[16][16];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const long t = (long)blockIdx.x * 16 + r;
+  const int at = t < T ? s.pos[t] : -1;
+  CePart p = {-__builtin_inff(), 0.f};
+  if (at >= 0)
+#pragma unroll 4
+    for (int i = q; i < tiles; i += 16) p = ce_join<NPROD>(p, part[(long)i * T + at]);
+  red[q][r] = p;
+  __syncthreads();
+  if (q == 0 && t < T) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) p = ce_join<NPROD>(p, red[i][r]);
+    float l = 0.f;
+    if (at >= 0) {
+      const bool in = s.y[at] >= 0;
+      const float lse = in ? p.m + logf(p.s) : __builtin_nanf("");   // a target outside of the vocabulary: NaN, in the loss and in the gradients
+      s.lse[at] = lse;
+      l = in ? lse - tlogit[at] : lse;
+    }
+    rows[t] = l;
+  }
+}
+// sum or mean of the rows, in fp64 and in one order
+__global__ void __launch_bounds__(1024) k_ce_loss(const float* rows, long T, const int* n, int reduction, float* loss) {
+  __shared__ double red[16];
+  double v = 0;
+  for (long i = threadIdx.x; i < T; i += 1024) v += (double)rows[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) v += red[i];
+    *loss = (float)(reduction == FC_REDUCE_MEAN ? v / (double)*n : v);    // no row counts: 0 / 0, NaN, as torch's mean
+  }
+}
+
+// dL of the tile's logits, rounded once to the operands' precision
+template <class S, int NPROD>
+__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4, M = min(a.T, *a.n);
+  ft_f4 acc[S::NI][S::NJ];
+  FtTile t;
+  if (!ce_product<S, NPROD>(a, smem, acc, t, M, wave, lane)) return;
+  const int m0 = t.m * S::TM, c0 = wn * S::NJ * 16, n0 = a.v0 + t.n * S::TN + c0;
+#pragma unroll
+  for (int i = 0; i < S::NI; ++i) {
+    const int r = (wm * S::NI + i) * 16 + (lane & 15), m = m0 + r;
+    const bool live = m < M;
+    const float lse = live ? a.lse[m] : 0.f;
+    const int rel = (live ? a.y[m] : -1) - n0 - 4 * g;
+    float sc = live ? (a.reduction == FC_REDUCE_NONE ? a.g[a.idx[m]] : a.g[0]) : 0.f;
+    if (a.reduction == FC_REDUCE_MEAN) sc /= (float)M;
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float p = ce_exp<NPROD>(acc[i][j][x], lse);
+        if (rel == 16 * j + x) p -= 1.f;
+        acc[i][j][x] = live && n0 + 16 * j + 4 * g + x < a.V ? p * sc : 0.f;
+      }
+  }
+  const FtRows rows;
+#pragma unroll
+  for (int pl = 0; pl < (NPROD == 1 ? 1 : 3); ++pl) {
+    if (pl) ft_barrier();
+#pragma unroll
+    for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j) {
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (NPROD == 1) { v[x] = acc[i][j][x]; continue; }
+          float h[3];
+          ft_split(acc[i][j][x], h[0], h[1], h[2]);
+          v[x] = h[pl];
+        }
+        ft_img_put<S::TN>(smem, (wm * S::NI + i) * 16 + (lane & 15), c0 + 16 * j + 4 * g, v[0], v[1], v[2], v[3]);
+      }
+    ft_barrier();
+    ft_img_out<S::TM, S::TN, S::NT>(smem, a.dl + pl * a.plane, a.ldl, m0, t.n * S::TN, M, (int)a.ldl, rows, true);
+  }
+}
+
+// ---------------------------------------------------------------- host
+typedef FtShape<256, 256, 2, 4, 2> CeBig;
+typedef FtShape<128, 128, 2, 2, 2> CeMid;
+typedef FtShape<32, 64, 2, 2, 4> CeRow;
+// 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32 (the three planes of dL need registers), 32 x 64 for the few rows
+// of a scoring call
+static int ce_shape(int dt, long T, long V) {
+  if (T <= 32) return 2;
+  return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
+}
+static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
+
+template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, hipStream_t s) {
+  const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.nv + S::TN - 1) / S::TN);
+  FC_REQUIRE(tiles < (1L << 31), "linear_ce: too many tiles");
+  if (GRAD) {
+    FC_TRY(ft_allow_lds((const void*)k_ce_grad<S, NPROD>, S::LDS));
+    hipLaunchKernelGGL((k_ce_grad<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
+  } else {
+    FC_TRY(ft_allow_lds((const void*)k_ce_stats<S, NPROD>, S::LDS));
+    hipLaunchKernelGGL((k_ce_stats<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
+  }
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+template <bool GRAD> static int ce_run(int dt, int shape, const CeArgs& a, hipStream_t s) {
+  if (a.T == 0 || a.nv == 0) return 0;
+  if (dt) return shape == 0 ? ce_launch<CeBig, 1, GRAD>(a, s) : shape == 1 ? ce_launch<CeMid, 1, GRAD>(a, s) : ce_launch<CeRow, 1, GRAD>(a, s);
+  return shape == 1 ? ce_launch<CeMid, 6, GRAD>(a, s) : ce_launch<CeRow, 6, GRAD>(a, s);
+}
+
+// columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
+static long ce_piece(int dt, long T, long V) {
+  const long most = (192L << 20) / ((T ? T : 1) * (dt ? 2 : 6)) / 256 * 256, all = ft_up(V, 256);
+  return most < 256 ? 256 : most < all ? most : all;
+}
+struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx; };
+static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad) {
+  CeSizes z = {};
+  const int np = dt ? 1 : 6;
+  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 1 : 3) * V * ft_up(D, 8) * 2, 256);
+  if (!grad) {
+    const int tn = ce_tn(ce_shape(dt, T, V));
+    z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
+    z.rows = (size_t)ft_up(T * 4, 256) * 2;
+    return z;
+  }
+  z.piece = ce_piece(dt, T, V);
+  z.dl = (size_t)ft_up((dt ? 1 : 3) * T * z.piece * 2, 256);
+  z.dx = ft_plan(TK, TR, np, T, D, z.piece, true);
+  z.dxp = (size_t)ft_up(ft_part_floats(T, D, z.dx) * 4, 256);
+  z.dwp = (size_t)ft_up(ft_product_part_floats(TR, TR, np, z.piece < V ? z.piece : V, D, T) * 4, 256);
+  const long last = V % z.piece;
+  if (last) {
+    const size_t l = (size_t)ft_up(ft_product_part_floats(TR, TR, np, last, D, T) * 4, 256);
+    z.dwp = z.dwp > l ? z.dwp : l;
+  }
+  return z;
+}
+static int ce_args(const char* what, int dt, long T, long V, long D, long ldw, const void* w) {
+  FC_REQUIRE(dt == FC_PREC_FP32 || dt == FC_PREC_BF16, "%s: dt %d", what, dt);
+  FC_REQUIRE(T >= 0 && T <= (1L << 28) && V >= 1 && V <= (1L << 30) && D >= 1 && D <= (1L << 20), "%s: bad sizes (%ld rows, %ld classes, width %ld)", what, T, V, D);
+  FC_REQUIRE(w && ldw >= D && ldw < (1L << 21), "%s: weight missing or its rows %ld apart", what, ldw);
+  return ft_check_device(w, what);
+}
+// the weight as the products take it
+static int ce_weight(int dt, const void* w, long ldw, long V, long D, char*& ws, FtMat& m, hipStream_t s) {
+  if (ft_direct(dt, w, ldw, D)) {
+    m.p = (const bf16_t*)w;
+    m.ld = ldw;
+    return 0;
+  }
+  FtPack k;
+  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 8); k.Rd = V;
+  m.p = k.dst; m.ld = k.ldd; m.plane = V * k.ldd;
+  ws += (size_t)ft_up((dt ? 1 : 3) * V * k.ldd * 2, 256);
+  return ft_pack(k, s);
+}
+
+extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t D) { return T < 0 || D < 1 ? 0 : ce_saved(nullptr, dt, T, D).bytes; }
+extern "C" size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward) {
+  if (T < 0 || V < 1 || D < 1) return 0;
+  const CeSizes z = ce_sizes(dt, T, V, D, dt && !packed, backward != 0);
+  return z.w + z.part + z.rows + z.dl + z.dxp + z.dwp + 256;
+}
+extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
+                                int64_t ignore_index, int32_t reduction, float* loss, void* saved, size_t saved_bytes, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  FC_TRY(ce_args("fc_linear_ce_fwd", dt, T, V, D, ldw, w));
+  FC_REQUIRE(loss && saved && workspace && ((x && y && ldx >= D) || T == 0), "fc_linear_ce_fwd: null pointer, or rows %ld apart", (long)ldx);
+  FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_fwd: reduction %d", reduction);
+  FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_fwd: saved and workspace are aligned to 256 bytes");
+  const CeSaved sv = ce_saved(saved, dt, T, D);
+  const bool direct = ft_direct(dt, w, ldw, D);
+  const CeSizes z = ce_sizes(dt, T, V, D, direct, false);
+  FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.part + z.rows, "fc_linear_ce_fwd: saved or workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  CeArgs a = {};
+  FC_TRY(ce_weight(dt, w, ldw, V, D, ws, a.w, s));
+  a.x = sv.x;
+  a.T = T; a.V = V; a.D = D; a.v0 = 0; a.nv = V;
+  a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
+  a.part = (CePart*)ws;
+  a.tlogit = (float*)(ws + z.part);
+  float* rows = reduction == FC_REDUCE_NONE ? loss : (float*)(ws + z.part + z.rows / 2);
+  const int R = (int)ft_up(T > 65536 ? (T + 1023) / 1024 : 64, 64), blocks = T ? (T + R - 1) / R : 1;
+  if (dt) {
+    const bool vec = ft_direct(1, x, ldx, D);
+    hipLaunchKernelGGL((k_ce_rows<bf16_t, 1>), dim3(blocks), dim3(256), 0, s, (const bf16_t*)x, (long)ldx, y, (long)T, R, V, ignore_index, D, vec, sv);
+  } else {
+    hipLaunchKernelGGL((k_ce_rows<float, 3>), dim3(blocks), dim3(256), 0, s, (const float*)x, (long)ldx, y, (long)T, R, V, ignore_index, D, false, sv);
+  }
+  FC_LAUNCH_CHECK();
+  const int shape = ce_shape(dt, T, V), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
+  FC_TRY(ce_run<false>(dt, shape, a, s));
+  if (T) {
+    const dim3 gj((unsigned)((T + 15) / 16));
+    if (dt) hipLaunchKernelGGL(k_ce_join<1>, gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+    else hipLaunchKernelGGL(k_ce_join<6>, gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+    FC_LAUNCH_CHECK();
+  }
+  if (reduction != FC_REDUCE_NONE) {
+    hipLaunchKernelGGL(k_ce_loss, dim3(1), dim3(1024), 0, s, rows, (long)T, sv.n, reduction, loss);
+    FC_LAUNCH_CHECK();
+  }
+  return 0;
+}
+extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t T, int32_t V, int32_t D, int32_t reduction, const float* gloss,
+                                const void* saved, size_t saved_bytes, void* dx, int64_t lddx, void* dw, int64_t lddw, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  FC_TRY(ce_args("fc_linear_ce_bwd", dt, T, V, D, ldw, w));
+  FC_REQUIRE((gloss || T == 0) && saved && workspace && (!dx || lddx >= D) && (!dw || lddw >= D), "fc_linear_ce_bwd: null pointer, or an output's rows too close");
+  FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_bwd: reduction %d", reduction);
+  FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_bwd: saved and workspace are aligned to 256 bytes");
+  const CeSaved sv = ce_saved((void*)saved, dt, T, D);
+  const bool direct = ft_direct(dt, w, ldw, D);
+  const CeSizes z = ce_sizes(dt, T, V, D, direct, true);
+  FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.dl + z.dxp + z.dwp, "fc_linear_ce_bwd: saved or workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  CeArgs a = {};
+  FC_TRY(ce_weight(dt, w, ldw, V, D, ws, a.w, s));
+  a.x = sv.x;
+  a.T = T; a.V = V; a.D = D;
+  a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
+  a.lse = sv.lse; a.g = gloss; a.reduction = reduction;
+  a.dl = (bf16_t*)ws;
+  a.ldl = z.piece;
+  a.plane = (long)T * z.piece;
+  float* dxp = (float*)(ws + z.dl);
+  float* dwp = (float*)(ws + z.dl + z.dxp);
+  const int np = dt ? 1 : 6, es = dt ? 2 : 4;
+  FtProduct px, pw;
+  px.am = TK; px.bm = TR; px.nprod = np; px.M = T; px.N = D; px.Mdyn = sv.n; px.Ks = (int)z.piece; px.out = dx; px.ldo = lddx;
+  px.a.p = a.dl; px.a.ld = a.ldl; px.a.plane = a.plane;
+  pw.am = TR; pw.bm = TR; pw.nprod = np; pw.N = D; pw.K = T; pw.Kdyn = sv.n; pw.ldo = lddw;
+  pw.a = px.a;
+  pw.b = sv.x;
+  for (long v0 = 0; v0 < V; v0 += z.piece) {
+    a.v0 = (int)v0;
+    a.nv = (int)(V - v0 < z.piece ? V - v0 : z.piece);
+    FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv), a, s));
+    if (dw) {
+      pw.M = a.nv;
+      pw.out = (char*)dw + v0 * lddw * es;
+      FC_TRY(ft_product_out(pw, dwp, z.dwp / 4, s));
+    }
+    if (dx && T) {
+      px.K = a.nv;
+      px.b = a.w;
+      px.b.p = a.w.p + v0 * a.w.ld;
+      FC_TRY(ft_product(px, z.dx, dxp, v0 > 0, s));
+    }
+  }
+  if (dx && T) FC_TRY(ft_reduce(px, z.dx, dxp, sv.pos, T, s));
+  return 0;
+}

@@ -1,0 +1,363 @@
+// Between two branches of a block, in one pass over the rows:
+//
+//   n = norm(y) wp + bp;   r = alpha x + s_b gate n;   h = norm(r) wn + bn
+//
+// y the branch's output, x the residual stream, gate one vector for all rows or one for each sample, s_b a sample's drop-path multiplier;
+// norm: LayerNorm or RMSNorm.  Each part may be absent.  A multiplier of 0 drops the branch: y is not used and its gradient is 0, whatever
+// it holds.  h comes from r before r is rounded.
+// Backward: r and both norms' statistics are formed again from y and x, so nothing is kept and dwn, dwp are those of the unrounded r.
+// Bound: HBM, 4 T D elements forward (y, x in; r, h out), 6 T D backward (y, x, dr, dh in; dy, dx out).
+// A row is held in registers by a wave (D <= 512), 4 waves (<= 2048) or 8 (<= 8192): 8 or 16 values a lane.  A workgroup walks several
+// rows with the weight vectors in registers: read per row they would be 20 bytes an element from L2 beside the 8 from HBM.
+// dwp, dbp, dwn, dbn, dgate: each workgroup's sums over its rows (fp32) are one row of partial sums, added in fp64 in a fixed order by a
+// second launch.  A workgroup's rows share one gate vector.
+#include "../../include/fedcola_hip.h"
+#include "fc_tiles.h"
+
+struct NgArgs {
+  const void *y, *x, *dr, *dh;
+  long ldy, ldx, lddr, lddh;
+  void *r, *h, *dy, *dx;                       // rows D apart
+  const float *wp, *bp, *gate, *scale, *wn, *bn;
+  float alpha, eps;
+  int rms, post, pre, D;
+  long T, gate_rows, scale_rows;               // rows of one gate vector / one multiplier
+  long per, blocks;                            // rows of a workgroup, workgroups of a gate vector
+  float* part;                                 // [workgroups][5][D]: dwp, dbp, dwn, dbn, dgate
+};
+enum { NG_DWP = 0, NG_DBP, NG_DWN, NG_DBN, NG_DGATE, NG_SUMS };
+
+// E values of a row for lane l of NTH: VEC 8: chunks l, l + NTH, ... of 8; VEC 1: values l, l + NTH, ...
+template <int VEC, int NTH, int E, class F> __device__ __forceinline__ void ng_each(int l, int D, F f) {
+  if (VEC == 8) {
+#pragma unroll
+    for (int t = 0; t < E / 8; ++t)
+      if ((l + NTH * t) * 8 < D) f(t * 8, (l + NTH * t) * 8);
+  } else {
+#pragma unroll
+    for (int t = 0; t < E; ++t)
+      if (l + NTH * t < D) f(t, l + NTH * t);
+  }
+}
+__device__ __forceinline__ void ng_ld8(const bf16_t* p, float* v) {
+  const uint4 u = *(const uint4*)p;
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void ng_ld8(const float* p, float* v) {
+  const ft_f4 a = *(const ft_f4*)p, b = *(const ft_f4*)(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
+__device__ __forceinline__ void ng_st8(bf16_t* p, const float* v) { *(uint4*)p = make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7])); }
+__device__ __forceinline__ void ng_st8(float* p, const float* v) {
+  *(ft_f4*)p = ft_f4{v[0], v[1], v[2], v[3]};
+  *(ft_f4*)(p + 4) = ft_f4{v[4], v[5], v[6], v[7]};
+}
+template <typename T, int VEC, int NTH, int E> __device__ __forceinline__ void ng_load(const T* p, int l, int D, float (&v)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = 0.f;
+  if (!p) return;
+  ng_each<VEC, NTH, E>(l, D, [&](int k, int c) {
+    if constexpr (VEC == 8) ng_ld8(p + c, v + k); else v[k] = Io<T>::ld(p, c);
+  });
+}
+template <typename T, int VEC, int NTH, int E> __device__ __forceinline__ void ng_store(T* p, int l, int D, const float (&v)[E]) {
+  ng_each<VEC, NTH, E>(l, D, [&](int k, int c) {
+    if constexpr (VEC == 8) ng_st8(p + c, v + k); else Io<T>::st(p, c, v[k]);
+  });
+}
+// sums over a row's lanes.  W waves: through LDS, one barrier, two buffers in turn (a wave is never two sums ahead of another)
+template <int W> struct NgSum {
+  float2* red;     // [2][W]
+  int turn = 0;
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if (W == 1) return make_float2(a, b);
+    float2* q = red + turn * W;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) q[threadIdx.x >> 6] = make_float2(a, b);
+    ft_barrier();
+    float2 s = q[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) { s.x += q[i].x; s.y += q[i].y; }
+    return s;
+  }
+};
+// v -> normalised v; lanes past D keep 0.  Returns 1 / deviation
+template <int VEC, int NTH, int E, class SUM> __device__ __forceinline__ float ng_norm(float (&v)[E], int l, int D, int rms, float eps, SUM& sum) {
+  const float inv = 1.f / (float)D;
+  float a = 0.f;
+  if (!rms) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) a += v[i];
+    const float mu = sum(a, 0.f).x * inv;
+    constexpr int STEP = VEC == 8 ? 8 : 1;
+    ng_each<VEC, NTH, E>(l, D, [&](int k, int c) {
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) v[k + i] -= mu;
+    });
+    a = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) a += v[i] * v[i];
+  const float rs = 1.f / sqrtf(sum(a, 0.f).x * inv + eps);
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] *= rs;
+  return rs;
+}
+
+template <typename T, int VEC, int W, int E>
+__global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
+  constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;       // rows at once
+  __shared__ float2 red[2 * W];
+  NgSum<W> sum{red};
+  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? threadIdx.x >> 6 : 0, D = a.D;
+  const long grp = blockIdx.x / a.blocks, b0 = (blockIdx.x % a.blocks) * a.per;
+  const long first = grp * a.gate_rows + b0, left = a.gate_rows - b0, n = left < a.per ? left : a.per;
+  float wp[E], bp[E], gt[E], wn[E], bn[E];
+  ng_load<float, VEC, NTH, E>(a.wp, l, D, wp);
+  ng_load<float, VEC, NTH, E>(a.bp, l, D, bp);
+  ng_load<float, VEC, NTH, E>(a.gate ? a.gate + grp * D : nullptr, l, D, gt);
+  ng_load<float, VEC, NTH, E>(a.wn, l, D, wn);
+  ng_load<float, VEC, NTH, E>(a.bn, l, D, bn);
+  for (long i = sub; i < n; i += RB) {
+    const long row = first + i;
+    const float s = a.scale ? a.scale[row / a.scale_rows] : 1.f;
+    float y[E], x[E];
+    ng_load<T, VEC, NTH, E>(s == 0.f ? nullptr : (const T*)a.y + row * a.ldy, l, D, y);
+    ng_load<T, VEC, NTH, E>((const T*)a.x + row * a.ldx, l, D, x);
+    if (a.post) {
+      ng_norm<VEC, NTH, E>(y, l, D, a.rms, a.eps, sum);
+#pragma unroll
+      for (int k = 0; k < E; ++k) y[k] = y[k] * wp[k] + bp[k];
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + s * (a.gate ? gt[k] * y[k] : y[k]);
+    ng_store<T, VEC, NTH, E>((T*)a.r + row * D, l, D, x);
+    if (a.pre) {
+      ng_norm<VEC, NTH, E>(x, l, D, a.rms, a.eps, sum);
+#pragma unroll
+      for (int k = 0; k < E; ++k) x[k] = x[k] * wn[k] + bn[k];
+      ng_store<T, VEC, NTH, E>((T*)a.h + row * D, l, D, x);
+    }
+  }
+}
+
+template <typename T, int VEC, int W, int E>
+__global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_bwd(NgArgs a) {
+  constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;
+  __shared__ float2 red[2 * W];
+  __shared__ float acc4[W == 1 ? 4 * 512 : 1];
+  NgSum<W> sum{red};
+  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? threadIdx.x >> 6 : 0, D = a.D;
+  const float inv = 1.f / (float)D;
+  const long grp = blockIdx.x / a.blocks, b0 = (blockIdx.x % a.blocks) * a.per;
+  const long first = grp * a.gate_rows + b0, left = a.gate_rows - b0, n = left < a.per ? left : a.per;
+  float wp[E], bp[E], gt[E], wn[E], sums[NG_SUMS][E];
+  ng_load<float, VEC, NTH, E>(a.wp, l, D, wp);
+  ng_load<float, VEC, NTH, E>(a.bp, l, D, bp);
+  ng_load<float, VEC, NTH, E>(a.gate ? a.gate + grp * D : nullptr, l, D, gt);
+  ng_load<float, VEC, NTH, E>(a.wn, l, D, wn);
+#pragma unroll
+  for (int q = 0; q < NG_SUMS; ++q)
+#pragma unroll
+    for (int k = 0; k < E; ++k) sums[q][k] = 0.f;
+  for (long i = sub; i < n; i += RB) {
+    const long row = first + i;
+    const float s = a.scale ? a.scale[row / a.scale_rows] : 1.f;
+    float y[E], x[E], d[E], dn[E];
+    ng_load<T, VEC, NTH, E>(s == 0.f ? nullptr : (const T*)a.y + row * a.ldy, l, D, y);
+    ng_load<T, VEC, NTH, E>((const T*)a.x + row * a.ldx, l, D, x);
+    ng_load<T, VEC, NTH, E>(a.dr ? (const T*)a.dr + row * a.lddr : nullptr, l, D, d);
+    ng_load<T, VEC, NTH, E>(a.dh ? (const T*)a.dh + row * a.lddh : nullptr, l, D, dn);
+    const float rs1 = a.post ? ng_norm<VEC, NTH, E>(y, l, D, a.rms, a.eps, sum) : 1.f;      // y: its normalised row from here on
+    if (a.pre) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float p = a.post ? y[k] * wp[k] + bp[k] : y[k];
+        x[k] = a.alpha * x[k] + s * (a.gate ? gt[k] * p : p);
+      }
+      const float rs2 = ng_norm<VEC, NTH, E>(x, l, D, a.rms, a.eps, sum);
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        sums[NG_DWN][k] += dn[k] * x[k];
+        sums[NG_DBN][k] += dn[k];
+        dn[k] *= wn[k];
+        s1 += dn[k];
+        s2 += dn[k] * x[k];
+      }
+      const float2 m = sum(s1, s2);
+      const float m1 = a.rms ? 0.f : m.x * inv, m2 = m.y * inv;
+#pragma unroll
+      for (int k = 0; k < E; ++k) d[k] += rs2 * (dn[k] - m1 - x[k] * m2);
+    }
+    // d: the gradient of r
+#pragma unroll
+    for (int k = 0; k < E; ++k) dn[k] = a.alpha * d[k];
+    ng_store<T, VEC, NTH, E>((T*)a.dx + row * D, l, D, dn);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const float p = a.post ? y[k] * wp[k] + bp[k] : y[k], dp = s == 0.f ? 0.f : d[k] * s;
+      sums[NG_DGATE][k] += dp * p;
+      d[k] = a.gate ? dp * gt[k] : dp;
+      if (a.post) {
+        sums[NG_DWP][k] += d[k] * y[k];
+        sums[NG_DBP][k] += d[k];
+        d[k] *= wp[k];
+        s1 += d[k];
+        s2 += d[k] * y[k];
+      }
+    }
+    if (a.post) {
+      const float2 m = sum(s1, s2);
+      const float m1 = a.rms ? 0.f : m.x * inv, m2 = m.y * inv;
+#pragma unroll
+      for (int k = 0; k < E; ++k) d[k] = rs1 * (d[k] - m1 - y[k] * m2);
+    }
+    ng_store<T, VEC, NTH, E>((T*)a.dy + row * D, l, D, d);
+  }
+  if (!a.part) return;
+  float* o = a.part + (long)blockIdx.x * NG_SUMS * D;
+#pragma unroll
+  for (int q = 0; q < NG_SUMS; ++q) {
+    if (W == 1) {
+      __syncthreads();
+      ng_store<float, VEC, NTH, E>(acc4 + sub * 512, l, D, sums[q]);
+      __syncthreads();
+      for (int c = threadIdx.x; c < D; c += 256) o[q * D + c] = (acc4[c] + acc4[512 + c]) + (acc4[1024 + c] + acc4[1536 + c]);
+    } else {
+      ng_each<VEC, NTH, E>(l, D, [&](int k, int c) {
+        constexpr int STEP = VEC == 8 ? 8 : 1;
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) o[q * D + c + i] = sums[q][k + i];
+      });
+    }
+  }
+}
+
+// out[c] = sum over workgroups of their partial sums: 64 columns by 16 slices of the workgroups
+struct NgOut { float* p[NG_SUMS]; };
+__global__ void __launch_bounds__(1024) k_ng_sum(const float* part, int D, long blocks, long groups, NgOut out) {
+  __shared__ double red[16][64];
+  const int q = blockIdx.y < 4 ? blockIdx.y : NG_DGATE, c = blockIdx.x * 64 + (threadIdx.x & 63), sl = threadIdx.x >> 6;
+  const long g = blockIdx.y < 4 ? 0 : blockIdx.y - 4, b0 = g * blocks, b1 = q == NG_DGATE ? b0 + blocks : groups * blocks;
+  if (!out.p[q]) return;
+  double v = 0;
+  if (c < D)
+#pragma unroll 4
+    for (long b = b0 + sl; b < b1; b += 16) v += (double)part[(b * NG_SUMS + q) * D + c];
+  red[sl][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (sl == 0 && c < D) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += red[i][threadIdx.x & 63];
+    out.p[q][g * D + c] = (float)v;
+  }
+}
+
+// ---------------------------------------------------------------- host
+// workgroups of a gate vector's rows: about 1024 in all for wide rows (4 a CU; 2048 of the one-wave-a-row form), at least a few rows each
+static void ng_split(long T, long gate_rows, long D, long& per, long& blocks) {
+  const long groups = T / gate_rows, want = D <= 512 ? 1024 : 1024, at_once = D <= 512 ? 4 : 1;
+  long b = (want + groups - 1) / groups;
+  const long most = (gate_rows + 2 * at_once - 1) / (2 * at_once);
+  b = b < most ? b : most;
+  per = (gate_rows + b - 1) / b;
+  blocks = (gate_rows + per - 1) / per;
+}
+static bool ng_aligned(const NgArgs& a, int dt) {
+  size_t p = (size_t)a.y | (size_t)a.x | (size_t)a.dr | (size_t)a.dh | (size_t)a.r | (size_t)a.h | (size_t)a.dy | (size_t)a.dx | (size_t)a.wp | (size_t)a.bp |
+             (size_t)a.gate | (size_t)a.wn | (size_t)a.bn;
+  const long m = dt ? 8 : 4;
+  return (p & 15) == 0 && a.D % 8 == 0 && a.ldy % m == 0 && a.ldx % m == 0 && a.lddr % m == 0 && a.lddh % m == 0;
+}
+template <typename T, bool BWD> static int ng_launch(const NgArgs& a, int dt, hipStream_t s) {
+  const dim3 g((unsigned)(a.T / a.gate_rows * a.blocks));
+  const bool v = ng_aligned(a, dt);
+#define NG_RUN(VEC, W, E)                                                                                          \
+  do {                                                                                                             \
+    if (BWD) hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                   \
+    else hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                       \
+  } while (0)
+#define NG_PICK(W, E) do { if (v) NG_RUN(8, W, E); else NG_RUN(1, W, E); } while (0)
+  if (a.D <= 512) NG_PICK(1, 8);
+  else if (a.D <= 2048) NG_PICK(4, 8);
+  else if (a.D <= 4096) NG_PICK(8, 8);
+  else NG_PICK(8, 16);
+#undef NG_PICK
+#undef NG_RUN
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+static int ng_check(const char* what, int dt, int kind, const NgArgs& a, const void* out) {
+  FC_REQUIRE(dt == FC_PREC_FP32 || dt == FC_PREC_BF16, "%s: dt %d", what, dt);
+  FC_REQUIRE(kind == FC_NORM_LAYER || kind == FC_NORM_RMS, "%s: norm %d", what, kind);
+  FC_REQUIRE(a.T >= 0 && a.T < (1L << 40) && a.D >= 1 && a.D <= 8192, "%s: bad sizes (%ld rows, width %d: 1 to 8192)", what, a.T, a.D);
+  FC_REQUIRE(a.T == 0 || (a.y && a.x && out), "%s: null pointer", what);
+  FC_REQUIRE(a.ldy >= a.D && a.ldx >= a.D, "%s: rows %ld and %ld apart", what, a.ldy, a.ldx);
+  FC_REQUIRE(a.eps > 0.f, "%s: eps %g", what, (double)a.eps);
+  FC_REQUIRE(a.gate_rows >= 1 && a.scale_rows >= 1 && a.T % a.gate_rows == 0 && a.T % a.scale_rows == 0, "%s: %ld rows are no whole number of samples", what, a.T);
+  FC_REQUIRE((!a.bp || a.wp) && (!a.bn || a.wn), "%s: a bias without its weight", what);
+  FC_REQUIRE(kind == FC_NORM_LAYER || (!a.bp && !a.bn), "%s: RMSNorm has no bias", what);
+  return ft_check_device(a.x, what);
+}
+extern "C" size_t fc_norm_gate_workspace_bytes(int64_t T, int32_t D, int64_t gate_rows) {
+  if (T <= 0 || D < 1 || gate_rows < 0) return 256;
+  long per, blocks;
+  const long gr = gate_rows ? gate_rows : T;
+  if (T % gr) return 256;
+  ng_split(T, gr, D, per, blocks);
+  return (size_t)(T / gr) * blocks * NG_SUMS * D * sizeof(float) + 256;
+}
+extern "C" int fc_norm_gate_fwd(int32_t dt, int32_t kind, const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t T, int32_t D, const float* post_w,
+                                const float* post_b, const float* gate, int64_t gate_rows, const float* row_scale, int64_t scale_rows, float alpha,
+                                const float* pre_w, const float* pre_b, float eps, void* r, void* h, void* stream) {
+  NgArgs a = {};
+  a.y = y; a.x = x; a.ldy = ldy; a.ldx = ldx; a.r = r; a.h = h;
+  a.wp = post_w; a.bp = post_b; a.gate = gate; a.scale = row_scale; a.wn = pre_w; a.bn = pre_b;
+  a.alpha = alpha; a.eps = eps; a.rms = kind == FC_NORM_RMS; a.post = post_w != nullptr; a.pre = pre_w != nullptr; a.D = D; a.T = T;
+  a.gate_rows = gate && gate_rows ? gate_rows : T ? T : 1;
+  a.scale_rows = row_scale && scale_rows ? scale_rows : T ? T : 1;
+  FC_TRY(ng_check("fc_norm_gate_fwd", dt, kind, a, r));
+  FC_REQUIRE(!a.pre || h || T == 0, "fc_norm_gate_fwd: no place for the second norm's output");
+  if (T == 0) return 0;
+  ng_split(T, a.gate_rows, D, a.per, a.blocks);
+  FC_REQUIRE(T / a.gate_rows * a.blocks < (1L << 31), "fc_norm_gate_fwd: too many samples");
+  return dt ? ng_launch<bf16_t, false>(a, dt, (hipStream_t)stream) : ng_launch<float, false>(a, dt, (hipStream_t)stream);
+}
+extern "C" int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_t lddr, const void* dh, int64_t lddh, const void* y, int64_t ldy, const void* x,
+                                int64_t ldx, int64_t T, int32_t D, const float* post_w, const float* post_b, const float* gate, int64_t gate_rows,
+                                const float* row_scale, int64_t scale_rows, float alpha, const float* pre_w, float eps, void* dy, void* dx, float* d_post_w,
+                                float* d_post_b, float* d_pre_w, float* d_pre_b, float* d_gate, void* workspace, size_t workspace_bytes, void* stream) {
+  NgArgs a = {};
+  a.y = y; a.x = x; a.ldy = ldy; a.ldx = ldx; a.dr = dr; a.dh = dh; a.lddr = dr ? lddr : 0; a.lddh = dh ? lddh : 0; a.dy = dy; a.dx = dx;
+  a.wp = post_w; a.bp = post_b; a.gate = gate; a.scale = row_scale; a.wn = pre_w;
+  a.alpha = alpha; a.eps = eps; a.rms = kind == FC_NORM_RMS; a.post = post_w != nullptr; a.pre = pre_w != nullptr && dh != nullptr; a.D = D; a.T = T;
+  a.gate_rows = gate && gate_rows ? gate_rows : T ? T : 1;
+  a.scale_rows = row_scale && scale_rows ? scale_rows : T ? T : 1;
+  FC_TRY(ng_check("fc_norm_gate_bwd", dt, kind, a, dy));
+  FC_REQUIRE((dx || T == 0) && (!dr || lddr >= D) && (!dh || lddh >= D) && (!dh || pre_w), "fc_norm_gate_bwd: null pointer, rows too close, or a gradient without its norm");
+  const long groups = T ? T / a.gate_rows : 0;
+  NgOut out = {{d_post_w, d_post_b, d_pre_w, d_pre_b, gate ? d_gate : nullptr}};
+  const bool sums = out.p[0] || out.p[1] || out.p[2] || out.p[3] || out.p[4];
+  hipStream_t s = (hipStream_t)stream;
+  if (T) {
+    ng_split(T, a.gate_rows, D, a.per, a.blocks);
+    FC_REQUIRE(groups * a.blocks < (1L << 31) && groups < 65000, "fc_norm_gate_bwd: too many samples");
+    if (sums) {
+      FC_REQUIRE(workspace && ((size_t)workspace & 255) == 0 && workspace_bytes >= (size_t)groups * a.blocks * NG_SUMS * D * sizeof(float), "fc_norm_gate_bwd: workspace too small or not aligned to 256 bytes");
+      a.part = (float*)workspace;
+    }
+    FC_TRY(dt ? (ng_launch<bf16_t, true>(a, dt, s)) : (ng_launch<float, true>(a, dt, s)));
+  }
+  if (sums) {
+    hipLaunchKernelGGL(k_ng_sum, dim3((D + 63) / 64, (unsigned)(4 + (out.p[NG_DGATE] ? groups : 0))), dim3(1024), 0, s, a.part, D, a.blocks, groups, out);
+    FC_LAUNCH_CHECK();
+  }
+  return 0;
+}

@@ -1,0 +1,288 @@
+// Tiled products for the fused vocabulary cross entropy (fc_linear_ce.hip) and the gated feed-forward block (fc_gated_mlp.hip):
+//
+//     C[m, n] = sum_k A(m, k) B(n, k)
+//
+// with each operand stored either with k contiguous ("TK": rows are m or n) or with k as its row index ("TR"), bf16, on
+// v_mfma_f32_16x16x32_bf16.  fp32 operands come as three bf16 planes hi + mid + lo (24 bits of mantissa); a k-step is then run six
+// times, over the plane pairs whose product is above 2^-24 of the whole (NPROD = 6), so that the result is that of an fp32 product.
+//
+// One k-step is 64 deep.  Operand tiles go global -> LDS by buffer_load ... lds (16 B a lane), NS stages deep, one barrier a step.  The
+// loads are issued by inline asm: with the builtin the compiler waits for every load in flight in front of the LDS reads it cannot tell
+// apart from the load's destination.  They have no register results; dma_wait() in front of each barrier waits for them.
+// Rows, columns and k past the end read as zero: by the descriptor's size or by an offset outside of it.
+// LDS images (both conflict-free): TK [rows][64 k], 128-B rows, 16-B chunk c of row r at chunk c ^ ((r >> 1) & 7), read by ds_read_b128;
+// TR [64 k][W cols], 32-B unit u of row k at unit u ^ (((k >> 3) & 1) << 2 | (k & 3)), read by ds_read_b64_tr_b16.
+// The MFMA's operands are swapped, so a lane's accumulator acc[i][j] is row 16 i + (lane & 15), columns 16 j + 4 (lane >> 4) .. + 3.
+#pragma once
+#include "fc_common.h"
+
+typedef __attribute__((ext_vector_type(8))) short ft_b8;
+typedef __attribute__((ext_vector_type(4))) short ft_b4;
+typedef __attribute__((ext_vector_type(4))) float ft_f4;
+typedef __attribute__((ext_vector_type(4))) int ft_i4;
+typedef __attribute__((address_space(3))) ft_b4 ft_lds_b4;
+
+enum { TK = 0, TR = 1 };
+#define FT_OOB 0x80000000u       // outside of every descriptor below (their sizes stay under 2^31)
+#define FT_MAX_BYTES 0x7fffff00L
+
+// one operand: element (row, k) of plane q at p[q * plane + row * ld + k] (TK), (k, col) at p[q * plane + k * ld + col] (TR)
+struct FtMat {
+  const bf16_t* p = nullptr;
+  long ld = 0, plane = 0;
+};
+
+__device__ __forceinline__ int ft_wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+__device__ __forceinline__ unsigned ft_lds_addr(const char* p) {
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)(size_t)(__attribute__((address_space(3))) const char*)p);
+}
+template <int N> __device__ __forceinline__ void ft_dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ft_barrier() {   // LDS hand-off: this wave's LDS traffic is done, its global stores need not be
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// m0 (a reserved register, no operand of anything else in these kernels) takes the LDS address of the wave's piece
+__device__ __forceinline__ void ft_dma16(ft_i4 rsrc, unsigned lds, unsigned voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ ft_i4 ft_rsrc(const void* p, long bytes) {
+  const unsigned long long a = (unsigned long long)p;
+  const long b = bytes < 0 ? 0 : bytes > FT_MAX_BYTES ? FT_MAX_BYTES : bytes;
+  ft_i4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
+  r[1] = __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32) & 0xffff);
+  r[2] = __builtin_amdgcn_readfirstlane((int)b);
+  r[3] = 0x00020000;
+  return r;
+}
+
+// Stages one operand's tile of W rows (TK) or columns (TR) by NW waves, W / 8 pieces of 1 KB.
+template <int MODE, int W, int NW> struct FtStager {
+  static constexpr int NP = W / 8 / NW;
+  static_assert(NP >= 1 && NP * NW * 8 == W, "a wave moves whole pieces");
+  static_assert(MODE == TK || W >= 128, "a TR row holds at least the swizzle's eight units");
+  const bf16_t* p;
+  long ld, plane;
+  int K, kc[MODE == TK ? NP : 1];   // kc: first k of the lane's chunk inside the step
+  unsigned voff[NP];
+
+  // map(r): row (TK) / column (TR) of the matrix that tile position r takes, < 0 for none.  TR positions come in eights: map(r + i) = map(r) + i.
+  // TK: offsets are taken from row `base`, the least row of the tile.
+  template <class F> __device__ __forceinline__ void init(const FtMat& m, long base, int K_, int wave, int lane, F map) {
+    ld = m.ld; plane = m.plane; K = K_;
+    p = m.p + (MODE == TK ? base * ld : 0);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int piece = wave * NP + i;
+      if (MODE == TK) {
+        const int r = piece * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        const long row = map(r);
+        kc[i] = c * 8;
+        voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + c * 8) * 2) : FT_OOB;
+      } else {
+        const int k = piece * (512 / W) + lane * 8 / W, pc = lane % (W / 8);
+        const int s = (((k >> 3) & 1) << 2) | (k & 3);
+        const int c = (((pc >> 1) ^ s) << 1) | (pc & 1);
+        const long col = map(c * 8);
+        voff[i] = col >= 0 ? (unsigned)(((long)k * ld + col) * 2) : FT_OOB;
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(unsigned lds, long k0, int pl, int wave) const {
+    const ft_i4 r = MODE == TK ? ft_rsrc(p + pl * plane + k0, FT_MAX_BYTES) : ft_rsrc(p + pl * plane + k0 * ld, (K - k0) * ld * 2);
+    const int left = K - k0 < 64 ? (int)(K - k0) : 64;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const unsigned vo = MODE == TK ? (kc[i] < left ? voff[i] : FT_OOB) : voff[i];
+      ft_dma16(r, lds + (wave * NP + i) * 1024, vo);
+    }
+  }
+};
+
+// one wave's fragment of 16 rows / columns starting at rb (a multiple of 16) for the 32-deep half ks of a step
+template <int MODE, int W> __device__ __forceinline__ ft_b8 ft_frag(const char* tile, int rb, int ks, int lane) {
+  const int g = lane >> 4;
+  if (MODE == TK) {
+    const int c = (ks * 4 + g) ^ ((lane >> 1) & 7);
+    return *(const ft_b8*)(tile + (rb + (lane & 15)) * 128 + (c << 4));
+  }
+  const int q = (lane >> 2) & 3, s = ((g & 1) << 2) | q;
+  const char* a = tile + (ks * 32 + 8 * g + q) * (W * 2) + ((((rb >> 4) ^ s)) << 5) + (lane & 3) * 8;
+  const ft_b4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ft_lds_b4*)a);
+  const ft_b4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ft_lds_b4*)(a + 4 * W * 2));
+  return ft_b8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// tile shape: TM x TN by WM x WN waves, NS LDS stages
+template <int TM_, int TN_, int WM_, int WN_, int NS_> struct FtShape {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, NW = WM * WN, NT = NW * 64;
+  static constexpr int NI = TM / WM / 16, NJ = TN / WN / 16, STAGE = (TM + TN) * 128, LDS = NS * STAGE;
+};
+// plane pairs of the six products, least k first: (0,0) (0,1) (1,0) (1,1) (0,2) (2,0); one nibble each
+__device__ __forceinline__ int ft_pa(int c) { return (0x201100 >> (4 * c)) & 3; }
+__device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; }
+
+// acc += the k-steps [kt0, kt1).  On return every wave has left the loop's LDS reads behind and no load into LDS is in flight.
+template <class S, int AM, int BMO, int NPROD, int NJ>
+__device__ __forceinline__ void ft_loop(const FtStager<AM, S::TM, S::NW>& sa, const FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+                                        ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
+  constexpr int TNL = NJ * 16 * S::WN;      // columns staged (the shape's TN, or less in a second loop over the same tile)
+  constexpr int PIECES = FtStager<AM, S::TM, S::NW>::NP + FtStager<BMO, TNL, S::NW>::NP;
+  const unsigned lds0 = ft_lds_addr(smem);
+  const int steps = (kt1 - kt0) * NPROD;
+  int ic = 0, slot = 0, c = 0;
+  long ik = (long)kt0 * 64;
+  auto put = [&](int at) {                  // steps past the end load zeros (k >= K), so every step issues the same number of loads
+    const bool in = ic < steps;
+    const long k0 = in ? ik : (long)sa.K + 64;
+    const long k0b = in ? ik : (long)sb.K + 64;
+    sa.issue(lds0 + at * S::STAGE, k0, NPROD == 1 ? 0 : ft_pa(c), wave);
+    sb.issue(lds0 + at * S::STAGE + S::TM * 128, k0b, NPROD == 1 ? 0 : ft_pb(c), wave);
+    ++ic;
+    if (NPROD == 1) ik += 64;
+    else if (++c == NPROD) { c = 0; ik += 64; }
+  };
+#pragma unroll
+  for (int s = 0; s < S::NS - 1; ++s) put(s);
+  int free_slot = S::NS - 1;
+  for (int s = 0; s < steps; ++s) {
+    ft_dma_wait<(S::NS - 2) * PIECES>();
+    ft_barrier();
+    put(free_slot);
+    const char* ta = smem + slot * S::STAGE;
+    const char* tb = ta + S::TM * 128;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      ft_b8 af[S::NI], bf[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) bf[j] = ft_frag<BMO, TNL>(tb, (wn * NJ + j) * 16, ks, lane);
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i) af[i] = ft_frag<AM, S::TM>(ta, (wm * S::NI + i) * 16, ks, lane);
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
+    }
+    free_slot = slot;
+    slot = slot + 1 == S::NS ? 0 : slot + 1;
+  }
+  ft_dma_wait<0>();
+  ft_barrier();
+}
+
+// ---- which tile a workgroup takes.  Consecutive ids share an XCD's L2 (workgroups are dealt to the 8 XCDs in turn), and ids walk the
+// tiles in groups of 8 tile rows, column by column, so that the tiles in flight on an XCD share few operand panels.
+struct FtTile { int m, n, split; bool any; };
+__device__ __forceinline__ FtTile ft_tile(int tm, int tn, int splits) {
+  FtTile t;
+  const int total = tm * tn * splits, b = blockIdx.x;
+  t.any = b < total;
+  if (!t.any) { t.m = t.n = t.split = 0; return t; }
+  const int q = total >> 3, r = total & 7, xcd = b & 7;
+  int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
+  t.split = id / (tm * tn);
+  id -= t.split * tm * tn;
+  const int per = 8 * tn, gi = id / per, first = gi * 8, gs = tm - first < 8 ? tm - first : 8, in = id - gi * per;
+  t.m = first + in % gs;
+  t.n = in / gs;
+  return t;
+}
+
+// ---- rows of an output: position i of `half` rows each goes to row (i / half) * to + i % half, none where i % half >= to (0: as it is)
+struct FtRows {
+  int half = 0, to = 0;
+  __device__ __forceinline__ long at(int i) const {
+    if (!half) return i;
+    const int h = i >= half ? 1 : 0, f = i - h * half;
+    return f < to ? (long)h * to + f : -1;
+  }
+};
+
+// a bf16 image of the tile in LDS, rows of IW columns: 16-B chunk c of row r at chunk c ^ (r & 15)
+template <int IW> __device__ __forceinline__ int ft_img(int row, int chunk) { return row * (IW * 2) + ((chunk ^ (row & 15 & (IW / 8 - 1))) << 4); }
+template <int IW> __device__ __forceinline__ void ft_img_put(char* img, int row, int col, float a, float b, float c, float d) {
+  *(uint2*)(img + ft_img<IW>(row, col >> 3) + (col & 4) * 2) = make_uint2(f2bf2(a, b), f2bf2(c, d));
+}
+// image -> global: rows m0 + r < M, columns n0 + c < N of a row-major bf16 matrix
+template <int IR, int IW, int NT>
+__device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld, int m0, int n0, int M, int N, const FtRows& rows, bool vec) {
+#pragma unroll 4
+  for (int e = threadIdx.x; e < IR * (IW / 8); e += NT) {
+    const int r = e / (IW / 8), c = e % (IW / 8), m = m0 + r, n = n0 + c * 8;
+    if (m >= M || n >= N) continue;
+    const long row = rows.at(m);
+    if (row < 0) continue;
+    const uint4 v = *(const uint4*)(img + ft_img<IW>(r, c));
+    bf16_t* o = out + row * ld + n;
+    if (vec && n + 8 <= N) {
+      *(uint4*)o = v;
+    } else {
+      const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < N) o[i] = (bf16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+// the three planes of an fp32 value.  A value that is no number or infinite is its first plane alone.
+__device__ __forceinline__ void ft_split(float x, float& hi, float& mid, float& lo) {
+  hi = bf2f(f2bf(x));
+  const float r = x - hi;
+  const bool fin = __builtin_fabsf(hi) < __builtin_inff();
+  mid = fin ? bf2f(f2bf(r)) : 0.f;
+  lo = fin ? r - mid : 0.f;
+}
+
+// ---------------------------------------------------------------- host side (fc_tiles.hip)
+// C = A B^T written to `out` (bf16 for nprod 1, fp32 for 6), or as fp32 partial sums for ft_reduce().
+struct FtProduct {
+  int am = TK, bm = TK, nprod = 1;
+  FtMat a, b;
+  int M = 0, N = 0, K = 0;
+  int Ks = 0;                     // > 0: the length that the slices are cut from, >= K (products added onto each other's partial sums)
+  const int* Mdyn = nullptr;      // device: the rows (M) / reduction length (K) really there, at most M / K
+  const int* Kdyn = nullptr;
+  void* out = nullptr;
+  long ldo = 0;
+  FtRows rows;
+};
+// shape: index of the tile shape; target: workgroups wanted, by which the reduction is sliced (0: it is not)
+struct FtPlan { int shape = 0, target = 0; };
+FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_rows);
+__host__ __device__ static inline long ft_part_ld(long N) { return (N + 7) / 8 * 8; }
+// slices of a reduction of length K for `tiles` output tiles: as many as the target asks for, none under four k-steps
+__host__ __device__ static inline int ft_slices(long tiles, long K, int target) {
+  if (target <= 0 || tiles <= 0) return 1;
+  long s = target / tiles;
+  const long most = (K + 63) / 64 / 4;
+  s = s < most ? s : most;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+size_t ft_part_floats(long M, long N, const FtPlan& plan);     // for any number of rows up to M
+// partial sums [slices][rows there][ft_part_ld(N)] into `part` (or, part null, the product into p.out); add: onto what is there
+int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s);
+// out = the sum over the slices, in their order, of ft_product's partial sums; with `pos`: out[r] = row pos[r] of the sums, 0 where pos[r] < 0, for R rows
+int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s);
+// the product into p.out, by way of partial sums in `part` where the plan slices the reduction
+int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s);
+size_t ft_product_part_floats(int am, int bm, int nprod, long M, long N, long K);
+
+// an operand as the products take it: aligned, and in planes for fp32.  Rows come from `rows` halves (FtRows the other way round) or idx.
+struct FtPack {
+  const void* src = nullptr;
+  long lds = 0;                   // elements between source rows
+  int dt = 1;
+  long R = 0, C = 0;              // rows and columns there
+  bf16_t* dst = nullptr;
+  long ldd = 0;                   // multiple of 8, >= C: the columns in between are written as zeros
+  long Rd = 0;                    // rows written
+  long half = 0, to = 0;          // half > 0: row i of dst is row (i / half) * to + i % half of src, zeros where i % half >= to
+};
+int ft_pack(const FtPack& p, hipStream_t s);
+static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
+static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }
+// > 64 KB of LDS for a kernel, once for each device
+int ft_allow_lds(const void* kernel, int bytes);
+// the device that holds p has to be the current one
+int ft_check_device(const void* p, const char* what);

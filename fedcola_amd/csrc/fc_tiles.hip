@@ -1,0 +1,257 @@
+// The plain tiled product of fc_tiles.h with its choice of tile and of slices of the reduction, the sum of the slices, and the packing
+// of operands that the tile loads cannot take as they are.
+#include "fc_tiles.h"
+
+#include <atomic>
+#include <mutex>
+#include <set>
+#include <utility>
+
+int ft_allow_lds(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>>* done = new std::set<std::pair<int, const void*>>;
+  int dev = 0;
+  FC_CHECK_HIP(hipGetDevice(&dev));
+  std::lock_guard<std::mutex> l(mu);
+  if (done->count({dev, kernel})) return 0;
+  FC_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done->insert({dev, kernel});
+  return 0;
+}
+
+int ft_check_device(const void* p, const char* what) {
+  hipPointerAttribute_t at;
+  int cur = 0;
+  if (!p) return 0;
+  if (hipPointerGetAttributes(&at, p) != hipSuccess) { (void)hipGetLastError(); fc_set_error("%s: not a device pointer", what); return -1; }
+  FC_CHECK_HIP(hipGetDevice(&cur));
+  FC_REQUIRE(at.type == hipMemoryTypeDevice || at.type == hipMemoryTypeManaged, "%s: not a device pointer", what);
+  FC_REQUIRE(at.device == cur, "%s: the buffers are on device %d, the current device is %d", what, at.device, cur);
+  return 0;
+}
+
+// ---------------------------------------------------------------- packing
+template <typename T, int PL>
+__global__ void __launch_bounds__(256) k_ft_pack(FtPack a) {
+  const long cw = a.ldd / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= a.Rd * cw) return;
+  const long i = e / cw;
+  const int c0 = (int)(e - i * cw) * 8;
+  long r = i;
+  if (a.half > 0) { const long h = i / a.half, f = i - h * a.half; r = f < a.to ? h * a.to + f : -1; }
+  if (r >= a.R) r = -1;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = r >= 0 && c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
+  float h[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (PL == 1) h[0][j] = v[j]; else ft_split(v[j], h[0][j], h[1][j], h[2][j]);
+  }
+#pragma unroll
+  for (int p = 0; p < PL; ++p)
+    *(uint4*)(a.dst + (size_t)p * a.Rd * a.ldd + i * a.ldd + c0) =
+        make_uint4(f2bf2(h[p][0], h[p][1]), f2bf2(h[p][2], h[p][3]), f2bf2(h[p][4], h[p][5]), f2bf2(h[p][6], h[p][7]));
+}
+int ft_pack(const FtPack& p, hipStream_t s) {
+  const long n = p.Rd * (p.ldd / 8);
+  if (n == 0) return 0;
+  const dim3 g((unsigned)((n + 255) / 256));
+  if (p.dt) hipLaunchKernelGGL((k_ft_pack<bf16_t, 1>), g, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((k_ft_pack<float, 3>), g, dim3(256), 0, s, p);
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+
+// ---------------------------------------------------------------- the product
+template <class S, int AM, int BMO, int NPROD, bool PART>
+__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtProduct p, float* part, int target, int add) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
+  const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = p.Ks ? p.Ks : K, splits = ft_slices((long)tm * tn, Ks, target);
+  const FtTile t = ft_tile(tm, tn, splits);
+  if (!t.any) return;
+  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = t.n * S::TN;
+  FtStager<AM, S::TM, S::NW> sa;
+  FtStager<BMO, S::TN, S::NW> sb;
+  sa.init(p.a, m0, K, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
+  sb.init(p.b, n0, K, wave, lane, [&](int r) { return n0 + r < N ? (long)n0 + r : -1L; });
+  ft_f4 acc[S::NI][S::NJ];
+#pragma unroll
+  for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
+  const int nk = (K + 63) / 64, per = ((Ks + 63) / 64 + splits - 1) / splits, kt0 = min(nk, t.split * per);
+  ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0, min(nk, kt0 + per), acc, wm, wn, wave, lane);
+  const int mr = wm * S::NI * 16 + (lane & 15), nc = wn * S::NJ * 16 + 4 * (lane >> 4);
+  if (PART) {
+    const long ldp = ft_part_ld(N);
+    float* o = part + (long)t.split * M * ldp;
+#pragma unroll
+    for (int i = 0; i < S::NI; ++i) {
+      const int m = m0 + mr + 16 * i;
+      if (m >= M) continue;
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j) {
+        const int n = n0 + nc + 16 * j;
+        if (n >= ldp) continue;
+        ft_f4* q = (ft_f4*)(o + (long)m * ldp + n);
+        *q = add ? *q + acc[i][j] : acc[i][j];
+      }
+    }
+  } else if (NPROD == 1) {
+#pragma unroll
+    for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j) ft_img_put<S::TN>(smem, mr + 16 * i, nc + 16 * j, acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+    ft_barrier();
+    const bool vec = p.ldo % 8 == 0 && ((size_t)p.out & 15) == 0;
+    ft_img_out<S::TM, S::TN, S::NT>(smem, (bf16_t*)p.out, p.ldo, m0, n0, M, N, p.rows, vec);
+  } else {
+    const bool vec = p.ldo % 4 == 0 && ((size_t)p.out & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < S::NI; ++i) {
+      const int m = m0 + mr + 16 * i;
+      const long row = m < M ? p.rows.at(m) : -1;
+      if (row < 0) continue;
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j) {
+        const int n = n0 + nc + 16 * j;
+        float* q = (float*)p.out + row * p.ldo + n;
+        if (vec && n + 4 <= N) {
+          *(ft_f4*)q = acc[i][j];
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (n + x < N) q[x] = acc[i][j][x];
+        }
+      }
+    }
+  }
+}
+
+typedef FtShape<256, 256, 2, 4, 2> FtBig;      // 128 KB of LDS, one workgroup a CU
+typedef FtShape<128, 128, 2, 2, 2> FtMid;      // 64 KB, two
+typedef FtShape<32, 64, 2, 2, 4> FtRow;        // 48 KB, three: few rows, the reading of B is what counts (TK x TK alone)
+
+struct FtCost { double step, fixed; int slots; };   // us a k-step with the chip full, us a tile besides, tiles at once
+static const FtCost kCost[3] = {{1.9, 7.0, 256}, {1.1, 5.0, 512}, {0.45, 4.0, 768}};
+static const int kTM[3] = {256, 128, 32}, kTN[3] = {256, 128, 64};
+
+// The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
+// step + time of a tile's start and end), plus the partial sums' way to memory and back.
+FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_rows) {
+  FtPlan best;
+  double least = 1e30;
+  for (int sh = 0; sh < 3; ++sh) {
+    if (sh == 2 && (am != TK || bm != TK || M > 64)) continue;
+    const long tiles = ((M + kTM[sh] - 1) / kTM[sh]) * ((N + kTN[sh] - 1) / kTN[sh]), nk = (K + 63) / 64;
+    for (int want = 1; want <= 64; want = want < 4 ? want + 1 : want + want / 2) {
+      const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want));
+      const long per = (nk + sp - 1) / sp, wg = tiles * sp;
+      const double rounds = wg <= kCost[sh].slots ? 1.0 : (double)wg / kCost[sh].slots + 0.5;
+      double t = rounds * ((double)(per * nprod) * kCost[sh].step * (wg < kCost[sh].slots ? 0.7 : 1.0) + kCost[sh].fixed);
+      if (sp > 1) t += 4.0 + (double)sp * M * N * 8.0 / 4e6;
+      if (t < least) {
+        least = t;
+        best.shape = sh;
+        best.target = sp > 1 ? (int)(tiles * sp) : 0;
+        if (dynamic_rows && best.target < kCost[sh].slots) best.target = kCost[sh].slots;
+      }
+      if (sp < want) break;
+    }
+  }
+  return best;
+}
+static long tiles_of(const FtPlan& pl, long M, long N) { return ((M + kTM[pl.shape] - 1) / kTM[pl.shape]) * ((N + kTN[pl.shape] - 1) / kTN[pl.shape]); }
+// slices x tiles stays under max(target, tiles), and rows x columns under tiles x a tile
+size_t ft_part_floats(long M, long N, const FtPlan& pl) {
+  const long tiles = tiles_of(pl, M, N), wg = tiles > pl.target ? tiles : pl.target;
+  return (size_t)wg * kTM[pl.shape] * kTN[pl.shape];
+}
+
+template <class S, int AM, int BMO, int NPROD>
+static int launch(const FtProduct& p, int target, float* part, bool add, hipStream_t s) {
+  long tiles = (long)((p.M + S::TM - 1) / S::TM) * ((p.N + S::TN - 1) / S::TN);
+  if (part) {     // rows really there may be fewer, and the slices then more: never more workgroups than this
+    if (p.Mdyn) tiles = tiles > target ? tiles : target;
+    else tiles *= ft_slices(tiles, p.Ks ? p.Ks : p.K, target);
+  }
+  FC_REQUIRE(tiles < (1L << 31), "product of %d x %d: too many tiles", p.M, p.N);
+  if (tiles == 0) return 0;
+  const void* k = part ? (const void*)k_ft_product<S, AM, BMO, NPROD, true> : (const void*)k_ft_product<S, AM, BMO, NPROD, false>;
+  FC_TRY(ft_allow_lds(k, S::LDS));
+  if (part) hipLaunchKernelGGL((k_ft_product<S, AM, BMO, NPROD, true>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, p, part, target, add ? 1 : 0);
+  else hipLaunchKernelGGL((k_ft_product<S, AM, BMO, NPROD, false>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, p, part, 0, 0);
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+template <class S, int NPROD> static int by_mode(const FtProduct& p, int target, float* part, bool add, hipStream_t s) {
+  if (p.am == TK && p.bm == TK) return launch<S, TK, TK, NPROD>(p, target, part, add, s);
+  if constexpr (S::TN >= 128) {
+    if (p.am == TK) return launch<S, TK, TR, NPROD>(p, target, part, add, s);
+    if (p.bm == TR) return launch<S, TR, TR, NPROD>(p, target, part, add, s);
+  }
+  fc_set_error("no such product");
+  return -1;
+}
+template <int NPROD> static int by_shape(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s) {
+  if (plan.shape == 0) return by_mode<FtBig, NPROD>(p, plan.target, part, add, s);
+  if (plan.shape == 1) return by_mode<FtMid, NPROD>(p, plan.target, part, add, s);
+  return by_mode<FtRow, NPROD>(p, plan.target, part, add, s);
+}
+int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s) {
+  // 32-bit offsets inside a tile: 256 rows of a TK operand, 64 of a TR one, and a whole row of columns
+  FC_REQUIRE(p.a.ld < (1L << 21) && p.b.ld < (1L << 21), "an operand's rows are too far apart (%ld, %ld elements)", p.a.ld, p.b.ld);
+  return p.nprod == 1 ? by_shape<1>(p, plan, part, add, s) : by_shape<6>(p, plan, part, add, s);
+}
+
+// ---------------------------------------------------------------- sums of the slices
+template <typename T>
+__global__ void __launch_bounds__(256) k_ft_reduce(FtProduct p, const float* part, int target, int TM, int TN, const int* pos, long R) {
+  const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
+  const long ldp = ft_part_ld(N), cw = ldp / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= R * cw) return;
+  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), p.Ks ? p.Ks : K, target);
+  const long m = e / cw;
+  const int n = (int)(e - m * cw) * 8;
+  const long src = pos ? pos[m] : m, row = pos ? m : p.rows.at((int)m);
+  if (row < 0) return;
+  ft_f4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  if (src >= 0 && src < M)
+#pragma unroll 4
+    for (int q = 0; q < splits; ++q) {
+      const ft_f4* a = (const ft_f4*)(part + ((long)q * M + src) * ldp + n);
+      v[0] += a[0];
+      v[1] += a[1];
+    }
+  T* o = (T*)p.out + row * p.ldo + n;
+  if (sizeof(T) == 2 && n + 8 <= N && p.ldo % 8 == 0 && ((size_t)p.out & 15) == 0) {
+    *(uint4*)o = make_uint4(f2bf2(v[0][0], v[0][1]), f2bf2(v[0][2], v[0][3]), f2bf2(v[1][0], v[1][1]), f2bf2(v[1][2], v[1][3]));
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < 8; ++x)
+    if (n + x < N) Io<T>::st(o, x, v[x >> 2][x & 3]);
+}
+int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s) {
+  const long n = R * (ft_part_ld(p.N) / 8);
+  if (n == 0) return 0;
+  const dim3 g((unsigned)((n + 255) / 256));
+  if (p.nprod == 1) hipLaunchKernelGGL(k_ft_reduce<bf16_t>, g, dim3(256), 0, s, p, part, plan.target, kTM[plan.shape], kTN[plan.shape], pos, R);
+  else hipLaunchKernelGGL(k_ft_reduce<float>, g, dim3(256), 0, s, p, part, plan.target, kTM[plan.shape], kTN[plan.shape], pos, R);
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+
+size_t ft_product_part_floats(int am, int bm, int nprod, long M, long N, long K) {
+  const FtPlan p = ft_plan(am, bm, nprod, M, N, K, false);
+  return p.target ? ft_part_floats(M, N, p) : 0;
+}
+int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s) {
+  const FtPlan plan = ft_plan(p.am, p.bm, p.nprod, p.M, p.N, p.K, false);
+  if (!plan.target) return ft_product(p, plan, nullptr, false, s);
+  FC_REQUIRE(part && part_floats >= ft_part_floats(p.M, p.N, plan), "workspace too small for the partial sums");
+  FC_TRY(ft_product(p, plan, part, false, s));
+  return ft_reduce(p, plan, part, nullptr, p.M, s);
+}

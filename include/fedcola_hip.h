@@ -109,6 +109,53 @@ size_t fc_contrastive_scratch_floats(int32_t B);
 /* nn.CrossEntropyLoss() (fedavgclient.py:85,90) */
 int fc_ce_loss_fwd_bwd(const float* logits, const int64_t* y, int32_t B, int32_t C, float* lossbuf, float* dlogits, void* stream);
 
+/* ---- operators of a current transformer block and its loss, beside the ones above (dt: FC_PREC_*; activations and their weights have that type).
+ * All work goes to `stream`; nothing is allocated, copied from the host or synchronised, so every call may be captured into a graph.
+ * A row-major matrix is given by its first element and its row stride in elements (ld*, at least the row's length, below 2^21), any
+ * alignment of the element's own type.  bf16 operands whose base is 16-byte aligned and whose stride and row length are multiples of 8
+ * are read in place; others, and fp32 ones (three bf16 planes, products exact to fp32), are first laid out in the workspace: pass
+ * packed = 1 to the workspace functions for them.  Workspaces and `saved` are aligned to 256 bytes; what they hold before does not matter.
+ * Two calls that may run at once need workspaces of their own.  Results are bitwise reproducible (no atomics). */
+enum { FC_REDUCE_NONE = 0, FC_REDUCE_MEAN = 1, FC_REDUCE_SUM = 2 };
+enum { FC_ACT_SILU = 0, FC_ACT_GELU = 1 };
+enum { FC_NORM_LAYER = 0, FC_NORM_RMS = 1 };
+
+/* softmax cross entropy of logits x w^T, x [T, D], w [V, D], which are never kept: loss (fp32: one value, or T with FC_REDUCE_NONE).  Rows with
+ * y = ignore_index have loss 0, cost nothing, and what they hold reaches no output; MEAN divides by the rows that count (none: NaN).  A target
+ * outside of [0, V) makes its row's loss and the gradients NaN.  `saved` (fc_linear_ce_saved_bytes) is what fc_linear_ce_bwd reads in x's place. */
+size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t D);
+size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward);
+int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
+                     int64_t ignore_index, int32_t reduction, float* loss, void* saved, size_t saved_bytes, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* gloss: device gradient of the loss (one value, or T with FC_REDUCE_NONE); dx [T, D] (0 in ignored rows), dw [V, D]: either may be NULL */
+int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t T, int32_t V, int32_t D, int32_t reduction, const float* gloss,
+                     const void* saved, size_t saved_bytes, void* dx, int64_t lddx, void* dw, int64_t lddw, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* gated feed-forward block: y = (act(x wg^T) * (x wu^T)) w_out^T, w_in [2F, D] = wg over wu, w_out [D, F], x and y [T, D].  The backward forms the
+ * hidden units again from x (nothing is kept); dx, dw_in, dw_out: any may be NULL */
+size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward);
+int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t ldx, const void* w_in, int64_t ld_in, const void* w_out, int64_t ld_out,
+                     int32_t T, int32_t D, int32_t F, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_in, int64_t ld_in,
+                     const void* w_out, int64_t ld_out, int32_t T, int32_t D, int32_t F, void* dx, int64_t lddx, void* dw_in,
+                     int64_t ldd_in, void* dw_out, int64_t ldd_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* between two branches: n = norm(y) post_w + post_b; r = alpha x + row_scale[t / scale_rows] gate[t / gate_rows] n; h = norm(r) pre_w + pre_b, for y the
+ * branch's output and x the residual stream [T, D], D <= 8192; r and h are contiguous.  post_w NULL: n = y; pre_w NULL: no h; gate / row_scale NULL:
+ * 1; gate_rows / scale_rows 0: one vector / value for all rows.  Weights, gate and row_scale are fp32.  A row_scale of 0 drops the branch: its rows
+ * of y are not read and their gradient is 0.  The backward takes dr and / or dh (the other NULL) and reads y and x again; the five weight gradients
+ * (fp32; d_gate one row for each gate vector) are NULL where not wanted. */
+size_t fc_norm_gate_workspace_bytes(int64_t T, int32_t D, int64_t gate_rows);
+int fc_norm_gate_fwd(int32_t dt, int32_t kind, const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t T, int32_t D, const float* post_w,
+                     const float* post_b, const float* gate, int64_t gate_rows, const float* row_scale, int64_t scale_rows, float alpha,
+                     const float* pre_w, const float* pre_b, float eps, void* r, void* h, void* stream);
+int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_t lddr, const void* dh, int64_t lddh, const void* y, int64_t ldy, const void* x,
+                     int64_t ldx, int64_t T, int32_t D, const float* post_w, const float* post_b, const float* gate, int64_t gate_rows,
+                     const float* row_scale, int64_t scale_rows, float alpha, const float* pre_w, float eps, void* dy, void* dx, float* d_post_w,
+                     float* d_post_b, float* d_pre_w, float* d_pre_b, float* d_gate, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- torch.optim.AdamW.step over the trainable ranges of the flat buffers (fedavgclient.py:63,100). step is 1-based. */
 int fc_adamw_step(const fc_model_t* m, float* params, float* grads, float* exp_avg, float* exp_avg_sq, float lr, float beta1,
                   float beta2, float eps, float weight_decay, int32_t step, void* stream);

@@ -1,0 +1,428 @@
+"""The block operators and the vocabulary loss on the GPU against float64, elementwise within the rounding bounds of oracle/blocks_oracle.py."""
+import math
+
+import pytest
+import torch
+
+from oracle import blocks_oracle as O
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+TINY = 1e-30
+
+
+def rnd(gen, *shape, scale=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def within(got, want, bound, what):
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    off = (got.double() - want).abs()
+    bad = ~(off <= bound + TINY)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside; worst {float((off / (bound + TINY)).nan_to_num(1e9).max()):.3g} bounds, off {float(off.nan_to_num(1e9).max()):.3g}"
+
+
+def layout(t, how):
+    """the same values in another memory layout"""
+    if how == "wide":                                     # rows of a wider buffer
+        b = torch.full((t.shape[0], t.shape[1] + 8), 7.0, dtype=t.dtype, device=t.device)
+        b[:, :t.shape[1]] = t
+        return b[:, :t.shape[1]]
+    if how == "odd":                                      # an odd row stride and an odd first element
+        b = torch.full((t.shape[0] * (t.shape[1] + 3) + 1,), 7.0, dtype=t.dtype, device=t.device)
+        v = b[1:].view(t.shape[0], t.shape[1] + 3)[:, :t.shape[1]]
+        v.copy_(t)
+        return v
+    if how == "turned":
+        return t.t().contiguous().t()
+    return t
+
+
+# ------------------------------------------------------------------------------------------------ cross entropy over a vocabulary
+def ce_case(T, V, D, dt, ignored, seed):
+    g = gen(seed)
+    x, w = rnd(g, T, D, dtype=DT[dt]), rnd(g, V, D, scale=2 / math.sqrt(D), dtype=DT[dt])
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    y[torch.rand(T, generator=g, device="cuda") < ignored] = -100
+    return x, w, y
+
+
+CE = [(1, 2, 1, 0.0, "", ""), (1, 1003, 384, 0.0, "", ""), (7, 50, 16, 0.0, "wide", ""), (33, 257, 64, 0.5, "", "odd"), (64, 1000, 100, 0.0, "odd", ""),
+      (65, 513, 7, 0.3, "turned", "turned"), (300, 999, 72, 0.0, "", "wide"), (200, 4100, 136, 0.85, "", ""), (129, 130, 520, 0.0, "", ""), (1030, 6000, 64, 0.2, "", "")]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,V,D,ignored,xl,wl", CE)
+def test_linear_cross_entropy(T, V, D, ignored, xl, wl, dt):
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(T, V, D, dt, ignored, T + V + D)
+    if ignored == 0.0 and T > 3:
+        y[2] = V - 1
+        y[3] = 0
+    for reduction in ("mean", "sum", "none"):
+        g = rnd(gen(5), T) if reduction == "none" else torch.tensor(0.7, device="cuda")
+        want, bound = O.linear_ce(x, w, y, g, -100, reduction, DT[dt])
+        loss, saved = linear_cross_entropy_forward(layout(x, xl), layout(w, wl), y, reduction=reduction)
+        dx, dw = linear_cross_entropy_backward(g, saved, layout(w, wl))
+        assert loss.dtype == torch.float32 and dx.dtype == dw.dtype == DT[dt]
+        if bool((y != -100).any()) or reduction != "mean":
+            within(loss, want["loss"], bound["loss"], f"loss {reduction}")
+        within(dx, want["dx"], bound["dx"], f"dx {reduction}")
+        within(dw, want["dw"], bound["dw"], f"dw {reduction}")
+
+
+@pytest.mark.parametrize("dt,T", [("bf16", 131072), ("fp32", 44000)])
+def test_linear_cross_entropy_in_pieces(dt, T):
+    """so many rows that the backward takes the vocabulary in several pieces (768 and 512 columns), the last one ragged"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(T, 1700, 24, dt, 0.4, 11)
+    g = rnd(gen(6), T)
+    want, bound = O.linear_ce(x, w, y, g, -100, "none", DT[dt])
+    loss, saved = linear_cross_entropy_forward(x, w, y, reduction="none")
+    dx, dw = linear_cross_entropy_backward(g, saved, w)
+    within(loss, want["loss"], bound["loss"], "loss")
+    within(dx, want["dx"], bound["dx"], "dx")
+    within(dw, want["dw"], bound["dw"], "dw")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_linear_cross_entropy_masked_rows_hold_anything(dt):
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(90, 300, 64, dt, 0.4, 3)
+    one = torch.tensor(1.0, device="cuda")
+    clean = torch.where((y == -100)[:, None], 0.0, x)
+    dirty = x.clone()
+    dirty[y == -100] = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(x.dtype).min], device="cuda", dtype=x.dtype).repeat(16)
+    got = []
+    for v in (clean, dirty):
+        loss, saved = linear_cross_entropy_forward(v, w, y)
+        got.append((loss, *linear_cross_entropy_backward(one, saved, w)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert not got[1][1][y == -100].any()
+    # nothing counts: torch's mean, and gradients of zero; no rows at all
+    for rows in (90, 0):
+        none = torch.full((rows,), -100, device="cuda")
+        loss, saved = linear_cross_entropy_forward(dirty[:rows], w, none)
+        dx, dw = linear_cross_entropy_backward(one, saved, w)
+        assert torch.isnan(loss) and dx.shape == (rows, 64) and not dx.any() and not dw.any()
+        loss, saved = linear_cross_entropy_forward(dirty[:rows], w, none, reduction="sum")
+        assert float(loss) == 0.0
+
+
+def test_linear_cross_entropy_extreme_values():
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    w = torch.zeros(300, 64, device="cuda")
+    w[:, 0] = torch.linspace(-1, 1, 300, device="cuda")
+    x = torch.zeros(4, 64, device="cuda")
+    x[0, 0], x[1, 0], x[2, 0], x[3, 0] = 1e4, -1e4, 1e-30, 0.0          # logits of +-1e4: one class alone; all alike
+    y = torch.tensor([299, 0, 5, 299], device="cuda")
+    for dt in (torch.bfloat16, torch.float32):
+        loss, saved = linear_cross_entropy_forward(x.to(dt), w.to(dt), y, reduction="none")
+        want = torch.nn.functional.cross_entropy(x.to(dt).double() @ w.to(dt).double().t(), y, reduction="none")
+        within(loss, want, 1e-5 + 2e-3 * 0 * want, "loss")
+    # a target outside of the vocabulary, and a row of NaN: loud, and in their own rows
+    for bad in (300, -1):
+        y2 = y.clone()
+        y2[1] = bad
+        loss, saved = linear_cross_entropy_forward(x, w, y2, reduction="none")
+        assert torch.isnan(loss).tolist() == [False, True, False, False]
+        dx, dw = linear_cross_entropy_backward(torch.ones(4, device="cuda"), saved, w)
+        assert torch.isnan(dx[1]).any() and not torch.isnan(dx[[0, 2, 3]]).any() and torch.isnan(dw).any()
+    x[2] = math.nan
+    loss, _ = linear_cross_entropy_forward(x, w, y, reduction="none")
+    assert torch.isnan(loss).tolist() == [False, False, True, False]
+
+
+def test_linear_cross_entropy_module():
+    """autograd, leading dimensions, upstream factor, one gradient alone; against differences of the loss in a direction"""
+    from fedcola_amd.criterions import LinearCrossEntropyLoss
+    x, w, y = ce_case(6 * 9, 77, 40, "fp32", 0.2, 21)
+    x = x.view(6, 9, 40).requires_grad_(True)
+    w = w.requires_grad_(True)
+    loss = LinearCrossEntropyLoss()(x, w, y.view(6, 9))
+    (3 * loss).backward()
+    assert x.grad.shape == x.shape
+    d = rnd(gen(1), 6, 9, 40)
+    e = rnd(gen(2), 77, 40)
+    f = lambda t: float(torch.nn.functional.cross_entropy((x.detach().double() + t * d.double()).view(-1, 40) @ (w.detach().double() + t * e.double()).t(), y))  # noqa: E731
+    slope = 3 * (f(1e-4) - f(-1e-4)) / 2e-4
+    got = float((x.grad.double() * d.double()).sum() + (w.grad.double() * e.double()).sum())
+    assert abs(got - slope) <= 1e-5 * max(1.0, abs(slope)), (got, slope)
+    (gx,) = torch.autograd.grad(LinearCrossEntropyLoss()(x, w.detach(), y.view(6, 9)), x)
+    assert torch.equal(gx * 3, x.grad) or (gx * 3 - x.grad).abs().max() <= 1e-6
+    (gw,) = torch.autograd.grad(LinearCrossEntropyLoss(reduction="sum")(x.detach(), w, y.view(6, 9)), w)
+    n = int((y != -100).sum())
+    assert (gw * 3 / n - w.grad).abs().max() <= 1e-5 * gw.abs().max()
+
+
+# ------------------------------------------------------------------------------------------------ gated feed-forward
+MLP = [(1, 16, 8, "", ""), (1, 384, 1024, "", ""), (5, 7, 3, "", ""), (33, 64, 48, "wide", ""), (64, 1, 5, "", ""), (130, 100, 37, "odd", ""), (257, 192, 515, "", ""),
+       (300, 136, 264, "", "turned"), (1000, 64, 24, "turned", "odd"), (700, 320, 640, "", "")]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,D,F,xl,wl", MLP)
+def test_gated_mlp(T, D, F, xl, wl, dt):
+    from fedcola_amd.blocks import gated_mlp_backward, gated_mlp_forward
+    g = gen(T + D + F)
+    x, wi, wo, dy = rnd(g, T, D, dtype=DT[dt]), rnd(g, 2 * F, D, scale=1 / math.sqrt(D), dtype=DT[dt]), rnd(g, D, F, scale=1 / math.sqrt(F), dtype=DT[dt]), rnd(g, T, D, dtype=DT[dt])
+    for act in ("silu", "gelu"):
+        want, bound = O.gated_mlp(x, wi, wo, dy, act, DT[dt])
+        a = layout(x, xl), layout(wi, wl), layout(wo, wl)
+        got = dict(y=gated_mlp_forward(*a, act=act))
+        got["dx"], got["dw_in"], got["dw_out"] = gated_mlp_backward(layout(dy, xl), *a, act=act)
+        for k in want:
+            assert got[k].dtype == DT[dt]
+            within(got[k], want[k], bound[k], f"{act} {k}")
+
+
+def test_gated_mlp_extreme_values():
+    """gates far out: the activation is 0 or the gate itself, its derivative 0 or 1, nothing overflows; no rows; no gradient wanted"""
+    from fedcola_amd.blocks import gated_mlp_backward, gated_mlp_forward
+    for dt in DT.values():
+        x = torch.zeros(3, 8, device="cuda", dtype=dt)
+        x[0, 0], x[1, 0], x[2, 0] = 200.0, -200.0, 0.0
+        wi, wo = torch.zeros(8, 8, device="cuda", dtype=dt), torch.zeros(8, 4, device="cuda", dtype=dt)
+        wi[:4, 0], wi[4:, 0], wo[0] = 1.0, 0.5, 1.0
+        dy = torch.ones(3, 8, device="cuda", dtype=dt)
+        for act in ("silu", "gelu"):
+            y = gated_mlp_forward(x, wi, wo, act=act)
+            assert y[:, 0].tolist() == [float(torch.tensor(4 * 200 * 100.0).to(dt)), 0.0, 0.0] and \
+                 not y[:, 1:].any()
+            dx, dwi, dwo = gated_mlp_backward(dy, x, wi, wo, act=act)
+            assert dx[0, 0] == 4 * (100 + 0.5 * 200) and dx[1, 0] == 0.0 and all(torch.isfinite(t).all() for t in (dx, dwi, dwo))
+        empty = gated_mlp_forward(x[:0], wi, wo)
+        dx, dwi, dwo = gated_mlp_backward(dy[:0], x[:0], wi, wo)
+        assert empty.shape == (0, 8) and dx.shape == (0, 8) and not dwi.any() and not dwo.any()
+        assert gated_mlp_backward(dy, x, wi, wo, need=(False, False, True))[:2] == (None, None)
+
+
+def test_gated_mlp_module():
+    from fedcola_amd.blocks import GatedMlp
+    m = GatedMlp(96, act="gelu", device="cuda")
+    assert m.w_in.shape == (512, 96) and m.w_out.shape == (96, 256)
+    x = rnd(gen(0), 4, 11, 96).requires_grad_(True)
+    y = m(x)
+    dy = rnd(gen(1), 4, 11, 96)
+    y.backward(dy)
+    xr, wi, wo = x.detach().double().requires_grad_(True), m.w_in.detach().double().requires_grad_(True), m.w_out.detach().double().requires_grad_(True)
+    g, u = (xr @ wi.t()).chunk(2, -1)
+    ref = (torch.nn.functional.gelu(g) * u) @ wo.t()
+    ref.backward(dy.double())
+    for a, b in ((y, ref), (x.grad, xr.grad), (m.w_in.grad, wi.grad), (m.w_out.grad, wo.grad)):
+        assert (a.double() - b).norm() <= 2e-6 * b.norm()
+
+
+# ------------------------------------------------------------------------------------------------ norm, gate, residual, norm
+def norm_case(S, N, D, dt, kind, post, pre, gate, scale, seed):
+    g = gen(seed)
+    v = dict(post_weight=1 + 0.2 * rnd(g, D) if post else None, post_bias=0.1 * rnd(g, D) if post and kind == "layer" else None,
+             pre_weight=1 + 0.2 * rnd(g, D) if pre else None, pre_bias=0.1 * rnd(g, D) if pre and kind == "layer" else None,
+             gate={"": None, "all": rnd(g, D), "sample": rnd(g, S, D)}[gate], residual_scale=0.9, norm=kind, eps=1e-5,
+             row_scale=((torch.rand(S, generator=g, device="cuda") < 0.6).float() / 0.6) if scale else None)
+    b, r = rnd(g, S, N, D, scale=0.7, dtype=DT[dt]), rnd(g, S, N, D, scale=1.5, dtype=DT[dt])
+    return b, r, rnd(g, S, N, D, dtype=DT[dt]), rnd(g, S, N, D, dtype=DT[dt]), v
+
+
+NORM = [(1, 1, 384, "layer", 1, 1, "sample", 0), (3, 5, 1, "layer", 1, 1, "all", 1), (3, 5, 1, "rms", 1, 1, "sample", 0), (2, 7, 3, "rms", 1, 1, "", 1),
+        (4, 197, 384, "layer", 1, 1, "sample", 1), (5, 40, 511, "layer", 1, 1, "all", 0), (2, 33, 512, "rms", 0, 1, "sample", 1), (3, 9, 513, "layer", 1, 0, "sample", 1),
+        (2, 50, 1000, "layer", 0, 1, "", 0), (7, 3, 2048, "rms", 1, 1, "all", 1), (2, 6, 2051, "layer", 1, 1, "sample", 0), (1, 300, 4096, "rms", 1, 1, "all", 0),
+        (2, 5, 4100, "layer", 1, 1, "all", 1), (3, 4, 5001, "rms", 1, 1, "sample", 0), (2, 3, 8192, "layer", 1, 1, "sample", 1), (2, 3, 64, "layer", 0, 0, "sample", 1),
+        (1500, 2, 64, "layer", 1, 1, "sample", 1)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("S,N,D,kind,post,pre,gate,scale", NORM)
+def test_norm_gate_residual(S, N, D, kind, post, pre, gate, scale, dt):
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    b, r, dr, dh, v = norm_case(S, N, D, dt, kind, post, pre, gate, scale, S + N + D)
+    for mode in ("both", "r", "h"):
+        a = dict(d_residual=dr if mode != "h" else None, d_normed=dh if mode != "r" and pre else None)
+        if a["d_residual"] is None and a["d_normed"] is None:
+            continue
+        want, bound = O.norm_gate(b, r, DT[dt], **v, **a)
+        gr, gh = norm_gate_residual_forward(b, r, **v)
+        got = norm_gate_residual_backward(a["d_residual"], a["d_normed"], b, r, **v)
+        within(gr, want["r"], bound["r"], "r")
+        if pre:
+            within(gh, want["h"], bound["h"], "h")
+        else:
+            assert gh is None
+        for k, t in got.items():
+            if k.startswith("pre") and a["d_normed"] is None:
+                assert not t.any()
+                continue
+            within(t, want[k], bound[k], f"{mode} {k}")
+
+
+def test_norm_gate_residual_layouts():
+    """rows of wider buffers, odd strides, unaligned vectors: the same bits as contiguous operands where the values a lane holds are the same"""
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    for dt in DT.values():
+        b, r, dr, dh, v = norm_case(2, 30, 96, "bf16" if dt == torch.bfloat16 else "fp32", "layer", 1, 1, "sample", 1, 4)
+        two = lambda t, how: layout(t.reshape(60, 96), how)  # noqa: E731
+        ref = norm_gate_residual_forward(b.view(60, 96), r.view(60, 96), **v), norm_gate_residual_backward(dr.view(60, 96), dh.view(60, 96), b.view(60, 96), r.view(60, 96), **v)
+        for how in ("wide", "odd", "turned"):
+            a = two(b, how), two(r, how)
+            o = norm_gate_residual_forward(*a, **v)
+            g = norm_gate_residual_backward(two(dr, how), two(dh, how), *a, **v)
+            tol = 2 * O.half_step(dt) + 64 * O.F24
+            for x, y in [*zip(o, ref[0]), *((g[k], ref[1][k]) for k in g)]:
+                assert (x.double() - y.double()).abs().max() <= tol * 4 * y.double().abs().max()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_norm_gate_residual_dropped_branch_holds_anything(dt):
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    b, r, dr, dh, v = norm_case(4, 6, 200, dt, "layer", 1, 1, "sample", 1, 8)
+    v["row_scale"] = torch.tensor([1.5, 0.0, 0.0, 1.0], device="cuda")
+    dirty = b.clone()
+    dirty[1], dirty[2] = math.nan, math.inf
+    out = [(*norm_gate_residual_forward(t, r, **v), *norm_gate_residual_backward(dr, dh, t, r, **v).values()) for t in (b, dirty)]
+    for x, y in zip(*out):
+        assert torch.isfinite(y).all() and torch.equal(x, y)
+    g = norm_gate_residual_backward(dr, dh, dirty, r, **v)
+    assert not g["branch"][1:3].any() and g["branch"][0].any() and not g["gate"][1:3].any()
+
+
+def test_norm_gate_residual_module():
+    from fedcola_amd.blocks import NormGateResidual
+    for kind in ("layer", "rms"):
+        m = NormGateResidual(48, norm=kind, gate_init=0.5, residual_scale=0.8, device="cuda")
+        b, r = rnd(gen(0), 3, 7, 48).requires_grad_(True), rnd(gen(1), 3, 7, 48).requires_grad_(True)
+        s = torch.tensor([1.0, 0.0, 2.0], device="cuda")
+        x, h = m(b, r, row_scale=s)
+        dh = rnd(gen(2), 3, 7, 48)
+        h.backward(dh)                                               # r's own gradient absent
+        want, _ = O.norm_gate(b.detach(), r.detach(), torch.float32, post_weight=m.post_weight.detach(), post_bias=None if m.post_bias is None else m.post_bias.detach(),
+                              gate=m.gate.detach(), row_scale=s, residual_scale=0.8, pre_weight=m.pre_weight.detach(),
+                              pre_bias=None if m.pre_bias is None else m.pre_bias.detach(), norm=kind, d_normed=dh)
+        for got, k in ((x, "r"), (h, "h"), (b.grad, "branch"), (r.grad, "residual"), (m.gate.grad, "gate"), (m.post_weight.grad, "post_weight"), (m.pre_weight.grad, "pre_weight")):
+            assert (got.double() - want[k]).norm() <= 2e-6 * want[k].norm(), k
+
+
+# ------------------------------------------------------------------------------------------------ together, as a program uses them
+def tower(x, y, P, act="silu", s=None):
+    """a residual stream through two gated feed-forward branches to the vocabulary loss; returns the loss"""
+    from fedcola_amd.blocks import gated_mlp, norm_gate_residual
+    from fedcola_amd.criterions import LinearCrossEntropyLoss
+    r = x
+    zero = torch.zeros_like(x)
+    r, h = norm_gate_residual(zero, r, pre_weight=P["n0"], norm="rms")
+    for i in range(2):
+        b = gated_mlp(h, P[f"wi{i}"], P[f"wo{i}"], act)
+        r, h = norm_gate_residual(b, r, post_weight=P[f"p{i}"], gate=P[f"g{i}"], row_scale=s, pre_weight=P[f"n{i + 1}"], norm="rms")
+    return LinearCrossEntropyLoss()(h, P["w"], y)
+
+
+def tower64(x, y, P, s):
+    norm = lambda v, w: v / (v.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w  # noqa: E731
+    r, h = x, norm(x, P["n0"])
+    for i in range(2):
+        g, u = (h @ P[f"wi{i}"].t()).chunk(2, -1)
+        b = (torch.nn.functional.silu(g) * u) @ P[f"wo{i}"].t()
+        r = r + s.double()[:, None, None] * norm(b, P[f"p{i}"]) * P[f"g{i}"]
+        h = norm(r, P[f"n{i + 1}"])
+    return torch.nn.functional.cross_entropy((h @ P["w"].t()).flatten(0, 1), y.flatten())
+
+
+def tower_case(dt, B=3, N=41, D=64, F=136, V=500, seed=0):
+    g = gen(seed)
+    P = dict(w=rnd(g, V, D, scale=0.2, dtype=dt))
+    for i in range(2):
+        P.update({f"wi{i}": rnd(g, 2 * F, D, scale=1 / math.sqrt(D), dtype=dt), f"wo{i}": rnd(g, D, F, scale=1 / math.sqrt(F), dtype=dt),
+                  f"p{i}": 1 + 0.1 * rnd(g, D), f"g{i}": 0.5 + 0.1 * rnd(g, D)})
+    P.update({f"n{i}": 1 + 0.1 * rnd(g, D) for i in range(3)})
+    y = torch.randint(0, V, (B, N), generator=g, device="cuda")
+    y[:, -9:] = -100
+    return rnd(g, B, N, D, dtype=dt), y, P, torch.tensor([1.0, 0.0, 2.0], device="cuda")[:B]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_operators_together(dt):
+    x, y, P, s = tower_case(DT[dt])
+    leaves = {"x": x.requires_grad_(True), **{k: v.requires_grad_(True) for k, v in P.items()}}
+    loss = tower(x, y, P, s=s)
+    got = torch.autograd.grad(loss, list(leaves.values()))
+    wide = {k: v.detach().double().requires_grad_(True) for k, v in leaves.items()}
+    ref = tower64(wide["x"], y, wide, s)
+    want = torch.autograd.grad(ref, list(wide.values()))
+    # a gradient passes at most 16 stored roundings of u each, which are independent: their sum in norm stays under 16 u, and in fp32 under that
+    # of 16 sums of about 500 terms
+    tol = 16 * O.half_step(DT[dt]) if dt == "bf16" else 16 * O.acc(500)
+    assert abs(loss.item() - ref.item()) <= tol * abs(ref.item())
+    for k, a, b in zip(leaves, got, want):
+        assert a.dtype == leaves[k].dtype
+        assert (a.double() - b).norm() <= tol * b.norm(), (k, float((a.double() - b).norm() / b.norm()))
+
+
+def test_operators_captured_into_a_graph():
+    """forward and backward of the tower captured once and replayed on new inputs, eager work in between: the eager results, to the bit"""
+    x, y, P, s = tower_case(torch.bfloat16)
+    st = torch.cuda.Stream()
+    names = ["x", *P]
+    sx, sy = x.clone(), y.clone()
+
+    def step(x_, y_):
+        leaves = {"x": x_.detach().requires_grad_(True), **{k: v.detach().requires_grad_(True) for k, v in P.items()}}
+        loss = tower(leaves["x"], y_, leaves, s=s)
+        return [loss.detach(), *torch.autograd.grad(loss, [leaves[k] for k in names])]
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            step(sx, sy)
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(sx, sy)
+    for k in range(4):
+        x2, y2, _, _ = tower_case(torch.bfloat16, seed=20 + k)
+        eager = step(x2, y2)
+        sx.copy_(x2)
+        sy.copy_(y2)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, eager):
+            assert torch.equal(a, b)
+
+
+def test_operators_on_two_streams_at_once_and_twice():
+    """two calls at once on streams of their own, and again: the same bits as one after the other"""
+    cases = [tower_case(torch.bfloat16, N=41 + 7 * i, seed=i) for i in range(2)]
+
+    def step(c):
+        x, y, P, s = c
+        leaves = [t.detach().requires_grad_(True) for t in (x, *P.values())]
+        loss = tower(leaves[0], y, dict(zip(P, leaves[1:])), s=s)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    alone = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        got = []
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(step(c))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_operator_refusals_on_the_device():
+    from fedcola_amd import blocks, criterions
+    x, w, y = ce_case(8, 20, 16, "bf16", 0.0, 0)
+    ce = criterions.linear_cross_entropy_forward
+    for bad in (lambda: ce(x, w.float(), y), lambda: ce(x, w[:, :8], y), lambda: ce(x, w, y.int()), lambda: ce(x, w, y[:4]), lambda: ce(x, w, y, reduction="max"),
+                lambda: ce(x.half(), w.half(), y), lambda: ce(x, w, y.cpu()), lambda: ce(x, w[:0], y), lambda: blocks.gated_mlp_forward(x, w, w),
+                lambda: blocks.gated_mlp_forward(x, w, w[:16, :10].contiguous(), act="relu"), lambda: blocks.norm_gate_residual_forward(x, x[:4]),
+                lambda: blocks.norm_gate_residual_forward(x, x, gate=torch.ones(3, 16, device="cuda")), lambda: blocks.norm_gate_residual_forward(x, x, pre_bias=torch.ones(16, device="cuda")),
+                lambda: blocks.norm_gate_residual_forward(x, x, gate=x[0]), lambda: blocks.norm_gate_residual_forward(x, x, eps=0.0),
+                lambda: blocks.norm_gate_residual_forward(torch.ones(2, 8193, device="cuda"), torch.ones(2, 8193, device="cuda"))):
+        with pytest.raises(ValueError):
+            bad()
