@@ -8,7 +8,9 @@
 // Backward: r and both norms' statistics are formed again from y and x, so nothing is kept and dwn, dwp are those of the unrounded r.
 // Bound: HBM, 4 T D elements forward (y, x in; r, h out), 6 T D backward (y, x, dr, dh in; dy, dx out).
 // A row is held in registers by a wave (D <= 512), 4 waves (<= 2048) or 8 (<= 8192): 8 or 16 values a lane.  A workgroup walks several
-// rows with the weight vectors in registers: read per row they would be 20 bytes an element from L2 beside the 8 from HBM.
+// rows with the weight vectors in registers (forward) or LDS (backward): read per row they would be 20 bytes an element from L2 beside the 8
+// from HBM.  The next row is loaded while this one is summed.  Measured at the rate of a large copy (4.9 TB/s) for 65536 x 4096 bf16: 417 us
+// forward (5.1 TB/s), 667 us backward (4.8 TB/s); 12608 x 384: 13 and 27 us, where filling and draining the chip is most of the time.
 // dwp, dbp, dwn, dbn, dgate: each workgroup's sums over its rows (fp32) are one row of partial sums, added in fp64 in a fixed order by a
 // second launch.  A workgroup's rows share one gate vector.
 #include "../../include/fedcola_hip.h"
@@ -68,13 +70,58 @@ template <typename T, int VEC, int NTH, int E> __device__ __forceinline__ void n
     if constexpr (VEC == 8) ng_st8(p + c, v + k); else Io<T>::st(p, c, v[k]);
   });
 }
+// a row as it lies in memory, so that the next row's loads can be in flight under this row's sums.  Every lane loads, from inside the row;
+// lanes past its end, and rows that are not there, become zeros in get(), whose asm keeps the conversion in front of the next row's loads.
+template <typename T, int VEC, int NTH, int E> struct NgRaw {
+  T v[E] __attribute__((aligned(16)));
+  __device__ __forceinline__ void load(const T* p, int l, int D) {
+    if (VEC == 8) {
+#pragma unroll
+      for (int t = 0; t < E / 8; ++t) {
+        const int c = (l + NTH * t) * 8;
+        const uint4* q = (const uint4*)(p + (c < D ? c : 0));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) *(uint4*)&v[t * 8 + i * 16 / sizeof(T)] = q[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = p[l + NTH * i < D ? l + NTH * i : 0];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[E], int l, int D, bool there) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = VEC == 8 ? (l + NTH * (i / 8)) * 8 : l + NTH * i;
+      const float u = Io<T>::ld(v, i);
+      f[i] = there && c < D ? u : 0.f;
+      asm volatile("" : "+v"(f[i]));
+    }
+  }
+};
+// a wave's sum in every lane, by DPP: pairs, quads, eights, sixteens, then the four rows of sixteen (shuffles through LDS cost six round trips
+// instead; the rows' sums stand in the way of every row's loads)
+__device__ __forceinline__ float ng_wave_sum(float v) {
+#define NG_DPP(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, false))
+  NG_DPP(0xb1);     // quad_perm 1 0 3 2
+  NG_DPP(0x4e);     // quad_perm 2 3 0 1
+  NG_DPP(0x141);    // row_half_mirror
+  NG_DPP(0x140);    // row_mirror
+#undef NG_DPP
+  const int i = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+}
 // sums over a row's lanes.  W waves: through LDS, one barrier, two buffers in turn (a wave is never two sums ahead of another)
 template <int W> struct NgSum {
   float2* red;     // [2][W]
   int turn = 0;
   __device__ __forceinline__ float2 operator()(float a, float b) {
-    a = wave_sum(a);
-    b = wave_sum(b);
+    a = ng_wave_sum(a);
+    b = ng_wave_sum(b);
+    return join(a, b);
+  }
+  __device__ __forceinline__ float operator()(float a) { return join(ng_wave_sum(a), 0.f).x; }
+  __device__ __forceinline__ float2 join(float a, float b) {
     if (W == 1) return make_float2(a, b);
     float2* q = red + turn * W;
     turn ^= 1;
@@ -93,7 +140,7 @@ template <int VEC, int NTH, int E, class SUM> __device__ __forceinline__ float n
   if (!rms) {
 #pragma unroll
     for (int i = 0; i < E; ++i) a += v[i];
-    const float mu = sum(a, 0.f).x * inv;
+    const float mu = sum(a) * inv;
     constexpr int STEP = VEC == 8 ? 8 : 1;
     ng_each<VEC, NTH, E>(l, D, [&](int k, int c) {
 #pragma unroll
@@ -103,32 +150,60 @@ template <int VEC, int NTH, int E, class SUM> __device__ __forceinline__ float n
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) a += v[i] * v[i];
-  const float rs = 1.f / sqrtf(sum(a, 0.f).x * inv + eps);
+  const float rs = 1.f / sqrtf(sum(a) * inv + eps);
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] *= rs;
   return rs;
 }
+
+__device__ __forceinline__ float ng_uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+// the multiplier of a workgroup's rows, which come in order: one division in all
+struct NgSample {
+  long q, rem;
+  __device__ __forceinline__ NgSample(const NgArgs& a, long row) {
+    q = rem = 0;
+    if (a.scale) { q = row / a.scale_rows; rem = row - q * a.scale_rows; }
+  }
+  __device__ __forceinline__ float scale(const NgArgs& a, int step) {     // of the row; then `step` rows on
+    if (!a.scale) return 1.f;
+    const float s = a.scale[q];
+    for (rem += step; rem >= a.scale_rows; rem -= a.scale_rows) ++q;
+    return s;
+  }
+};
 
 template <typename T, int VEC, int W, int E>
 __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
   constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;       // rows at once
   __shared__ float2 red[2 * W];
   NgSum<W> sum{red};
-  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? threadIdx.x >> 6 : 0, D = a.D;
-  const long grp = blockIdx.x / a.blocks, b0 = (blockIdx.x % a.blocks) * a.per;
-  const long first = grp * a.gate_rows + b0, left = a.gate_rows - b0, n = left < a.per ? left : a.per;
+  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D;
+  const unsigned grp = blockIdx.x / (unsigned)a.blocks;
+  const long b0 = (long)(blockIdx.x - grp * (unsigned)a.blocks) * a.per, first = (long)grp * a.gate_rows + b0, left = a.gate_rows - b0;
+  const int n = (int)(left < a.per ? left : a.per);
+  NgSample smp(a, first + sub);
+  NgRaw<T, VEC, NTH, E> ry, rx;
+  float s = 1.f, snext = 1.f;
+  auto fetch = [&](int i) {
+    const long row = first + (i < n ? i : n - 1);
+    snext = i < n ? smp.scale(a, RB) : 0.f;
+    ry.load((const T*)a.y + row * a.ldy, l, D);
+    rx.load((const T*)a.x + row * a.ldx, l, D);
+  };
+  if (sub < n) fetch(sub);
   float wp[E], bp[E], gt[E], wn[E], bn[E];
   ng_load<float, VEC, NTH, E>(a.wp, l, D, wp);
   ng_load<float, VEC, NTH, E>(a.bp, l, D, bp);
   ng_load<float, VEC, NTH, E>(a.gate ? a.gate + grp * D : nullptr, l, D, gt);
   ng_load<float, VEC, NTH, E>(a.wn, l, D, wn);
   ng_load<float, VEC, NTH, E>(a.bn, l, D, bn);
-  for (long i = sub; i < n; i += RB) {
+  for (int i = sub; i < n; i += RB) {
     const long row = first + i;
-    const float s = a.scale ? a.scale[row / a.scale_rows] : 1.f;
     float y[E], x[E];
-    ng_load<T, VEC, NTH, E>(s == 0.f ? nullptr : (const T*)a.y + row * a.ldy, l, D, y);
-    ng_load<T, VEC, NTH, E>((const T*)a.x + row * a.ldx, l, D, x);
+    s = ng_uniform(snext);
+    ry.get(y, l, D, s != 0.f);
+    rx.get(x, l, D, true);
+    fetch(i + RB);
     if (a.post) {
       ng_norm<VEC, NTH, E>(y, l, D, a.rms, a.eps, sum);
 #pragma unroll
@@ -146,47 +221,82 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
   }
 }
 
+// The weight vectors stand in LDS here: with the five running sums and the next row's loads they do not fit the registers.
+enum { NG_WP = 0, NG_BP, NG_GT, NG_WN, NG_VECS };
 template <typename T, int VEC, int W, int E>
-__global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_bwd(NgArgs a) {
+__global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 && VEC == 8 ? 4 : 3) : 2) k_ng_bwd(NgArgs a) {
   constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;
+  extern __shared__ __attribute__((aligned(16))) float vec[];   // [NG_VECS][Dp], then for W = 1 [4][NG_SUMS][Dp] over it
   __shared__ float2 red[2 * W];
-  __shared__ float acc4[W == 1 ? 4 * 512 : 1];
   NgSum<W> sum{red};
-  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? threadIdx.x >> 6 : 0, D = a.D;
+  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D, Dp = (D + 7) & ~7;
   const float inv = 1.f / (float)D;
-  const long grp = blockIdx.x / a.blocks, b0 = (blockIdx.x % a.blocks) * a.per;
-  const long first = grp * a.gate_rows + b0, left = a.gate_rows - b0, n = left < a.per ? left : a.per;
-  float wp[E], bp[E], gt[E], wn[E], sums[NG_SUMS][E];
-  ng_load<float, VEC, NTH, E>(a.wp, l, D, wp);
-  ng_load<float, VEC, NTH, E>(a.bp, l, D, bp);
-  ng_load<float, VEC, NTH, E>(a.gate ? a.gate + grp * D : nullptr, l, D, gt);
-  ng_load<float, VEC, NTH, E>(a.wn, l, D, wn);
+  const unsigned grp = blockIdx.x / (unsigned)a.blocks;
+  const long b0 = (long)(blockIdx.x - grp * (unsigned)a.blocks) * a.per, first = (long)grp * a.gate_rows + b0, left = a.gate_rows - b0;
+  const int n = (int)(left < a.per ? left : a.per);
+  NgSample smp(a, first + sub);
+  NgRaw<T, VEC, NTH, E> ry, rx, rr, rh;
+  float s = 1.f, snext = 1.f;
+  auto fetch = [&](int i) {
+    const long row = first + (i < n ? i : n - 1);
+    snext = i < n ? smp.scale(a, RB) : 0.f;
+    ry.load((const T*)a.y + row * a.ldy, l, D);
+    rx.load((const T*)a.x + row * a.ldx, l, D);
+    rr.load(a.dr ? (const T*)a.dr + row * a.lddr : (const T*)a.x + row * a.ldx, l, D);
+    rh.load(a.dh ? (const T*)a.dh + row * a.lddh : (const T*)a.x + row * a.ldx, l, D);
+  };
+  if (sub < n) fetch(sub);
+  for (int c = threadIdx.x; c < Dp; c += W == 8 ? 512 : 256) {
+    const bool in = c < D;
+    vec[NG_WP * Dp + c] = in && a.wp ? a.wp[c] : 0.f;
+    vec[NG_BP * Dp + c] = in && a.bp ? a.bp[c] : 0.f;
+    vec[NG_GT * Dp + c] = in ? (a.gate ? a.gate[grp * D + c] : 1.f) : 0.f;
+    vec[NG_WN * Dp + c] = in && a.wn ? a.wn[c] : 0.f;
+  }
+  float sums[NG_SUMS][E];
 #pragma unroll
   for (int q = 0; q < NG_SUMS; ++q)
 #pragma unroll
     for (int k = 0; k < E; ++k) sums[q][k] = 0.f;
-  for (long i = sub; i < n; i += RB) {
+  __syncthreads();
+  auto get = [&](int q, float (&w)[E]) {
+    asm volatile("" ::: "memory");                       // read again for every row: hoisted out of the loop they take the registers they are to save
+    ng_load<float, VEC, NTH, E>(vec + q * Dp, l, D, w);
+  };
+  for (int i = sub; i < n; i += RB) {
     const long row = first + i;
-    const float s = a.scale ? a.scale[row / a.scale_rows] : 1.f;
-    float y[E], x[E], d[E], dn[E];
-    ng_load<T, VEC, NTH, E>(s == 0.f ? nullptr : (const T*)a.y + row * a.ldy, l, D, y);
-    ng_load<T, VEC, NTH, E>((const T*)a.x + row * a.ldx, l, D, x);
-    ng_load<T, VEC, NTH, E>(a.dr ? (const T*)a.dr + row * a.lddr : nullptr, l, D, d);
-    ng_load<T, VEC, NTH, E>(a.dh ? (const T*)a.dh + row * a.lddh : nullptr, l, D, dn);
+    float y[E], x[E], d[E], dn[E], w[E], v[E];
+    s = ng_uniform(snext);
+    ry.get(y, l, D, s != 0.f);
+    rx.get(x, l, D, true);
+    rr.get(d, l, D, a.dr != nullptr);
+    rh.get(dn, l, D, a.dh != nullptr);
+    fetch(i + RB);       // here alone: in two branches the loads' registers would be copied, and so waited for, where these meet
     const float rs1 = a.post ? ng_norm<VEC, NTH, E>(y, l, D, a.rms, a.eps, sum) : 1.f;      // y: its normalised row from here on
-    if (a.pre) {
+    auto branch = [&](float (&p)[E]) {                                                      // the branch as the gate sees it
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        const float p = a.post ? y[k] * wp[k] + bp[k] : y[k];
-        x[k] = a.alpha * x[k] + s * (a.gate ? gt[k] * p : p);
-      }
+      for (int k = 0; k < E; ++k) p[k] = y[k];
+      if (!a.post) return;
+      get(NG_WP, w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) p[k] *= w[k];
+      get(NG_BP, w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) p[k] += w[k];
+    };
+    if (a.pre) {
+      branch(v);
+      get(NG_GT, w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + s * (w[k] * v[k]);
       const float rs2 = ng_norm<VEC, NTH, E>(x, l, D, a.rms, a.eps, sum);
+      get(NG_WN, w);
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < E; ++k) {
         sums[NG_DWN][k] += dn[k] * x[k];
         sums[NG_DBN][k] += dn[k];
-        dn[k] *= wn[k];
+        dn[k] *= w[k];
         s1 += dn[k];
         s2 += dn[k] * x[k];
       }
@@ -197,23 +307,27 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_bwd(NgArgs a) {
     }
     // d: the gradient of r
 #pragma unroll
-    for (int k = 0; k < E; ++k) dn[k] = a.alpha * d[k];
-    ng_store<T, VEC, NTH, E>((T*)a.dx + row * D, l, D, dn);
-    float s1 = 0.f, s2 = 0.f;
+    for (int k = 0; k < E; ++k) v[k] = a.alpha * d[k];
+    ng_store<T, VEC, NTH, E>((T*)a.dx + row * D, l, D, v);
+    branch(v);
+    get(NG_GT, w);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      const float p = a.post ? y[k] * wp[k] + bp[k] : y[k], dp = s == 0.f ? 0.f : d[k] * s;
-      sums[NG_DGATE][k] += dp * p;
-      d[k] = a.gate ? dp * gt[k] : dp;
-      if (a.post) {
+      const float dp = s == 0.f ? 0.f : d[k] * s;
+      sums[NG_DGATE][k] += dp * v[k];
+      d[k] = dp * w[k];
+    }
+    if (a.post) {
+      float s1 = 0.f, s2 = 0.f;
+      get(NG_WP, w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
         sums[NG_DWP][k] += d[k] * y[k];
         sums[NG_DBP][k] += d[k];
-        d[k] *= wp[k];
+        d[k] *= w[k];
         s1 += d[k];
         s2 += d[k] * y[k];
       }
-    }
-    if (a.post) {
       const float2 m = sum(s1, s2);
       const float m1 = a.rms ? 0.f : m.x * inv, m2 = m.y * inv;
 #pragma unroll
@@ -223,20 +337,24 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_bwd(NgArgs a) {
   }
   if (!a.part) return;
   float* o = a.part + (long)blockIdx.x * NG_SUMS * D;
+  if (W == 1) {
+    __syncthreads();
 #pragma unroll
-  for (int q = 0; q < NG_SUMS; ++q) {
-    if (W == 1) {
-      __syncthreads();
-      ng_store<float, VEC, NTH, E>(acc4 + sub * 512, l, D, sums[q]);
-      __syncthreads();
-      for (int c = threadIdx.x; c < D; c += 256) o[q * D + c] = (acc4[c] + acc4[512 + c]) + (acc4[1024 + c] + acc4[1536 + c]);
-    } else {
+    for (int q = 0; q < NG_SUMS; ++q) ng_store<float, VEC, NTH, E>(vec + (sub * NG_SUMS + q) * Dp, l, D, sums[q]);
+    __syncthreads();
+    const int st = NG_SUMS * Dp;
+    for (int c = threadIdx.x; c < NG_SUMS * D; c += 256) {
+      const float* f = vec + c / D * Dp + c % D;
+      o[c] = (f[0] + f[st]) + (f[2 * st] + f[3 * st]);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < NG_SUMS; ++q)
       ng_each<VEC, NTH, E>(l, D, [&](int k, int c) {
         constexpr int STEP = VEC == 8 ? 8 : 1;
 #pragma unroll
         for (int i = 0; i < STEP; ++i) o[q * D + c + i] = sums[q][k + i];
       });
-    }
   }
 }
 
@@ -261,13 +379,20 @@ __global__ void __launch_bounds__(1024) k_ng_sum(const float* part, int D, long 
 }
 
 // ---------------------------------------------------------------- host
-// workgroups of a gate vector's rows: about 1024 in all for wide rows (4 a CU; 2048 of the one-wave-a-row form), at least a few rows each
-static void ng_split(long T, long gate_rows, long D, long& per, long& blocks) {
-  const long groups = T / gate_rows, want = D <= 512 ? 1024 : 1024, at_once = D <= 512 ? 4 : 1;
-  long b = (want + groups - 1) / groups;
-  const long most = (gate_rows + 2 * at_once - 1) / (2 * at_once);
-  b = b < most ? b : most;
-  per = (gate_rows + b - 1) / b;
+// waves of a row and values of a lane.  Forward: 8 values, whose vectors fit the registers five waves deep.  Backward: 16 where that leaves two
+// workgroups a CU instead of one of twice the waves (65536 x 4096 bf16: 693 us against 1151; forward the other way, 454 against 408)
+static void ng_form(long D, bool bwd, int& W, int& E) {
+  W = D <= 512 ? 1 : D <= 2048 || (bwd && D <= 4096) ? 4 : 8;
+  E = D <= 2048 || (!bwd && D <= 4096) ? 8 : 16;
+}
+// workgroups of a gate vector's rows: in all as many as the chip holds at once (the registers allow 5 waves a SIMD forward, 4 backward, 2 with 16
+// values a lane), each wave with the same number of rows
+static void ng_split(long T, long gate_rows, long D, bool bwd, long& per, long& blocks) {
+  int W, E;
+  ng_form(D, bwd, W, E);
+  const long groups = T / gate_rows, at_once = W == 1 ? 4 : 1, waves = 4 * 256 * (E == 16 ? 2 : bwd ? 4 : W == 8 ? 4 : 5), want = waves / (W == 1 ? 4 : W);
+  const long b = (want + groups - 1) / groups;
+  per = ft_up((gate_rows + b - 1) / b, at_once);
   blocks = (gate_rows + per - 1) / per;
 }
 static bool ng_aligned(const NgArgs& a, int dt) {
@@ -281,13 +406,20 @@ template <typename T, bool BWD> static int ng_launch(const NgArgs& a, int dt, hi
   const bool v = ng_aligned(a, dt);
 #define NG_RUN(VEC, W, E)                                                                                          \
   do {                                                                                                             \
-    if (BWD) hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                   \
-    else hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                       \
+    if constexpr (BWD) {                                                                                                  \
+      const int lds = (W == 1 ? 4 * NG_SUMS : NG_VECS) * ((a.D + 7) & ~7) * 4;                                     \
+      FC_TRY(ft_allow_lds((const void*)k_ng_bwd<T, VEC, W, E>, (W == 1 ? 4 * NG_SUMS * 512 : NG_VECS * 8192) * 4)); \
+      hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), lds, s, a);                        \
+    }                                                                                                              \
+    if constexpr (!BWD) hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                       \
   } while (0)
 #define NG_PICK(W, E) do { if (v) NG_RUN(8, W, E); else NG_RUN(1, W, E); } while (0)
-  if (a.D <= 512) NG_PICK(1, 8);
-  else if (a.D <= 2048) NG_PICK(4, 8);
-  else if (a.D <= 4096) NG_PICK(8, 8);
+  int W, E;
+  ng_form(a.D, BWD, W, E);
+  if (W == 1) NG_PICK(1, 8);
+  else if (W == 4 && E == 8) NG_PICK(4, 8);
+  else if (W == 4) { if constexpr (BWD) NG_PICK(4, 16); }
+  else if (E == 8) { if constexpr (!BWD) NG_PICK(8, 8); }
   else NG_PICK(8, 16);
 #undef NG_PICK
 #undef NG_RUN
@@ -311,7 +443,7 @@ extern "C" size_t fc_norm_gate_workspace_bytes(int64_t T, int32_t D, int64_t gat
   long per, blocks;
   const long gr = gate_rows ? gate_rows : T;
   if (T % gr) return 256;
-  ng_split(T, gr, D, per, blocks);
+  ng_split(T, gr, D, true, per, blocks);
   return (size_t)(T / gr) * blocks * NG_SUMS * D * sizeof(float) + 256;
 }
 extern "C" int fc_norm_gate_fwd(int32_t dt, int32_t kind, const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t T, int32_t D, const float* post_w,
@@ -326,7 +458,7 @@ extern "C" int fc_norm_gate_fwd(int32_t dt, int32_t kind, const void* y, int64_t
   FC_TRY(ng_check("fc_norm_gate_fwd", dt, kind, a, r));
   FC_REQUIRE(!a.pre || h || T == 0, "fc_norm_gate_fwd: no place for the second norm's output");
   if (T == 0) return 0;
-  ng_split(T, a.gate_rows, D, a.per, a.blocks);
+  ng_split(T, a.gate_rows, D, false, a.per, a.blocks);
   FC_REQUIRE(T / a.gate_rows * a.blocks < (1L << 31), "fc_norm_gate_fwd: too many samples");
   return dt ? ng_launch<bf16_t, false>(a, dt, (hipStream_t)stream) : ng_launch<float, false>(a, dt, (hipStream_t)stream);
 }
@@ -347,7 +479,7 @@ extern "C" int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_
   const bool sums = out.p[0] || out.p[1] || out.p[2] || out.p[3] || out.p[4];
   hipStream_t s = (hipStream_t)stream;
   if (T) {
-    ng_split(T, a.gate_rows, D, a.per, a.blocks);
+    ng_split(T, a.gate_rows, D, true, a.per, a.blocks);
     FC_REQUIRE(groups * a.blocks < (1L << 31) && groups < 65000, "fc_norm_gate_bwd: too many samples");
     if (sums) {
       FC_REQUIRE(workspace && ((size_t)workspace & 255) == 0 && workspace_bytes >= (size_t)groups * a.blocks * NG_SUMS * D * sizeof(float), "fc_norm_gate_bwd: workspace too small or not aligned to 256 bytes");
