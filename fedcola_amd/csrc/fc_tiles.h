@@ -64,8 +64,13 @@ template <int MODE, int W, int NW> struct FtStager {
   static_assert(MODE == TK || W >= 128, "a TR row holds at least the swizzle's eight units");
   const bf16_t* p;
   long ld, plane;
-  int K, kc[MODE == TK ? NP : 1];   // kc: first k of the lane's chunk inside the step
+  int K, kc[2];                     // TK: first k, inside the step, of the lane's chunk in an even and an odd piece
   unsigned voff[NP];
+  // of the step that is being staged: descriptor, k left; and where the next one starts
+  ft_i4 r;
+  int left, left_next;
+  const bf16_t* at;
+  long bytes;
 
   // map(r): row (TK) / column (TR) of the matrix that tile position r takes, < 0 for none.  TR positions come in eights: map(r + i) = map(r) + i.
   // TK: offsets are taken from row `base`, the least row of the tile.
@@ -73,13 +78,14 @@ template <int MODE, int W, int NW> struct FtStager {
     ld = m.ld; plane = m.plane; K = K_;
     p = m.p + (MODE == TK ? base * ld : 0);
 #pragma unroll
+    for (int i = 0; i < 2; ++i) kc[i] = ((lane & 7) ^ (i * 4 + (lane >> 4))) * 8;
+#pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int piece = wave * NP + i;
       if (MODE == TK) {
-        const int r = piece * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-        const long row = map(r);
-        kc[i] = c * 8;
-        voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + c * 8) * 2) : FT_OOB;
+        const int t = piece * 8 + (lane >> 3);
+        const long row = map(t);
+        voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + ((lane & 7) ^ ((t >> 1) & 7)) * 8) * 2) : FT_OOB;
       } else {
         const int k = piece * (512 / W) + lane * 8 / W, pc = lane % (W / 8);
         const int s = (((k >> 3) & 1) << 2) | (k & 3);
@@ -89,14 +95,21 @@ template <int MODE, int W, int NW> struct FtStager {
       }
     }
   }
-  __device__ __forceinline__ void issue(unsigned lds, long k0, int pl, int wave) const {
-    const ft_i4 r = MODE == TK ? ft_rsrc(p + pl * plane + k0, FT_MAX_BYTES) : ft_rsrc(p + pl * plane + k0 * ld, (K - k0) * ld * 2);
-    const int left = K - k0 < 64 ? (int)(K - k0) : 64;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const unsigned vo = MODE == TK ? (kc[i] < left ? voff[i] : FT_OOB) : voff[i];
-      ft_dma16(r, lds + (wave * NP + i) * 1024, vo);
-    }
+  __device__ __forceinline__ void seek(long k0, int pl) {      // the next step is the one at k0, of plane pl
+    at = p + pl * plane + (MODE == TK ? k0 : k0 * ld);
+    left_next = K - k0 < -64 ? -64 : (int)(K - k0);
+    bytes = (K - k0) * ld * 2;
+  }
+  __device__ __forceinline__ void step() {                     // past the end: no k left, no bytes, and so zeros
+    r = MODE == TK ? ft_rsrc(at, FT_MAX_BYTES) : ft_rsrc(at, bytes);
+    left = left_next;
+    left_next -= 64;
+    at += MODE == TK ? 64 : 64 * ld;
+    bytes -= 128 * ld;
+  }
+  __device__ __forceinline__ void piece(int i, unsigned lds, int wave) const {
+    const int k = NP % 2 == 0 ? kc[i & 1] : (wave * NP + i) & 1 ? kc[1] : kc[0];
+    ft_dma16(r, lds + (wave * NP + i) * 1024, MODE == TK ? (k < left ? voff[i] : FT_OOB) : voff[i]);
   }
 };
 
@@ -124,30 +137,109 @@ __device__ __forceinline__ int ft_pa(int c) { return (0x201100 >> (4 * c)) & 3; 
 __device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; }
 
 // acc += the k-steps [kt0, kt1).  On return every wave has left the loop's LDS reads behind and no load into LDS is in flight.
+//
+// Two stages.  A step's two halves of 32 k are held in registers in turn: while the MFMAs of one run, the fragments of the next are read,
+// one read to every few MFMAs, so that neither the LDS nor the matrix pipe waits for the other.  The one barrier stands between the halves:
+// there a wave has the step's second half in registers, so the stage is free for the loads of the step after the next, and the next stage,
+// loaded for a whole step by then, is read from there on.
 template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_loop(const FtStager<AM, S::TM, S::NW>& sa, const FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
-                                        ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
+__device__ __forceinline__ void ft_loop2(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+                                         ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
+  static_assert(S::NS == 2, "two stages");
   constexpr int TNL = NJ * 16 * S::WN;      // columns staged (the shape's TN, or less in a second loop over the same tile)
-  constexpr int PIECES = FtStager<AM, S::TM, S::NW>::NP + FtStager<BMO, TNL, S::NW>::NP;
+  constexpr int PA = FtStager<AM, S::TM, S::NW>::NP, PB = FtStager<BMO, TNL, S::NW>::NP, NF = S::NI + NJ, NM = S::NI * NJ;
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * NPROD;
-  int ic = 0, slot = 0, c = 0;
+  int c = 0;
   long ik = (long)kt0 * 64;
-  auto put = [&](int at) {                  // steps past the end load zeros (k >= K), so every step issues the same number of loads
-    const bool in = ic < steps;
-    const long k0 = in ? ik : (long)sa.K + 64;
-    const long k0b = in ? ik : (long)sb.K + 64;
-    sa.issue(lds0 + at * S::STAGE, k0, NPROD == 1 ? 0 : ft_pa(c), wave);
-    sb.issue(lds0 + at * S::STAGE + S::TM * 128, k0b, NPROD == 1 ? 0 : ft_pb(c), wave);
-    ++ic;
-    if (NPROD == 1) ik += 64;
-    else if (++c == NPROD) { c = 0; ik += 64; }
+  if (NPROD == 1) { sa.seek(ik, 0); sb.seek(ik, 0); }
+  auto next = [&]() {                       // steps past a slice's end, or the matrices', are loaded and not used: every step issues as many loads
+    if (NPROD > 1) {
+      sa.seek(ik, ft_pa(c));
+      sb.seek(ik, ft_pb(c));
+      if (++c == NPROD) { c = 0; ik += 64; }
+    }
+    sa.step();
+    sb.step();
+  };
+  auto piece = [&](int i, int at) {
+    if (i < PA) sa.piece(i, lds0 + at * S::STAGE, wave); else sb.piece(i - PA, lds0 + at * S::STAGE + S::TM * 128, wave);
+  };
+  ft_b8 f[2][NF];                           // [half][B fragments, then A fragments]
+  auto read = [&](int i, int ks, int at) {
+    const char* t = smem + at * S::STAGE;
+    f[ks][i] = i < NJ ? ft_frag<BMO, TNL>(t + S::TM * 128, (wn * NJ + i) * 16, ks, lane) : ft_frag<AM, S::TM>(t, (wm * S::NI + i - NJ) * 16, ks, lane);
+  };
+  auto mfma = [&](int m, int ks) {
+    const int i = m / NJ, j = m % NJ;
+    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[ks][j], f[ks][NJ + i], acc[i][j], 0, 0, 0);
+  };
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    next();
+#pragma unroll
+    for (int i = 0; i < PA + PB; ++i) piece(i, st);
+  }
+  ft_dma_wait<PA + PB>();
+  ft_barrier();
+#pragma unroll
+  for (int i = 0; i < NF; ++i) read(i, 0, 0);
+  // a half: reads spread over the first three quarters of its MFMAs, so that the last ones cover the last read's way
+  constexpr int RM = NM * 3 / 4 / NF > 0 ? NM * 3 / 4 / NF : 1;
+  auto half = [&](int ks, int at, auto before) {
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+      before(g);
+      read(g, ks ^ 1, at);
+#pragma unroll
+      for (int m = g * RM; m < (g + 1 < NF ? (g + 1) * RM : NM); ++m) mfma(m, ks);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  int at = 0;
+  for (int s = 0; s < steps; ++s) {
+    half(0, at, [&](int g) { if (g == 0) next(); });
+    ft_dma_wait<0>();
+    ft_barrier();
+    half(1, at ^ 1, [&](int g) {
+#pragma unroll
+      for (int i = g * (PA + PB) / NF; i < (g + 1) * (PA + PB) / NF; ++i) piece(i, at);
+    });
+    at ^= 1;
+  }
+  ft_dma_wait<0>();
+  ft_barrier();
+}
+
+// the same with NS stages in flight and no halves: few rows, where a step is short and its loads' way from memory is long
+template <class S, int AM, int BMO, int NPROD, int NJ>
+__device__ __forceinline__ void ft_loop_deep(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+                                             ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
+  constexpr int TNL = NJ * 16 * S::WN;
+  constexpr int PA = FtStager<AM, S::TM, S::NW>::NP, PB = FtStager<BMO, TNL, S::NW>::NP;
+  const unsigned lds0 = ft_lds_addr(smem);
+  const int steps = (kt1 - kt0) * NPROD;
+  int slot = 0, c = 0;
+  long ik = (long)kt0 * 64;
+  if (NPROD == 1) { sa.seek(ik, 0); sb.seek(ik, 0); }
+  auto put = [&](int at) {
+    if (NPROD > 1) {
+      sa.seek(ik, ft_pa(c));
+      sb.seek(ik, ft_pb(c));
+      if (++c == NPROD) { c = 0; ik += 64; }
+    }
+    sa.step();
+    sb.step();
+#pragma unroll
+    for (int i = 0; i < PA; ++i) sa.piece(i, lds0 + at * S::STAGE, wave);
+#pragma unroll
+    for (int i = 0; i < PB; ++i) sb.piece(i, lds0 + at * S::STAGE + S::TM * 128, wave);
   };
 #pragma unroll
   for (int s = 0; s < S::NS - 1; ++s) put(s);
   int free_slot = S::NS - 1;
   for (int s = 0; s < steps; ++s) {
-    ft_dma_wait<(S::NS - 2) * PIECES>();
+    ft_dma_wait<(S::NS - 2) * (PA + PB)>();
     ft_barrier();
     put(free_slot);
     const char* ta = smem + slot * S::STAGE;
@@ -169,6 +261,12 @@ __device__ __forceinline__ void ft_loop(const FtStager<AM, S::TM, S::NW>& sa, co
   }
   ft_dma_wait<0>();
   ft_barrier();
+}
+template <class S, int AM, int BMO, int NPROD, int NJ>
+__device__ __forceinline__ void ft_loop(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+                                        ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
+  if constexpr (S::NS == 2) ft_loop2<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  else ft_loop_deep<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
 }
 
 // ---- which tile a workgroup takes.  Consecutive ids share an XCD's L2 (workgroups are dealt to the 8 XCDs in turn), and ids walk the
