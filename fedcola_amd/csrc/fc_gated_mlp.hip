@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_grad(GmArgs 
 typedef FtShape<256, 256, 2, 4, 2> GmBig;
 typedef FtShape<128, 128, 2, 2, 2> GmMid;
 typedef FtShape<32, 64, 2, 2, 4> GmRow;
-typedef FtShape<128, 256, 2, 4, 2> GmGrad;     // 96 KB; 64 + 32 accumulators a lane
+typedef FtShape<128, 256, 2, 4, 3> GmGrad;     // 144 KB; 64 + 32 accumulators a lane
 
 template <class S, int NPROD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));

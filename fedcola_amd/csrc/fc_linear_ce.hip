@@ -28,7 +28,7 @@ struct CeSaved {
 static CeSaved ce_saved(void* base, int dt, long T, long D) {
   CeSaved s;
   char* p = (char*)base;
-  const long ld = ft_up(D, 8), t4 = ft_up(T * 4, 256);
+  const long ld = ft_up(D, 64), t4 = ft_up(T * 4, 256);
   s.n = (int*)p;
   s.pos = (int*)(p + 256);
   s.idx = (int*)(p + 256 + t4);
@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(1024) k_ce_loss(const float* rows, long T, con
   }
 }
 
-// dL of the tile's logits, rounded once to the operands' precision
+// dL of the tile's logits, rounded once to the operands' precision.  A factor that all rows share (g, g / count) is applied to the products'
+// results instead: multiplied in here, it gives the targets' entries, which are all close to -1, all the same rounding error.
 template <class S, int NPROD>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -251,8 +252,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs 
     const bool live = m < M;
     const float lse = live ? a.lse[m] : 0.f;
     const int rel = (live ? a.y[m] : -1) - n0 - 4 * g;
-    float sc = live ? (a.reduction == FC_REDUCE_NONE ? a.g[a.idx[m]] : a.g[0]) : 0.f;
-    if (a.reduction == FC_REDUCE_MEAN) sc /= (float)M;
+    const float sc = live && a.reduction == FC_REDUCE_NONE ? a.g[a.idx[m]] : 1.f;
 #pragma unroll
     for (int j = 0; j < S::NJ; ++j)
 #pragma unroll
@@ -325,7 +325,7 @@ struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx; };
 static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad) {
   CeSizes z = {};
   const int np = dt ? 1 : 6;
-  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 1 : 3) * V * ft_up(D, 8) * 2, 256);
+  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 1 : 3) * V * ft_up(D, 64) * 2, 256);
   if (!grad) {
     const int tn = ce_tn(ce_shape(dt, T, V));
     z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
@@ -358,7 +358,7 @@ static int ce_weight(int dt, const void* w, long ldw, long V, long D, char*& ws,
     return 0;
   }
   FtPack k;
-  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 8); k.Rd = V;
+  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64); k.Rd = V;
   m.p = k.dst; m.ld = k.ldd; m.plane = V * k.ldd;
   ws += (size_t)ft_up((dt ? 1 : 3) * V * k.ldd * 2, 256);
   return ft_pack(k, s);
@@ -391,7 +391,8 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
   a.part = (CePart*)ws;
   a.tlogit = (float*)(ws + z.part);
   float* rows = reduction == FC_REDUCE_NONE ? loss : (float*)(ws + z.part + z.rows / 2);
-  const int R = (int)ft_up(T > 65536 ? (T + 1023) / 1024 : 64, 64), blocks = T ? (T + R - 1) / R : 1;
+  // 16 rows a workgroup, more where its count of the targets before it would cost more than the copy
+  const int R = (int)ft_up(T > 16384 ? (T + 1023) / 1024 : 16, 16), blocks = T ? (T + R - 1) / R : 1;
   if (dt) {
     const bool vec = ft_direct(1, x, ldx, D);
     hipLaunchKernelGGL((k_ce_rows<bf16_t, 1>), dim3(blocks), dim3(256), 0, s, (const bf16_t*)x, (long)ldx, y, (long)T, R, V, ignore_index, D, vec, sv);
@@ -444,6 +445,10 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   pw.am = TR; pw.bm = TR; pw.nprod = np; pw.N = D; pw.K = T; pw.Kdyn = sv.n; pw.ldo = lddw;
   pw.a = px.a;
   pw.b = sv.x;
+  if (reduction != FC_REDUCE_NONE) {
+    px.alpha = pw.alpha = gloss;
+    if (reduction == FC_REDUCE_MEAN) px.alpha_over = pw.alpha_over = sv.n;
+  }
   for (long v0 = 0; v0 < V; v0 += z.piece) {
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < z.piece ? V - v0 : z.piece);

@@ -138,14 +138,13 @@ __device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; 
 
 // acc += the k-steps [kt0, kt1).  On return every wave has left the loop's LDS reads behind and no load into LDS is in flight.
 //
-// Two stages.  A step's two halves of 32 k are held in registers in turn: while the MFMAs of one run, the fragments of the next are read,
-// one read to every few MFMAs, so that neither the LDS nor the matrix pipe waits for the other.  The one barrier stands between the halves:
-// there a wave has the step's second half in registers, so the stage is free for the loads of the step after the next, and the next stage,
-// loaded for a whole step by then, is read from there on.
+// A step's two halves of 32 k are held in registers in turn: while the MFMAs of one run, the fragments of the next are read, one read to every
+// few MFMAs, so that neither the LDS nor the matrix pipe waits for the other.  The one barrier stands between the halves: there a wave has the
+// step's second half in registers, so its stage is free for the loads of the step NS on, and the next stage, loaded for NS - 1 steps by then, is
+// read from there on.
 template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_loop2(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+__device__ __forceinline__ void ft_halves(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
                                          ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  static_assert(S::NS == 2, "two stages");
   constexpr int TNL = NJ * 16 * S::WN;      // columns staged (the shape's TN, or less in a second loop over the same tile)
   constexpr int PA = FtStager<AM, S::TM, S::NW>::NP, PB = FtStager<BMO, TNL, S::NW>::NP, NF = S::NI + NJ, NM = S::NI * NJ;
   const unsigned lds0 = ft_lds_addr(smem);
@@ -175,12 +174,12 @@ __device__ __forceinline__ void ft_loop2(FtStager<AM, S::TM, S::NW>& sa, FtStage
     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[ks][j], f[ks][NJ + i], acc[i][j], 0, 0, 0);
   };
 #pragma unroll
-  for (int st = 0; st < 2; ++st) {
+  for (int st = 0; st < S::NS; ++st) {
     next();
 #pragma unroll
     for (int i = 0; i < PA + PB; ++i) piece(i, st);
   }
-  ft_dma_wait<PA + PB>();
+  ft_dma_wait<(S::NS - 1) * (PA + PB)>();
   ft_barrier();
 #pragma unroll
   for (int i = 0; i < NF; ++i) read(i, 0, 0);
@@ -199,21 +198,22 @@ __device__ __forceinline__ void ft_loop2(FtStager<AM, S::TM, S::NW>& sa, FtStage
   int at = 0;
   for (int s = 0; s < steps; ++s) {
     half(0, at, [&](int g) { if (g == 0) next(); });
-    ft_dma_wait<0>();
+    ft_dma_wait<(S::NS - 2) * (PA + PB)>();
     ft_barrier();
-    half(1, at ^ 1, [&](int g) {
+    const int to = at + 1 == S::NS ? 0 : at + 1;
+    half(1, to, [&](int g) {
 #pragma unroll
       for (int i = g * (PA + PB) / NF; i < (g + 1) * (PA + PB) / NF; ++i) piece(i, at);
     });
-    at ^= 1;
+    at = to;
   }
   ft_dma_wait<0>();
   ft_barrier();
 }
 
-// the same with NS stages in flight and no halves: few rows, where a step is short and its loads' way from memory is long
+// the same without halves, for few rows: a step is short, and its loads' way from memory long
 template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_loop_deep(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+__device__ __forceinline__ void ft_rows(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
                                              ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
   constexpr int TNL = NJ * 16 * S::WN;
   constexpr int PA = FtStager<AM, S::TM, S::NW>::NP, PB = FtStager<BMO, TNL, S::NW>::NP;
@@ -265,8 +265,8 @@ __device__ __forceinline__ void ft_loop_deep(FtStager<AM, S::TM, S::NW>& sa, FtS
 template <class S, int AM, int BMO, int NPROD, int NJ>
 __device__ __forceinline__ void ft_loop(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
                                         ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  if constexpr (S::NS == 2) ft_loop2<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
-  else ft_loop_deep<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  else ft_rows<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
 }
 
 // ---- which tile a workgroup takes.  Consecutive ids share an XCD's L2 (workgroups are dealt to the 8 XCDs in turn), and ids walk the
@@ -341,9 +341,15 @@ struct FtProduct {
   int Ks = 0;                     // > 0: the length that the slices are cut from, >= K (products added onto each other's partial sums)
   const int* Mdyn = nullptr;      // device: the rows (M) / reduction length (K) really there, at most M / K
   const int* Kdyn = nullptr;
+  const float* alpha = nullptr;   // device: factor of the result (null: 1), over *alpha_over where that is given
+  const int* alpha_over = nullptr;
   void* out = nullptr;
   long ldo = 0;
   FtRows rows;
+  __device__ __forceinline__ float factor() const {
+    if (!alpha) return 1.f;
+    return alpha_over ? (*alpha_over > 0 ? *alpha / (float)*alpha_over : 0.f) : *alpha;
+  }
 };
 // shape: index of the tile shape; target: workgroups wanted, by which the reduction is sliced (0: it is not)
 struct FtPlan { int shape = 0, target = 0; };
