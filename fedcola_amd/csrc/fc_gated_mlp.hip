@@ -3,11 +3,13 @@
 // Forward: one product computes both projections -- a tile's columns are gate and up rows of the same hidden units, interleaved by half a
 // wave's columns, so that g and u of a unit are in one lane -- and its epilogue applies the activation and the product; h is all that
 // reaches memory.  A second product gives y.
-// Backward: nothing but the inputs is kept.  One kernel forms g and u again and, on the same tile, dh = dy w_out, and writes
+// Backward: nothing but the inputs is kept.  dh = dy w_out goes to the workspace in 32 bits; the product of the forward is run again, and its
+// epilogue, which has g and u in 32 bits, reads dh and writes
 //   h = act(g) u,   dg = dh u act'(g),   du = dh act(g)
-// each rounded once from 32 bits; then dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h.  That is 16 T D F operations for the
-// 12 of a backward pass that reads g and u back; these would have to be stored in 32 bits (16 bytes a hidden unit to write and read, as
-// much time as the 4 D operations at D of about 1000) or rounded once more than here.
+// each rounded once; then dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h.  That is 16 T D F operations for the 12 of a backward
+// pass that reads g and u back; these would have to be stored in 32 bits too, or rounded once more than here.  (dh on the same tile as g and
+// u, without its 8 bytes a unit through memory, leaves registers for 128 x 256 tiles only: 2300 us for 8192 x 4096 x 11000, TIME_TWO in two
+// kernels.)
 #include <math.h>
 
 #include "../../include/fedcola_hip.h"
@@ -18,7 +20,9 @@ struct GmArgs {
   int T, D, F, act;
   long up;                      // rows between a unit's gate and up row in w_in
   bf16_t *h, *dgu;              // planes of [T][ldh], [T][2 ldh]: h; dg | du
-  long ldh;
+  long ldh;                     // whole 128-byte lines: a row that straddles one more costs every tile load an L2 request more
+  const float* dh;              // [T][ldd]
+  long ldd;
 };
 
 // act(g) and act'(g); FAST: through v_exp_f32 and v_rcp_f32, for bf16 operands
@@ -57,161 +61,140 @@ __device__ __forceinline__ void gm_gate_up(const GmArgs& a, char* smem, ft_f4 (&
   ft_loop<S, TK, TK, NPROD, S::NJ>(sa, sb, smem, 0, (a.D + 63) / 64, acc, wm, wn, wave, lane);
 }
 
-// one plane of v[i][j], the values of S::TM rows and S::TN / 2 units, as an LDS image
-template <class S, int NPROD, int J>
-__device__ __forceinline__ void gm_image(char* img, const ft_f4 (&v)[S::NI][J], int pl, int wm, int wn, int lane) {
-#pragma unroll
-  for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float o[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (NPROD == 1) { o[x] = v[i][j][x]; continue; }
-        float h[3];
-        ft_split(v[i][j][x], h[0], h[1], h[2]);
-        o[x] = h[pl];
-      }
-      ft_img_put<S::TN / 2>(img, (wm * S::NI + i) * 16 + (lane & 15), wn * J * 16 + 16 * j + 4 * (lane >> 4), o[0], o[1], o[2], o[3]);
-    }
-}
-
+// one row block of values, J columns of 16, into the planes' LDS images
 template <class S, int NPROD>
-__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN;
-  const FtTile t = ft_tile((a.T + S::TM - 1) / S::TM, (a.F + S::TN / 2 - 1) / (S::TN / 2), 1);
-  if (!t.any) return;
-  ft_f4 acc[S::NI][S::NJ], h[S::NI][S::NJ / 2];
-  gm_gate_up<S, NPROD>(a, smem, acc, t, wave, lane);
+__device__ __forceinline__ void gm_put(char* img, int i, const ft_f4 (&v)[S::NJ / 2], int wm, int wn, int lane) {
+  constexpr int J = S::NJ / 2, FC = S::TN / 2, IMG = S::TM * FC * 2;
 #pragma unroll
-  for (int i = 0; i < S::NI; ++i)
+  for (int j = 0; j < J; ++j) {
+    const int r = (wm * S::NI + i) * 16 + (lane & 15), c = wn * J * 16 + 16 * j + 4 * (lane >> 4);
+    if (NPROD == 1) {
+      ft_img_put<FC>(img, r, c, v[j][0], v[j][1], v[j][2], v[j][3]);
+    } else {
+      float h[3][4];
 #pragma unroll
-    for (int j = 0; j < S::NJ / 2; ++j)
+      for (int x = 0; x < 4; ++x) ft_split(v[j][x], h[0][x], h[1][x], h[2][x]);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float v, dv;
-        gm_act<NPROD == 1>(a.act, acc[i][j][x], v, dv);
-        h[i][j][x] = v * acc[i][j + S::NJ / 2][x];
-      }
-  const FtRows rows;
-#pragma unroll
-  for (int pl = 0; pl < (NPROD == 1 ? 1 : 3); ++pl) {
-    if (pl) ft_barrier();
-    gm_image<S, NPROD, S::NJ / 2>(smem, h, pl, wm, wn, lane);
-    ft_barrier();
-    ft_img_out<S::TM, S::TN / 2, S::NT>(smem, a.h + pl * a.T * a.ldh, a.ldh, t.m * S::TM, t.n * (S::TN / 2), a.T, (int)a.ldh, rows, true);
+      for (int p = 0; p < 3; ++p) ft_img_put<FC>(img + p * IMG, r, c, h[p][0], h[p][1], h[p][2], h[p][3]);
+    }
   }
 }
+// the planes' images to the columns f0.. of rows of `ld` values
+template <class S, int NPROD> __device__ __forceinline__ void gm_out(const char* img, bf16_t* out, long plane, long ld, const GmArgs& a, int m0, int f0) {
+  constexpr int FC = S::TN / 2, IMG = S::TM * FC * 2;
+  const FtRows rows;
+#pragma unroll
+  for (int p = 0; p < (NPROD == 1 ? 1 : 3); ++p) ft_img_out<S::TM, FC, S::NT>(img + p * IMG, out + p * plane, ld, m0, f0, a.T, (int)a.ldh, rows, true);
+}
 
-template <class S, int NPROD>
-__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_grad(GmArgs a) {
+// GRAD: the backward's pass over the same product
+template <class S, int NPROD, bool GRAD>
+__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int J = S::NJ / 2, FC = S::TN / 2;
+  constexpr int J = S::NJ / 2, FC = S::TN / 2, SET = (NPROD == 1 ? 1 : 3) * S::TM * FC * 2;     // bytes of an output's images
+  constexpr bool TURN = 2 * SET <= S::LDS;                                                      // room for two outputs' in turn
+  static_assert(SET <= S::LDS, "an output's images fit");
   const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN;
   const FtTile t = ft_tile((a.T + S::TM - 1) / S::TM, (a.F + FC - 1) / FC, 1);
   if (!t.any) return;
   const int m0 = t.m * S::TM, f0 = t.n * FC;
-  ft_f4 acc[S::NI][S::NJ], dh[S::NI][J];
+  ft_f4 acc[S::NI][S::NJ];
   gm_gate_up<S, NPROD>(a, smem, acc, t, wave, lane);
-  FtStager<TK, S::TM, S::NW> sa;
-  FtStager<TR, FC, S::NW> sb;
-  sa.init(a.dy, m0, a.D, wave, lane, [&](int r) { return m0 + r < a.T ? (long)m0 + r : -1L; });
-  sb.init(a.w_out, f0, a.D, wave, lane, [&](int r) { return f0 + r < a.F ? (long)f0 + r : -1L; });
 #pragma unroll
-  for (int i = 0; i < S::NI; ++i)
+  for (int i = 0; i < S::NI; ++i) {
+    ft_f4 h[J], d[J];
+    if (GRAD) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) dh[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
-  ft_loop<S, TK, TR, NPROD, J>(sa, sb, smem, 0, (a.D + 63) / 64, dh, wm, wn, wave, lane);
-#pragma unroll
-  for (int i = 0; i < S::NI; ++i)
+      for (int j = 0; j < J; ++j) {
+        const int m = m0 + (wm * S::NI + i) * 16 + (lane & 15), f = f0 + wn * J * 16 + 16 * j + 4 * (lane >> 4);
+        const bool in = m < a.T && f < a.ldd;                   // (ldd is F in whole eights, the columns in between are zeros)
+        const ft_f4 v = *(const ft_f4*)(a.dh + (in ? (long)m * a.ldd + f : 0));
+        d[j] = in ? v : ft_f4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         float v, dv;
-        const float u = acc[i][j + J][x], d = dh[i][j][x];
+        const float u = acc[i][j + J][x];
         gm_act<NPROD == 1>(a.act, acc[i][j][x], v, dv);
-        acc[i][j][x] = d * u * dv;
-        acc[i][j + J][x] = d * v;
-        dh[i][j][x] = v * u;
+        if (GRAD) {
+          acc[i][j][x] = d[j][x] * u * dv;
+          acc[i][j + J][x] = d[j][x] * v;
+        }
+        h[j][x] = v * u;
       }
-  const FtRows rows;
-  ft_f4 dv[S::NI][J];
-#pragma unroll
-  for (int pl = 0; pl < (NPROD == 1 ? 1 : 3); ++pl) {
-    if (pl) ft_barrier();
-    constexpr int IMG = S::TM * FC * 2;
-    static_assert(3 * IMG <= S::LDS, "three images at once");
-    gm_image<S, NPROD, J>(smem, dh, pl, wm, wn, lane);
+    gm_put<S, NPROD>(smem, i, h, wm, wn, lane);
+    if (GRAD && (i & 1)) __builtin_amdgcn_sched_barrier(0);      // two rows' loads at a time: all of them together do not fit the registers
+  }
+  ft_barrier();
+  gm_out<S, NPROD>(smem, a.h, a.T * a.ldh, a.ldh, a, m0, f0);
+  if (GRAD) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
+      char* img = smem + (TURN ? (q ^ 1) * SET : 0);
+      if (!TURN) ft_barrier();
 #pragma unroll
-      for (int i = 0; i < S::NI; ++i)
+      for (int i = 0; i < S::NI; ++i) {
+        ft_f4 v[J];
 #pragma unroll
-        for (int j = 0; j < J; ++j) dv[i][j] = acc[i][j + q * J];
-      gm_image<S, NPROD, J>(smem + (1 + q) * IMG, dv, pl, wm, wn, lane);
+        for (int j = 0; j < J; ++j) v[j] = acc[i][j + q * J];
+        gm_put<S, NPROD>(img, i, v, wm, wn, lane);
+      }
+      ft_barrier();
+      gm_out<S, NPROD>(img, a.dgu + q * a.ldh, a.T * 2 * a.ldh, 2 * a.ldh, a, m0, f0);
     }
-    ft_barrier();
-    ft_img_out<S::TM, FC, S::NT>(smem, a.h + pl * a.T * a.ldh, a.ldh, m0, f0, a.T, (int)a.ldh, rows, true);
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      ft_img_out<S::TM, FC, S::NT>(smem + (1 + q) * IMG, a.dgu + pl * a.T * 2 * a.ldh + q * a.ldh, 2 * a.ldh, m0, f0, a.T, (int)a.ldh, rows, true);
   }
 }
 
 // ---------------------------------------------------------------- host
 typedef FtShape<256, 256, 2, 4, 2> GmBig;
 typedef FtShape<128, 128, 2, 2, 2> GmMid;
-typedef FtShape<32, 64, 2, 2, 4> GmRow;
-typedef FtShape<128, 256, 2, 4, 3> GmGrad;     // 144 KB; 64 + 32 accumulators a lane
+typedef FtShape<32, 64, 2, 2, 6> GmRow;
 
-template <class S, int NPROD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
+template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));
   FC_REQUIRE(tiles < (1L << 31), "gated_mlp: too many tiles");
-  FC_TRY(ft_allow_lds((const void*)k_gm_act<S, NPROD>, S::LDS));
-  hipLaunchKernelGGL((k_gm_act<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
+  FC_TRY(ft_allow_lds((const void*)k_gm_act<S, NPROD, GRAD>, S::LDS));
+  hipLaunchKernelGGL((k_gm_act<S, NPROD, GRAD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
   FC_LAUNCH_CHECK();
   return 0;
 }
-template <int NPROD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
-  if (a.T <= 32) return gm_act_launch<GmRow, NPROD>(a, s);
-  if ((long)((a.T + 255) / 256) * ((a.F + 127) / 128) >= 128) return gm_act_launch<GmBig, NPROD>(a, s);
-  return gm_act_launch<GmMid, NPROD>(a, s);
-}
-template <int NPROD> static int gm_grad_run(const GmArgs& a, hipStream_t s) {
-  typedef GmGrad S;
-  const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));
-  FC_REQUIRE(tiles < (1L << 31), "gated_mlp: too many tiles");
-  FC_TRY(ft_allow_lds((const void*)k_gm_grad<S, NPROD>, S::LDS));
-  hipLaunchKernelGGL((k_gm_grad<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
-  FC_LAUNCH_CHECK();
-  return 0;
+// 256 x 256 tiles once they fill half of the chip, 128 x 128 below, 32 x 64 for a few rows.  Backward: 256 x 256 only where the product is long;
+// the epilogue (8 bytes a unit in, 6 out) stands still while it runs, and two 128 x 128 workgroups a CU cover each other's (12608 x 384 x 1024:
+// 50 us against 70; 8192 x 4096 x 11000 the other way, TIME_MID against 1333)
+template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
+  if (a.T <= 32) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
+  if constexpr (NPROD == 1)       // (an output's three planes do not fit the LDS at 256 x 256)
+    if ((long)((a.T + 255) / 256) * ((a.F + 127) / 128) >= 128 && (!GRAD || a.D >= 1024)) return gm_act_launch<GmBig, NPROD, GRAD>(a, s);
+  return gm_act_launch<GmMid, NPROD, GRAD>(a, s);
 }
 
-struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, part; };
+struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; };
 static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backward) {
   GmSizes z = {};
-  const long D8 = ft_up(D, 8), F8 = ft_up(F, 8), e = dt ? 2 : 6;
+  const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6;
   const int np = dt ? 1 : 6;
   if (packed) {
-    z.x = ft_up(T * D8 * e, 256);
-    z.w_in = ft_up(2 * F8 * D8 * e, 256);
-    z.w_out = ft_up(D * F8 * e, 256);
+    z.x = ft_up(T * Dp * e, 256);
+    z.w_in = ft_up(2 * F * Dp * e, 256);
+    z.w_out = ft_up(D * Fp * e, 256);
     z.dy = backward ? z.x : 0;
   }
-  z.h = ft_up(T * F8 * e, 256);
+  z.h = ft_up(T * Fp * e, 256);
   if (!backward) {
     z.part = ft_product_part_floats(TK, TK, np, T, D, F) * 4;
     return z;
   }
-  z.dgu = ft_up(T * 2 * F8 * e, 256);
-  const size_t a = ft_product_part_floats(TK, TR, np, T, D, 2 * F8), b = ft_product_part_floats(TR, TR, np, 2 * F8, D, T),
+  z.dgu = ft_up(T * 2 * Fp * e, 256);
+  z.dh = ft_up(ft_part_ld(F) * T * 4, 256);
+  const size_t a = ft_product_part_floats(TK, TR, np, T, D, 2 * F), b = ft_product_part_floats(TR, TR, np, 2 * Fp, D, T),
                c = ft_product_part_floats(TR, TR, np, D, F, T);
   z.part = 4 * (a > b ? a > c ? a : c : b > c ? b : c);
   return z;
 }
-static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.part; }
+static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.dh + z.part; }
 
 static int gm_matrix(int dt, const void* p, long ld, long R, long C, bool use_direct, char*& ws, FtMat& m, hipStream_t s) {
   if (use_direct) {
@@ -220,7 +203,7 @@ static int gm_matrix(int dt, const void* p, long ld, long R, long C, bool use_di
     return 0;
   }
   FtPack k;
-  k.src = p; k.lds = ld; k.dt = dt; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 8); k.Rd = R;
+  k.src = p; k.lds = ld; k.dt = dt; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 64);
   m.p = k.dst; m.ld = k.ldd; m.plane = R * k.ldd;
   ws += ft_up((dt ? 1 : 3) * R * k.ldd * 2, 256);
   return ft_pack(k, s);
@@ -234,7 +217,7 @@ static int gm_check(const char* what, const GmCall& c, const void* ws) {
   FC_REQUIRE(c.w_in && c.w_out && ws && (c.x || c.T == 0), "%s: null pointer", what);
   FC_REQUIRE(c.ldx >= c.D && c.ld_in >= c.D && c.ld_out >= c.F && c.ldx < (1L << 21) && c.ld_in < (1L << 21) && c.ld_out < (1L << 21), "%s: row strides %ld, %ld, %ld", what,
              c.ldx, c.ld_in, c.ld_out);
-  FC_REQUIRE((c.F + 512) * (c.ld_in > c.D + 8 ? c.ld_in : c.D + 8) < (1L << 30), "%s: the up rows are past a tile load's reach (%ld x %ld)", what, c.F, c.ld_in);
+  FC_REQUIRE((c.F + 512) * (c.ld_in > c.D + 64 ? c.ld_in : c.D + 64) < (1L << 30), "%s: the up rows are past a tile load's reach (%ld x %ld)", what, c.F, c.ld_in);
   FC_REQUIRE(((size_t)ws & 255) == 0, "%s: the workspace is aligned to 256 bytes", what);
   return ft_check_device(c.w_in, what);
 }
@@ -244,25 +227,11 @@ static bool gm_direct(const GmCall& c) {
 }
 // the operands as the products take them; what of them cannot be taken as it is goes to the workspace
 static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
-  const long F8 = ft_up(c.F, 8);
-  a.T = (int)c.T; a.D = (int)c.D; a.F = (int)c.F; a.act = c.act;
+  a.T = (int)c.T; a.D = (int)c.D; a.F = (int)c.F; a.act = c.act; a.up = c.F; a.ldh = ft_up(c.F, 64);
   FC_TRY(gm_matrix(c.dt, c.x, c.ldx, c.T, c.D, ft_direct(c.dt, c.x, c.ldx, c.D), ws, a.x, s));
   if (c.dy) FC_TRY(gm_matrix(c.dt, c.dy, c.lddy, c.T, c.D, ft_direct(c.dt, c.dy, c.lddy, c.D), ws, a.dy, s));
   FC_TRY(gm_matrix(c.dt, c.w_out, c.ld_out, c.D, c.F, ft_direct(c.dt, c.w_out, c.ld_out, c.F), ws, a.w_out, s));
-  if (ft_direct(c.dt, c.w_in, c.ld_in, c.D) && F8 == c.F) {
-    a.w_in.p = (const bf16_t*)c.w_in;
-    a.w_in.ld = c.ld_in;
-    a.up = c.F;
-  } else {     // halves of F8 rows, so that [dg | du] has 16-byte columns and meets w_in row by row
-    FtPack k;
-    k.src = c.w_in; k.lds = c.ld_in; k.dt = c.dt; k.R = 2 * c.F; k.C = c.D; k.dst = (bf16_t*)ws; k.ldd = ft_up(c.D, 8); k.Rd = 2 * F8; k.half = F8; k.to = c.F;
-    a.w_in.p = k.dst; a.w_in.ld = k.ldd; a.w_in.plane = k.Rd * k.ldd;
-    a.up = F8;
-    ws += ft_up((c.dt ? 1 : 3) * k.Rd * k.ldd * 2, 256);
-    FC_TRY(ft_pack(k, s));
-  }
-  a.ldh = F8;
-  return 0;
+  return gm_matrix(c.dt, c.w_in, c.ld_in, 2 * c.F, c.D, ft_direct(c.dt, c.w_in, c.ld_in, c.D), ws, a.w_in, s);
 }
 
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
@@ -283,7 +252,7 @@ extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t 
   FC_TRY(gm_operands(c, ws, a, s));
   a.h = (bf16_t*)ws;
   ws += z.h;
-  FC_TRY(dt ? gm_act_run<1>(a, s) : gm_act_run<6>(a, s));
+  FC_TRY(dt ? (gm_act_run<1, false>(a, s)) : (gm_act_run<6, false>(a, s)));
   FtProduct p;
   p.nprod = dt ? 1 : 6;
   p.a.p = a.h; p.a.ld = a.ldh; p.a.plane = (long)T * a.ldh;
@@ -308,15 +277,29 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   ws += z.h;
   a.dgu = (bf16_t*)ws;
   ws += z.dgu;
-  if (T) FC_TRY(dt ? gm_grad_run<1>(a, s) : gm_grad_run<6>(a, s));
+  float* part = (float*)(ws + z.dh);
   FtProduct p;
   p.nprod = dt ? 1 : 6;
+  if (T) {
+    p.am = TK; p.bm = TR;
+    p.a = a.dy;
+    p.b = a.w_out;
+    p.M = T; p.N = F; p.K = D;
+    FtPlan plan = ft_plan(TK, TR, p.nprod, T, F, D, false);
+    plan.target = 0;                                           // one slice: its partial sums are dh
+    FC_TRY(ft_product(p, plan, (float*)ws, false, s));
+    a.dh = (const float*)ws;
+    a.ldd = ft_part_ld(F);
+    FC_TRY(dt ? (gm_act_run<1, true>(a, s)) : (gm_act_run<6, true>(a, s)));
+  }
   p.a.p = a.dgu; p.a.ld = 2 * a.ldh; p.a.plane = (long)T * 2 * a.ldh;
   if (dx && T) {
-    p.am = TK; p.bm = TR;
+    p.segs = 2;
+    p.a2 = a.ldh; p.b2 = (long)F * a.w_in.ld;
     p.b = a.w_in;
-    p.M = T; p.N = D; p.K = (int)(2 * a.ldh); p.out = dx; p.ldo = lddx;
-    FC_TRY(ft_product_out(p, (float*)ws, z.part / 4, s));
+    p.M = T; p.N = D; p.K = F; p.out = dx; p.ldo = lddx;
+    FC_TRY(ft_product_out(p, part, z.part / 4, s));
+    p.segs = 1;
   }
   p.am = TR; p.bm = TR;
   p.K = T;
@@ -324,14 +307,14 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
     p.b = a.x;
     p.M = (int)(2 * a.ldh); p.N = D; p.out = dw_in; p.ldo = ldd_in;
     if (a.ldh != F) { p.rows.half = (int)a.ldh; p.rows.to = F; }
-    FC_TRY(ft_product_out(p, (float*)ws, z.part / 4, s));
+    FC_TRY(ft_product_out(p, part, z.part / 4, s));
     p.rows = FtRows();
   }
   if (dw_out) {
     p.a = a.dy;
     p.b.p = a.h; p.b.ld = a.ldh; p.b.plane = (long)T * a.ldh;
     p.M = D; p.N = F; p.out = dw_out; p.ldo = ldd_out;
-    FC_TRY(ft_product_out(p, (float*)ws, z.part / 4, s));
+    FC_TRY(ft_product_out(p, part, z.part / 4, s));
   }
   return 0;
 }

@@ -195,19 +195,26 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_stats(CeArgs
     }
 }
 
-// joins the tiles' partial sums of 16 rows a workgroup, 16 lanes a row
-template <int NPROD>
+// joins the tiles' partial sums: ROWS rows a workgroup, 256 / ROWS lanes a row (16: whole lines of neighbouring rows; 1: a scoring call's few rows)
+template <int NPROD, int ROWS>
 __global__ void __launch_bounds__(256) k_ce_join(const CePart* part, int tiles, const float* tlogit, CeSaved s, float* rows, long T) {
-  __shared__ CePart red[16][16];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const long t = (long)blockIdx.x * 16 + r;
+  constexpr int LANES = 256 / ROWS;
+  __shared__ CePart red[LANES][ROWS];
+  const int r = threadIdx.x % ROWS, q = threadIdx.x / ROWS;
+  const long t = (long)blockIdx.x * ROWS + r;
   const int at = t < T ? s.pos[t] : -1;
   CePart p = {-__builtin_inff(), 0.f};
   if (at >= 0)
 #pragma unroll 4
-    for (int i = q; i < tiles; i += 16) p = ce_join<NPROD>(p, part[(long)i * T + at]);
+    for (int i = q; i < tiles; i += LANES) p = ce_join<NPROD>(p, part[(long)i * T + at]);
   red[q][r] = p;
   __syncthreads();
+  if (q < 16 && LANES > 16) {
+#pragma unroll
+    for (int i = 1; i < LANES / 16; ++i) p = ce_join<NPROD>(p, red[q + 16 * i][r]);
+    red[q][r] = p;
+  }
+  if (LANES > 16) __syncthreads();
   if (q == 0 && t < T) {
 #pragma unroll
     for (int i = 1; i < 16; ++i) p = ce_join<NPROD>(p, red[i][r]);
@@ -288,7 +295,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs 
 // ---------------------------------------------------------------- host
 typedef FtShape<256, 256, 2, 4, 2> CeBig;
 typedef FtShape<128, 128, 2, 2, 2> CeMid;
-typedef FtShape<32, 64, 2, 2, 4> CeRow;
+typedef FtShape<32, 64, 2, 2, 6> CeRow;
 // 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32 (the three planes of dL need registers), 32 x 64 for the few rows
 // of a scoring call
 static int ce_shape(int dt, long T, long V) {
@@ -358,7 +365,7 @@ static int ce_weight(int dt, const void* w, long ldw, long V, long D, char*& ws,
     return 0;
   }
   FtPack k;
-  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64); k.Rd = V;
+  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64);
   m.p = k.dst; m.ld = k.ldd; m.plane = V * k.ldd;
   ws += (size_t)ft_up((dt ? 1 : 3) * V * k.ldd * 2, 256);
   return ft_pack(k, s);
@@ -403,9 +410,11 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
   const int shape = ce_shape(dt, T, V), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
   FC_TRY(ce_run<false>(dt, shape, a, s));
   if (T) {
-    const dim3 gj((unsigned)((T + 15) / 16));
-    if (dt) hipLaunchKernelGGL(k_ce_join<1>, gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
-    else hipLaunchKernelGGL(k_ce_join<6>, gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+    const dim3 gj((unsigned)(T <= 64 ? T : (T + 15) / 16));
+    if (dt && T <= 64) hipLaunchKernelGGL((k_ce_join<1, 1>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+    else if (dt) hipLaunchKernelGGL((k_ce_join<1, 16>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+    else if (T <= 64) hipLaunchKernelGGL((k_ce_join<6, 1>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+    else hipLaunchKernelGGL((k_ce_join<6, 16>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
     FC_LAUNCH_CHECK();
   }
   if (reduction != FC_REDUCE_NONE) {

@@ -341,6 +341,8 @@ struct FtProduct {
   int Ks = 0;                     // > 0: the length that the slices are cut from, >= K (products added onto each other's partial sums)
   const int* Mdyn = nullptr;      // device: the rows (M) / reduction length (K) really there, at most M / K
   const int* Kdyn = nullptr;
+  int segs = 1;                   // 2: the reduction is two pieces of length K, the second a2 / b2 elements on in A / B
+  long a2 = 0, b2 = 0;
   const float* alpha = nullptr;   // device: factor of the result (null: 1), over *alpha_over where that is given
   const int* alpha_over = nullptr;
   void* out = nullptr;
@@ -372,16 +374,14 @@ int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const i
 int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s);
 size_t ft_product_part_floats(int am, int bm, int nprod, long M, long N, long K);
 
-// an operand as the products take it: aligned, and in planes for fp32.  Rows come from `rows` halves (FtRows the other way round) or idx.
+// an operand as the products take it: rows of whole 128-byte lines, and in planes for fp32
 struct FtPack {
   const void* src = nullptr;
   long lds = 0;                   // elements between source rows
   int dt = 1;
-  long R = 0, C = 0;              // rows and columns there
+  long R = 0, C = 0;
   bf16_t* dst = nullptr;
-  long ldd = 0;                   // multiple of 8, >= C: the columns in between are written as zeros
-  long Rd = 0;                    // rows written
-  long half = 0, to = 0;          // half > 0: row i of dst is row (i / half) * to + i % half of src, zeros where i % half >= to
+  long ldd = 0;                   // multiple of 64, >= C: the columns in between are written as zeros
 };
 int ft_pack(const FtPack& p, hipStream_t s);
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }

@@ -34,15 +34,12 @@ int ft_check_device(const void* p, const char* what) {
 template <typename T, int PL>
 __global__ void __launch_bounds__(256) k_ft_pack(FtPack a) {
   const long cw = a.ldd / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
-  if (e >= a.Rd * cw) return;
-  const long i = e / cw;
-  const int c0 = (int)(e - i * cw) * 8;
-  long r = i;
-  if (a.half > 0) { const long h = i / a.half, f = i - h * a.half; r = f < a.to ? h * a.to + f : -1; }
-  if (r >= a.R) r = -1;
+  if (e >= a.R * cw) return;
+  const long r = e / cw;
+  const int c0 = (int)(e - r * cw) * 8;
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = r >= 0 && c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
+  for (int j = 0; j < 8; ++j) v[j] = c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
   float h[3][8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -50,11 +47,11 @@ __global__ void __launch_bounds__(256) k_ft_pack(FtPack a) {
   }
 #pragma unroll
   for (int p = 0; p < PL; ++p)
-    *(uint4*)(a.dst + (size_t)p * a.Rd * a.ldd + i * a.ldd + c0) =
+    *(uint4*)(a.dst + (size_t)p * a.R * a.ldd + r * a.ldd + c0) =
         make_uint4(f2bf2(h[p][0], h[p][1]), f2bf2(h[p][2], h[p][3]), f2bf2(h[p][4], h[p][5]), f2bf2(h[p][6], h[p][7]));
 }
 int ft_pack(const FtPack& p, hipStream_t s) {
-  const long n = p.Rd * (p.ldd / 8);
+  const long n = p.R * (p.ldd / 8);
   if (n == 0) return 0;
   const dim3 g((unsigned)((n + 255) / 256));
   if (p.dt) hipLaunchKernelGGL((k_ft_pack<bf16_t, 1>), g, dim3(256), 0, s, p);
@@ -68,7 +65,7 @@ template <class S, int AM, int BMO, int NPROD, bool PART>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtProduct p, float* part, int target, int add) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
-  const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = p.Ks ? p.Ks : K, splits = ft_slices((long)tm * tn, Ks, target);
+  const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = (p.Ks ? p.Ks : K) * p.segs, splits = ft_slices((long)tm * tn, Ks, target);
   const FtTile t = ft_tile(tm, tn, splits);
   if (!t.any) return;
   const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = t.n * S::TN;
@@ -81,8 +78,14 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtPr
   for (int i = 0; i < S::NI; ++i)
 #pragma unroll
     for (int j = 0; j < S::NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
-  const int nk = (K + 63) / 64, per = ((Ks + 63) / 64 + splits - 1) / splits, kt0 = min(nk, t.split * per);
-  ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0, min(nk, kt0 + per), acc, wm, wn, wave, lane);
+  const int nk = (K + 63) / 64, all = nk * p.segs, per = (p.segs == 1 ? (Ks + 63) / 64 + splits - 1 : all + splits - 1) / splits, kt0 = min(all, t.split * per),
+            kt1 = min(all, kt0 + per);
+  ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0 < nk ? kt0 : nk, kt1 < nk ? kt1 : nk, acc, wm, wn, wave, lane);
+  if (kt1 > nk) {
+    sa.p += p.a2;
+    sb.p += p.b2;
+    ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0 > nk ? kt0 - nk : 0, kt1 - nk, acc, wm, wn, wave, lane);
+  }
   const int mr = wm * S::NI * 16 + (lane & 15), nc = wn * S::NJ * 16 + 4 * (lane >> 4);
   if (PART) {
     const long ldp = ft_part_ld(N);
@@ -139,10 +142,10 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtPr
 
 typedef FtShape<256, 256, 2, 4, 2> FtBig;      // 128 KB of LDS, one workgroup a CU
 typedef FtShape<128, 128, 2, 2, 2> FtMid;      // 64 KB, two
-typedef FtShape<32, 64, 2, 2, 4> FtRow;        // 48 KB, three: few rows, the reading of B is what counts (TK x TK alone)
+typedef FtShape<32, 64, 2, 2, 6> FtRow;        // 72 KB, two: few rows, the reading of B is what counts (TK x TK alone)
 
 struct FtCost { double step, fixed; int slots; };   // us a k-step with the chip full, us a tile besides, tiles at once
-static const FtCost kCost[3] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 768}};
+static const FtCost kCost[3] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}};
 static const int kTM[3] = {256, 128, 32}, kTN[3] = {256, 128, 64};
 
 // The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
@@ -183,7 +186,7 @@ static int launch(const FtProduct& p, int target, float* part, bool add, hipStre
   long tiles = (long)((p.M + S::TM - 1) / S::TM) * ((p.N + S::TN - 1) / S::TN);
   if (part) {     // rows really there may be fewer, and the slices then more: never more workgroups than this
     if (p.Mdyn) tiles = tiles > target ? tiles : target;
-    else tiles *= ft_slices(tiles, p.Ks ? p.Ks : p.K, target);
+    else tiles *= ft_slices(tiles, (p.Ks ? p.Ks : p.K) * p.segs, target);
   }
   FC_REQUIRE(tiles < (1L << 31), "product of %d x %d: too many tiles", p.M, p.N);
   if (tiles == 0) return 0;
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(256) k_ft_reduce(FtProduct p, const float* par
   const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
   const long ldp = ft_part_ld(N), cw = ldp / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
   if (e >= R * cw) return;
-  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), p.Ks ? p.Ks : K, target);
+  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), (p.Ks ? p.Ks : K) * p.segs, target);
   const long m = e / cw;
   const int n = (int)(e - m * cw) * 8;
   const long src = pos ? pos[m] : m, row = pos ? m : p.rows.at((int)m);
@@ -260,7 +263,7 @@ size_t ft_product_part_floats(int am, int bm, int nprod, long M, long N, long K)
   return p.target ? ft_part_floats(M, N, p) : 0;
 }
 int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s) {
-  const FtPlan plan = ft_plan(p.am, p.bm, p.nprod, p.M, p.N, p.K, false);
+  const FtPlan plan = ft_plan(p.am, p.bm, p.nprod, p.M, p.N, (long)p.K * p.segs, false);
   if (!plan.target) return ft_product(p, plan, nullptr, false, s);
   FC_REQUIRE(part && part_floats >= ft_part_floats(p.M, p.N, plan), "workspace too small for the partial sums");
   FC_TRY(ft_product(p, plan, part, false, s));
