@@ -171,57 +171,3 @@ def ptr(t):
 def stream_ptr():
     import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-# ------------------------------------------------------------------ operands of the row-wise operators (criterions.py, blocks.py)
-def operand_type(what, *tensors):
-    """(type code, device) that the tensors share; raises where they do not."""
-    import torch
-    t = tensors[0]
-    for u in tensors:
-        if not torch.is_tensor(u):
-            raise ValueError(f"{what}: a tensor is expected, not {type(u).__name__}")
-        if not u.is_cuda:
-            raise FedcolaHipError(f"{what}: needs its tensors on an MI355X (cuda) device: the operator is HIP-only (no CPU fallback)")
-        if u.dtype != t.dtype or u.device != t.device:
-            raise ValueError(f"{what}: operands of one type on one device are expected: {t.dtype} on {t.device}, {u.dtype} on {u.device}")
-    if t.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{what}: {t.dtype}: bfloat16 or float32")
-    return FC_PREC_BF16 if t.dtype == torch.bfloat16 else FC_PREC_FP32, t.device
-
-
-def as_rows(t):
-    """(2-D view or copy of t with its last dimension contiguous, row stride in elements)"""
-    D = t.shape[-1]
-    if t.dim() != 2:
-        t = t.reshape(-1, D) if t.numel() else t.new_empty(t.shape[:-1].numel(), D)
-    if t.shape[0] <= 1 and (D == 1 or t.stride(1) == 1):
-        return t, D
-    if (D > 1 and t.stride(1) != 1) or not D <= t.stride(0) < 1 << 21:
-        t = t.contiguous()
-    return t, t.stride(0)
-
-
-def in_place(t, ld):
-    """whether the tiled products read a matrix where it is (include/fedcola_hip.h)"""
-    return t.element_size() == 2 and ld % 8 == 0 and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0
-
-
-class on_device:
-    """``with on_device(dev) as stream``: the device current, and its current stream's handle"""
-
-    def __init__(self, dev):
-        self.dev = dev
-
-    def __enter__(self):
-        import torch
-        cur = torch.cuda.current_device()
-        self.back = cur if cur != self.dev.index else None
-        if self.back is not None:
-            torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            import torch
-            torch.cuda.set_device(self.back)

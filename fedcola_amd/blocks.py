@@ -14,7 +14,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import as_rows, check, in_place, on_device, operand_type, ptr
+from ._lib import check
+from .operands import address, as_rows, in_place, on_device, operand_type
 
 _ACTS = {"silu": 0, "gelu": 1}
 _NORMS = {"layer": 0, "rms": 1}
@@ -58,8 +59,8 @@ def gated_mlp_backward(dy, x, w_in, w_out, act="silu", need=(True, True, True)):
     packed = not (in_place(x2, ldx) and in_place(dy2, ldy) and in_place(wi, ldi) and in_place(wo, ldo))
     with on_device(dev) as stream:
         ws = torch.empty(L.fc_gated_mlp_workspace_bytes(code, T, D, F, packed, 1), dtype=torch.uint8, device=dev)
-        check(L.fc_gated_mlp_bwd(code, _ACTS[act], dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wi.data_ptr(), ldi, wo.data_ptr(), ldo, T, D, F, ptr(dx), D,
-                                 ptr(dwi), D, ptr(dwo), F, ws.data_ptr(), ws.numel(), stream))
+        check(L.fc_gated_mlp_bwd(code, _ACTS[act], dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wi.data_ptr(), ldi, wo.data_ptr(), ldo, T, D, F, address(dx), D,
+                                 address(dwi), D, address(dwo), F, ws.data_ptr(), ws.numel(), stream))
     return dx, dwi, dwo
 
 
@@ -104,36 +105,38 @@ class GatedMlp(nn.Module):
 _VECTORS = ("post_weight", "post_bias", "gate", "row_scale", "pre_weight", "pre_bias")
 
 
-def _norm_operands(branch, residual, norm, eps, residual_scale, vectors):
+def _norm_operands(branch, residual, norm, eps, vectors):
+    """type code, device, T, D, rows of a gate vector, rows of a multiplier, and the vectors, contiguous, in _VECTORS' order"""
     if norm not in _NORMS:
         raise ValueError(f"norm_gate_residual: norm {norm!r}: layer or rms")
     code, dev = operand_type("norm_gate_residual", branch, residual)
-    if branch.shape != residual.shape or branch.dim() < 1 or not 1 <= branch.shape[-1] <= 8192:
+    shape = branch.shape
+    if shape != residual.shape or not shape or not 1 <= shape[-1] <= 8192:
         raise ValueError(f"norm_gate_residual: branch {tuple(branch.shape)} and residual {tuple(residual.shape)} of one shape [..., D], D <= 8192, are expected")
     if not eps > 0:
         raise ValueError(f"norm_gate_residual: eps {eps}")
-    D = branch.shape[-1]
-    T = branch.shape[:-1].numel()
-    for name, v in vectors.items():
+    D = shape[-1]
+    T = shape[:-1].numel()
+    pw, pb, gate, scale, nw, nb = vectors
+    gate_rows = scale_rows = 0
+    for i, v in enumerate(vectors):
         if v is None:
             continue
-        if v.dtype != torch.float32 or v.device != dev:
-            raise ValueError(f"norm_gate_residual: {name} is float32 on {dev}, not {v.dtype} on {v.device}")
-        if name == "gate":
-            ok = v.shape == (D,) or (v.dim() == 2 and v.shape[1] == D and v.shape[0] >= 1 and T % v.shape[0] == 0)
-        elif name == "row_scale":
-            ok = v.dim() == 1 and v.shape[0] >= 1 and T % v.shape[0] == 0
-        else:
-            ok = v.shape == (D,)
-        if not ok:
-            raise ValueError(f"norm_gate_residual: {name} {tuple(v.shape)} does not match {T} rows of {D}")
-    for part in ("post", "pre"):
-        if vectors[part + "_bias"] is not None and (vectors[part + "_weight"] is None or norm == "rms"):
-            raise ValueError(f"norm_gate_residual: {part}_bias goes with {part}_weight and norm='layer'")
-    v = {k: None if t is None else t.contiguous() for k, t in vectors.items()}
-    gate_rows = T // v["gate"].shape[0] if v["gate"] is not None and v["gate"].dim() == 2 else 0
-    scale_rows = T // v["row_scale"].shape[0] if v["row_scale"] is not None else 0
-    return code, dev, T, D, v, gate_rows, scale_rows
+        if v.dtype is not torch.float32 or v.device != dev:
+            raise ValueError(f"norm_gate_residual: {_VECTORS[i]} is float32 on {dev}, not {v.dtype} on {v.device}")
+        s = v.shape
+        if i == 3 or (i == 2 and len(s) == 2):       # one for each sample
+            if len(s) != (1 if i == 3 else 2) or s[0] < 1 or T % s[0] or (i == 2 and s[1] != D):
+                raise ValueError(f"norm_gate_residual: {_VECTORS[i]} {tuple(s)} does not match {T} rows of {D}")
+            if i == 3:
+                scale_rows = T // s[0]
+            else:
+                gate_rows = T // s[0]
+        elif len(s) != 1 or s[0] != D:
+            raise ValueError(f"norm_gate_residual: {_VECTORS[i]} {tuple(s)} does not match {T} rows of {D}")
+    if (pb is not None and (pw is None or norm == "rms")) or (nb is not None and (nw is None or norm == "rms")):
+        raise ValueError("norm_gate_residual: a bias goes with its weight and norm='layer'")
+    return code, dev, T, D, gate_rows, scale_rows, [None if v is None else v.contiguous() for v in vectors]
 
 
 def norm_gate_residual_forward(branch, residual, *, post_weight=None, post_bias=None, gate=None, row_scale=None, residual_scale=1.0, pre_weight=None,
@@ -144,16 +147,15 @@ def norm_gate_residual_forward(branch, residual, *, post_weight=None, post_bias=
     norm).  gate [D] for all rows or [S, D], one for each of S samples of equally many consecutive rows.  row_scale [S]: a sample's drop-path
     multiplier; 0 drops the branch, whatever it holds.  pre_weight / pre_bias [D]: the norm in front of the next branch.  norm: "layer" or
     "rms" (which has no bias)."""
-    vectors = dict(post_weight=post_weight, post_bias=post_bias, gate=gate, row_scale=row_scale, pre_weight=pre_weight, pre_bias=pre_bias)
-    code, dev, T, D, v, gate_rows, scale_rows = _norm_operands(branch, residual, norm, eps, residual_scale, vectors)
+    code, dev, T, D, gate_rows, scale_rows, v = _norm_operands(branch, residual, norm, eps, (post_weight, post_bias, gate, row_scale, pre_weight, pre_bias))
     y, ldy = as_rows(branch)
     x, ldx = as_rows(residual)
     r = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
     h = torch.empty(residual.shape, dtype=residual.dtype, device=dev) if pre_weight is not None else None
+    pw, pb, g, s, nw, nb = map(address, v)
     with on_device(dev) as stream:
-        check(_lib.lib().fc_norm_gate_fwd(code, _NORMS[norm], y.data_ptr(), ldy, x.data_ptr(), ldx, T, D, ptr(v["post_weight"]), ptr(v["post_bias"]), ptr(v["gate"]),
-                                          gate_rows, ptr(v["row_scale"]), scale_rows, residual_scale, ptr(v["pre_weight"]), ptr(v["pre_bias"]), eps,
-                                          r.data_ptr(), ptr(h), stream))
+        check(_lib.lib().fc_norm_gate_fwd(code, _NORMS[norm], y.data_ptr(), ldy, x.data_ptr(), ldx, T, D, pw, pb, g, gate_rows, s, scale_rows, residual_scale,
+                                          nw, nb, eps, r.data_ptr(), address(h), stream))
     return r, h
 
 
@@ -161,29 +163,32 @@ def norm_gate_residual_backward(d_residual, d_normed, branch, residual, *, post_
                                 pre_weight=None, pre_bias=None, norm="layer", eps=1e-5, weight_grads=True):
     """Gradients for those of r (d_residual) and h (d_normed), either None: a dict of ``branch``, ``residual`` and, for each vector that was
     given and with weight_grads, ``post_weight``, ``post_bias``, ``gate``, ``pre_weight``, ``pre_bias`` (fp32)."""
-    vectors = dict(post_weight=post_weight, post_bias=post_bias, gate=gate, row_scale=row_scale, pre_weight=pre_weight, pre_bias=pre_bias)
-    code, dev, T, D, v, gate_rows, scale_rows = _norm_operands(branch, residual, norm, eps, residual_scale, vectors)
-    for g in (d_residual, d_normed):
-        if g is not None:
-            operand_type("norm_gate_residual", branch, g)
-            if g.shape != branch.shape:
-                raise ValueError(f"norm_gate_residual: a gradient of shape {tuple(g.shape)} for rows of shape {tuple(branch.shape)}")
+    code, dev, T, D, gate_rows, scale_rows, v = _norm_operands(branch, residual, norm, eps, (post_weight, post_bias, gate, row_scale, pre_weight, pre_bias))
+    for t in (d_residual, d_normed):
+        if t is not None:
+            operand_type("norm_gate_residual", branch, t)
+            if t.shape != branch.shape:
+                raise ValueError(f"norm_gate_residual: a gradient of shape {tuple(t.shape)} for rows of shape {tuple(branch.shape)}")
     if d_normed is not None and pre_weight is None:
         raise ValueError("norm_gate_residual: d_normed without pre_weight")
     y, ldy = as_rows(branch)
     x, ldx = as_rows(residual)
     dr, lddr = as_rows(d_residual) if d_residual is not None else (None, 0)
     dh, lddh = as_rows(d_normed) if d_normed is not None else (None, 0)
-    out = dict(branch=torch.empty(branch.shape, dtype=branch.dtype, device=dev), residual=torch.empty(branch.shape, dtype=branch.dtype, device=dev))
-    grads = {k: torch.empty(t.shape, device=dev) if t is not None and weight_grads and k != "row_scale" else None for k, t in v.items()}
-    L = _lib.lib()
+    dy = torch.empty(branch.shape, dtype=branch.dtype, device=dev)
+    dx = torch.empty(branch.shape, dtype=branch.dtype, device=dev)
+    grads = [torch.empty(t.shape, device=dev) if t is not None and weight_grads and i != 3 else None for i, t in enumerate(v)]
+    pw, pb, g, s, nw, _ = map(address, v)
+    gpw, gpb, gg, _, gnw, gnb = map(address, grads)
+    L, ws, n = _lib.lib(), None, 0
     with on_device(dev) as stream:
-        ws = torch.empty(L.fc_norm_gate_workspace_bytes(T, D, gate_rows), dtype=torch.uint8, device=dev) if any(t is not None for t in grads.values()) else None
-        check(L.fc_norm_gate_bwd(code, _NORMS[norm], ptr(dr), lddr, ptr(dh), lddh, y.data_ptr(), ldy, x.data_ptr(), ldx, T, D, ptr(v["post_weight"]),
-                                 ptr(v["post_bias"]), ptr(v["gate"]), gate_rows, ptr(v["row_scale"]), scale_rows, residual_scale, ptr(v["pre_weight"]),
-                                 eps, out["branch"].data_ptr(), out["residual"].data_ptr(), ptr(grads["post_weight"]), ptr(grads["post_bias"]),
-                                 ptr(grads["pre_weight"]), ptr(grads["pre_bias"]), ptr(grads["gate"]), ptr(ws), ws.numel() if ws is not None else 0, stream))
-    out.update((k, g) for k, g in grads.items() if g is not None)
+        if weight_grads:
+            n = L.fc_norm_gate_workspace_bytes(T, D, gate_rows)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        check(L.fc_norm_gate_bwd(code, _NORMS[norm], address(dr), lddr, address(dh), lddh, y.data_ptr(), ldy, x.data_ptr(), ldx, T, D, pw, pb, g, gate_rows, s,
+                                 scale_rows, residual_scale, nw, eps, dy.data_ptr(), dx.data_ptr(), gpw, gpb, gnw, gnb, gg, address(ws), n, stream))
+    out = dict(branch=dy, residual=dx)
+    out.update((k, t) for k, t in zip(_VECTORS, grads) if t is not None)
     return out
 
 

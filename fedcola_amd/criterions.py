@@ -13,7 +13,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import as_rows, check, in_place, on_device, operand_type, ptr
+from ._lib import check, ptr
+from .operands import address, as_rows, in_place, on_device, operand_type
 
 
 def contrastive_tau() -> float:
@@ -115,7 +116,7 @@ def linear_cross_entropy_backward(gloss, saved, weight, need_hidden=True, need_w
     dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if need_weight else None
     with on_device(dev) as stream:
         ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw), 1), dtype=torch.uint8, device=dev)
-        check(L.fc_linear_ce_bwd(code, w.data_ptr(), ldw, T, V, D, red, g.data_ptr(), saved.data_ptr(), saved.numel(), ptr(dx), D, ptr(dw), D,
+        check(L.fc_linear_ce_bwd(code, w.data_ptr(), ldw, T, V, D, red, g.data_ptr(), saved.data_ptr(), saved.numel(), address(dx), D, address(dw), D,
                                  ws.data_ptr(), ws.numel(), stream))
     return dx, dw
 

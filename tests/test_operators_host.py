@@ -70,7 +70,7 @@ def test_python_refuses_host_tensors_and_bad_choices():
 
 
 def test_rows_of_a_tensor():
-    from fedcola_amd._lib import as_rows
+    from fedcola_amd.operands import as_rows
     base = torch.arange(240.0).view(10, 24)
     for t, copied in ((base, False), (base[:, :7], False), (base.view(2, 5, 24), False), (base[::2, :5], False), (base.t(), True), (base[:1].expand(6, 24), True),
                       (base[:, ::2], True), (base[3:4, :9], False), (torch.zeros(0, 5), False), (torch.zeros(3, 0, 5), False), (base[0], False)):
