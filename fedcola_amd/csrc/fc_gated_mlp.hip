@@ -47,8 +47,8 @@ template <class S, int NPROD>
 __device__ __forceinline__ void gm_gate_up(const GmArgs& a, char* smem, ft_f4 (&acc)[S::NI][S::NJ], const FtTile& t, int wave, int lane) {
   constexpr int WC = S::NJ * 16, HC = WC / 2;            // columns of a wave: HC gate rows and the HC up rows of the same units
   const int wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, f0 = t.n * (S::TN / 2);
-  FtStager<TK, S::TM, S::NW> sa;
-  FtStager<TK, S::TN, S::NW> sb;
+  FtStageA<S, TK> sa;
+  FtStageB<S, TK> sb;
   sa.init(a.x, m0, a.D, wave, lane, [&](int r) { return m0 + r < a.T ? (long)m0 + r : -1L; });
   sb.init(a.w_in, f0, a.D, wave, lane, [&](int r) {
     const int in = r % WC, f = f0 + (r / WC) * HC + in % HC;
@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a
 typedef FtShape<256, 256, 2, 4, 2> GmBig;
 typedef FtShape<128, 128, 2, 2, 2> GmMid;
 typedef FtShape<32, 64, 2, 2, 6> GmRow;
+typedef FtShape<128, 128, 2, 4, 3, 32, 3> GmPlanes;
 
 template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));
@@ -166,9 +167,12 @@ template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& 
 // 50 us against 70; 8192 x 4096 x 11000 the other way, TIME_MID against 1333)
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
   if (a.T <= 32) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
-  if constexpr (NPROD == 1)       // (an output's three planes do not fit the LDS at 256 x 256)
+  if constexpr (NPROD == 6) {
+    return gm_act_launch<GmPlanes, NPROD, GRAD>(a, s);
+  } else {
     if ((long)((a.T + 255) / 256) * ((a.F + 127) / 128) >= 128 && (!GRAD || a.D >= 1024)) return gm_act_launch<GmBig, NPROD, GRAD>(a, s);
-  return gm_act_launch<GmMid, NPROD, GRAD>(a, s);
+    return gm_act_launch<GmMid, NPROD, GRAD>(a, s);
+  }
 }
 
 struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; };

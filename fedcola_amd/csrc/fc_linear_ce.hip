@@ -125,8 +125,8 @@ __device__ __forceinline__ bool ce_product(const CeArgs& a, char* smem, ft_f4 (&
   t = ft_tile((M + S::TM - 1) / S::TM, (a.nv + S::TN - 1) / S::TN, 1);
   if (!t.any) return false;
   const int wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = a.v0 + t.n * S::TN;
-  FtStager<TK, S::TM, S::NW> sa;
-  FtStager<TK, S::TN, S::NW> sb;
+  FtStageA<S, TK> sa;
+  FtStageB<S, TK> sb;
   sa.init(a.x, m0, a.D, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
   sb.init(a.w, n0, a.D, wave, lane, [&](int r) { return n0 + r < a.V ? (long)n0 + r : -1L; });
 #pragma unroll
@@ -296,8 +296,8 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs 
 typedef FtShape<256, 256, 2, 4, 2> CeBig;
 typedef FtShape<128, 128, 2, 2, 2> CeMid;
 typedef FtShape<32, 64, 2, 2, 6> CeRow;
-// 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32 (the three planes of dL need registers), 32 x 64 for the few rows
-// of a scoring call
+typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
+// 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32, 32 x 64 for the few rows of a scoring call
 static int ce_shape(int dt, long T, long V) {
   if (T <= 32) return 2;
   return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
@@ -320,7 +320,7 @@ template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, h
 template <bool GRAD> static int ce_run(int dt, int shape, const CeArgs& a, hipStream_t s) {
   if (a.T == 0 || a.nv == 0) return 0;
   if (dt) return shape == 0 ? ce_launch<CeBig, 1, GRAD>(a, s) : shape == 1 ? ce_launch<CeMid, 1, GRAD>(a, s) : ce_launch<CeRow, 1, GRAD>(a, s);
-  return shape == 1 ? ce_launch<CeMid, 6, GRAD>(a, s) : ce_launch<CeRow, 6, GRAD>(a, s);
+  return shape == 1 ? ce_launch<CePlanes, 6, GRAD>(a, s) : ce_launch<CeRow, 6, GRAD>(a, s);
 }
 
 // columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles

@@ -57,20 +57,23 @@ __device__ __forceinline__ ft_i4 ft_rsrc(const void* p, long bytes) {
   return r;
 }
 
-// Stages one operand's tile of W rows (TK) or columns (TR) by NW waves, W / 8 pieces of 1 KB.
-template <int MODE, int W, int NW> struct FtStager {
-  static constexpr int NP = W / 8 / NW;
-  static_assert(NP >= 1 && NP * NW * 8 == W, "a wave moves whole pieces");
+// the XOR of a TK row's 16-B chunks: rows that would meet in a bank differ in it
+template <int KS> __device__ __forceinline__ int ft_tk_swz(int row) { return KS == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
+
+// Stages one operand's tile of W rows (TK) or columns (TR), KS k deep, by NW waves, in pieces of 1 KB.
+template <int MODE, int W, int KS, int NW> struct FtStager {
+  static constexpr int NP = W * KS / 512 / NW, RP = 512 / KS, CR = KS / 8;      // pieces of a wave; TK: rows of a piece, chunks of a row
+  static_assert(NP >= 1 && NP * NW * 512 == W * KS, "a wave moves whole pieces");
   static_assert(MODE == TK || W >= 128, "a TR row holds at least the swizzle's eight units");
   const bf16_t* p;
   long ld, plane;
-  int K, kc[2];                     // TK: first k, inside the step, of the lane's chunk in an even and an odd piece
+  int K, kc[2];                     // TK: first k, inside the stage, of the lane's chunk in an even and an odd piece
   unsigned voff[NP];
-  // of the step that is being staged: descriptor, k left; and where the next one starts
+  // of the stage that is being loaded: descriptor, start, bytes and k left; and where the next one starts
   ft_i4 r;
+  const bf16_t *cur, *at;
+  long cur_bytes, bytes;
   int left, left_next;
-  const bf16_t* at;
-  long bytes;
 
   // map(r): row (TK) / column (TR) of the matrix that tile position r takes, < 0 for none.  TR positions come in eights: map(r + i) = map(r) + i.
   // TK: offsets are taken from row `base`, the least row of the tile.
@@ -78,14 +81,14 @@ template <int MODE, int W, int NW> struct FtStager {
     ld = m.ld; plane = m.plane; K = K_;
     p = m.p + (MODE == TK ? base * ld : 0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) kc[i] = ((lane & 7) ^ (i * 4 + (lane >> 4))) * 8;
+    for (int i = 0; i < 2; ++i) kc[i] = (lane % CR ^ ft_tk_swz<KS>(i * RP + lane / CR)) * 8;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int piece = wave * NP + i;
       if (MODE == TK) {
-        const int t = piece * 8 + (lane >> 3);
+        const int t = piece * RP + lane / CR;
         const long row = map(t);
-        voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + ((lane & 7) ^ ((t >> 1) & 7)) * 8) * 2) : FT_OOB;
+        voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + (lane % CR ^ ft_tk_swz<KS>(t)) * 8) * 2) : FT_OOB;
       } else {
         const int k = piece * (512 / W) + lane * 8 / W, pc = lane % (W / 8);
         const int s = (((k >> 3) & 1) << 2) | (k & 3);
@@ -95,30 +98,36 @@ template <int MODE, int W, int NW> struct FtStager {
       }
     }
   }
-  __device__ __forceinline__ void seek(long k0, int pl) {      // the next step is the one at k0, of plane pl
+  __device__ __forceinline__ void seek(long k0, int pl) {      // the next stage is the one at k0, of plane pl
     at = p + pl * plane + (MODE == TK ? k0 : k0 * ld);
-    left_next = K - k0 < -64 ? -64 : (int)(K - k0);
+    left_next = K - k0 < -KS ? -KS : (int)(K - k0);
     bytes = (K - k0) * ld * 2;
   }
   __device__ __forceinline__ void step() {                     // past the end: no k left, no bytes, and so zeros
-    r = MODE == TK ? ft_rsrc(at, FT_MAX_BYTES) : ft_rsrc(at, bytes);
+    cur = at;
+    cur_bytes = bytes;
+    r = ft_rsrc(cur, MODE == TK ? FT_MAX_BYTES : cur_bytes);
     left = left_next;
-    left_next -= 64;
-    at += MODE == TK ? 64 : 64 * ld;
-    bytes -= 128 * ld;
+    left_next -= KS;
+    at += MODE == TK ? KS : KS * ld;
+    bytes -= 2 * KS * ld;
   }
-  __device__ __forceinline__ void piece(int i, unsigned lds, int wave) const {
+  __device__ __forceinline__ unsigned offset(int i, int wave) const {
     const int k = NP % 2 == 0 ? kc[i & 1] : (wave * NP + i) & 1 ? kc[1] : kc[0];
-    ft_dma16(r, lds + (wave * NP + i) * 1024, MODE == TK ? (k < left ? voff[i] : FT_OOB) : voff[i]);
+    return MODE == TK ? (k < left ? voff[i] : FT_OOB) : voff[i];
+  }
+  __device__ __forceinline__ void piece(int i, unsigned lds, int wave) const { ft_dma16(r, lds + (wave * NP + i) * 1024, offset(i, wave)); }
+  __device__ __forceinline__ void piece_of(int pl, int i, unsigned lds, int wave) const {      // the same k of plane pl, sought at plane 0
+    ft_dma16(ft_rsrc(cur + pl * plane, MODE == TK ? FT_MAX_BYTES : cur_bytes), lds + (wave * NP + i) * 1024, offset(i, wave));
   }
 };
 
-// one wave's fragment of 16 rows / columns starting at rb (a multiple of 16) for the 32-deep half ks of a step
-template <int MODE, int W> __device__ __forceinline__ ft_b8 ft_frag(const char* tile, int rb, int ks, int lane) {
+// one wave's fragment of 16 rows / columns starting at rb (a multiple of 16) for 32 k, the ks-th of a stage
+template <int MODE, int W, int KS> __device__ __forceinline__ ft_b8 ft_frag(const char* tile, int rb, int ks, int lane) {
   const int g = lane >> 4;
   if (MODE == TK) {
-    const int c = (ks * 4 + g) ^ ((lane >> 1) & 7);
-    return *(const ft_b8*)(tile + (rb + (lane & 15)) * 128 + (c << 4));
+    const int c = (ks * 4 + g) ^ ft_tk_swz<KS>(lane & 15);
+    return *(const ft_b8*)(tile + (rb + (lane & 15)) * (KS * 2) + (c << 4));
   }
   const int q = (lane >> 2) & 3, s = ((g & 1) << 2) | q;
   const char* a = tile + (ks * 32 + 8 * g + q) * (W * 2) + ((((rb >> 4) ^ s)) << 5) + (lane & 3) * 8;
@@ -127,11 +136,13 @@ template <int MODE, int W> __device__ __forceinline__ ft_b8 ft_frag(const char* 
   return ft_b8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// tile shape: TM x TN by WM x WN waves, NS LDS stages
-template <int TM_, int TN_, int WM_, int WN_, int NS_> struct FtShape {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, NW = WM * WN, NT = NW * 64;
-  static constexpr int NI = TM / WM / 16, NJ = TN / WN / 16, STAGE = (TM + TN) * 128, LDS = NS * STAGE;
+// tile shape: TM x TN by WM x WN waves, NS LDS stages of KS k and PL planes
+template <int TM_, int TN_, int WM_, int WN_, int NS_, int KS_ = 64, int PL_ = 1> struct FtShape {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, KS = KS_, PL = PL_, NW = WM * WN, NT = NW * 64;
+  static constexpr int NI = TM / WM / 16, NJ = TN / WN / 16, STAGE = (TM + TN) * KS * 2 * PL, LDS = NS * STAGE;
 };
+template <class S, int MODE> using FtStageA = FtStager<MODE, S::TM, S::KS, S::NW>;
+template <class S, int MODE, int NJ = S::NJ> using FtStageB = FtStager<MODE, NJ * 16 * S::WN, S::KS, S::NW>;
 // plane pairs of the six products, least k first: (0,0) (0,1) (1,0) (1,1) (0,2) (2,0); one nibble each
 __device__ __forceinline__ int ft_pa(int c) { return (0x201100 >> (4 * c)) & 3; }
 __device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; }
@@ -143,10 +154,10 @@ __device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; 
 // step's second half in registers, so its stage is free for the loads of the step NS on, and the next stage, loaded for NS - 1 steps by then, is
 // read from there on.
 template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_halves(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+__device__ __forceinline__ void ft_halves(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                          ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
   constexpr int TNL = NJ * 16 * S::WN;      // columns staged (the shape's TN, or less in a second loop over the same tile)
-  constexpr int PA = FtStager<AM, S::TM, S::NW>::NP, PB = FtStager<BMO, TNL, S::NW>::NP, NF = S::NI + NJ, NM = S::NI * NJ;
+  constexpr int PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO, NJ>::NP, NF = S::NI + NJ, NM = S::NI * NJ;
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * NPROD;
   int c = 0;
@@ -167,7 +178,7 @@ __device__ __forceinline__ void ft_halves(FtStager<AM, S::TM, S::NW>& sa, FtStag
   ft_b8 f[2][NF];                           // [half][B fragments, then A fragments]
   auto read = [&](int i, int ks, int at) {
     const char* t = smem + at * S::STAGE;
-    f[ks][i] = i < NJ ? ft_frag<BMO, TNL>(t + S::TM * 128, (wn * NJ + i) * 16, ks, lane) : ft_frag<AM, S::TM>(t, (wm * S::NI + i - NJ) * 16, ks, lane);
+    f[ks][i] = i < NJ ? ft_frag<BMO, TNL, 64>(t + S::TM * 128, (wn * NJ + i) * 16, ks, lane) : ft_frag<AM, S::TM, 64>(t, (wm * S::NI + i - NJ) * 16, ks, lane);
   };
   auto mfma = [&](int m, int ks) {
     const int i = m / NJ, j = m % NJ;
@@ -213,10 +224,10 @@ __device__ __forceinline__ void ft_halves(FtStager<AM, S::TM, S::NW>& sa, FtStag
 
 // the same without halves, for few rows: a step is short, and its loads' way from memory long
 template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_rows(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+__device__ __forceinline__ void ft_rows(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                              ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
   constexpr int TNL = NJ * 16 * S::WN;
-  constexpr int PA = FtStager<AM, S::TM, S::NW>::NP, PB = FtStager<BMO, TNL, S::NW>::NP;
+  constexpr int PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO, NJ>::NP;
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * NPROD;
   int slot = 0, c = 0;
@@ -248,9 +259,9 @@ __device__ __forceinline__ void ft_rows(FtStager<AM, S::TM, S::NW>& sa, FtStager
     for (int ks = 0; ks < 2; ++ks) {
       ft_b8 af[S::NI], bf[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) bf[j] = ft_frag<BMO, TNL>(tb, (wn * NJ + j) * 16, ks, lane);
+      for (int j = 0; j < NJ; ++j) bf[j] = ft_frag<BMO, TNL, 64>(tb, (wn * NJ + j) * 16, ks, lane);
 #pragma unroll
-      for (int i = 0; i < S::NI; ++i) af[i] = ft_frag<AM, S::TM>(ta, (wm * S::NI + i) * 16, ks, lane);
+      for (int i = 0; i < S::NI; ++i) af[i] = ft_frag<AM, S::TM, 64>(ta, (wm * S::NI + i) * 16, ks, lane);
 #pragma unroll
       for (int i = 0; i < S::NI; ++i)
 #pragma unroll
@@ -262,10 +273,82 @@ __device__ __forceinline__ void ft_rows(FtStager<AM, S::TM, S::NW>& sa, FtStager
   ft_dma_wait<0>();
   ft_barrier();
 }
+// fp32 operands with all three planes of both in a stage of 32 k: six products from one read of each fragment.  (A plane pair a step, as above
+// with nprod 6, loads every plane twice and meets six barriers for one here; it is left for the few rows of ft_rows.)  The fragments of the
+// next stage are read under the MFMAs of this one, whose barrier stands under the first of them.
+template <class S, int AM, int BMO>
+__device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
+                                          int lane) {
+  static_assert(S::KS == 32 && S::PL == 3, "a stage is one fragment deep");
+  constexpr int NI = S::NI, NJ = S::NJ, PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO>::NP, P = 3 * (PA + PB), NF = 3 * (NI + NJ), NM = 6 * NI * NJ;
+  constexpr int TA = S::TM * 64, TB = S::TN * 64;     // bytes of a plane's tile
+  const unsigned lds0 = ft_lds_addr(smem);
+  const int steps = (kt1 - kt0) * 2;
+  sa.seek((long)kt0 * 64, 0);
+  sb.seek((long)kt0 * 64, 0);
+  auto next = [&]() { sa.step(); sb.step(); };
+  auto piece = [&](int i, int at) {
+    const unsigned l = lds0 + at * S::STAGE;
+    if (i < 3 * PA) sa.piece_of(i / PA, i % PA, l + i / PA * TA, wave);
+    else sb.piece_of((i - 3 * PA) / PB, (i - 3 * PA) % PB, l + 3 * TA + (i - 3 * PA) / PB * TB, wave);
+  };
+  ft_b8 fa[2][3][NI], fb[2][3][NJ];
+  auto read = [&](int i, int h, int at) {             // in the order of use: both first planes, then the others
+    const char* t = smem + at * S::STAGE;
+    const int pl = i / (NI + NJ), k = i % (NI + NJ);
+    if (k < NJ) fb[h][pl][k] = ft_frag<BMO, S::TN, 32>(t + 3 * TA + pl * TB, (wn * NJ + k) * 16, 0, lane);
+    else fa[h][pl][k - NJ] = ft_frag<AM, S::TM, 32>(t + pl * TA, (wm * NI + k - NJ) * 16, 0, lane);
+  };
+  auto mfma = [&](int m, int h) {
+    constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
+    const int q = m / (NI * NJ), i = m % (NI * NJ) / NJ, j = m % NJ;
+    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[h][qb[q]][j], fa[h][qa[q]][i], acc[i][j], 0, 0, 0);
+  };
+#pragma unroll
+  for (int st = 0; st < S::NS; ++st) {
+    next();
+#pragma unroll
+    for (int i = 0; i < P; ++i) piece(i, st);
+  }
+  ft_dma_wait<(S::NS - 1) * P>();
+  ft_barrier();
+#pragma unroll
+  for (int i = 0; i < NF; ++i) read(i, 0, 0);
+  constexpr int M0 = NM / 8, RM = (NM - M0) / NF;
+  static_assert(RM >= 1, "an MFMA to every read");
+  int at = 0;
+  auto stage = [&](int h) {
+    const int to = at + 1 == S::NS ? 0 : at + 1;
+    next();
+#pragma unroll
+    for (int m = 0; m < M0; ++m) mfma(m, h);
+    __builtin_amdgcn_sched_barrier(0);
+    ft_dma_wait<(S::NS - 2) * P>();
+    ft_barrier();                                     // slot `to` is there, and slot `at` read by everybody
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+#pragma unroll
+      for (int i = g * P / NF; i < (g + 1) * P / NF; ++i) piece(i, at);
+      read(g, h ^ 1, to);
+#pragma unroll
+      for (int m = M0 + g * RM; m < (g + 1 < NF ? M0 + (g + 1) * RM : NM); ++m) mfma(m, h);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    at = to;
+  };
+  for (int s = 0; s < steps; s += 2) {
+    stage(0);
+    stage(1);
+  }
+  ft_dma_wait<0>();
+  ft_barrier();
+}
+
 template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_loop(FtStager<AM, S::TM, S::NW>& sa, FtStager<BMO, NJ * 16 * S::WN, S::NW>& sb, char* smem, int kt0, int kt1,
+__device__ __forceinline__ void ft_loop(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                         ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  if constexpr (S::PL == 3) ft_planes<S, AM, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  else if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
   else ft_rows<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
 }
 
@@ -357,11 +440,11 @@ struct FtProduct {
 struct FtPlan { int shape = 0, target = 0; };
 FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_rows);
 __host__ __device__ static inline long ft_part_ld(long N) { return (N + 7) / 8 * 8; }
-// slices of a reduction of length K for `tiles` output tiles: as many as the target asks for, none under four k-steps
-__host__ __device__ static inline int ft_slices(long tiles, long K, int target) {
+// slices of a reduction of length K for `tiles` output tiles: as many as the target asks for, none under four k-steps (one of fp32's six products)
+__host__ __device__ static inline int ft_slices(long tiles, long K, int target, int nprod) {
   if (target <= 0 || tiles <= 0) return 1;
   long s = target / tiles;
-  const long most = (K + 63) / 64 / 4;
+  const long most = nprod == 1 ? (K + 63) / 64 / 4 : (K + 63) / 64;
   s = s < most ? s : most;
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }

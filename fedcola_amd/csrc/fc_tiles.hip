@@ -65,12 +65,12 @@ template <class S, int AM, int BMO, int NPROD, bool PART>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtProduct p, float* part, int target, int add) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
-  const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = (p.Ks ? p.Ks : K) * p.segs, splits = ft_slices((long)tm * tn, Ks, target);
+  const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = (p.Ks ? p.Ks : K) * p.segs, splits = ft_slices((long)tm * tn, Ks, target, NPROD);
   const FtTile t = ft_tile(tm, tn, splits);
   if (!t.any) return;
   const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = t.n * S::TN;
-  FtStager<AM, S::TM, S::NW> sa;
-  FtStager<BMO, S::TN, S::NW> sb;
+  FtStageA<S, AM> sa;
+  FtStageB<S, BMO> sb;
   sa.init(p.a, m0, K, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
   sb.init(p.b, n0, K, wave, lane, [&](int r) { return n0 + r < N ? (long)n0 + r : -1L; });
   ft_f4 acc[S::NI][S::NJ];
@@ -144,9 +144,11 @@ typedef FtShape<256, 256, 2, 4, 2> FtBig;      // 128 KB of LDS, one workgroup a
 typedef FtShape<128, 128, 2, 2, 2> FtMid;      // 64 KB, two
 typedef FtShape<32, 64, 2, 2, 6> FtRow;        // 72 KB, two: few rows, the reading of B is what counts (TK x TK alone)
 
+typedef FtShape<128, 128, 2, 4, 3, 32, 3> FtPlanes;   // fp32's only large tile: 144 KB, one workgroup of eight waves a CU
+
 struct FtCost { double step, fixed; int slots; };   // us a k-step with the chip full, us a tile besides, tiles at once
-static const FtCost kCost[3] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}};
-static const int kTM[3] = {256, 128, 32}, kTN[3] = {256, 128, 64};
+static const FtCost kCost[4] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}, {2.6, 6.0, 256}};
+static const int kTM[4] = {256, 128, 32, 128}, kTN[4] = {256, 128, 64, 128};
 
 // The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
 // step + time of a tile's start and end), plus the partial sums' way to memory and back.  The constants are measured: 256 x 256 tiles run
@@ -154,14 +156,14 @@ static const int kTM[3] = {256, 128, 32}, kTN[3] = {256, 128, 64};
 FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_rows) {
   FtPlan best;
   double least = 1e30;
-  for (int sh = 0; sh < 3; ++sh) {
-    if (sh == 2 && (am != TK || bm != TK || M > 64)) continue;
+  for (int sh = 0; sh < 4; ++sh) {
+    if (sh == 2 ? am != TK || bm != TK || M > 64 : (sh == 3) != (nprod == 6)) continue;
     const long tiles = ((M + kTM[sh] - 1) / kTM[sh]) * ((N + kTN[sh] - 1) / kTN[sh]), nk = (K + 63) / 64;
     for (int want = 1; want <= 64; ++want) {
-      const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want));
+      const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want), nprod);
       const long per = (nk + sp - 1) / sp, wg = tiles * sp, slots = kCost[sh].slots;
       const double rounds = wg <= 4 * slots ? (double)((wg + slots - 1) / slots) : (double)wg / slots + 0.5;
-      double t = rounds * ((double)(per * nprod) * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
+      double t = rounds * ((double)(sh == 2 ? per * nprod : per) * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
       if (sp > 1) t += 4.0 + (double)sp * M * N * 8.0 / 4e6;
       if (t < least) {
         least = t;
@@ -186,7 +188,7 @@ static int launch(const FtProduct& p, int target, float* part, bool add, hipStre
   long tiles = (long)((p.M + S::TM - 1) / S::TM) * ((p.N + S::TN - 1) / S::TN);
   if (part) {     // rows really there may be fewer, and the slices then more: never more workgroups than this
     if (p.Mdyn) tiles = tiles > target ? tiles : target;
-    else tiles *= ft_slices(tiles, (p.Ks ? p.Ks : p.K) * p.segs, target);
+    else tiles *= ft_slices(tiles, (p.Ks ? p.Ks : p.K) * p.segs, target, p.nprod);
   }
   FC_REQUIRE(tiles < (1L << 31), "product of %d x %d: too many tiles", p.M, p.N);
   if (tiles == 0) return 0;
@@ -206,15 +208,15 @@ template <class S, int NPROD> static int by_mode(const FtProduct& p, int target,
   fc_set_error("no such product");
   return -1;
 }
-template <int NPROD> static int by_shape(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s) {
-  if (plan.shape == 0) return by_mode<FtBig, NPROD>(p, plan.target, part, add, s);
-  if (plan.shape == 1) return by_mode<FtMid, NPROD>(p, plan.target, part, add, s);
-  return by_mode<FtRow, NPROD>(p, plan.target, part, add, s);
-}
 int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s) {
   // 32-bit offsets inside a tile: 256 rows of a TK operand, 64 of a TR one, and a whole row of columns
   FC_REQUIRE(p.a.ld < (1L << 21) && p.b.ld < (1L << 21), "an operand's rows are too far apart (%ld, %ld elements)", p.a.ld, p.b.ld);
-  return p.nprod == 1 ? by_shape<1>(p, plan, part, add, s) : by_shape<6>(p, plan, part, add, s);
+  switch (plan.shape) {
+    case 0: return by_mode<FtBig, 1>(p, plan.target, part, add, s);
+    case 1: return by_mode<FtMid, 1>(p, plan.target, part, add, s);
+    case 2: return p.nprod == 1 ? by_mode<FtRow, 1>(p, plan.target, part, add, s) : by_mode<FtRow, 6>(p, plan.target, part, add, s);
+    default: return by_mode<FtPlanes, 6>(p, plan.target, part, add, s);
+  }
 }
 
 // ---------------------------------------------------------------- sums of the slices
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(256) k_ft_reduce(FtProduct p, const float* par
   const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
   const long ldp = ft_part_ld(N), cw = ldp / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
   if (e >= R * cw) return;
-  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), (p.Ks ? p.Ks : K) * p.segs, target);
+  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), (p.Ks ? p.Ks : K) * p.segs, target, p.nprod);
   const long m = e / cw;
   const int n = (int)(e - m * cw) * 8;
   const long src = pos ? pos[m] : m, row = pos ? m : p.rows.at((int)m);
