@@ -200,17 +200,18 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backwa
 }
 static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.dh + z.part; }
 
-static int gm_matrix(int dt, const void* p, long ld, long R, long C, bool use_direct, char*& ws, FtMat& m, hipStream_t s) {
-  if (use_direct) {
+// a matrix as the products take it: where it is, or as one of the packs
+static void gm_matrix(int dt, const void* p, long ld, long R, long C, char*& ws, FtMat& m, FtPacks& l) {
+  if (ft_direct(dt, p, ld, C)) {
     m.p = (const bf16_t*)p;
     m.ld = ld;
-    return 0;
+    return;
   }
   FtPack k;
   k.src = p; k.lds = ld; k.dt = dt; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 64);
   m.p = k.dst; m.ld = k.ldd; m.plane = R * k.ldd;
   ws += ft_up((dt ? 1 : 3) * R * k.ldd * 2, 256);
-  return ft_pack(k, s);
+  l.add(k);
 }
 struct GmCall { int dt, act; long T, D, F; const void *x, *w_in, *w_out, *dy; long ldx, ld_in, ld_out, lddy; };
 static int gm_check(const char* what, const GmCall& c, const void* ws) {
@@ -232,10 +233,12 @@ static bool gm_direct(const GmCall& c) {
 // the operands as the products take them; what of them cannot be taken as it is goes to the workspace
 static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
   a.T = (int)c.T; a.D = (int)c.D; a.F = (int)c.F; a.act = c.act; a.up = c.F; a.ldh = ft_up(c.F, 64);
-  FC_TRY(gm_matrix(c.dt, c.x, c.ldx, c.T, c.D, ft_direct(c.dt, c.x, c.ldx, c.D), ws, a.x, s));
-  if (c.dy) FC_TRY(gm_matrix(c.dt, c.dy, c.lddy, c.T, c.D, ft_direct(c.dt, c.dy, c.lddy, c.D), ws, a.dy, s));
-  FC_TRY(gm_matrix(c.dt, c.w_out, c.ld_out, c.D, c.F, ft_direct(c.dt, c.w_out, c.ld_out, c.F), ws, a.w_out, s));
-  return gm_matrix(c.dt, c.w_in, c.ld_in, 2 * c.F, c.D, ft_direct(c.dt, c.w_in, c.ld_in, c.D), ws, a.w_in, s);
+  FtPacks l;
+  gm_matrix(c.dt, c.x, c.ldx, c.T, c.D, ws, a.x, l);
+  if (c.dy) gm_matrix(c.dt, c.dy, c.lddy, c.T, c.D, ws, a.dy, l);
+  gm_matrix(c.dt, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
+  gm_matrix(c.dt, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
+  return ft_pack(l, s);
 }
 
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {

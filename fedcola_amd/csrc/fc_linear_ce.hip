@@ -368,7 +368,9 @@ static int ce_weight(int dt, const void* w, long ldw, long V, long D, char*& ws,
   k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64);
   m.p = k.dst; m.ld = k.ldd; m.plane = V * k.ldd;
   ws += (size_t)ft_up((dt ? 1 : 3) * V * k.ldd * 2, 256);
-  return ft_pack(k, s);
+  FtPacks l;
+  l.add(k);
+  return ft_pack(l, s);
 }
 
 extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t D) { return T < 0 || D < 1 ? 0 : ce_saved(nullptr, dt, T, D).bytes; }

@@ -466,7 +466,13 @@ struct FtPack {
   bf16_t* dst = nullptr;
   long ldd = 0;                   // multiple of 64, >= C: the columns in between are written as zeros
 };
-int ft_pack(const FtPack& p, hipStream_t s);
+struct FtPacks {                  // up to four of one type in one launch
+  FtPack p[4];
+  int n = 0;
+  long first[5] = {0, 0, 0, 0, 0};   // 16-byte chunks before each
+  void add(const FtPack& q) { p[n] = q; first[n + 1] = first[n] + q.R * (q.ldd / 8); ++n; }
+};
+int ft_pack(const FtPacks& p, hipStream_t s);
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
 static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }
 // > 64 KB of LDS for a kernel, once for each device

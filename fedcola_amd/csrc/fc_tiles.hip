@@ -32,11 +32,20 @@ int ft_check_device(const void* p, const char* what) {
 
 // ---------------------------------------------------------------- packing
 template <typename T, int PL>
-__global__ void __launch_bounds__(256) k_ft_pack(FtPack a) {
-  const long cw = a.ldd / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
-  if (e >= a.R * cw) return;
-  const long r = e / cw;
-  const int c0 = (int)(e - r * cw) * 8;
+__global__ void __launch_bounds__(256) k_ft_pack(FtPacks l) {
+  const long e = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= l.first[l.n]) return;
+  int w = 0;
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+    if (i < l.n && e >= l.first[i]) w = i;
+  FtPack a = l.p[0];
+  long e0 = 0;
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+    if (w == i) { a = l.p[i]; e0 = l.first[i]; }
+  const long cw = a.ldd / 8, r = (e - e0) / cw;
+  const int c0 = (int)(e - e0 - r * cw) * 8;
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
@@ -50,11 +59,11 @@ __global__ void __launch_bounds__(256) k_ft_pack(FtPack a) {
     *(uint4*)(a.dst + (size_t)p * a.R * a.ldd + r * a.ldd + c0) =
         make_uint4(f2bf2(h[p][0], h[p][1]), f2bf2(h[p][2], h[p][3]), f2bf2(h[p][4], h[p][5]), f2bf2(h[p][6], h[p][7]));
 }
-int ft_pack(const FtPack& p, hipStream_t s) {
-  const long n = p.R * (p.ldd / 8);
+int ft_pack(const FtPacks& p, hipStream_t s) {
+  const long n = p.first[p.n];
   if (n == 0) return 0;
   const dim3 g((unsigned)((n + 255) / 256));
-  if (p.dt) hipLaunchKernelGGL((k_ft_pack<bf16_t, 1>), g, dim3(256), 0, s, p);
+  if (p.p[0].dt) hipLaunchKernelGGL((k_ft_pack<bf16_t, 1>), g, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((k_ft_pack<float, 3>), g, dim3(256), 0, s, p);
   FC_LAUNCH_CHECK();
   return 0;
