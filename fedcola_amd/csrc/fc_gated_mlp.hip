@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a
   constexpr bool TURN = 2 * SET <= S::LDS;                                                      // room for two outputs' in turn
   static_assert(SET <= S::LDS, "an output's images fit");
   const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN;
-  const FtTile t = ft_tile((a.T + S::TM - 1) / S::TM, (a.F + FC - 1) / FC, 1);
+  const FtTile t = ft_tile((a.T + S::TM - 1) / S::TM, (a.F + FC - 1) / FC, 1, blockIdx.x);
   if (!t.any) return;
   const int m0 = t.m * S::TM, f0 = t.n * FC;
   ft_f4 acc[S::NI][S::NJ];
@@ -175,7 +175,25 @@ template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream
   }
 }
 
-struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; };
+struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan[3]; bool group; };
+// dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
+static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProduct (&p)[3]) {
+  const long Fp = ft_up(F, 64);
+  for (FtProduct& q : p) { q.am = TR; q.bm = TR; q.nprod = dt ? 1 : 6; q.K = (int)T; }
+  p[0].am = TK;
+  p[0].M = (int)T; p[0].N = (int)D; p[0].K = (int)F;
+  p[0].segs = 2; p[0].a2 = Fp; p[0].b2 = F * a.w_in.ld;
+  p[0].a.p = p[1].a.p = a.dgu;
+  p[0].a.ld = p[1].a.ld = 2 * Fp;
+  p[0].a.plane = p[1].a.plane = T * 2 * Fp;
+  p[0].b = a.w_in;
+  p[1].M = (int)(2 * Fp); p[1].N = (int)D;
+  if (Fp != F) { p[1].rows.half = (int)Fp; p[1].rows.to = (int)F; }
+  p[1].b = a.x;
+  p[2].M = (int)D; p[2].N = (int)F;
+  p[2].a = a.dy;
+  p[2].b.p = a.h; p[2].b.ld = Fp; p[2].b.plane = T * Fp;
+}
 static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backward) {
   GmSizes z = {};
   const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6;
@@ -193,9 +211,17 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backwa
   }
   z.dgu = ft_up(T * 2 * Fp * e, 256);
   z.dh = ft_up(ft_part_ld(F) * T * 4, 256);
-  const size_t a = ft_product_part_floats(TK, TR, np, T, D, 2 * F), b = ft_product_part_floats(TR, TR, np, 2 * Fp, D, T),
-               c = ft_product_part_floats(TR, TR, np, D, F, T);
-  z.part = 4 * (a > b ? a > c ? a : c : b > c ? b : c);
+  FtProduct p[3];
+  gm_products(dt, T, D, F, GmArgs(), p);
+  z.group = ft_group_plan(p, 3, z.plan);
+  for (int i = 0; i < 3; ++i) {
+    if (z.group) {
+      z.part += z.plan[i].target ? ft_up(ft_part_floats(p[i].M, p[i].N, z.plan[i]) * 4, 256) : 0;
+    } else {
+      const size_t n = ft_product_part_floats(p[i].am, p[i].bm, np, p[i].M, p[i].N, (long)p[i].K * p[i].segs) * 4;
+      z.part = z.part > n ? z.part : n;
+    }
+  }
   return z;
 }
 static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.dh + z.part; }
@@ -284,10 +310,10 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   ws += z.h;
   a.dgu = (bf16_t*)ws;
   ws += z.dgu;
-  float* part = (float*)(ws + z.dh);
-  FtProduct p;
-  p.nprod = dt ? 1 : 6;
+  char* part = ws + z.dh;
   if (T) {
+    FtProduct p;
+    p.nprod = dt ? 1 : 6;
     p.am = TK; p.bm = TR;
     p.a = a.dy;
     p.b = a.w_out;
@@ -299,29 +325,31 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
     a.ldd = ft_part_ld(F);
     FC_TRY(dt ? (gm_act_run<1, true>(a, s)) : (gm_act_run<6, true>(a, s)));
   }
-  p.a.p = a.dgu; p.a.ld = 2 * a.ldh; p.a.plane = (long)T * 2 * a.ldh;
-  if (dx && T) {
-    p.segs = 2;
-    p.a2 = a.ldh; p.b2 = (long)F * a.w_in.ld;
-    p.b = a.w_in;
-    p.M = T; p.N = D; p.K = F; p.out = dx; p.ldo = lddx;
-    FC_TRY(ft_product_out(p, part, z.part / 4, s));
-    p.segs = 1;
+  FtProduct p[3], q[3];
+  FtPlan plan[3];
+  float* at[3];
+  FtSums sums;
+  int n = 0;
+  gm_products(dt, T, D, F, a, p);
+  p[0].out = T ? dx : nullptr; p[0].ldo = lddx;
+  p[1].out = dw_in; p[1].ldo = ldd_in;
+  p[2].out = dw_out; p[2].ldo = ldd_out;
+  for (int i = 0; i < 3; ++i) {
+    if (!p[i].out) continue;
+    if (!z.group) {
+      FC_TRY(ft_product_out(p[i], (float*)part, z.part / 4, s));
+      continue;
+    }
+    q[n] = p[i];
+    plan[n] = z.plan[i];
+    at[n] = z.plan[i].target ? (float*)part : nullptr;
+    if (at[n]) {
+      sums.add(q[n], plan[n], at[n], nullptr, q[n].M);
+      part += ft_up(ft_part_floats(q[n].M, q[n].N, plan[n]) * 4, 256);
+    }
+    ++n;
   }
-  p.am = TR; p.bm = TR;
-  p.K = T;
-  if (dw_in) {
-    p.b = a.x;
-    p.M = (int)(2 * a.ldh); p.N = D; p.out = dw_in; p.ldo = ldd_in;
-    if (a.ldh != F) { p.rows.half = (int)a.ldh; p.rows.to = F; }
-    FC_TRY(ft_product_out(p, part, z.part / 4, s));
-    p.rows = FtRows();
-  }
-  if (dw_out) {
-    p.a = a.dy;
-    p.b.p = a.h; p.b.ld = a.ldh; p.b.plane = (long)T * a.ldh;
-    p.M = D; p.N = F; p.out = dw_out; p.ldo = ldd_out;
-    FC_TRY(ft_product_out(p, part, z.part / 4, s));
-  }
-  return 0;
+  if (!n) return 0;
+  FC_TRY(ft_group(q, plan, n, at, s));
+  return ft_reduce(sums, s);
 }

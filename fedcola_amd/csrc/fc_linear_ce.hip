@@ -122,7 +122,7 @@ struct CeArgs {
 
 template <class S, int NPROD>
 __device__ __forceinline__ bool ce_product(const CeArgs& a, char* smem, ft_f4 (&acc)[S::NI][S::NJ], FtTile& t, int M, int wave, int lane) {
-  t = ft_tile((M + S::TM - 1) / S::TM, (a.nv + S::TN - 1) / S::TN, 1);
+  t = ft_tile((M + S::TM - 1) / S::TM, (a.nv + S::TN - 1) / S::TN, 1, blockIdx.x);
   if (!t.any) return false;
   const int wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = a.v0 + t.n * S::TN;
   FtStageA<S, TK> sa;
@@ -328,7 +328,12 @@ static long ce_piece(int dt, long T, long V) {
   const long most = (192L << 20) / ((T ? T : 1) * (dt ? 2 : 6)) / 256 * 256, all = ft_up(V, 256);
   return most < 256 ? 256 : most < all ? most : all;
 }
-struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx; };
+struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx, dw; bool group; };
+// dx = dL w and dw = dL^T x of nv columns; n: device, the rows that count
+static void ce_products(int dt, long T, long D, long nv, const int* n, FtProduct& x, FtProduct& w) {
+  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
+  w.am = TR; w.bm = TR; w.nprod = x.nprod; w.M = (int)nv; w.N = (int)D; w.K = (int)T; w.Kdyn = n;
+}
 static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad) {
   CeSizes z = {};
   const int np = dt ? 1 : 6;
@@ -341,6 +346,19 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
   }
   z.piece = ce_piece(dt, T, V);
   z.dl = (size_t)ft_up((dt ? 1 : 3) * T * z.piece * 2, 256);
+  if (z.piece >= V) {                     // one piece: its two products may run together
+    FtProduct p[2];
+    FtPlan plan[2];
+    ce_products(dt, T, D, V, nullptr, p[0], p[1]);
+    if (ft_group_plan(p, 2, plan)) {
+      z.group = true;
+      z.dx = plan[0];
+      z.dw = plan[1];
+      z.dxp = (size_t)ft_up(ft_part_floats(T, D, z.dx) * 4, 256);
+      z.dwp = z.dw.target ? (size_t)ft_up(ft_part_floats(V, D, z.dw) * 4, 256) : 0;
+      return z;
+    }
+  }
   z.dx = ft_plan(TK, TR, np, T, D, z.piece, true);
   z.dxp = (size_t)ft_up(ft_part_floats(T, D, z.dx) * 4, 256);
   z.dwp = (size_t)ft_up(ft_product_part_floats(TR, TR, np, z.piece < V ? z.piece : V, D, T) * 4, 256);
@@ -449,13 +467,14 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   a.plane = (long)T * z.piece;
   float* dxp = (float*)(ws + z.dl);
   float* dwp = (float*)(ws + z.dl + z.dxp);
-  const int np = dt ? 1 : 6, es = dt ? 2 : 4;
+  const int es = dt ? 2 : 4;
   FtProduct px, pw;
-  px.am = TK; px.bm = TR; px.nprod = np; px.M = T; px.N = D; px.Mdyn = sv.n; px.Ks = (int)z.piece; px.out = dx; px.ldo = lddx;
+  ce_products(dt, T, D, z.piece, sv.n, px, pw);
+  px.out = dx; px.ldo = lddx;
   px.a.p = a.dl; px.a.ld = a.ldl; px.a.plane = a.plane;
-  pw.am = TR; pw.bm = TR; pw.nprod = np; pw.N = D; pw.K = T; pw.Kdyn = sv.n; pw.ldo = lddw;
   pw.a = px.a;
   pw.b = sv.x;
+  pw.ldo = lddw;
   if (reduction != FC_REDUCE_NONE) {
     px.alpha = pw.alpha = gloss;
     if (reduction == FC_REDUCE_MEAN) px.alpha_over = pw.alpha_over = sv.n;
@@ -464,6 +483,28 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < z.piece ? V - v0 : z.piece);
     FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv), a, s));
+    if (z.group) {
+      px.K = pw.M = a.nv;
+      px.b = a.w;
+      pw.out = dw;
+      FtProduct p[2];
+      FtPlan plan[2];
+      float* part[2];
+      FtSums l;
+      int n = 0;
+      if (dx && T) {
+        p[n] = px; plan[n] = z.dx; part[n++] = dxp;
+        l.add(px, z.dx, dxp, sv.pos, T);
+      }
+      if (dw) {
+        p[n] = pw; plan[n] = z.dw; part[n++] = z.dw.target ? dwp : nullptr;
+        if (z.dw.target) l.add(pw, z.dw, dwp, nullptr, V);
+      }
+      if (!n) return 0;
+      FC_TRY(ft_group(p, plan, n, part, s));
+      return ft_reduce(l, s);
+    }
+    px.Ks = (int)z.piece;
     if (dw) {
       pw.M = a.nv;
       pw.out = (char*)dw + v0 * lddw * es;

@@ -355,9 +355,9 @@ __device__ __forceinline__ void ft_loop(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ
 // ---- which tile a workgroup takes.  Consecutive ids share an XCD's L2 (workgroups are dealt to the 8 XCDs in turn), and ids walk the
 // tiles in groups of 8 tile rows, column by column, so that the tiles in flight on an XCD share few operand panels.
 struct FtTile { int m, n, split; bool any; };
-__device__ __forceinline__ FtTile ft_tile(int tm, int tn, int splits) {
+__device__ __forceinline__ FtTile ft_tile(int tm, int tn, int splits, int b) {
   FtTile t;
-  const int total = tm * tn * splits, b = blockIdx.x;
+  const int total = tm * tn * splits;
   t.any = b < total;
   if (!t.any) { t.m = t.n = t.split = 0; return t; }
   const int q = total >> 3, r = total & 7, xcd = b & 7;
@@ -451,6 +451,24 @@ __host__ __device__ static inline int ft_slices(long tiles, long K, int target, 
 size_t ft_part_floats(long M, long N, const FtPlan& plan);     // for any number of rows up to M
 // partial sums [slices][rows there][ft_part_ld(N)] into `part` (or, part null, the product into p.out); add: onto what is there
 int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s);
+// up to three products in one launch, and the sums of their slices in one
+struct FtGroup {
+  FtProduct p[3];
+  float* part[3] = {nullptr, nullptr, nullptr};
+  int target[3] = {0, 0, 0}, add[3] = {0, 0, 0}, first[4] = {0, 0, 0, 0};      // first workgroup of each
+};
+struct FtSums {
+  FtProduct p[3];
+  const float* part[3] = {nullptr, nullptr, nullptr};
+  const int* pos[3] = {nullptr, nullptr, nullptr};
+  int target[3] = {0, 0, 0}, TM[3] = {0, 0, 0}, TN[3] = {0, 0, 0}, n = 0;
+  long first[4] = {0, 0, 0, 0};                                                // first group of eight columns of each
+  void add(const FtProduct& q, const FtPlan& plan, const float* partial, const int* places, long rows);
+};
+int ft_reduce(const FtSums& l, hipStream_t s);
+// whether they are better run as a group, and how; part[i] null: straight into out
+bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan);
+int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, hipStream_t s);
 // out = the sum over the slices, in their order, of ft_product's partial sums; with `pos`: out[r] = row pos[r] of the sums, 0 where pos[r] < 0, for R rows
 int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s);
 // the product into p.out, by way of partial sums in `part` where the plan slices the reduction

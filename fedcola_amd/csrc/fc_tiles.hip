@@ -70,12 +70,12 @@ int ft_pack(const FtPacks& p, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- the product
-template <class S, int AM, int BMO, int NPROD, bool PART>
-__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtProduct p, float* part, int target, int add) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+// workgroup b of a product: into p.out, or (part) as partial sums
+template <class S, int AM, int BMO, int NPROD>
+__device__ __forceinline__ void ft_product_tile(const FtProduct& p, float* part, int target, int add, int b, char* smem) {
   const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
   const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = (p.Ks ? p.Ks : K) * p.segs, splits = ft_slices((long)tm * tn, Ks, target, NPROD);
-  const FtTile t = ft_tile(tm, tn, splits);
+  const FtTile t = ft_tile(tm, tn, splits, b);
   if (!t.any) return;
   const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = t.n * S::TN;
   FtStageA<S, AM> sa;
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtPr
     ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0 > nk ? kt0 - nk : 0, kt1 - nk, acc, wm, wn, wave, lane);
   }
   const int mr = wm * S::NI * 16 + (lane & 15), nc = wn * S::NJ * 16 + 4 * (lane >> 4);
-  if (PART) {
+  if (part) {
     const long ldp = ft_part_ld(N);
     float* o = part + (long)t.split * M * ldp;
 #pragma unroll
@@ -149,6 +149,21 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtPr
   }
 }
 
+template <class S, int AM, int BMO, int NPROD>
+__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_product(FtProduct p, float* part, int target, int add) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  ft_product_tile<S, AM, BMO, NPROD>(p, part, target, add, blockIdx.x, smem);
+}
+// several products in one launch: B is TR in all of them
+template <class S, int NPROD>
+__global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_group(FtGroup g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int b = blockIdx.x, i = b < g.first[1] ? 0 : b < g.first[2] ? 1 : 2;
+  const FtProduct& p = g.p[i];
+  if (p.am == TK) ft_product_tile<S, TK, TR, NPROD>(p, g.part[i], g.target[i], g.add[i], b - g.first[i], smem);
+  else ft_product_tile<S, TR, TR, NPROD>(p, g.part[i], g.target[i], g.add[i], b - g.first[i], smem);
+}
+
 typedef FtShape<256, 256, 2, 4, 2> FtBig;      // 128 KB of LDS, one workgroup a CU
 typedef FtShape<128, 128, 2, 2, 2> FtMid;      // 64 KB, two
 typedef FtShape<32, 64, 2, 2, 6> FtRow;        // 72 KB, two: few rows, the reading of B is what counts (TK x TK alone)
@@ -192,27 +207,28 @@ size_t ft_part_floats(long M, long N, const FtPlan& pl) {
   return (size_t)wg * kTM[pl.shape] * kTN[pl.shape];
 }
 
+// workgroups of a product: rows really there may be fewer, and the slices then more, but never more of both than this
+static long workgroups(const FtProduct& p, const FtPlan& pl, bool part) {
+  const long tiles = tiles_of(pl, p.M, p.N);
+  if (!part) return tiles;
+  if (p.Mdyn) return tiles > pl.target ? tiles : pl.target;
+  return tiles * ft_slices(tiles, (long)(p.Ks ? p.Ks : p.K) * p.segs, pl.target, p.nprod);
+}
 template <class S, int AM, int BMO, int NPROD>
-static int launch(const FtProduct& p, int target, float* part, bool add, hipStream_t s) {
-  long tiles = (long)((p.M + S::TM - 1) / S::TM) * ((p.N + S::TN - 1) / S::TN);
-  if (part) {     // rows really there may be fewer, and the slices then more: never more workgroups than this
-    if (p.Mdyn) tiles = tiles > target ? tiles : target;
-    else tiles *= ft_slices(tiles, (p.Ks ? p.Ks : p.K) * p.segs, target, p.nprod);
-  }
-  FC_REQUIRE(tiles < (1L << 31), "product of %d x %d: too many tiles", p.M, p.N);
-  if (tiles == 0) return 0;
-  const void* k = part ? (const void*)k_ft_product<S, AM, BMO, NPROD, true> : (const void*)k_ft_product<S, AM, BMO, NPROD, false>;
-  FC_TRY(ft_allow_lds(k, S::LDS));
-  if (part) hipLaunchKernelGGL((k_ft_product<S, AM, BMO, NPROD, true>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, p, part, target, add ? 1 : 0);
-  else hipLaunchKernelGGL((k_ft_product<S, AM, BMO, NPROD, false>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, p, part, 0, 0);
+static int launch(const FtProduct& p, const FtPlan& pl, float* part, bool add, hipStream_t s) {
+  const long n = workgroups(p, pl, part != nullptr);
+  FC_REQUIRE(n < (1L << 31), "product of %d x %d: too many tiles", p.M, p.N);
+  if (n == 0) return 0;
+  FC_TRY(ft_allow_lds((const void*)k_ft_product<S, AM, BMO, NPROD>, S::LDS));
+  hipLaunchKernelGGL((k_ft_product<S, AM, BMO, NPROD>), dim3((unsigned)n), dim3(S::NT), S::LDS, s, p, part, part ? pl.target : 0, add ? 1 : 0);
   FC_LAUNCH_CHECK();
   return 0;
 }
-template <class S, int NPROD> static int by_mode(const FtProduct& p, int target, float* part, bool add, hipStream_t s) {
-  if (p.am == TK && p.bm == TK) return launch<S, TK, TK, NPROD>(p, target, part, add, s);
+template <class S, int NPROD> static int by_mode(const FtProduct& p, const FtPlan& pl, float* part, bool add, hipStream_t s) {
+  if (p.am == TK && p.bm == TK) return launch<S, TK, TK, NPROD>(p, pl, part, add, s);
   if constexpr (S::TN >= 128) {
-    if (p.am == TK) return launch<S, TK, TR, NPROD>(p, target, part, add, s);
-    if (p.bm == TR) return launch<S, TR, TR, NPROD>(p, target, part, add, s);
+    if (p.am == TK) return launch<S, TK, TR, NPROD>(p, pl, part, add, s);
+    if (p.bm == TR) return launch<S, TR, TR, NPROD>(p, pl, part, add, s);
   }
   fc_set_error("no such product");
   return -1;
@@ -221,20 +237,25 @@ int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hi
   // 32-bit offsets inside a tile: 256 rows of a TK operand, 64 of a TR one, and a whole row of columns
   FC_REQUIRE(p.a.ld < (1L << 21) && p.b.ld < (1L << 21), "an operand's rows are too far apart (%ld, %ld elements)", p.a.ld, p.b.ld);
   switch (plan.shape) {
-    case 0: return by_mode<FtBig, 1>(p, plan.target, part, add, s);
-    case 1: return by_mode<FtMid, 1>(p, plan.target, part, add, s);
-    case 2: return p.nprod == 1 ? by_mode<FtRow, 1>(p, plan.target, part, add, s) : by_mode<FtRow, 6>(p, plan.target, part, add, s);
-    default: return by_mode<FtPlanes, 6>(p, plan.target, part, add, s);
+    case 0: return by_mode<FtBig, 1>(p, plan, part, add, s);
+    case 1: return by_mode<FtMid, 1>(p, plan, part, add, s);
+    case 2: return p.nprod == 1 ? by_mode<FtRow, 1>(p, plan, part, add, s) : by_mode<FtRow, 6>(p, plan, part, add, s);
+    default: return by_mode<FtPlanes, 6>(p, plan, part, add, s);
   }
 }
 
 // ---------------------------------------------------------------- sums of the slices
 template <typename T>
-__global__ void __launch_bounds__(256) k_ft_reduce(FtProduct p, const float* part, int target, int TM, int TN, const int* pos, long R) {
-  const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N;
-  const long ldp = ft_part_ld(N), cw = ldp / 8, e = (long)blockIdx.x * 256 + threadIdx.x;
-  if (e >= R * cw) return;
-  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), (p.Ks ? p.Ks : K) * p.segs, target, p.nprod);
+__global__ void __launch_bounds__(256) k_ft_reduce(FtSums l) {
+  const long e0 = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e0 >= l.first[l.n]) return;
+  const int w = e0 < l.first[1] ? 0 : e0 < l.first[2] ? 1 : 2;
+  const long e = e0 - l.first[w];
+  const FtProduct& p = l.p[w];
+  const int M = p.Mdyn ? min(p.M, *p.Mdyn) : p.M, K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, N = p.N, TM = l.TM[w], TN = l.TN[w];
+  const long ldp = ft_part_ld(N), cw = ldp / 8;
+  const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), (long)(p.Ks ? p.Ks : K) * p.segs, l.target[w], p.nprod);
+  const int* pos = l.pos[w];
   const long m = e / cw;
   const int n = (int)(e - m * cw) * 8;
   const long src = pos ? pos[m] : m, row = pos ? m : p.rows.at((int)m);
@@ -243,7 +264,7 @@ __global__ void __launch_bounds__(256) k_ft_reduce(FtProduct p, const float* par
   if (src >= 0 && src < M)
 #pragma unroll 4
     for (int q = 0; q < splits; ++q) {
-      const ft_f4* a = (const ft_f4*)(part + ((long)q * M + src) * ldp + n);
+      const ft_f4* a = (const ft_f4*)(l.part[w] + ((long)q * M + src) * ldp + n);
       v[0] += a[0];
       v[1] += a[1];
     }
@@ -259,12 +280,64 @@ __global__ void __launch_bounds__(256) k_ft_reduce(FtProduct p, const float* par
   for (int x = 0; x < 8; ++x)
     if (n + x < N) Io<T>::st(o, x, v[x >> 2][x & 3]);
 }
-int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s) {
-  const long n = R * (ft_part_ld(p.N) / 8);
+void FtSums::add(const FtProduct& q, const FtPlan& plan, const float* partial, const int* places, long rows) {
+  p[n] = q; part[n] = partial; pos[n] = places; target[n] = plan.target; TM[n] = kTM[plan.shape]; TN[n] = kTN[plan.shape];
+  first[n + 1] = first[n] + rows * (ft_part_ld(q.N) / 8);
+  for (int i = ++n; i < 3; ++i) first[i + 1] = first[i];
+}
+int ft_reduce(const FtSums& l, hipStream_t s) {
+  const long n = l.first[l.n];
   if (n == 0) return 0;
   const dim3 g((unsigned)((n + 255) / 256));
-  if (p.nprod == 1) hipLaunchKernelGGL(k_ft_reduce<bf16_t>, g, dim3(256), 0, s, p, part, plan.target, kTM[plan.shape], kTN[plan.shape], pos, R);
-  else hipLaunchKernelGGL(k_ft_reduce<float>, g, dim3(256), 0, s, p, part, plan.target, kTM[plan.shape], kTN[plan.shape], pos, R);
+  if (l.p[0].nprod == 1) hipLaunchKernelGGL(k_ft_reduce<bf16_t>, g, dim3(256), 0, s, l);
+  else hipLaunchKernelGGL(k_ft_reduce<float>, g, dim3(256), 0, s, l);
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s) {
+  FtSums l;
+  l.add(p, plan, part, pos, R);
+  return ft_reduce(l, s);
+}
+
+// ---------------------------------------------------------------- products that wait for nothing of each other
+// One launch of 128 x 128 tiles while the chip would run less than about 160 k-steps of them: launches of 100 to 500 workgroups one after
+// the other leave part of it idle each (12608 x 384 x 1024, three products: TIME_SEP us apart, TIME_GRP together).  Above, tiles of 256 x 256
+// in launches of their own are faster.  Slices: of about half of a slot's share of the work, so that what is long and what is short packs well.
+bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan) {
+  const int sh = p[0].nprod == 1 ? 1 : 3, slots = kCost[sh].slots;
+  double work = 0;
+  for (int i = 0; i < n; ++i) work += (double)tiles_of(FtPlan{sh, 0}, p[i].M, p[i].N) * (double)((p[i].K + 63) / 64 * p[i].segs);
+  if (work > 160.0 * slots) return false;
+  const double share = work / slots / 2 > 4 ? work / slots / 2 : 4;
+  for (int i = 0; i < n; ++i) {
+    const long tiles = tiles_of(FtPlan{sh, 0}, p[i].M, p[i].N), nk = (long)(p[i].K + 63) / 64 * p[i].segs;
+    const long want = nk <= 2 * share ? 1 : (long)((double)nk / share + 0.5);
+    plan[i].shape = sh;
+    plan[i].target = want > 1 ? (int)(tiles * want < (1 << 20) ? tiles * want : 0) : 0;
+    if (p[i].Mdyn && plan[i].target < slots) plan[i].target = slots;
+  }
+  return true;
+}
+int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, hipStream_t s) {
+  FtGroup g;
+  for (int i = 0; i < n; ++i) {
+    FC_REQUIRE(p[i].bm == TR && p[i].a.ld < (1L << 21) && p[i].b.ld < (1L << 21), "an operand's rows are too far apart");
+    g.p[i] = p[i];
+    g.part[i] = part[i];
+    g.target[i] = part[i] ? plan[i].target : 0;
+    g.add[i] = 0;
+    g.first[i + 1] = g.first[i] + (int)ft_up(workgroups(p[i], plan[i], part[i] != nullptr), 8);      // whole rounds over the XCDs
+  }
+  for (int i = n; i < 3; ++i) g.first[i + 1] = g.first[i];
+  if (g.first[n] == 0) return 0;
+  if (plan[0].shape == 1) {
+    FC_TRY(ft_allow_lds((const void*)k_ft_group<FtMid, 1>, FtMid::LDS));
+    hipLaunchKernelGGL((k_ft_group<FtMid, 1>), dim3(g.first[n]), dim3(FtMid::NT), FtMid::LDS, s, g);
+  } else {
+    FC_TRY(ft_allow_lds((const void*)k_ft_group<FtPlanes, 6>, FtPlanes::LDS));
+    hipLaunchKernelGGL((k_ft_group<FtPlanes, 6>), dim3(g.first[n]), dim3(FtPlanes::NT), FtPlanes::LDS, s, g);
+  }
   FC_LAUNCH_CHECK();
   return 0;
 }
