@@ -8,8 +8,8 @@
 //   h = act(g) u,   dg = dh u act'(g),   du = dh act(g)
 // each rounded once; then dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h.  That is 16 T D F operations for the 12 of a backward
 // pass that reads g and u back; these would have to be stored in 32 bits too, or rounded once more than here.  (dh on the same tile as g and
-// u, without its 8 bytes a unit through memory, leaves registers for 128 x 256 tiles only: 2300 us for 8192 x 4096 x 11000, TIME_TWO in two
-// kernels.)
+// u, without its 8 bytes a unit through memory, leaves registers for 128 x 256 tiles only: 2300 us for 8192 x 4096 x 11000, 2000 in two kernels;
+// 70 against 74 for 12608 x 384 x 1024.)
 #include <math.h>
 
 #include "../../include/fedcola_hip.h"
@@ -157,14 +157,15 @@ typedef FtShape<128, 128, 2, 4, 3, 32, 3> GmPlanes;
 template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));
   FC_REQUIRE(tiles < (1L << 31), "gated_mlp: too many tiles");
-  FC_TRY(ft_allow_lds((const void*)k_gm_act<S, NPROD, GRAD>, S::LDS));
+  static FtLds lds;
+  FC_TRY(lds.allow((const void*)k_gm_act<S, NPROD, GRAD>, S::LDS));
   hipLaunchKernelGGL((k_gm_act<S, NPROD, GRAD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
   FC_LAUNCH_CHECK();
   return 0;
 }
 // 256 x 256 tiles once they fill half of the chip, 128 x 128 below, 32 x 64 for a few rows.  Backward: 256 x 256 only where the product is long;
 // the epilogue (8 bytes a unit in, 6 out) stands still while it runs, and two 128 x 128 workgroups a CU cover each other's (12608 x 384 x 1024:
-// 50 us against 70; 8192 x 4096 x 11000 the other way, TIME_MID against 1333)
+// 50 us against 70; 8192 x 4096 x 11000 the other way, 1571 against 1333)
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
   if (a.T <= 32) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
   if constexpr (NPROD == 6) {

@@ -308,10 +308,12 @@ template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, h
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.nv + S::TN - 1) / S::TN);
   FC_REQUIRE(tiles < (1L << 31), "linear_ce: too many tiles");
   if (GRAD) {
-    FC_TRY(ft_allow_lds((const void*)k_ce_grad<S, NPROD>, S::LDS));
+    static FtLds lds;
+    FC_TRY(lds.allow((const void*)k_ce_grad<S, NPROD>, S::LDS));
     hipLaunchKernelGGL((k_ce_grad<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
   } else {
-    FC_TRY(ft_allow_lds((const void*)k_ce_stats<S, NPROD>, S::LDS));
+    static FtLds lds;
+    FC_TRY(lds.allow((const void*)k_ce_stats<S, NPROD>, S::LDS));
     hipLaunchKernelGGL((k_ce_stats<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
   }
   FC_LAUNCH_CHECK();

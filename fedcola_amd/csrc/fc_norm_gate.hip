@@ -408,7 +408,8 @@ template <typename T, bool BWD> static int ng_launch(const NgArgs& a, int dt, hi
   do {                                                                                                             \
     if constexpr (BWD) {                                                                                                  \
       const int lds = (W == 1 ? 4 * NG_SUMS : NG_VECS) * ((a.D + 7) & ~7) * 4;                                     \
-      FC_TRY(ft_allow_lds((const void*)k_ng_bwd<T, VEC, W, E>, (W == 1 ? 4 * NG_SUMS * 512 : NG_VECS * 8192) * 4)); \
+      static FtLds allowed;                                                                                        \
+      FC_TRY(allowed.allow((const void*)k_ng_bwd<T, VEC, W, E>, (W == 1 ? 4 * NG_SUMS * 512 : NG_VECS * 8192) * 4)); \
       hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), lds, s, a);                        \
     }                                                                                                              \
     if constexpr (!BWD) hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                       \

@@ -14,6 +14,8 @@
 // TR [64 k][W cols], 32-B unit u of row k at unit u ^ (((k >> 3) & 1) << 2 | (k & 3)), read by ds_read_b64_tr_b16.
 // The MFMA's operands are swapped, so a lane's accumulator acc[i][j] is row 16 i + (lane & 15), columns 16 j + 4 (lane >> 4) .. + 3.
 #pragma once
+#include <atomic>
+
 #include "fc_common.h"
 
 typedef __attribute__((ext_vector_type(8))) short ft_b8;
@@ -446,7 +448,7 @@ __host__ __device__ static inline int ft_slices(long tiles, long K, int target, 
   long s = target / tiles;
   const long most = nprod == 1 ? (K + 63) / 64 / 4 : (K + 63) / 64;
   s = s < most ? s : most;
-  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+  return s < 1 ? 1 : s > 32 ? 32 : (int)s;
 }
 size_t ft_part_floats(long M, long N, const FtPlan& plan);     // for any number of rows up to M
 // partial sums [slices][rows there][ft_part_ld(N)] into `part` (or, part null, the product into p.out); add: onto what is there
@@ -493,7 +495,18 @@ struct FtPacks {                  // up to four of one type in one launch
 int ft_pack(const FtPacks& p, hipStream_t s);
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
 static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }
-// > 64 KB of LDS for a kernel, once for each device
-int ft_allow_lds(const void* kernel, int bytes);
+// > 64 KB of LDS for a kernel: asked for once on each device (a static of the launch that needs it)
+struct FtLds {
+  std::atomic<unsigned long long> done{0};      // a bit for each of the first 64 devices
+  int allow(const void* kernel, int bytes) {
+    int dev = 0;
+    FC_CHECK_HIP(hipGetDevice(&dev));
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    FC_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+  }
+};
 // the device that holds p has to be the current one
 int ft_check_device(const void* p, const char* what);

@@ -2,23 +2,6 @@
 // of operands that the tile loads cannot take as they are.
 #include "fc_tiles.h"
 
-#include <atomic>
-#include <mutex>
-#include <set>
-#include <utility>
-
-int ft_allow_lds(const void* kernel, int bytes) {
-  static std::mutex mu;
-  static std::set<std::pair<int, const void*>>* done = new std::set<std::pair<int, const void*>>;
-  int dev = 0;
-  FC_CHECK_HIP(hipGetDevice(&dev));
-  std::lock_guard<std::mutex> l(mu);
-  if (done->count({dev, kernel})) return 0;
-  FC_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done->insert({dev, kernel});
-  return 0;
-}
-
 int ft_check_device(const void* p, const char* what) {
   hipPointerAttribute_t at;
   int cur = 0;
@@ -183,7 +166,7 @@ FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_r
   for (int sh = 0; sh < 4; ++sh) {
     if (sh == 2 ? am != TK || bm != TK || M > 64 : (sh == 3) != (nprod == 6)) continue;
     const long tiles = ((M + kTM[sh] - 1) / kTM[sh]) * ((N + kTN[sh] - 1) / kTN[sh]), nk = (K + 63) / 64;
-    for (int want = 1; want <= 64; ++want) {
+    for (int want = 1; want <= 32; ++want) {
       const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want), nprod);
       const long per = (nk + sp - 1) / sp, wg = tiles * sp, slots = kCost[sh].slots;
       const double rounds = wg <= 4 * slots ? (double)((wg + slots - 1) / slots) : (double)wg / slots + 0.5;
@@ -219,7 +202,8 @@ static int launch(const FtProduct& p, const FtPlan& pl, float* part, bool add, h
   const long n = workgroups(p, pl, part != nullptr);
   FC_REQUIRE(n < (1L << 31), "product of %d x %d: too many tiles", p.M, p.N);
   if (n == 0) return 0;
-  FC_TRY(ft_allow_lds((const void*)k_ft_product<S, AM, BMO, NPROD>, S::LDS));
+  static FtLds lds;
+  FC_TRY(lds.allow((const void*)k_ft_product<S, AM, BMO, NPROD>, S::LDS));
   hipLaunchKernelGGL((k_ft_product<S, AM, BMO, NPROD>), dim3((unsigned)n), dim3(S::NT), S::LDS, s, p, part, part ? pl.target : 0, add ? 1 : 0);
   FC_LAUNCH_CHECK();
   return 0;
@@ -302,7 +286,7 @@ int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const i
 
 // ---------------------------------------------------------------- products that wait for nothing of each other
 // One launch of 128 x 128 tiles while the chip would run less than about 160 k-steps of them: launches of 100 to 500 workgroups one after
-// the other leave part of it idle each (12608 x 384 x 1024, three products: TIME_SEP us apart, TIME_GRP together).  Above, tiles of 256 x 256
+// the other leave part of it idle each (12608 x 384 x 1024, three products and their sums: 109 us apart, 80 together).  Above, tiles of 256 x 256
 // in launches of their own are faster.  Slices: of about half of a slot's share of the work, so that what is long and what is short packs well.
 bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan) {
   const int sh = p[0].nprod == 1 ? 1 : 3, slots = kCost[sh].slots;
@@ -332,10 +316,12 @@ int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, 
   for (int i = n; i < 3; ++i) g.first[i + 1] = g.first[i];
   if (g.first[n] == 0) return 0;
   if (plan[0].shape == 1) {
-    FC_TRY(ft_allow_lds((const void*)k_ft_group<FtMid, 1>, FtMid::LDS));
+    static FtLds lds;
+    FC_TRY(lds.allow((const void*)k_ft_group<FtMid, 1>, FtMid::LDS));
     hipLaunchKernelGGL((k_ft_group<FtMid, 1>), dim3(g.first[n]), dim3(FtMid::NT), FtMid::LDS, s, g);
   } else {
-    FC_TRY(ft_allow_lds((const void*)k_ft_group<FtPlanes, 6>, FtPlanes::LDS));
+    static FtLds lds;
+    FC_TRY(lds.allow((const void*)k_ft_group<FtPlanes, 6>, FtPlanes::LDS));
     hipLaunchKernelGGL((k_ft_group<FtPlanes, 6>), dim3(g.first[n]), dim3(FtPlanes::NT), FtPlanes::LDS, s, g);
   }
   FC_LAUNCH_CHECK();

@@ -426,3 +426,58 @@ def test_operator_refusals_on_the_device():
                 lambda: blocks.norm_gate_residual_forward(torch.ones(2, 8193, device="cuda"), torch.ones(2, 8193, device="cuda"))):
         with pytest.raises(ValueError):
             bad()
+
+
+# ------------------------------------------------------------------------------------------------ offsets past 32 bits
+def test_offsets_past_32_bits_in_the_vocabulary():
+    """a weight of 4.9 GB, zeros but for three rows: everything has a closed form"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    V, D, T = 1_200_000, 2048, 5
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    hot = torch.tensor([0, V // 2 + 1, V - 1], device="cuda")
+    w[hot] = rnd(gen(0), 3, D, scale=0.2).bfloat16()
+    x = rnd(gen(1), T, D).bfloat16()
+    y = torch.tensor([V - 1, 0, V // 2 + 1, 77, V - 2], device="cuda")
+    loss, saved = linear_cross_entropy_forward(x, w, y, reduction="sum")
+    dx, dw = linear_cross_entropy_backward(torch.tensor(1.0, device="cuda"), saved, w)
+    wide = torch.cat([w[hot].double(), torch.zeros(1, D, device="cuda", dtype=torch.float64)])
+    logits = x.double() @ wide.t()
+    lse = torch.log(torch.exp(logits[:, :3]).sum(1) + (V - 3))
+    at = torch.tensor([2, 0, 1, 3, 3], device="cuda")
+    rows = lse - logits.gather(1, at[:, None])[:, 0]
+    assert abs(loss.double() - rows.sum()) <= 1e-6 * rows.sum()
+    p = torch.exp(logits - lse[:, None])
+    # two roundings of u; a logit of 2048 products of about 0.13 each is off by at most (64 + 32) 2^-24 x 270 = 1.6e-3 (64 accumulations of 32
+    # products), and so are lse and, twice, p
+    tol = 1.1 * (2 * O.half_step(torch.bfloat16) + 4e-3)
+    for k, v in enumerate(hot.tolist()):
+        d = p[:, k] - (y == v).double()
+        want = d @ x.double()
+        within(dw[v], want, tol * (d.abs() @ x.double().abs()), f"dw row {v}")
+    for v in (1, V // 2, V - 3):                                              # rows that nothing points at: 1 / V each
+        d = p[:, 3]
+        within(dw[v], d @ x.double(), tol * (d.abs() @ x.double().abs()), f"dw row {v}")
+    d = p[:, :3] - (y[:, None] == hot).double()
+    within(dx, d @ wide[:3], tol * (d.abs() @ wide[:3].abs()), "dx")
+
+
+def test_offsets_past_32_bits_in_the_rows():
+    """more than 4 GB of rows: the first, the last and some in between against the same rows alone"""
+    from fedcola_amd.blocks import gated_mlp_backward, gated_mlp_forward, norm_gate_residual_backward, norm_gate_residual_forward
+    T, D = 1_100_000, 2048
+    x = torch.empty(T, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen(0))
+    some = torch.tensor([0, 1, 524_288, 1_048_575, 1_048_577, T - 2, T - 1], device="cuda")
+    wi, wo = rnd(gen(1), 32, D, scale=0.02).bfloat16(), rnd(gen(2), D, 16, scale=0.2).bfloat16()
+    y = gated_mlp_forward(x, wi, wo)
+    dx, _, _ = gated_mlp_backward(x, x, wi, wo, need=(True, False, False))
+    want, bound = O.gated_mlp(x[some], wi, wo, x[some], "silu", torch.bfloat16)
+    within(y[some], want["y"], bound["y"], "y")
+    within(dx[some], want["dx"], bound["dx"], "dx")
+    del y, dx
+    v = dict(post_weight=torch.ones(D, device="cuda"), gate=rnd(gen(3), D), pre_weight=torch.ones(D, device="cuda"), norm="rms")
+    r, h = norm_gate_residual_forward(x, x, **v)
+    d = norm_gate_residual_backward(x, x, x, x, weight_grads=False, **v)
+    one = x[some][None]
+    want, bound = O.norm_gate(one, one, torch.bfloat16, **v, d_residual=one, d_normed=one)
+    for got, k in ((r, "r"), (h, "h"), (d["branch"], "branch"), (d["residual"], "residual")):
+        within(got[some][None], want[k], bound[k], k)
