@@ -172,27 +172,12 @@ struct NgSample {
   }
 };
 
-enum { NG_WP = 0, NG_BP, NG_GT, NG_WN, NG_BN, NG_VECS };
-// the weight vectors of a workgroup's rows in LDS, [NG_VECS][D in whole eights]: they do not fit the registers beside the next row's loads
-template <int NT> __device__ __forceinline__ void ng_vectors(const NgArgs& a, float* vec, unsigned grp, int count) {
-  const int D = a.D, Dp = (D + 7) & ~7;
-  for (int c = threadIdx.x; c < Dp; c += NT) {
-    const bool in = c < D;
-    vec[NG_WP * Dp + c] = in && a.wp ? a.wp[c] : 0.f;
-    vec[NG_BP * Dp + c] = in && a.bp ? a.bp[c] : 0.f;
-    vec[NG_GT * Dp + c] = in ? (a.gate ? a.gate[(long)grp * D + c] : 1.f) : 0.f;
-    vec[NG_WN * Dp + c] = in && a.wn ? a.wn[c] : 0.f;
-    if (count > NG_BN) vec[NG_BN * Dp + c] = in && a.bn ? a.bn[c] : 0.f;
-  }
-}
-
 template <typename T, int VEC, int W, int E>
 __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
   constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;       // rows at once
-  extern __shared__ __attribute__((aligned(16))) float vec[];
   __shared__ float2 red[2 * W];
   NgSum<W> sum{red};
-  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D, Dp = (D + 7) & ~7;
+  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D;
   const unsigned grp = blockIdx.x / (unsigned)a.blocks;
   const long b0 = (long)(blockIdx.x - grp * (unsigned)a.blocks) * a.per, first = (long)grp * a.gate_rows + b0, left = a.gate_rows - b0;
   const int n = (int)(left < a.per ? left : a.per);
@@ -206,67 +191,42 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
     rx.load((const T*)a.x + row * a.ldx, l, D);
   };
   if (sub < n) fetch(sub);
-  constexpr bool REGS = W == 8 || E == 8;                // (five vectors of a row of eight waves do not fit the LDS)
-  float v[REGS ? NG_VECS : 1][E];
-  if constexpr (REGS) {
-    ng_load<float, VEC, NTH, E>(a.wp, l, D, v[NG_WP]);
-    ng_load<float, VEC, NTH, E>(a.bp, l, D, v[NG_BP]);
-    ng_load<float, VEC, NTH, E>(a.wn, l, D, v[NG_WN]);
-    ng_load<float, VEC, NTH, E>(a.bn, l, D, v[NG_BN]);
-    ng_load<float, VEC, NTH, E>(a.gate ? a.gate + (long)grp * D : nullptr, l, D, v[NG_GT]);
-    if (!a.gate)
-#pragma unroll
-      for (int k = 0; k < E; ++k) v[NG_GT][k] = 1.f;
-  } else {
-    ng_vectors<256>(a, vec, grp, NG_VECS);
-    __syncthreads();
-  }
-  auto get = [&](int q, float (&w)[E]) {
-    if constexpr (REGS) {
-#pragma unroll
-      for (int k = 0; k < E; ++k) w[k] = v[q][k];
-    } else {
-      asm volatile("" ::: "memory");                     // read again for every row: hoisted out of the loop they take the registers they are to save
-      ng_load<float, VEC, NTH, E>(vec + q * Dp, l, D, w);
-    }
-  };
+  float wp[E], bp[E], gt[E], wn[E], bn[E];
+  ng_load<float, VEC, NTH, E>(a.wp, l, D, wp);
+  ng_load<float, VEC, NTH, E>(a.bp, l, D, bp);
+  ng_load<float, VEC, NTH, E>(a.gate ? a.gate + (long)grp * D : nullptr, l, D, gt);
+  ng_load<float, VEC, NTH, E>(a.wn, l, D, wn);
+  ng_load<float, VEC, NTH, E>(a.bn, l, D, bn);
   for (int i = sub; i < n; i += RB) {
     const long row = first + i;
-    float y[E], x[E], w[E];
+    float y[E], x[E];
     s = ng_uniform(snext);
     ry.get(y, l, D, s != 0.f);
     rx.get(x, l, D, true);
     fetch(i + RB);
     if (a.post) {
       ng_norm<VEC, NTH, E>(y, l, D, a.rms, a.eps, sum);
-      get(NG_WP, w);
 #pragma unroll
-      for (int k = 0; k < E; ++k) y[k] *= w[k];
-      get(NG_BP, w);
-#pragma unroll
-      for (int k = 0; k < E; ++k) y[k] += w[k];
+      for (int k = 0; k < E; ++k) y[k] = y[k] * wp[k] + bp[k];
     }
-    get(NG_GT, w);
 #pragma unroll
-    for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + s * (w[k] * y[k]);
+    for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + s * (a.gate ? gt[k] * y[k] : y[k]);
     ng_store<T, VEC, NTH, E>((T*)a.r + row * D, l, D, x);
     if (a.pre) {
       ng_norm<VEC, NTH, E>(x, l, D, a.rms, a.eps, sum);
-      get(NG_WN, w);
 #pragma unroll
-      for (int k = 0; k < E; ++k) x[k] *= w[k];
-      get(NG_BN, w);
-#pragma unroll
-      for (int k = 0; k < E; ++k) x[k] += w[k];
+      for (int k = 0; k < E; ++k) x[k] = x[k] * wn[k] + bn[k];
       ng_store<T, VEC, NTH, E>((T*)a.h + row * D, l, D, x);
     }
   }
 }
 
+// The weight vectors stand in LDS here: with the five running sums and the next row's loads they do not fit the registers.
+enum { NG_WP = 0, NG_BP, NG_GT, NG_WN, NG_VECS };
 template <typename T, int VEC, int W, int E>
 __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 && VEC == 8 ? 4 : 3) : 2) k_ng_bwd(NgArgs a) {
   constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;
-  extern __shared__ __attribute__((aligned(16))) float vec[];   // the vectors but the last, then for W = 1 [4][NG_SUMS][Dp] over them
+  extern __shared__ __attribute__((aligned(16))) float vec[];   // [NG_VECS][Dp], then for W = 1 [4][NG_SUMS][Dp] over them
   __shared__ float2 red[2 * W];
   NgSum<W> sum{red};
   const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D, Dp = (D + 7) & ~7;
@@ -286,7 +246,13 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 &
     rh.load(a.dh ? (const T*)a.dh + row * a.lddh : (const T*)a.x + row * a.ldx, l, D);
   };
   if (sub < n) fetch(sub);
-  ng_vectors<W == 8 ? 512 : 256>(a, vec, grp, NG_BN);
+  for (int c = threadIdx.x; c < Dp; c += W == 8 ? 512 : 256) {
+    const bool in = c < D;
+    vec[NG_WP * Dp + c] = in && a.wp ? a.wp[c] : 0.f;
+    vec[NG_BP * Dp + c] = in && a.bp ? a.bp[c] : 0.f;
+    vec[NG_GT * Dp + c] = in ? (a.gate ? a.gate[(long)grp * D + c] : 1.f) : 0.f;
+    vec[NG_WN * Dp + c] = in && a.wn ? a.wn[c] : 0.f;
+  }
   float sums[NG_SUMS][E];
 #pragma unroll
   for (int q = 0; q < NG_SUMS; ++q)
@@ -414,7 +380,7 @@ __global__ void __launch_bounds__(1024) k_ng_sum(const float* part, int D, long 
 
 // ---------------------------------------------------------------- host
 // Waves of a row and values of a lane.  A wave alone needs no barriers for its sums, so one takes a row as long as 16 values a lane are enough
-// (12608 x 768 bf16: NEWF and NEWB us forward and backward; four waves of 8 values: 65 and 100); above, backward 16 values leave two workgroups a
+// (12608 x 768 bf16: 14 and 40 us forward and backward, of four waves of 8 values about 80 and 90); above, backward 16 values leave two workgroups a
 // CU instead of one of twice the waves (65536 x 4096 bf16: 667 us against 1151), forward 8 are as good.
 static void ng_form(long D, bool bwd, int& W, int& E) {
   W = D <= 1024 ? 1 : D <= 2048 || (bwd && D <= 4096) ? 4 : 8;
@@ -434,7 +400,7 @@ static int ng_deep(long D, bool bwd, int dt) {
   int W, E;
   ng_form(D, bwd, W, E);
   if (bwd) return E == 16 ? 2 : dt ? 4 : 3;
-  return W == 8 ? (E == 16 ? 2 : 4) : E == 16 ? 4 : 5;
+  return W == 8 ? (E == 16 ? 2 : 4) : E == 16 ? 3 : 5;
 }
 static bool ng_aligned(const NgArgs& a, int dt) {
   size_t p = (size_t)a.y | (size_t)a.x | (size_t)a.dr | (size_t)a.dh | (size_t)a.r | (size_t)a.h | (size_t)a.dy | (size_t)a.dx | (size_t)a.wp | (size_t)a.bp |
@@ -445,16 +411,16 @@ static bool ng_aligned(const NgArgs& a, int dt) {
 template <typename T, bool BWD> static int ng_launch(const NgArgs& a, int dt, hipStream_t s) {
   const dim3 g((unsigned)(a.T / a.gate_rows * a.blocks));
   const bool v = ng_aligned(a, dt);
-#define NG_RUN(VEC, W, E)                                                                                            \
-  do {                                                                                                               \
-    static FtLds allowed;                                                                                            \
-    const int row = ((a.D + 7) & ~7) * 4, most = W * 64 * E * 4;                                                     \
-    constexpr int rows = BWD ? (W == 1 ? 4 * NG_SUMS : NG_BN) : W == 8 || E == 8 ? 0 : NG_VECS;                                             \
-    const void* k;                                                                                                   \
-    if constexpr (BWD) k = (const void*)k_ng_bwd<T, VEC, W, E>; else k = (const void*)k_ng_fwd<T, VEC, W, E>;        \
-    FC_TRY(allowed.allow(k, rows * most));                                                                           \
-    if constexpr (BWD) hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), rows * row, s, a);  \
-    else hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), rows * row, s, a);                \
+#define NG_RUN(VEC, W, E)                                                                                             \
+  do {                                                                                                                \
+    if constexpr (BWD) {                                                                                              \
+      static FtLds allowed;                                                                                           \
+      constexpr int rows = W == 1 ? 4 * NG_SUMS : NG_VECS;                                                            \
+      FC_TRY(allowed.allow((const void*)k_ng_bwd<T, VEC, W, E>, rows * W * 64 * E * 4));                              \
+      hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), rows * ((a.D + 7) & ~7) * 4, s, a);   \
+    } else {                                                                                                          \
+      hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                             \
+    }                                                                                                                 \
   } while (0)
 #define NG_PICK(W, E) do { if (v) NG_RUN(8, W, E); else NG_RUN(1, W, E); } while (0)
   int W, E;
