@@ -167,7 +167,7 @@ template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& 
 // the epilogue (8 bytes a unit in, 6 out) stands still while it runs, and two 128 x 128 workgroups a CU cover each other's (12608 x 384 x 1024:
 // 50 us against 70; 8192 x 4096 x 11000 the other way, 1571 against 1333)
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
-  if (a.T <= 32) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
+  if (a.T <= 64) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
   if constexpr (NPROD == 6) {
     return gm_act_launch<GmPlanes, NPROD, GRAD>(a, s);
   } else {

@@ -299,7 +299,7 @@ typedef FtShape<32, 64, 2, 2, 6> CeRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
 // 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32, 32 x 64 for the few rows of a scoring call
 static int ce_shape(int dt, long T, long V) {
-  if (T <= 32) return 2;
+  if (T <= 64) return 2;
   return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
