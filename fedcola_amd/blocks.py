@@ -32,12 +32,18 @@ def _mlp_operands(x, w_in, w_out, act):
     return code, dev, as_rows(x), as_rows(w_in), as_rows(w_out)
 
 
+def _packed(T, F, w_in, w_out, *rows):
+    if w_in[0].element_size() == 4:             # x and dy are laid out in planes anyway; the up rows are reached from the gate rows
+        return not (in_place(*w_in, T) and in_place(*w_out, T) and (F + 512) * w_in[1] < 1 << 29)
+    return not all(in_place(t, ld, T) for t, ld in (w_in, w_out, *rows))
+
+
 def gated_mlp_forward(x, w_in, w_out, act="silu"):
     """y = (act(x wg^T) * (x wu^T)) w_out^T.  x [..., D]; w_in [2F, D]: wg over wu; w_out [D, F]; one type, bf16 or fp32.  act: "silu", "gelu" (erf)."""
     code, dev, (x2, ldx), (wi, ldi), (wo, ldo) = _mlp_operands(x, w_in, w_out, act)
     T, D, F, L = x2.shape[0], wi.shape[1], wo.shape[1], _lib.lib()
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    packed = not (in_place(x2, ldx) and in_place(wi, ldi) and in_place(wo, ldo))
+    packed = _packed(T, F, (wi, ldi), (wo, ldo), (x2, ldx))
     with on_device(dev) as stream:
         ws = torch.empty(L.fc_gated_mlp_workspace_bytes(code, T, D, F, packed, 0), dtype=torch.uint8, device=dev)
         check(L.fc_gated_mlp_fwd(code, _ACTS[act], x2.data_ptr(), ldx, wi.data_ptr(), ldi, wo.data_ptr(), ldo, T, D, F, y.data_ptr(), D, ws.data_ptr(),
@@ -56,7 +62,7 @@ def gated_mlp_backward(dy, x, w_in, w_out, act="silu", need=(True, True, True)):
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
     dwi = torch.empty(2 * F, D, dtype=x.dtype, device=dev) if need[1] else None
     dwo = torch.empty(D, F, dtype=x.dtype, device=dev) if need[2] else None
-    packed = not (in_place(x2, ldx) and in_place(dy2, ldy) and in_place(wi, ldi) and in_place(wo, ldo))
+    packed = _packed(T, F, (wi, ldi), (wo, ldo), (x2, ldx), (dy2, ldy))
     with on_device(dev) as stream:
         ws = torch.empty(L.fc_gated_mlp_workspace_bytes(code, T, D, F, packed, 1), dtype=torch.uint8, device=dev)
         check(L.fc_gated_mlp_bwd(code, _ACTS[act], dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wi.data_ptr(), ldi, wo.data_ptr(), ldo, T, D, F, address(dx), D,

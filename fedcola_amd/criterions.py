@@ -97,7 +97,7 @@ def linear_cross_entropy_forward(hidden, weight, targets, ignore_index=-100, red
     loss = torch.empty(targets.shape if red == 0 else (), device=dev)
     with on_device(dev) as stream:
         saved = torch.empty(L.fc_linear_ce_saved_bytes(code, T, D), dtype=torch.uint8, device=dev)
-        ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw), 0), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw, T), 0), dtype=torch.uint8, device=dev)
         check(L.fc_linear_ce_fwd(code, x.data_ptr(), ldx, w.data_ptr(), ldw, y.data_ptr(), T, V, D, ignore_index, red, loss.data_ptr(), saved.data_ptr(),
                                  saved.numel(), ws.data_ptr(), ws.numel(), stream))
     return loss, (saved, hidden.shape, red)
@@ -115,7 +115,7 @@ def linear_cross_entropy_backward(gloss, saved, weight, need_hidden=True, need_w
     dx = torch.empty(shape, dtype=weight.dtype, device=dev) if need_hidden else None
     dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if need_weight else None
     with on_device(dev) as stream:
-        ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw), 1), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw, T), 1), dtype=torch.uint8, device=dev)
         check(L.fc_linear_ce_bwd(code, w.data_ptr(), ldw, T, V, D, red, g.data_ptr(), saved.data_ptr(), saved.numel(), address(dx), D, address(dw), D,
                                  ws.data_ptr(), ws.numel(), stream))
     return dx, dw

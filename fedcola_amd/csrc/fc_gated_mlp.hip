@@ -18,6 +18,7 @@
 struct GmArgs {
   FtMat x, w_in, w_out, dy;
   int T, D, F, act;
+  bool rows32;                  // fp32, few rows: w_in and w_out are the fp32 matrices themselves
   long up;                      // rows between a unit's gate and up row in w_in
   bf16_t *h, *dgu;              // planes of [T][ldh], [T][2 ldh]: h; dg | du
   long ldh;                     // whole 128-byte lines: a row that straddles one more costs every tile load an L2 request more
@@ -153,6 +154,7 @@ typedef FtShape<256, 256, 2, 4, 2> GmBig;
 typedef FtShape<128, 128, 2, 2, 2> GmMid;
 typedef FtShape<32, 64, 2, 2, 6> GmRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> GmPlanes;
+typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> GmRows32;
 
 template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));
@@ -167,18 +169,21 @@ template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& 
 // the epilogue (8 bytes a unit in, 6 out) stands still while it runs, and two 128 x 128 workgroups a CU cover each other's (12608 x 384 x 1024:
 // 50 us against 70; 8192 x 4096 x 11000 the other way, 1571 against 1333)
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
-  if (a.T <= 64) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
   if constexpr (NPROD == 6) {
-    return gm_act_launch<GmPlanes, NPROD, GRAD>(a, s);
+    return a.rows32 ? gm_act_launch<GmRows32, NPROD, GRAD>(a, s) : gm_act_launch<GmPlanes, NPROD, GRAD>(a, s);
   } else {
+    if (a.T <= 64) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
     if ((long)((a.T + 255) / 256) * ((a.F + 127) / 128) >= 128 && (!GRAD || a.D >= 1024)) return gm_act_launch<GmBig, NPROD, GRAD>(a, s);
     return gm_act_launch<GmMid, NPROD, GRAD>(a, s);
   }
 }
 
+// fp32, few rows: the weights are read where they are, or from a copy in 32 bits, and split in registers
+static bool gm_rows32(int dt, long T, long D, long F) { return !dt && T <= FT_ROWS32 && (F + 512) * ft_up(D, 64) < (1L << 29); }
 struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan[3]; bool group; };
 // dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
 static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProduct (&p)[3]) {
+  p[0].rows32 = a.rows32;
   const long Fp = ft_up(F, 64);
   for (FtProduct& q : p) { q.am = TR; q.bm = TR; q.nprod = dt ? 1 : 6; q.K = (int)T; }
   p[0].am = TK;
@@ -195,31 +200,43 @@ static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProdu
   p[2].a = a.dy;
   p[2].b.p = a.h; p[2].b.ld = Fp; p[2].b.plane = T * Fp;
 }
+static FtProduct gm_y_product(int dt, long T, long D, long F, bool rows32) {
+  FtProduct p;
+  p.nprod = dt ? 1 : 6;
+  p.rows32 = rows32;
+  p.M = (int)T; p.N = (int)D; p.K = (int)F;
+  return p;
+}
 static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backward) {
   GmSizes z = {};
   const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6;
-  const int np = dt ? 1 : 6;
-  if (packed) {
+  const bool r32 = gm_rows32(dt, T, D, F);
+  if (packed || !dt) {
     z.x = ft_up(T * Dp * e, 256);
-    z.w_in = ft_up(2 * F * Dp * e, 256);
-    z.w_out = ft_up(D * Fp * e, 256);
     z.dy = backward ? z.x : 0;
+  }
+  if (packed) {
+    const long we = r32 ? 4 : e;
+    z.w_in = ft_up(2 * F * Dp * we, 256);
+    z.w_out = ft_up(D * Fp * we, 256);
   }
   z.h = ft_up(T * Fp * e, 256);
   if (!backward) {
-    z.part = ft_product_part_floats(TK, TK, np, T, D, F) * 4;
+    z.part = ft_product_part_floats(gm_y_product(dt, T, D, F, r32)) * 4;
     return z;
   }
   z.dgu = ft_up(T * 2 * Fp * e, 256);
   z.dh = ft_up(ft_part_ld(F) * T * 4, 256);
   FtProduct p[3];
-  gm_products(dt, T, D, F, GmArgs(), p);
+  GmArgs a = {};
+  a.rows32 = r32;
+  gm_products(dt, T, D, F, a, p);
   z.group = ft_group_plan(p, 3, z.plan);
   for (int i = 0; i < 3; ++i) {
     if (z.group) {
       z.part += z.plan[i].target ? ft_up(ft_part_floats(p[i].M, p[i].N, z.plan[i]) * 4, 256) : 0;
     } else {
-      const size_t n = ft_product_part_floats(p[i].am, p[i].bm, np, p[i].M, p[i].N, (long)p[i].K * p[i].segs) * 4;
+      const size_t n = ft_product_part_floats(p[i]) * 4;
       z.part = z.part > n ? z.part : n;
     }
   }
@@ -227,17 +244,19 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backwa
 }
 static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.dh + z.part; }
 
-// a matrix as the products take it: where it is, or as one of the packs
-static void gm_matrix(int dt, const void* p, long ld, long R, long C, char*& ws, FtMat& m, FtPacks& l) {
-  if (ft_direct(dt, p, ld, C)) {
+// a matrix as the products take it: where it is, or as one of the packs.  whole: an fp32 one that is not split into planes.
+static bool gm_whole(const void* p, long ld, long R, long C) { return ft_direct32(p, ld, C) && (R + 512) * ld < (1L << 29); }
+static void gm_matrix(int dt, bool whole, bool direct, const void* p, long ld, long R, long C, char*& ws, FtMat& m, FtPacks& l) {
+  const int units = whole ? 2 : 1;
+  if (direct) {
     m.p = (const bf16_t*)p;
-    m.ld = ld;
+    m.ld = units * ld;
     return;
   }
   FtPack k;
-  k.src = p; k.lds = ld; k.dt = dt; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 64);
-  m.p = k.dst; m.ld = k.ldd; m.plane = R * k.ldd;
-  ws += ft_up((dt ? 1 : 3) * R * k.ldd * 2, 256);
+  k.src = p; k.lds = ld; k.dt = dt; k.whole = whole; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 64);
+  m.p = k.dst; m.ld = units * k.ldd; m.plane = R * k.ldd;
+  ws += ft_up((dt ? 2 : whole ? 4 : 6) * R * k.ldd, 256);
   l.add(k);
 }
 struct GmCall { int dt, act; long T, D, F; const void *x, *w_in, *w_out, *dy; long ldx, ld_in, ld_out, lddy; };
@@ -253,31 +272,40 @@ static int gm_check(const char* what, const GmCall& c, const void* ws) {
   FC_REQUIRE(((size_t)ws & 255) == 0, "%s: the workspace is aligned to 256 bytes", what);
   return ft_check_device(c.w_in, what);
 }
-static bool gm_direct(const GmCall& c) {
-  return ft_direct(c.dt, c.x, c.ldx, c.D) && ft_direct(c.dt, c.w_in, c.ld_in, c.D) && ft_direct(c.dt, c.w_out, c.ld_out, c.F) &&
-         (!c.dy || ft_direct(c.dt, c.dy, c.lddy, c.D));
+// which of w_in and w_out is read where it is, and whether all operands of the type's are (fp32: the weights alone, x and dy become planes)
+static bool gm_direct(const GmCall& c, bool r32, bool& in, bool& out) {
+  in = r32 ? gm_whole(c.w_in, c.ld_in, c.F, c.D) : ft_direct(c.dt, c.w_in, c.ld_in, c.D);
+  out = r32 ? gm_whole(c.w_out, c.ld_out, 0, c.F) : ft_direct(c.dt, c.w_out, c.ld_out, c.F);
+  return in && out && (!c.dt || (ft_direct(c.dt, c.x, c.ldx, c.D) && (!c.dy || ft_direct(c.dt, c.dy, c.lddy, c.D))));
 }
 // the operands as the products take them; what of them cannot be taken as it is goes to the workspace
 static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
+  bool in, out;
+  a.rows32 = gm_rows32(c.dt, c.T, c.D, c.F);
+  gm_direct(c, a.rows32, in, out);
   a.T = (int)c.T; a.D = (int)c.D; a.F = (int)c.F; a.act = c.act; a.up = c.F; a.ldh = ft_up(c.F, 64);
   FtPacks l;
-  gm_matrix(c.dt, c.x, c.ldx, c.T, c.D, ws, a.x, l);
-  if (c.dy) gm_matrix(c.dt, c.dy, c.lddy, c.T, c.D, ws, a.dy, l);
-  gm_matrix(c.dt, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
-  gm_matrix(c.dt, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
+  gm_matrix(c.dt, false, ft_direct(c.dt, c.x, c.ldx, c.D), c.x, c.ldx, c.T, c.D, ws, a.x, l);
+  if (c.dy) gm_matrix(c.dt, false, ft_direct(c.dt, c.dy, c.lddy, c.D), c.dy, c.lddy, c.T, c.D, ws, a.dy, l);
+  gm_matrix(c.dt, a.rows32, out, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
+  gm_matrix(c.dt, a.rows32, in, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
   return ft_pack(l, s);
+}
+static GmSizes gm_call_sizes(const GmCall& c, bool backward) {
+  bool in, out;
+  return gm_sizes(c.dt, c.T, c.D, c.F, !gm_direct(c, gm_rows32(c.dt, c.T, c.D, c.F), in, out), backward);
 }
 
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
   if (T < 0 || D < 1 || F < 1) return 0;
-  return gm_total(gm_sizes(dt, T, D, F, !dt || packed || F % 8 || D % 8, backward != 0)) + 256;
+  return gm_total(gm_sizes(dt, T, D, F, packed || (!dt && !gm_rows32(dt, T, D, F)), backward != 0)) + 256;
 }
 extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t ldx, const void* w_in, int64_t ld_in, const void* w_out, int64_t ld_out,
                                 int32_t T, int32_t D, int32_t F, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   GmCall c = {dt, act, T, D, F, x, w_in, w_out, nullptr, ldx, ld_in, ld_out, 0};
   FC_TRY(gm_check("fc_gated_mlp_fwd", c, workspace));
   FC_REQUIRE((y || T == 0) && ldy >= D, "fc_gated_mlp_fwd: output missing or its rows %ld apart", (long)ldy);
-  const GmSizes z = gm_sizes(dt, T, D, F, !gm_direct(c), false);
+  const GmSizes z = gm_call_sizes(c, false);
   FC_REQUIRE(workspace_bytes >= gm_total(z), "fc_gated_mlp_fwd: workspace too small");
   if (T == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
@@ -287,11 +315,10 @@ extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t 
   a.h = (bf16_t*)ws;
   ws += z.h;
   FC_TRY(dt ? (gm_act_run<1, false>(a, s)) : (gm_act_run<6, false>(a, s)));
-  FtProduct p;
-  p.nprod = dt ? 1 : 6;
+  FtProduct p = gm_y_product(dt, T, D, F, a.rows32);
   p.a.p = a.h; p.a.ld = a.ldh; p.a.plane = (long)T * a.ldh;
   p.b = a.w_out;
-  p.M = T; p.N = D; p.K = F; p.out = y; p.ldo = ldy;
+  p.out = y; p.ldo = ldy;
   return ft_product_out(p, (float*)ws, z.part / 4, s);
 }
 extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_in, int64_t ld_in,
@@ -301,7 +328,7 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   FC_TRY(gm_check("fc_gated_mlp_bwd", c, workspace));
   FC_REQUIRE((dy || T == 0) && lddy >= D && lddy < (1L << 21) && (!dx || lddx >= D) && (!dw_in || ldd_in >= D) && (!dw_out || ldd_out >= F),
              "fc_gated_mlp_bwd: dy missing, or rows too close");
-  const GmSizes z = gm_sizes(dt, T, D, F, !gm_direct(c), true);
+  const GmSizes z = gm_call_sizes(c, true);
   FC_REQUIRE(workspace_bytes >= gm_total(z), "fc_gated_mlp_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
@@ -315,11 +342,12 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   if (T) {
     FtProduct p;
     p.nprod = dt ? 1 : 6;
+    p.rows32 = a.rows32;
     p.am = TK; p.bm = TR;
     p.a = a.dy;
     p.b = a.w_out;
     p.M = T; p.N = F; p.K = D;
-    FtPlan plan = ft_plan(TK, TR, p.nprod, T, F, D, false);
+    FtPlan plan = ft_plan(p, false);
     plan.target = 0;                                           // one slice: its partial sums are dh
     FC_TRY(ft_product(p, plan, (float*)ws, false, s));
     a.dh = (const float*)ws;

@@ -297,9 +297,10 @@ typedef FtShape<256, 256, 2, 4, 2> CeBig;
 typedef FtShape<128, 128, 2, 2, 2> CeMid;
 typedef FtShape<32, 64, 2, 2, 6> CeRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
+typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> CeRows32;
 // 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32, 32 x 64 for the few rows of a scoring call
 static int ce_shape(int dt, long T, long V) {
-  if (T <= 64) return 2;
+  if (T <= FT_ROWS32) return 2;
   return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
@@ -322,7 +323,7 @@ template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, h
 template <bool GRAD> static int ce_run(int dt, int shape, const CeArgs& a, hipStream_t s) {
   if (a.T == 0 || a.nv == 0) return 0;
   if (dt) return shape == 0 ? ce_launch<CeBig, 1, GRAD>(a, s) : shape == 1 ? ce_launch<CeMid, 1, GRAD>(a, s) : ce_launch<CeRow, 1, GRAD>(a, s);
-  return shape == 1 ? ce_launch<CePlanes, 6, GRAD>(a, s) : ce_launch<CeRow, 6, GRAD>(a, s);
+  return shape == 1 ? ce_launch<CePlanes, 6, GRAD>(a, s) : ce_launch<CeRows32, 6, GRAD>(a, s);
 }
 
 // columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
@@ -333,13 +334,12 @@ static long ce_piece(int dt, long T, long V) {
 struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx, dw; bool group; };
 // dx = dL w and dw = dL^T x of nv columns; n: device, the rows that count
 static void ce_products(int dt, long T, long D, long nv, const int* n, FtProduct& x, FtProduct& w) {
-  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
+  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.rows32 = !dt && T <= FT_ROWS32; x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
   w.am = TR; w.bm = TR; w.nprod = x.nprod; w.M = (int)nv; w.N = (int)D; w.K = (int)T; w.Kdyn = n;
 }
 static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad) {
   CeSizes z = {};
-  const int np = dt ? 1 : 6;
-  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 1 : 3) * V * ft_up(D, 64) * 2, 256);
+  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : T <= FT_ROWS32 ? 4 : 6) * V * ft_up(D, 64), 256);
   if (!grad) {
     const int tn = ce_tn(ce_shape(dt, T, V));
     z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
@@ -361,13 +361,14 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
       return z;
     }
   }
-  z.dx = ft_plan(TK, TR, np, T, D, z.piece, true);
+  FtProduct px, pw;
+  ce_products(dt, T, D, z.piece, nullptr, px, pw);
+  z.dx = ft_plan(px, true);
   z.dxp = (size_t)ft_up(ft_part_floats(T, D, z.dx) * 4, 256);
-  z.dwp = (size_t)ft_up(ft_product_part_floats(TR, TR, np, z.piece < V ? z.piece : V, D, T) * 4, 256);
-  const long last = V % z.piece;
-  if (last) {
-    const size_t l = (size_t)ft_up(ft_product_part_floats(TR, TR, np, last, D, T) * 4, 256);
-    z.dwp = z.dwp > l ? z.dwp : l;
+  for (long nv : {z.piece < V ? z.piece : V, V % z.piece}) {
+    pw.M = (int)nv;
+    const size_t n = nv ? (size_t)ft_up(ft_product_part_floats(pw) * 4, 256) : 0;
+    z.dwp = z.dwp > n ? z.dwp : n;
   }
   return z;
 }
@@ -377,17 +378,20 @@ static int ce_args(const char* what, int dt, long T, long V, long D, long ldw, c
   FC_REQUIRE(w && ldw >= D && ldw < (1L << 21), "%s: weight missing or its rows %ld apart", what, ldw);
   return ft_check_device(w, what);
 }
-// the weight as the products take it
-static int ce_weight(int dt, const void* w, long ldw, long V, long D, char*& ws, FtMat& m, hipStream_t s) {
-  if (ft_direct(dt, w, ldw, D)) {
+// the weight as the products take it: where it is, or (few fp32 rows: in 32 bits) laid out in the workspace
+static bool ce_direct(int dt, const void* w, long ldw, long T, long D) { return dt || T > FT_ROWS32 ? ft_direct(dt, w, ldw, D) : ft_direct32(w, ldw, D); }
+static int ce_weight(int dt, const void* w, long ldw, long T, long V, long D, char*& ws, FtMat& m, hipStream_t s) {
+  const bool whole = !dt && T <= FT_ROWS32;
+  const int units = whole ? 2 : 1;
+  if (ce_direct(dt, w, ldw, T, D)) {
     m.p = (const bf16_t*)w;
-    m.ld = ldw;
+    m.ld = units * ldw;
     return 0;
   }
   FtPack k;
-  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64);
-  m.p = k.dst; m.ld = k.ldd; m.plane = V * k.ldd;
-  ws += (size_t)ft_up((dt ? 1 : 3) * V * k.ldd * 2, 256);
+  k.src = w; k.lds = ldw; k.dt = dt; k.whole = whole; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64);
+  m.p = k.dst; m.ld = units * k.ldd; m.plane = V * k.ldd;
+  ws += (size_t)ft_up((dt ? 2 : whole ? 4 : 6) * V * k.ldd, 256);
   FtPacks l;
   l.add(k);
   return ft_pack(l, s);
@@ -396,7 +400,7 @@ static int ce_weight(int dt, const void* w, long ldw, long V, long D, char*& ws,
 extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t D) { return T < 0 || D < 1 ? 0 : ce_saved(nullptr, dt, T, D).bytes; }
 extern "C" size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward) {
   if (T < 0 || V < 1 || D < 1) return 0;
-  const CeSizes z = ce_sizes(dt, T, V, D, dt && !packed, backward != 0);
+  const CeSizes z = ce_sizes(dt, T, V, D, !packed, backward != 0);
   return z.w + z.part + z.rows + z.dl + z.dxp + z.dwp + 256;
 }
 extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
@@ -407,13 +411,13 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
   FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_fwd: reduction %d", reduction);
   FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_fwd: saved and workspace are aligned to 256 bytes");
   const CeSaved sv = ce_saved(saved, dt, T, D);
-  const bool direct = ft_direct(dt, w, ldw, D);
+  const bool direct = ce_direct(dt, w, ldw, T, D);
   const CeSizes z = ce_sizes(dt, T, V, D, direct, false);
   FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.part + z.rows, "fc_linear_ce_fwd: saved or workspace too small");
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   CeArgs a = {};
-  FC_TRY(ce_weight(dt, w, ldw, V, D, ws, a.w, s));
+  FC_TRY(ce_weight(dt, w, ldw, T, V, D, ws, a.w, s));
   a.x = sv.x;
   a.T = T; a.V = V; a.D = D; a.v0 = 0; a.nv = V;
   a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
@@ -453,13 +457,13 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_bwd: reduction %d", reduction);
   FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_bwd: saved and workspace are aligned to 256 bytes");
   const CeSaved sv = ce_saved((void*)saved, dt, T, D);
-  const bool direct = ft_direct(dt, w, ldw, D);
+  const bool direct = ce_direct(dt, w, ldw, T, D);
   const CeSizes z = ce_sizes(dt, T, V, D, direct, true);
   FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.dl + z.dxp + z.dwp, "fc_linear_ce_bwd: saved or workspace too small");
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   CeArgs a = {};
-  FC_TRY(ce_weight(dt, w, ldw, V, D, ws, a.w, s));
+  FC_TRY(ce_weight(dt, w, ldw, T, V, D, ws, a.w, s));
   a.x = sv.x;
   a.T = T; a.V = V; a.D = D;
   a.n = sv.n; a.y = sv.y; a.idx = sv.idx;

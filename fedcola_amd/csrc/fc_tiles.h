@@ -3,10 +3,11 @@
 //     C[m, n] = sum_k A(m, k) B(n, k)
 //
 // with each operand stored either with k contiguous ("TK": rows are m or n) or with k as its row index ("TR"), bf16, on
-// v_mfma_f32_16x16x32_bf16.  fp32 operands come as three bf16 planes hi + mid + lo (24 bits of mantissa); a k-step is then run six
-// times, over the plane pairs whose product is above 2^-24 of the whole (NPROD = 6), so that the result is that of an fp32 product.
+// v_mfma_f32_16x16x32_bf16.  fp32 operands are taken as three bf16 planes hi + mid + lo (24 bits of mantissa) and the
+// products of the six plane pairs that are above 2^-24 of the whole (NPROD = 6), so that the result is that of an fp32 product.  The planes are
+// laid out in memory first, but for a B that few rows meet: that one is split when its fragments are formed (ft_rows32).
 //
-// One k-step is 64 deep.  Operand tiles go global -> LDS by buffer_load ... lds (16 B a lane), NS stages deep, one barrier a step.  The
+// One k-step is 64 deep (fp32: two stages of 32).  Operand tiles go global -> LDS by buffer_load ... lds (16 B a lane), NS stages deep, one barrier a step.  The
 // loads are issued by inline asm: with the builtin the compiler waits for every load in flight in front of the LDS reads it cannot tell
 // apart from the load's destination.  They have no register results; dma_wait() in front of each barrier waits for them.
 // Rows, columns and k past the end read as zero: by the descriptor's size or by an offset outside of it.
@@ -100,8 +101,8 @@ template <int MODE, int W, int KS, int NW> struct FtStager {
       }
     }
   }
-  __device__ __forceinline__ void seek(long k0, int pl) {      // the next stage is the one at k0, of plane pl
-    at = p + pl * plane + (MODE == TK ? k0 : k0 * ld);
+  __device__ __forceinline__ void seek(long k0) {              // the next stage is the one at k0, of the first plane
+    at = p + (MODE == TK ? k0 : k0 * ld);
     left_next = K - k0 < -KS ? -KS : (int)(K - k0);
     bytes = (K - k0) * ld * 2;
   }
@@ -119,7 +120,7 @@ template <int MODE, int W, int KS, int NW> struct FtStager {
     return MODE == TK ? (k < left ? voff[i] : FT_OOB) : voff[i];
   }
   __device__ __forceinline__ void piece(int i, unsigned lds, int wave) const { ft_dma16(r, lds + (wave * NP + i) * 1024, offset(i, wave)); }
-  __device__ __forceinline__ void piece_of(int pl, int i, unsigned lds, int wave) const {      // the same k of plane pl, sought at plane 0
+  __device__ __forceinline__ void piece_of(int pl, int i, unsigned lds, int wave) const {      // the same k of plane pl
     ft_dma16(ft_rsrc(cur + pl * plane, MODE == TK ? FT_MAX_BYTES : cur_bytes), lds + (wave * NP + i) * 1024, offset(i, wave));
   }
 };
@@ -138,16 +139,66 @@ template <int MODE, int W, int KS> __device__ __forceinline__ ft_b8 ft_frag(cons
   return ft_b8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// tile shape: TM x TN by WM x WN waves, NS LDS stages of KS k and PL planes
-template <int TM_, int TN_, int WM_, int WN_, int NS_, int KS_ = 64, int PL_ = 1> struct FtShape {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, KS = KS_, PL = PL_, NW = WM * WN, NT = NW * 64;
-  static constexpr int NI = TM / WM / 16, NJ = TN / WN / 16, STAGE = (TM + TN) * KS * 2 * PL, LDS = NS * STAGE;
+// the three planes of an fp32 value.  A value that is no number or infinite is its first plane alone.
+__device__ __forceinline__ void ft_split(float x, float& hi, float& mid, float& lo) {
+  hi = bf2f(f2bf(x));
+  const float r = x - hi;
+  const bool fin = __builtin_fabsf(hi) < __builtin_inff();
+  mid = fin ? bf2f(f2bf(r)) : 0.f;
+  lo = fin ? r - mid : 0.f;
+}
+
+// fp32 rows at a time as few as a scoring call's: A is planes (it is small), B is read where it is, in 32 bits, and split when its fragments
+// are formed.  A tile of B columns is the bf16 stager's, with two columns to a value: [rows][64] (TK) or [32][2 columns] (TR).
+// A: 32 rows of three planes, 32 k deep: six pieces by four waves, the last two of them moved twice so that every wave moves as many.
+struct FtRowsA {
+  static constexpr int NP = 2;
+  const bf16_t* p;
+  long ld, plane, at;
+  int K, kc[2];
+  unsigned voff[2];
+  template <class F> __device__ __forceinline__ void init(const FtMat& m, long base, int K_, int wave, int lane, F map) {
+    ld = m.ld; plane = m.plane; K = K_;
+    p = m.p + base * ld;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = (id(i, wave) & 1) * 16 + (lane >> 2), c = (lane & 3) ^ ft_tk_swz<32>(t);
+      const long row = map(t);
+      kc[i] = c * 8;
+      voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + c * 8) * 2) : FT_OOB;
+    }
+  }
+  static __device__ __forceinline__ int id(int i, int wave) { return i ? 4 + (wave & 1) : wave; }
+  __device__ __forceinline__ void load(int i, long k0, unsigned lds, int wave) const {
+    const int q = id(i, wave);
+    ft_dma16(ft_rsrc(p + (q >> 1) * plane + k0, FT_MAX_BYTES), lds + q * 1024, kc[i] < (K - k0 < 32 ? (int)(K - k0) : 32) ? voff[i] : FT_OOB);
+  }
 };
-template <class S, int MODE> using FtStageA = FtStager<MODE, S::TM, S::KS, S::NW>;
-template <class S, int MODE, int NJ = S::NJ> using FtStageB = FtStager<MODE, NJ * 16 * S::WN, S::KS, S::NW>;
-// plane pairs of the six products, least k first: (0,0) (0,1) (1,0) (1,1) (0,2) (2,0); one nibble each
-__device__ __forceinline__ int ft_pa(int c) { return (0x201100 >> (4 * c)) & 3; }
-__device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; }
+template <int MODE, int W> struct FtRowsB : FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, 4> {
+  typedef FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, 4> Base;
+  // the matrix' ld counts bf16 units, two to a value
+  template <class F> __device__ __forceinline__ void init(const FtMat& m, long base, int K_, int wave, int lane, F map) {
+    if (MODE == TK) Base::init(m, base, 2 * K_, wave, lane, map);
+    else Base::init(m, base, K_, wave, lane, [&](int r) { const long c = map(r >> 1); return c < 0 ? -1L : 2 * c; });
+  }
+};
+
+// tile shape: TM x TN by WM x WN waves, NS LDS stages of KS k and PL planes (F32: of A alone, B as it is)
+template <int TM_, int TN_, int WM_, int WN_, int NS_, int KS_ = 64, int PL_ = 1, bool F32_ = false> struct FtShape {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, KS = KS_, PL = PL_, NW = WM * WN, NT = NW * 64;
+  static constexpr bool F32 = F32_;
+  static constexpr int NI = TM / WM / 16, NJ = TN / WN / 16, STAGE = F32 ? TM * KS * 2 * PL + TN * KS * 4 : (TM + TN) * KS * 2 * PL, LDS = NS * STAGE;
+};
+template <class S, int MODE, int NJ, bool F32> struct FtStagers {
+  typedef FtStager<MODE, S::TM, S::KS, S::NW> A;
+  typedef FtStager<MODE, NJ * 16 * S::WN, S::KS, S::NW> B;
+};
+template <class S, int MODE, int NJ> struct FtStagers<S, MODE, NJ, true> {
+  typedef FtRowsA A;
+  typedef FtRowsB<MODE, S::TN> B;
+};
+template <class S, int MODE> using FtStageA = typename FtStagers<S, MODE, S::NJ, S::F32>::A;
+template <class S, int MODE, int NJ = S::NJ> using FtStageB = typename FtStagers<S, MODE, NJ, S::F32>::B;
 
 // acc += the k-steps [kt0, kt1).  On return every wave has left the loop's LDS reads behind and no load into LDS is in flight.
 //
@@ -155,25 +206,16 @@ __device__ __forceinline__ int ft_pb(int c) { return (0x021010 >> (4 * c)) & 3; 
 // few MFMAs, so that neither the LDS nor the matrix pipe waits for the other.  The one barrier stands between the halves: there a wave has the
 // step's second half in registers, so its stage is free for the loads of the step NS on, and the next stage, loaded for NS - 1 steps by then, is
 // read from there on.
-template <class S, int AM, int BMO, int NPROD, int NJ>
+template <class S, int AM, int BMO, int NJ>
 __device__ __forceinline__ void ft_halves(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                          ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
   constexpr int TNL = NJ * 16 * S::WN;      // columns staged (the shape's TN, or less in a second loop over the same tile)
   constexpr int PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO, NJ>::NP, NF = S::NI + NJ, NM = S::NI * NJ;
   const unsigned lds0 = ft_lds_addr(smem);
-  const int steps = (kt1 - kt0) * NPROD;
-  int c = 0;
-  long ik = (long)kt0 * 64;
-  if (NPROD == 1) { sa.seek(ik, 0); sb.seek(ik, 0); }
-  auto next = [&]() {                       // steps past a slice's end, or the matrices', are loaded and not used: every step issues as many loads
-    if (NPROD > 1) {
-      sa.seek(ik, ft_pa(c));
-      sb.seek(ik, ft_pb(c));
-      if (++c == NPROD) { c = 0; ik += 64; }
-    }
-    sa.step();
-    sb.step();
-  };
+  const int steps = kt1 - kt0;
+  sa.seek((long)kt0 * 64);
+  sb.seek((long)kt0 * 64);
+  auto next = [&]() { sa.step(); sb.step(); };   // steps past a slice's end, or the matrices', are loaded and not used: every step issues as many loads
   auto piece = [&](int i, int at) {
     if (i < PA) sa.piece(i, lds0 + at * S::STAGE, wave); else sb.piece(i - PA, lds0 + at * S::STAGE + S::TM * 128, wave);
   };
@@ -225,22 +267,17 @@ __device__ __forceinline__ void ft_halves(FtStageA<S, AM>& sa, FtStageB<S, BMO, 
 }
 
 // the same without halves, for few rows: a step is short, and its loads' way from memory long
-template <class S, int AM, int BMO, int NPROD, int NJ>
+template <class S, int AM, int BMO, int NJ>
 __device__ __forceinline__ void ft_rows(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                              ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
   constexpr int TNL = NJ * 16 * S::WN;
   constexpr int PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO, NJ>::NP;
   const unsigned lds0 = ft_lds_addr(smem);
-  const int steps = (kt1 - kt0) * NPROD;
-  int slot = 0, c = 0;
-  long ik = (long)kt0 * 64;
-  if (NPROD == 1) { sa.seek(ik, 0); sb.seek(ik, 0); }
+  const int steps = kt1 - kt0;
+  int slot = 0;
+  sa.seek((long)kt0 * 64);
+  sb.seek((long)kt0 * 64);
   auto put = [&](int at) {
-    if (NPROD > 1) {
-      sa.seek(ik, ft_pa(c));
-      sb.seek(ik, ft_pb(c));
-      if (++c == NPROD) { c = 0; ik += 64; }
-    }
     sa.step();
     sb.step();
 #pragma unroll
@@ -275,19 +312,19 @@ __device__ __forceinline__ void ft_rows(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ
   ft_dma_wait<0>();
   ft_barrier();
 }
-// fp32 operands with all three planes of both in a stage of 32 k: six products from one read of each fragment.  (A plane pair a step, as above
-// with nprod 6, loads every plane twice and meets six barriers for one here; it is left for the few rows of ft_rows.)  The fragments of the
-// next stage are read under the MFMAs of this one, whose barrier stands under the first of them.
+// fp32 operands with all three planes of both in a stage of 32 k: six products from one read of each fragment.  (A plane pair a step
+// would load every plane twice and meet six barriers for one here.)  The fragments of the next stage are read under the MFMAs of this one,
+// whose barrier stands under the first of them.
 template <class S, int AM, int BMO>
 __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
                                           int lane) {
-  static_assert(S::KS == 32 && S::PL == 3, "a stage is one fragment deep");
+  static_assert(S::KS == 32 && S::PL == 3 && !S::F32, "a stage is one fragment deep");
   constexpr int NI = S::NI, NJ = S::NJ, PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO>::NP, P = 3 * (PA + PB), NF = 3 * (NI + NJ), NM = 6 * NI * NJ;
   constexpr int TA = S::TM * 64, TB = S::TN * 64;     // bytes of a plane's tile
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * 2;
-  sa.seek((long)kt0 * 64, 0);
-  sb.seek((long)kt0 * 64, 0);
+  sa.seek((long)kt0 * 64);
+  sb.seek((long)kt0 * 64);
   auto next = [&]() { sa.step(); sb.step(); };
   auto piece = [&](int i, int at) {
     const unsigned l = lds0 + at * S::STAGE;
@@ -346,12 +383,86 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
   ft_barrier();
 }
 
+// eight fp32 values of a B fragment as the fragments of their three planes
+__device__ __forceinline__ void ft_split8(const float (&v)[8], ft_b8 (&f)[3]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float h[2], m[2], l[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) ft_split(v[i + j], h[j], m[j], l[j]);
+    ((unsigned*)&f[0])[i / 2] = f2bf2(h[0], h[1]);
+    ((unsigned*)&f[1])[i / 2] = f2bf2(m[0], m[1]);
+    ((unsigned*)&f[2])[i / 2] = f2bf2(l[0], l[1]);
+  }
+}
+template <class S, int BMO>
+__device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtRowsB<BMO, S::TN>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
+                                          int lane) {
+  static_assert(S::TM == 32 && S::NW == 4 && S::KS == 32 && S::PL == 3 && S::NI == 1, "two waves by two");
+  constexpr int PB = FtRowsB<BMO, S::TN>::NP, P = 2 + PB, TA = S::TM * 64;
+  const unsigned lds0 = ft_lds_addr(smem);
+  const int steps = (kt1 - kt0) * 2, g = lane >> 4;
+  long k0 = (long)kt0 * 64;
+  sb.seek(BMO == TK ? 2 * k0 : k0);
+  auto put = [&](int at) {
+    const unsigned l = lds0 + at * S::STAGE;
+    sb.step();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sa.load(i, k0, l, wave);
+#pragma unroll
+    for (int i = 0; i < PB; ++i) sb.piece(i, l + 3 * TA, wave);
+    k0 += 32;
+  };
+#pragma unroll
+  for (int s = 0; s < S::NS - 1; ++s) put(s);
+  int slot = 0, free_slot = S::NS - 1;
+  for (int s = 0; s < steps; ++s) {
+    ft_dma_wait<(S::NS - 2) * P>();
+    ft_barrier();
+    put(free_slot);
+    const char* ta = smem + slot * S::STAGE;
+    const char* tb = ta + 3 * TA;
+    ft_b8 fa[3], fb[S::NJ][3];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) fa[p] = ft_frag<TK, 32, 32>(ta + p * TA, wm * 16, 0, lane);
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j) {
+      float v[8];
+      const int r = (wn * S::NJ + j) * 16 + (lane & 15);
+      if (BMO == TK) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const ft_f4 u = *(const ft_f4*)(tb + r * 128 + (((2 * g + h) ^ ft_tk_swz<64>(r)) << 4));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[4 * h + i] = u[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *(const float*)(tb + (8 * g + i) * (S::TN * 4) + (((r >> 3) ^ (((g & 1) << 2) | (i & 3))) << 5) + (r & 7) * 4);
+      }
+      ft_split8(v, fb[j]);
+    }
+#pragma unroll
+    for (int q = 0; q < 6; ++q)
+#pragma unroll
+      for (int j = 0; j < S::NJ; ++j) {
+        constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
+        acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j][qb[q]], fa[qa[q]], acc[0][j], 0, 0, 0);
+      }
+    free_slot = slot;
+    slot = slot + 1 == S::NS ? 0 : slot + 1;
+  }
+  ft_dma_wait<0>();
+  ft_barrier();
+}
+
 template <class S, int AM, int BMO, int NPROD, int NJ>
 __device__ __forceinline__ void ft_loop(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                         ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  if constexpr (S::PL == 3) ft_planes<S, AM, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
-  else if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
-  else ft_rows<S, AM, BMO, NPROD, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  if constexpr (S::F32) ft_rows32<S, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  else if constexpr (S::PL == 3) ft_planes<S, AM, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  else if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  else ft_rows<S, AM, BMO, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
 }
 
 // ---- which tile a workgroup takes.  Consecutive ids share an XCD's L2 (workgroups are dealt to the 8 XCDs in turn), and ids walk the
@@ -408,19 +519,11 @@ __device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld
     }
   }
 }
-// the three planes of an fp32 value.  A value that is no number or infinite is its first plane alone.
-__device__ __forceinline__ void ft_split(float x, float& hi, float& mid, float& lo) {
-  hi = bf2f(f2bf(x));
-  const float r = x - hi;
-  const bool fin = __builtin_fabsf(hi) < __builtin_inff();
-  mid = fin ? bf2f(f2bf(r)) : 0.f;
-  lo = fin ? r - mid : 0.f;
-}
-
 // ---------------------------------------------------------------- host side (fc_tiles.hip)
 // C = A B^T written to `out` (bf16 for nprod 1, fp32 for 6), or as fp32 partial sums for ft_reduce().
 struct FtProduct {
   int am = TK, bm = TK, nprod = 1;
+  bool rows32 = false;            // fp32, few rows: B is the fp32 matrix itself (its ld in bf16 units)
   FtMat a, b;
   int M = 0, N = 0, K = 0;
   int Ks = 0;                     // > 0: the length that the slices are cut from, >= K (products added onto each other's partial sums)
@@ -440,7 +543,7 @@ struct FtProduct {
 };
 // shape: index of the tile shape; target: workgroups wanted, by which the reduction is sliced (0: it is not)
 struct FtPlan { int shape = 0, target = 0; };
-FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_rows);
+FtPlan ft_plan(const FtProduct& p, bool dynamic_rows);
 __host__ __device__ static inline long ft_part_ld(long N) { return (N + 7) / 8 * 8; }
 // slices of a reduction of length K for `tiles` output tiles: as many as the target asks for, none under four k-steps (one of fp32's six products)
 __host__ __device__ static inline int ft_slices(long tiles, long K, int target, int nprod) {
@@ -475,13 +578,14 @@ int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, 
 int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s);
 // the product into p.out, by way of partial sums in `part` where the plan slices the reduction
 int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s);
-size_t ft_product_part_floats(int am, int bm, int nprod, long M, long N, long K);
+size_t ft_product_part_floats(const FtProduct& p);
 
 // an operand as the products take it: rows of whole 128-byte lines, and in planes for fp32
 struct FtPack {
   const void* src = nullptr;
   long lds = 0;                   // elements between source rows
   int dt = 1;
+  bool whole = false;             // fp32 kept in 32 bits: dst is fp32, ldd counts values
   long R = 0, C = 0;
   bf16_t* dst = nullptr;
   long ldd = 0;                   // multiple of 64, >= C: the columns in between are written as zeros
@@ -493,6 +597,9 @@ struct FtPacks {                  // up to four of one type in one launch
   void add(const FtPack& q) { p[n] = q; first[n + 1] = first[n] + q.R * (q.ldd / 8); ++n; }
 };
 int ft_pack(const FtPacks& p, hipStream_t s);
+// fp32 few rows: how many, and whether B can be read where it is
+#define FT_ROWS32 64
+static inline bool ft_direct32(const void* p, long ld, long cols) { return ((size_t)p & 15) == 0 && ld % 4 == 0 && cols % 4 == 0 && ld < (1L << 20); }
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
 static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }
 // > 64 KB of LDS for a kernel: asked for once on each device (a static of the launch that needs it)

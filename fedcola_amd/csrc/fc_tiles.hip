@@ -32,6 +32,12 @@ __global__ void __launch_bounds__(256) k_ft_pack(FtPacks l) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
+  if (PL == 3 && a.whole) {
+    ft_f4* d = (ft_f4*)((float*)a.dst + r * a.ldd + c0);
+    d[0] = ft_f4{v[0], v[1], v[2], v[3]};
+    d[1] = ft_f4{v[4], v[5], v[6], v[7]};
+    return;
+  }
   float h[3][8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -153,24 +159,28 @@ typedef FtShape<32, 64, 2, 2, 6> FtRow;        // 72 KB, two: few rows, the read
 
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> FtPlanes;   // fp32's only large tile: 144 KB, one workgroup of eight waves a CU
 
+typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> FtRows32;   // fp32, few rows: 70 KB, two
+
 struct FtCost { double step, fixed; int slots; };   // us a k-step with the chip full, us a tile besides, tiles at once
-static const FtCost kCost[4] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}, {2.6, 6.0, 256}};
-static const int kTM[4] = {256, 128, 32, 128}, kTN[4] = {256, 128, 64, 128};
+static const FtCost kCost[5] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}, {2.6, 6.0, 256}, {1.0, 5.0, 512}};
+static const int kTM[5] = {256, 128, 32, 128, 32}, kTN[5] = {256, 128, 64, 128, 64};
 
 // The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
 // step + time of a tile's start and end), plus the partial sums' way to memory and back.  The constants are measured: 256 x 256 tiles run
 // a k-step in 1.6 us on all CUs (1.3 PFLOP/s), 128 x 128 ones in 1.15 us, two a CU (0.93), and where they leave half of the chip idle, 0.8.
-FtPlan ft_plan(int am, int bm, int nprod, long M, long N, long K, bool dynamic_rows) {
+FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
+  const long M = p.M, N = p.N, K = (long)p.K * p.segs;
+  const int nprod = p.nprod;
   FtPlan best;
   double least = 1e30;
-  for (int sh = 0; sh < 4; ++sh) {
-    if (sh == 2 ? am != TK || bm != TK || M > 64 : (sh == 3) != (nprod == 6)) continue;
+  for (int sh = 0; sh < 5; ++sh) {
+    if (nprod == 6 ? sh != (p.rows32 ? 4 : 3) : sh > 2 || (sh == 2 && (p.am != TK || p.bm != TK || M > 64))) continue;
     const long tiles = ((M + kTM[sh] - 1) / kTM[sh]) * ((N + kTN[sh] - 1) / kTN[sh]), nk = (K + 63) / 64;
     for (int want = 1; want <= 32; ++want) {
       const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want), nprod);
       const long per = (nk + sp - 1) / sp, wg = tiles * sp, slots = kCost[sh].slots;
       const double rounds = wg <= 4 * slots ? (double)((wg + slots - 1) / slots) : (double)wg / slots + 0.5;
-      double t = rounds * ((double)(sh == 2 ? per * nprod : per) * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
+      double t = rounds * ((double)per * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
       if (sp > 1) t += 4.0 + (double)sp * M * N * 8.0 / 4e6;
       if (t < least) {
         least = t;
@@ -210,6 +220,9 @@ static int launch(const FtProduct& p, const FtPlan& pl, float* part, bool add, h
 }
 template <class S, int NPROD> static int by_mode(const FtProduct& p, const FtPlan& pl, float* part, bool add, hipStream_t s) {
   if (p.am == TK && p.bm == TK) return launch<S, TK, TK, NPROD>(p, pl, part, add, s);
+  if constexpr (S::F32) {
+    if (p.am == TK) return launch<S, TK, TR, NPROD>(p, pl, part, add, s);
+  }
   if constexpr (S::TN >= 128) {
     if (p.am == TK) return launch<S, TK, TR, NPROD>(p, pl, part, add, s);
     if (p.bm == TR) return launch<S, TR, TR, NPROD>(p, pl, part, add, s);
@@ -223,8 +236,9 @@ int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hi
   switch (plan.shape) {
     case 0: return by_mode<FtBig, 1>(p, plan, part, add, s);
     case 1: return by_mode<FtMid, 1>(p, plan, part, add, s);
-    case 2: return p.nprod == 1 ? by_mode<FtRow, 1>(p, plan, part, add, s) : by_mode<FtRow, 6>(p, plan, part, add, s);
-    default: return by_mode<FtPlanes, 6>(p, plan, part, add, s);
+    case 2: return by_mode<FtRow, 1>(p, plan, part, add, s);
+    case 3: return by_mode<FtPlanes, 6>(p, plan, part, add, s);
+    default: return by_mode<FtRows32, 6>(p, plan, part, add, s);
   }
 }
 
@@ -291,6 +305,8 @@ int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const i
 bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan) {
   const int sh = p[0].nprod == 1 ? 1 : 3, slots = kCost[sh].slots;
   double work = 0;
+  for (int i = 0; i < n; ++i)
+    if (p[i].rows32) return false;
   for (int i = 0; i < n; ++i) work += (double)tiles_of(FtPlan{sh, 0}, p[i].M, p[i].N) * (double)((p[i].K + 63) / 64 * p[i].segs);
   if (work > 160.0 * slots) return false;
   const double share = work / slots / 2 > 4 ? work / slots / 2 : 4;
@@ -328,12 +344,12 @@ int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, 
   return 0;
 }
 
-size_t ft_product_part_floats(int am, int bm, int nprod, long M, long N, long K) {
-  const FtPlan p = ft_plan(am, bm, nprod, M, N, K, false);
-  return p.target ? ft_part_floats(M, N, p) : 0;
+size_t ft_product_part_floats(const FtProduct& p) {
+  const FtPlan plan = ft_plan(p, false);
+  return plan.target ? ft_part_floats(p.M, p.N, plan) : 0;
 }
 int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s) {
-  const FtPlan plan = ft_plan(p.am, p.bm, p.nprod, p.M, p.N, (long)p.K * p.segs, false);
+  const FtPlan plan = ft_plan(p, false);
   if (!plan.target) return ft_product(p, plan, nullptr, false, s);
   FC_REQUIRE(part && part_floats >= ft_part_floats(p.M, p.N, plan), "workspace too small for the partial sums");
   FC_TRY(ft_product(p, plan, part, false, s));

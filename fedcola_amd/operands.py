@@ -45,9 +45,11 @@ def as_rows(t):
     return t, ld
 
 
-def in_place(t, ld):
-    """whether the tiled products read a matrix where it is (include/fedcola_hip.h)"""
-    return t.element_size() == 2 and ld % 8 == 0 and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0
+def in_place(t, ld, rows):
+    """whether the tiled products of `rows` rows read this matrix where it is (include/fedcola_hip.h)"""
+    if t.element_size() == 4:
+        return rows <= 64 and ld % 4 == 0 and t.shape[1] % 4 == 0 and t.data_ptr() % 16 == 0 and ld < 1 << 20
+    return ld % 8 == 0 and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 class on_device:
