@@ -18,7 +18,7 @@
 struct GmArgs {
   FtMat x, w_in, w_out, dy;
   int T, D, F, act;
-  bool rows32;                  // fp32, few rows: w_in and w_out are the fp32 matrices themselves
+  bool b32;                     // fp32: w_in and w_out are the fp32 matrices themselves
   long up;                      // rows between a unit's gate and up row in w_in
   bf16_t *h, *dgu;              // planes of [T][ldh], [T][2 ldh]: h; dg | du
   long ldh;                     // whole 128-byte lines: a row that straddles one more costs every tile load an L2 request more
@@ -155,6 +155,7 @@ typedef FtShape<128, 128, 2, 2, 2> GmMid;
 typedef FtShape<32, 64, 2, 2, 6> GmRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> GmPlanes;
 typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> GmRows32;
+typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> GmMid32;
 
 template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.F + S::TN / 2 - 1) / (S::TN / 2));
@@ -170,20 +171,20 @@ template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& 
 // 50 us against 70; 8192 x 4096 x 11000 the other way, 1571 against 1333)
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
   if constexpr (NPROD == 6) {
-    return a.rows32 ? gm_act_launch<GmRows32, NPROD, GRAD>(a, s) : gm_act_launch<GmPlanes, NPROD, GRAD>(a, s);
+    return !a.b32 ? gm_act_launch<GmPlanes, NPROD, GRAD>(a, s) : ft_few(6, a.T) ? gm_act_launch<GmRows32, NPROD, GRAD>(a, s) : gm_act_launch<GmMid32, NPROD, GRAD>(a, s);
   } else {
-    if (a.T <= 64) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
+    if (ft_few(1, a.T)) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
     if ((long)((a.T + 255) / 256) * ((a.F + 127) / 128) >= 128 && (!GRAD || a.D >= 1024)) return gm_act_launch<GmBig, NPROD, GRAD>(a, s);
     return gm_act_launch<GmMid, NPROD, GRAD>(a, s);
   }
 }
 
-// fp32, few rows: the weights are read where they are, or from a copy in 32 bits, and split in registers
-static bool gm_rows32(int dt, long T, long D, long F) { return !dt && T <= FT_ROWS32 && (F + 512) * ft_up(D, 64) < (1L << 29); }
+// fp32, few rows: the weights are read where they are, or from a copy in 32 bits (the up rows within a tile load's reach), and split in registers
+static bool gm_b32(int dt, long T, long D, long F) { return ft_b32(dt, T) && (F + 512) * ft_up(D, 64) < (1L << 29); }
 struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan[3]; bool group; };
 // dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
 static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProduct (&p)[3]) {
-  p[0].rows32 = a.rows32;
+  p[0].b32 = a.b32;
   const long Fp = ft_up(F, 64);
   for (FtProduct& q : p) { q.am = TR; q.bm = TR; q.nprod = dt ? 1 : 6; q.K = (int)T; }
   p[0].am = TK;
@@ -200,36 +201,36 @@ static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProdu
   p[2].a = a.dy;
   p[2].b.p = a.h; p[2].b.ld = Fp; p[2].b.plane = T * Fp;
 }
-static FtProduct gm_y_product(int dt, long T, long D, long F, bool rows32) {
+static FtProduct gm_y_product(int dt, long T, long D, long F, bool b32) {
   FtProduct p;
   p.nprod = dt ? 1 : 6;
-  p.rows32 = rows32;
+  p.b32 = b32;
   p.M = (int)T; p.N = (int)D; p.K = (int)F;
   return p;
 }
 static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backward) {
   GmSizes z = {};
   const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6;
-  const bool r32 = gm_rows32(dt, T, D, F);
+  const bool b32 = gm_b32(dt, T, D, F);
   if (packed || !dt) {
     z.x = ft_up(T * Dp * e, 256);
     z.dy = backward ? z.x : 0;
   }
   if (packed) {
-    const long we = r32 ? 4 : e;
+    const long we = b32 ? 4 : e;
     z.w_in = ft_up(2 * F * Dp * we, 256);
     z.w_out = ft_up(D * Fp * we, 256);
   }
   z.h = ft_up(T * Fp * e, 256);
   if (!backward) {
-    z.part = ft_product_part_floats(gm_y_product(dt, T, D, F, r32)) * 4;
+    z.part = ft_product_part_floats(gm_y_product(dt, T, D, F, b32)) * 4;
     return z;
   }
   z.dgu = ft_up(T * 2 * Fp * e, 256);
   z.dh = ft_up(ft_part_ld(F) * T * 4, 256);
   FtProduct p[3];
   GmArgs a = {};
-  a.rows32 = r32;
+  a.b32 = b32;
   gm_products(dt, T, D, F, a, p);
   z.group = ft_group_plan(p, 3, z.plan);
   for (int i = 0; i < 3; ++i) {
@@ -273,32 +274,32 @@ static int gm_check(const char* what, const GmCall& c, const void* ws) {
   return ft_check_device(c.w_in, what);
 }
 // which of w_in and w_out is read where it is, and whether all operands of the type's are (fp32: the weights alone, x and dy become planes)
-static bool gm_direct(const GmCall& c, bool r32, bool& in, bool& out) {
-  in = r32 ? gm_whole(c.w_in, c.ld_in, c.F, c.D) : ft_direct(c.dt, c.w_in, c.ld_in, c.D);
-  out = r32 ? gm_whole(c.w_out, c.ld_out, 0, c.F) : ft_direct(c.dt, c.w_out, c.ld_out, c.F);
+static bool gm_direct(const GmCall& c, bool b32, bool& in, bool& out) {
+  in = b32 ? gm_whole(c.w_in, c.ld_in, c.F, c.D) : ft_direct(c.dt, c.w_in, c.ld_in, c.D);
+  out = b32 ? gm_whole(c.w_out, c.ld_out, 0, c.F) : ft_direct(c.dt, c.w_out, c.ld_out, c.F);
   return in && out && (!c.dt || (ft_direct(c.dt, c.x, c.ldx, c.D) && (!c.dy || ft_direct(c.dt, c.dy, c.lddy, c.D))));
 }
 // the operands as the products take them; what of them cannot be taken as it is goes to the workspace
 static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
   bool in, out;
-  a.rows32 = gm_rows32(c.dt, c.T, c.D, c.F);
-  gm_direct(c, a.rows32, in, out);
+  a.b32 = gm_b32(c.dt, c.T, c.D, c.F);
+  gm_direct(c, a.b32, in, out);
   a.T = (int)c.T; a.D = (int)c.D; a.F = (int)c.F; a.act = c.act; a.up = c.F; a.ldh = ft_up(c.F, 64);
   FtPacks l;
   gm_matrix(c.dt, false, ft_direct(c.dt, c.x, c.ldx, c.D), c.x, c.ldx, c.T, c.D, ws, a.x, l);
   if (c.dy) gm_matrix(c.dt, false, ft_direct(c.dt, c.dy, c.lddy, c.D), c.dy, c.lddy, c.T, c.D, ws, a.dy, l);
-  gm_matrix(c.dt, a.rows32, out, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
-  gm_matrix(c.dt, a.rows32, in, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
+  gm_matrix(c.dt, a.b32, out, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
+  gm_matrix(c.dt, a.b32, in, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
   return ft_pack(l, s);
 }
 static GmSizes gm_call_sizes(const GmCall& c, bool backward) {
   bool in, out;
-  return gm_sizes(c.dt, c.T, c.D, c.F, !gm_direct(c, gm_rows32(c.dt, c.T, c.D, c.F), in, out), backward);
+  return gm_sizes(c.dt, c.T, c.D, c.F, !gm_direct(c, gm_b32(c.dt, c.T, c.D, c.F), in, out), backward);
 }
 
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
   if (T < 0 || D < 1 || F < 1) return 0;
-  return gm_total(gm_sizes(dt, T, D, F, packed || (!dt && !gm_rows32(dt, T, D, F)), backward != 0)) + 256;
+  return gm_total(gm_sizes(dt, T, D, F, packed || (!dt && !gm_b32(dt, T, D, F)), backward != 0)) + 256;
 }
 extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t ldx, const void* w_in, int64_t ld_in, const void* w_out, int64_t ld_out,
                                 int32_t T, int32_t D, int32_t F, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
@@ -315,7 +316,7 @@ extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t 
   a.h = (bf16_t*)ws;
   ws += z.h;
   FC_TRY(dt ? (gm_act_run<1, false>(a, s)) : (gm_act_run<6, false>(a, s)));
-  FtProduct p = gm_y_product(dt, T, D, F, a.rows32);
+  FtProduct p = gm_y_product(dt, T, D, F, a.b32);
   p.a.p = a.h; p.a.ld = a.ldh; p.a.plane = (long)T * a.ldh;
   p.b = a.w_out;
   p.out = y; p.ldo = ldy;
@@ -342,7 +343,7 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   if (T) {
     FtProduct p;
     p.nprod = dt ? 1 : 6;
-    p.rows32 = a.rows32;
+    p.b32 = a.b32;
     p.am = TK; p.bm = TR;
     p.a = a.dy;
     p.b = a.w_out;

@@ -298,9 +298,10 @@ typedef FtShape<128, 128, 2, 2, 2> CeMid;
 typedef FtShape<32, 64, 2, 2, 6> CeRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
 typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> CeRows32;
+typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> CeMid32;
 // 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32, 32 x 64 for the few rows of a scoring call
 static int ce_shape(int dt, long T, long V) {
-  if (T <= FT_ROWS32) return 2;
+  if (ft_few(dt ? 1 : 6, T)) return 2;
   return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
@@ -323,7 +324,7 @@ template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, h
 template <bool GRAD> static int ce_run(int dt, int shape, const CeArgs& a, hipStream_t s) {
   if (a.T == 0 || a.nv == 0) return 0;
   if (dt) return shape == 0 ? ce_launch<CeBig, 1, GRAD>(a, s) : shape == 1 ? ce_launch<CeMid, 1, GRAD>(a, s) : ce_launch<CeRow, 1, GRAD>(a, s);
-  return shape == 1 ? ce_launch<CePlanes, 6, GRAD>(a, s) : ce_launch<CeRows32, 6, GRAD>(a, s);
+  return shape != 1 ? ce_launch<CeRows32, 6, GRAD>(a, s) : ft_b32(dt, a.T) ? ce_launch<CeMid32, 6, GRAD>(a, s) : ce_launch<CePlanes, 6, GRAD>(a, s);
 }
 
 // columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
@@ -334,12 +335,12 @@ static long ce_piece(int dt, long T, long V) {
 struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx, dw; bool group; };
 // dx = dL w and dw = dL^T x of nv columns; n: device, the rows that count
 static void ce_products(int dt, long T, long D, long nv, const int* n, FtProduct& x, FtProduct& w) {
-  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.rows32 = !dt && T <= FT_ROWS32; x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
+  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.b32 = ft_b32(dt, T); x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
   w.am = TR; w.bm = TR; w.nprod = x.nprod; w.M = (int)nv; w.N = (int)D; w.K = (int)T; w.Kdyn = n;
 }
 static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad) {
   CeSizes z = {};
-  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : T <= FT_ROWS32 ? 4 : 6) * V * ft_up(D, 64), 256);
+  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : ft_b32(dt, T) ? 4 : 6) * V * ft_up(D, 64), 256);
   if (!grad) {
     const int tn = ce_tn(ce_shape(dt, T, V));
     z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
@@ -378,10 +379,10 @@ static int ce_args(const char* what, int dt, long T, long V, long D, long ldw, c
   FC_REQUIRE(w && ldw >= D && ldw < (1L << 21), "%s: weight missing or its rows %ld apart", what, ldw);
   return ft_check_device(w, what);
 }
-// the weight as the products take it: where it is, or (few fp32 rows: in 32 bits) laid out in the workspace
-static bool ce_direct(int dt, const void* w, long ldw, long T, long D) { return dt || T > FT_ROWS32 ? ft_direct(dt, w, ldw, D) : ft_direct32(w, ldw, D); }
+// the weight as the products take it: where it is, or laid out in the workspace
+static bool ce_direct(int dt, const void* w, long ldw, long T, long D) { return ft_b32(dt, T) ? ft_direct32(w, ldw, D) : ft_direct(dt, w, ldw, D); }
 static int ce_weight(int dt, const void* w, long ldw, long T, long V, long D, char*& ws, FtMat& m, hipStream_t s) {
-  const bool whole = !dt && T <= FT_ROWS32;
+  const bool whole = ft_b32(dt, T);
   const int units = whole ? 2 : 1;
   if (ce_direct(dt, w, ldw, T, D)) {
     m.p = (const bf16_t*)w;

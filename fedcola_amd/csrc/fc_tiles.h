@@ -5,7 +5,7 @@
 // with each operand stored either with k contiguous ("TK": rows are m or n) or with k as its row index ("TR"), bf16, on
 // v_mfma_f32_16x16x32_bf16.  fp32 operands are taken as three bf16 planes hi + mid + lo (24 bits of mantissa) and the
 // products of the six plane pairs that are above 2^-24 of the whole (NPROD = 6), so that the result is that of an fp32 product.  The planes are
-// laid out in memory first, but for a B that few rows meet: that one is split when its fragments are formed (ft_rows32).
+// laid out in memory first, but for a B that few rows meet: that one is split when its fragments are formed (FtB32).
 //
 // One k-step is 64 deep (fp32: two stages of 32).  Operand tiles go global -> LDS by buffer_load ... lds (16 B a lane), NS stages deep, one barrier a step.  The
 // loads are issued by inline asm: with the builtin the compiler waits for every load in flight in front of the LDS reads it cannot tell
@@ -16,6 +16,7 @@
 // The MFMA's operands are swapped, so a lane's accumulator acc[i][j] is row 16 i + (lane & 15), columns 16 j + 4 (lane >> 4) .. + 3.
 #pragma once
 #include <atomic>
+#include <type_traits>
 
 #include "fc_common.h"
 
@@ -148,9 +149,8 @@ __device__ __forceinline__ void ft_split(float x, float& hi, float& mid, float& 
   lo = fin ? r - mid : 0.f;
 }
 
-// fp32 rows at a time as few as a scoring call's: A is planes (it is small), B is read where it is, in 32 bits, and split when its fragments
-// are formed.  A tile of B columns is the bf16 stager's, with two columns to a value: [rows][64] (TK) or [32][2 columns] (TR).
-// A: 32 rows of three planes, 32 k deep: six pieces by four waves, the last two of them moved twice so that every wave moves as many.
+// fp32 tiles of 32 rows (a scoring call's): 32 rows of A's three planes, 32 k deep, are six pieces by four waves, the last two of them moved
+// twice so that every wave moves as many
 struct FtRowsA {
   static constexpr int NP = 2;
   const bf16_t* p;
@@ -174,14 +174,43 @@ struct FtRowsA {
     ft_dma16(ft_rsrc(p + (q >> 1) * plane + k0, FT_MAX_BYTES), lds + q * 1024, kc[i] < (K - k0 < 32 ? (int)(K - k0) : 32) ? voff[i] : FT_OOB);
   }
 };
-template <int MODE, int W> struct FtRowsB : FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, 4> {
-  typedef FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, 4> Base;
+// An fp32 B that is read where it is, in 32 bits, and split when its fragments are formed: its tile is a bf16 stager's with two columns to a
+// value, [rows][64] (TK) or [32][2 columns] (TR).
+template <int MODE, int W, int NW> struct FtB32 : FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, NW> {
+  typedef FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, NW> Base;
   // the matrix' ld counts bf16 units, two to a value
   template <class F> __device__ __forceinline__ void init(const FtMat& m, long base, int K_, int wave, int lane, F map) {
     if (MODE == TK) Base::init(m, base, 2 * K_, wave, lane, map);
     else Base::init(m, base, K_, wave, lane, [&](int r) { const long c = map(r >> 1); return c < 0 ? -1L : 2 * c; });
   }
+  __device__ __forceinline__ void seek(long k0) { Base::seek(MODE == TK ? 2 * k0 : k0); }
+  // eight k of column r (the lane's)
+  static __device__ __forceinline__ void read(const char* t, int r, int g, float (&v)[8]) {
+    if (MODE == TK) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const ft_f4 u = *(const ft_f4*)(t + r * 128 + (((2 * g + h) ^ ft_tk_swz<64>(r)) << 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * h + i] = u[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = *(const float*)(t + (8 * g + i) * (W * 4) + (((r >> 3) ^ (((g & 1) << 2) | (i & 3))) << 5) + (r & 7) * 4);
+    }
+  }
 };
+// eight fp32 values of a B fragment as the fragments of their three planes
+__device__ __forceinline__ void ft_split8(const float (&v)[8], ft_b8& f0, ft_b8& f1, ft_b8& f2) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float h[2], m[2], l[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) ft_split(v[i + j], h[j], m[j], l[j]);
+    ((unsigned*)&f0)[i / 2] = f2bf2(h[0], h[1]);
+    ((unsigned*)&f1)[i / 2] = f2bf2(m[0], m[1]);
+    ((unsigned*)&f2)[i / 2] = f2bf2(l[0], l[1]);
+  }
+}
 
 // tile shape: TM x TN by WM x WN waves, NS LDS stages of KS k and PL planes (F32: of A alone, B as it is)
 template <int TM_, int TN_, int WM_, int WN_, int NS_, int KS_ = 64, int PL_ = 1, bool F32_ = false> struct FtShape {
@@ -194,8 +223,8 @@ template <class S, int MODE, int NJ, bool F32> struct FtStagers {
   typedef FtStager<MODE, NJ * 16 * S::WN, S::KS, S::NW> B;
 };
 template <class S, int MODE, int NJ> struct FtStagers<S, MODE, NJ, true> {
-  typedef FtRowsA A;
-  typedef FtRowsB<MODE, S::TN> B;
+  typedef typename std::conditional<S::TM == 32, FtRowsA, FtStager<TK, S::TM < 128 ? 128 : S::TM, S::KS, S::NW>>::type A;
+  typedef FtB32<MODE, S::TN, S::NW> B;
 };
 template <class S, int MODE> using FtStageA = typename FtStagers<S, MODE, S::NJ, S::F32>::A;
 template <class S, int MODE, int NJ = S::NJ> using FtStageB = typename FtStagers<S, MODE, NJ, S::F32>::B;
@@ -315,11 +344,13 @@ __device__ __forceinline__ void ft_rows(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ
 // fp32 operands with all three planes of both in a stage of 32 k: six products from one read of each fragment.  (A plane pair a step
 // would load every plane twice and meet six barriers for one here.)  The fragments of the next stage are read under the MFMAs of this one,
 // whose barrier stands under the first of them.
+// F32: B's fragments are read in 32 bits and split a few groups of MFMAs later.
 template <class S, int AM, int BMO>
 __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
                                           int lane) {
-  static_assert(S::KS == 32 && S::PL == 3 && !S::F32, "a stage is one fragment deep");
-  constexpr int NI = S::NI, NJ = S::NJ, PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO>::NP, P = 3 * (PA + PB), NF = 3 * (NI + NJ), NM = 6 * NI * NJ;
+  static_assert(S::KS == 32 && S::PL == 3, "a stage is one fragment deep");
+  constexpr int NI = S::NI, NJ = S::NJ, PA = 3 * FtStageA<S, AM>::NP, PB1 = FtStageB<S, BMO>::NP, PB = S::F32 ? PB1 : 3 * PB1, P = PA + PB, NM = 6 * NI * NJ;
+  constexpr int NF = 3 * NI + (S::F32 ? NJ : 3 * NJ);
   constexpr int TA = S::TM * 64, TB = S::TN * 64;     // bytes of a plane's tile
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * 2;
@@ -328,15 +359,23 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
   auto next = [&]() { sa.step(); sb.step(); };
   auto piece = [&](int i, int at) {
     const unsigned l = lds0 + at * S::STAGE;
-    if (i < 3 * PA) sa.piece_of(i / PA, i % PA, l + i / PA * TA, wave);
-    else sb.piece_of((i - 3 * PA) / PB, (i - 3 * PA) % PB, l + 3 * TA + (i - 3 * PA) / PB * TB, wave);
+    if (i < PA) sa.piece_of(i / (PA / 3), i % (PA / 3), l + i / (PA / 3) * TA, wave);
+    else if (S::F32) sb.piece(i - PA, l + 3 * TA, wave);
+    else sb.piece_of((i - PA) / PB1, (i - PA) % PB1, l + 3 * TA + (i - PA) / PB1 * TB, wave);
   };
   ft_b8 fa[2][3][NI], fb[2][3][NJ];
+  float raw[NJ][8];
+  auto split = [&](int j, int h) { ft_split8(raw[j], fb[h][0][j], fb[h][1][j], fb[h][2][j]); };
   auto read = [&](int i, int h, int at) {             // in the order of use: both first planes, then the others
     const char* t = smem + at * S::STAGE;
-    const int pl = i / (NI + NJ), k = i % (NI + NJ);
-    if (k < NJ) fb[h][pl][k] = ft_frag<BMO, S::TN, 32>(t + 3 * TA + pl * TB, (wn * NJ + k) * 16, 0, lane);
-    else fa[h][pl][k - NJ] = ft_frag<AM, S::TM, 32>(t + pl * TA, (wm * NI + k - NJ) * 16, 0, lane);
+    if constexpr (S::F32) {
+      if (i < NJ) FtStageB<S, BMO>::read(t + 3 * TA, (wn * NJ + i) * 16 + (lane & 15), lane >> 4, raw[i]);
+      else fa[h][(i - NJ) / NI][(i - NJ) % NI] = ft_frag<AM, S::TM, 32>(t + (i - NJ) / NI * TA, (wm * NI + (i - NJ) % NI) * 16, 0, lane);
+    } else {
+      const int pl = i / (NI + NJ), k = i % (NI + NJ);
+      if (k < NJ) fb[h][pl][k] = ft_frag<BMO, S::TN, 32>(t + 3 * TA + pl * TB, (wn * NJ + k) * 16, 0, lane);
+      else fa[h][pl][k - NJ] = ft_frag<AM, S::TM, 32>(t + pl * TA, (wm * NI + k - NJ) * 16, 0, lane);
+    }
   };
   auto mfma = [&](int m, int h) {
     constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
@@ -353,8 +392,11 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
   ft_barrier();
 #pragma unroll
   for (int i = 0; i < NF; ++i) read(i, 0, 0);
-  constexpr int M0 = NM / 8, RM = (NM - M0) / NF;
-  static_assert(RM >= 1, "an MFMA to every read");
+  if constexpr (S::F32)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) split(j, 0);
+  constexpr int M0 = NM / 8, RM = (NM - M0) / NF, LATE = 4;
+  static_assert(RM >= 1 && (!S::F32 || LATE + 2 * NJ <= NF), "an MFMA to every read, and the splits' places");
   int at = 0;
   auto stage = [&](int h) {
     const int to = at + 1 == S::NS ? 0 : at + 1;
@@ -369,6 +411,8 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
 #pragma unroll
       for (int i = g * P / NF; i < (g + 1) * P / NF; ++i) piece(i, at);
       read(g, h ^ 1, to);
+      if constexpr (S::F32)
+        if (g >= LATE && (g - LATE) % 2 == 0 && (g - LATE) / 2 < NJ) split((g - LATE) / 2, h ^ 1);
 #pragma unroll
       for (int m = M0 + g * RM; m < (g + 1 < NF ? M0 + (g + 1) * RM : NM); ++m) mfma(m, h);
       __builtin_amdgcn_sched_barrier(0);
@@ -383,27 +427,15 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
   ft_barrier();
 }
 
-// eight fp32 values of a B fragment as the fragments of their three planes
-__device__ __forceinline__ void ft_split8(const float (&v)[8], ft_b8 (&f)[3]) {
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    float h[2], m[2], l[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) ft_split(v[i + j], h[j], m[j], l[j]);
-    ((unsigned*)&f[0])[i / 2] = f2bf2(h[0], h[1]);
-    ((unsigned*)&f[1])[i / 2] = f2bf2(m[0], m[1]);
-    ((unsigned*)&f[2])[i / 2] = f2bf2(l[0], l[1]);
-  }
-}
 template <class S, int BMO>
-__device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtRowsB<BMO, S::TN>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
+__device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtB32<BMO, S::TN, S::NW>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
                                           int lane) {
   static_assert(S::TM == 32 && S::NW == 4 && S::KS == 32 && S::PL == 3 && S::NI == 1, "two waves by two");
-  constexpr int PB = FtRowsB<BMO, S::TN>::NP, P = 2 + PB, TA = S::TM * 64;
+  constexpr int PB = FtB32<BMO, S::TN, S::NW>::NP, P = 2 + PB, TA = S::TM * 64;
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * 2, g = lane >> 4;
   long k0 = (long)kt0 * 64;
-  sb.seek(BMO == TK ? 2 * k0 : k0);
+  sb.seek(k0);
   auto put = [&](int at) {
     const unsigned l = lds0 + at * S::STAGE;
     sb.step();
@@ -428,19 +460,8 @@ __device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtRowsB<BMO, S::TN>& sb, 
 #pragma unroll
     for (int j = 0; j < S::NJ; ++j) {
       float v[8];
-      const int r = (wn * S::NJ + j) * 16 + (lane & 15);
-      if (BMO == TK) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const ft_f4 u = *(const ft_f4*)(tb + r * 128 + (((2 * g + h) ^ ft_tk_swz<64>(r)) << 4));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * h + i] = u[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = *(const float*)(tb + (8 * g + i) * (S::TN * 4) + (((r >> 3) ^ (((g & 1) << 2) | (i & 3))) << 5) + (r & 7) * 4);
-      }
-      ft_split8(v, fb[j]);
+      FtB32<BMO, S::TN, S::NW>::read(tb, (wn * S::NJ + j) * 16 + (lane & 15), g, v);
+      ft_split8(v, fb[j][0], fb[j][1], fb[j][2]);
     }
 #pragma unroll
     for (int q = 0; q < 6; ++q)
@@ -459,7 +480,7 @@ __device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtRowsB<BMO, S::TN>& sb, 
 template <class S, int AM, int BMO, int NPROD, int NJ>
 __device__ __forceinline__ void ft_loop(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
                                         ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  if constexpr (S::F32) ft_rows32<S, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  if constexpr (S::F32 && S::TM == 32) ft_rows32<S, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
   else if constexpr (S::PL == 3) ft_planes<S, AM, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
   else if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
   else ft_rows<S, AM, BMO, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
@@ -523,7 +544,7 @@ __device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld
 // C = A B^T written to `out` (bf16 for nprod 1, fp32 for 6), or as fp32 partial sums for ft_reduce().
 struct FtProduct {
   int am = TK, bm = TK, nprod = 1;
-  bool rows32 = false;            // fp32, few rows: B is the fp32 matrix itself (its ld in bf16 units)
+  bool b32 = false;               // fp32: B is the fp32 matrix itself (its ld in bf16 units), not its planes
   FtMat a, b;
   int M = 0, N = 0, K = 0;
   int Ks = 0;                     // > 0: the length that the slices are cut from, >= K (products added onto each other's partial sums)
@@ -597,8 +618,11 @@ struct FtPacks {                  // up to four of one type in one launch
   void add(const FtPack& q) { p[n] = q; first[n + 1] = first[n] + q.R * (q.ldd / 8); ++n; }
 };
 int ft_pack(const FtPacks& p, hipStream_t s);
-// fp32 few rows: how many, and whether B can be read where it is
-#define FT_ROWS32 64
+// rows up to which tiles are 32 rows high
+static inline bool ft_few(int nprod, long T) { return T <= (nprod == 1 ? 64 : 32); }
+// fp32: up to how many rows a weight is not worth laying out in planes, and whether it can be read where it is (or else from a copy)
+#define FT_B32 512
+static inline bool ft_b32(int dt, long T) { return !dt && T <= FT_B32; }
 static inline bool ft_direct32(const void* p, long ld, long cols) { return ((size_t)p & 15) == 0 && ld % 4 == 0 && cols % 4 == 0 && ld < (1L << 20); }
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
 static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }

@@ -58,6 +58,13 @@ int ft_pack(const FtPacks& p, hipStream_t s) {
   return 0;
 }
 
+typedef FtShape<256, 256, 2, 4, 2> FtBig;      // 128 KB of LDS, one workgroup a CU
+typedef FtShape<128, 128, 2, 2, 2> FtMid;      // 64 KB, two
+typedef FtShape<32, 64, 2, 2, 6> FtRow;        // 72 KB, two: few rows, the reading of B is what counts (TK x TK alone)
+typedef FtShape<128, 128, 2, 4, 3, 32, 3> FtPlanes;          // fp32, all in planes: 144 KB, one workgroup of eight waves a CU
+typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> FtMid32;     // fp32, B in 32 bits: 120 KB
+typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> FtRows32;      // the same of few rows: 70 KB, two
+
 // ---------------------------------------------------------------- the product
 // workgroup b of a product: into p.out, or (part) as partial sums
 template <class S, int AM, int BMO, int NPROD>
@@ -149,21 +156,16 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ft_group(FtGrou
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int b = blockIdx.x, i = b < g.first[1] ? 0 : b < g.first[2] ? 1 : 2;
   const FtProduct& p = g.p[i];
+  if constexpr (NPROD == 6) {
+    if (p.b32) return ft_product_tile<FtMid32, TK, TR, NPROD>(p, g.part[i], g.target[i], g.add[i], b - g.first[i], smem);
+  }
   if (p.am == TK) ft_product_tile<S, TK, TR, NPROD>(p, g.part[i], g.target[i], g.add[i], b - g.first[i], smem);
   else ft_product_tile<S, TR, TR, NPROD>(p, g.part[i], g.target[i], g.add[i], b - g.first[i], smem);
 }
 
-typedef FtShape<256, 256, 2, 4, 2> FtBig;      // 128 KB of LDS, one workgroup a CU
-typedef FtShape<128, 128, 2, 2, 2> FtMid;      // 64 KB, two
-typedef FtShape<32, 64, 2, 2, 6> FtRow;        // 72 KB, two: few rows, the reading of B is what counts (TK x TK alone)
-
-typedef FtShape<128, 128, 2, 4, 3, 32, 3> FtPlanes;   // fp32's only large tile: 144 KB, one workgroup of eight waves a CU
-
-typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> FtRows32;   // fp32, few rows: 70 KB, two
-
 struct FtCost { double step, fixed; int slots; };   // us a k-step with the chip full, us a tile besides, tiles at once
-static const FtCost kCost[5] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}, {2.6, 6.0, 256}, {1.0, 5.0, 512}};
-static const int kTM[5] = {256, 128, 32, 128, 32}, kTN[5] = {256, 128, 64, 128, 64};
+static const FtCost kCost[6] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}, {2.6, 6.0, 256}, {1.0, 5.0, 512}, {2.8, 6.0, 256}};
+static const int kTM[6] = {256, 128, 32, 128, 32, 128}, kTN[6] = {256, 128, 64, 128, 64, 128};
 
 // The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
 // step + time of a tile's start and end), plus the partial sums' way to memory and back.  The constants are measured: 256 x 256 tiles run
@@ -173,8 +175,8 @@ FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
   const int nprod = p.nprod;
   FtPlan best;
   double least = 1e30;
-  for (int sh = 0; sh < 5; ++sh) {
-    if (nprod == 6 ? sh != (p.rows32 ? 4 : 3) : sh > 2 || (sh == 2 && (p.am != TK || p.bm != TK || M > 64))) continue;
+  for (int sh = 0; sh < 6; ++sh) {
+    if (nprod == 6 ? sh != (!p.b32 ? 3 : ft_few(6, M) ? 4 : 5) : sh > 2 || (sh == 2 && (p.am != TK || p.bm != TK || !ft_few(1, M)))) continue;
     const long tiles = ((M + kTM[sh] - 1) / kTM[sh]) * ((N + kTN[sh] - 1) / kTN[sh]), nk = (K + 63) / 64;
     for (int want = 1; want <= 32; ++want) {
       const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want), nprod);
@@ -223,7 +225,7 @@ template <class S, int NPROD> static int by_mode(const FtProduct& p, const FtPla
   if constexpr (S::F32) {
     if (p.am == TK) return launch<S, TK, TR, NPROD>(p, pl, part, add, s);
   }
-  if constexpr (S::TN >= 128) {
+  if constexpr (S::TN >= 128 && !S::F32) {
     if (p.am == TK) return launch<S, TK, TR, NPROD>(p, pl, part, add, s);
     if (p.bm == TR) return launch<S, TR, TR, NPROD>(p, pl, part, add, s);
   }
@@ -238,7 +240,8 @@ int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hi
     case 1: return by_mode<FtMid, 1>(p, plan, part, add, s);
     case 2: return by_mode<FtRow, 1>(p, plan, part, add, s);
     case 3: return by_mode<FtPlanes, 6>(p, plan, part, add, s);
-    default: return by_mode<FtRows32, 6>(p, plan, part, add, s);
+    case 4: return by_mode<FtRows32, 6>(p, plan, part, add, s);
+    default: return by_mode<FtMid32, 6>(p, plan, part, add, s);
   }
 }
 
@@ -306,7 +309,7 @@ bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan) {
   const int sh = p[0].nprod == 1 ? 1 : 3, slots = kCost[sh].slots;
   double work = 0;
   for (int i = 0; i < n; ++i)
-    if (p[i].rows32) return false;
+    if (p[i].b32 && ft_few(6, p[i].M)) return false;
   for (int i = 0; i < n; ++i) work += (double)tiles_of(FtPlan{sh, 0}, p[i].M, p[i].N) * (double)((p[i].K + 63) / 64 * p[i].segs);
   if (work > 160.0 * slots) return false;
   const double share = work / slots / 2 > 4 ? work / slots / 2 : 4;

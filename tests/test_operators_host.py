@@ -51,7 +51,7 @@ def test_sizes_of_workspaces():
         # fp32: of few rows the weights are copied as they are or not at all; of many they become planes
         few = [L.fc_gated_mlp_workspace_bytes(0, 64, 64, 128, p, backward) for p in (0, 1)]
         assert few[1] == few[0] + 3 * 64 * 128 * 4
-        assert L.fc_gated_mlp_workspace_bytes(0, 65, 64, 128, 0, backward) == L.fc_gated_mlp_workspace_bytes(0, 65, 64, 128, 1, backward) > few[1]
+        assert L.fc_gated_mlp_workspace_bytes(0, 513, 64, 128, 0, backward) == L.fc_gated_mlp_workspace_bytes(0, 513, 64, 128, 1, backward) > few[1]
         few = [L.fc_linear_ce_workspace_bytes(0, 64, 1000, 64, p, backward) for p in (0, 1)]
         assert few[1] == few[0] + 1000 * 64 * 4
     # the logits' gradient is held in pieces, however large the vocabulary
