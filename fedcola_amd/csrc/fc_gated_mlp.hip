@@ -22,8 +22,9 @@ struct GmArgs {
   long up;                      // rows between a unit's gate and up row in w_in
   bf16_t *h, *dgu;              // planes of [T][ldh], [T][2 ldh]: h; dg | du
   long ldh;                     // whole 128-byte lines: a row that straddles one more costs every tile load an L2 request more
-  const float* dh;              // [T][ldd]
+  const float* dh;              // [dh_parts][T][ldd], to be added up
   long ldd;
+  int dh_parts;
 };
 
 // act(g) and act'(g); FAST: through v_exp_f32 and v_rcp_f32, for bf16 operands
@@ -109,7 +110,10 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a
       for (int j = 0; j < J; ++j) {
         const int m = m0 + (wm * S::NI + i) * 16 + (lane & 15), f = f0 + wn * J * 16 + 16 * j + 4 * (lane >> 4);
         const bool in = m < a.T && f < a.ldd;                   // (ldd is F in whole eights, the columns in between are zeros)
-        const ft_f4 v = *(const ft_f4*)(a.dh + (in ? (long)m * a.ldd + f : 0));
+        const float* at = a.dh + (in ? (long)m * a.ldd + f : 0);
+        ft_f4 v = *(const ft_f4*)at;
+        if (S::TM < 256)                                        // (the large tile's registers are full, and its products are long enough unsliced)
+          for (int q = 1; q < a.dh_parts; ++q) v += *(const ft_f4*)(at + (long)q * a.T * a.ldd);
         d[j] = in ? v : ft_f4{0.f, 0.f, 0.f, 0.f};
       }
     }
@@ -169,19 +173,20 @@ template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& 
 // 256 x 256 tiles once they fill half of the chip, 128 x 128 below, 32 x 64 for a few rows.  Backward: 256 x 256 only where the product is long;
 // the epilogue (8 bytes a unit in, 6 out) stands still while it runs, and two 128 x 128 workgroups a CU cover each other's (12608 x 384 x 1024:
 // 50 us against 70; 8192 x 4096 x 11000 the other way, 1571 against 1333)
+static bool gm_big(int dt, long T, long D, long F, bool grad) { return dt && ((T + 255) / 256) * ((F + 127) / 128) >= 128 && (!grad || D >= 1024); }
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
   if constexpr (NPROD == 6) {
     return !a.b32 ? gm_act_launch<GmPlanes, NPROD, GRAD>(a, s) : ft_few(6, a.T) ? gm_act_launch<GmRows32, NPROD, GRAD>(a, s) : gm_act_launch<GmMid32, NPROD, GRAD>(a, s);
   } else {
     if (ft_few(1, a.T)) return gm_act_launch<GmRow, NPROD, GRAD>(a, s);
-    if ((long)((a.T + 255) / 256) * ((a.F + 127) / 128) >= 128 && (!GRAD || a.D >= 1024)) return gm_act_launch<GmBig, NPROD, GRAD>(a, s);
+    if (gm_big(1, a.T, a.D, a.F, GRAD)) return gm_act_launch<GmBig, NPROD, GRAD>(a, s);
     return gm_act_launch<GmMid, NPROD, GRAD>(a, s);
   }
 }
 
 // fp32, few rows: the weights are read where they are, or from a copy in 32 bits (the up rows within a tile load's reach), and split in registers
 static bool gm_b32(int dt, long T, long D, long F) { return ft_b32(dt, T) && (F + 512) * ft_up(D, 64) < (1L << 29); }
-struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan[3]; bool group; };
+struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan_dh, plan[3]; bool group; };
 // dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
 static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProduct (&p)[3]) {
   p[0].b32 = a.b32;
@@ -200,6 +205,13 @@ static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProdu
   p[2].M = (int)D; p[2].N = (int)F;
   p[2].a = a.dy;
   p[2].b.p = a.h; p[2].b.ld = Fp; p[2].b.plane = T * Fp;
+}
+// dh = dy w_out, whose slices' sums the activation's pass adds up
+static FtProduct gm_dh_product(int dt, long T, long D, long F, bool b32) {
+  FtProduct p;
+  p.am = TK; p.bm = TR; p.nprod = dt ? 1 : 6; p.b32 = b32;
+  p.M = (int)T; p.N = (int)F; p.K = (int)D;
+  return p;
 }
 static FtProduct gm_y_product(int dt, long T, long D, long F, bool b32) {
   FtProduct p;
@@ -227,7 +239,9 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backwa
     return z;
   }
   z.dgu = ft_up(T * 2 * Fp * e, 256);
-  z.dh = ft_up(ft_part_ld(F) * T * 4, 256);
+  z.plan_dh = ft_plan(gm_dh_product(dt, T, D, F, b32), false);
+  if (gm_big(dt, T, D, F, true)) z.plan_dh.target = 0;
+  z.dh = ft_up(ft_part_floats(T, F, z.plan_dh) * 4, 256);
   FtProduct p[3];
   GmArgs a = {};
   a.b32 = b32;
@@ -341,16 +355,11 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   ws += z.dgu;
   char* part = ws + z.dh;
   if (T) {
-    FtProduct p;
-    p.nprod = dt ? 1 : 6;
-    p.b32 = a.b32;
-    p.am = TK; p.bm = TR;
+    FtProduct p = gm_dh_product(dt, T, D, F, a.b32);
     p.a = a.dy;
     p.b = a.w_out;
-    p.M = T; p.N = F; p.K = D;
-    FtPlan plan = ft_plan(p, false);
-    plan.target = 0;                                           // one slice: its partial sums are dh
-    FC_TRY(ft_product(p, plan, (float*)ws, false, s));
+    FC_TRY(ft_product(p, z.plan_dh, (float*)ws, false, s));
+    a.dh_parts = ft_parts(p, z.plan_dh);
     a.dh = (const float*)ws;
     a.ldd = ft_part_ld(F);
     FC_TRY(dt ? (gm_act_run<1, true>(a, s)) : (gm_act_run<6, true>(a, s)));

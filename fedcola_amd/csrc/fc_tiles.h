@@ -575,6 +575,7 @@ __host__ __device__ static inline int ft_slices(long tiles, long K, int target, 
   return s < 1 ? 1 : s > 32 ? 32 : (int)s;
 }
 size_t ft_part_floats(long M, long N, const FtPlan& plan);     // for any number of rows up to M
+int ft_parts(const FtProduct& p, const FtPlan& plan);          // slices of a product whose rows are all there
 // partial sums [slices][rows there][ft_part_ld(N)] into `part` (or, part null, the product into p.out); add: onto what is there
 int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hipStream_t s);
 // up to three products in one launch, and the sums of their slices in one

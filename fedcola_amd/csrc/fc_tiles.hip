@@ -202,12 +202,13 @@ size_t ft_part_floats(long M, long N, const FtPlan& pl) {
   return (size_t)wg * kTM[pl.shape] * kTN[pl.shape];
 }
 
+int ft_parts(const FtProduct& p, const FtPlan& pl) { return ft_slices(tiles_of(pl, p.M, p.N), (long)(p.Ks ? p.Ks : p.K) * p.segs, pl.target, p.nprod); }
 // workgroups of a product: rows really there may be fewer, and the slices then more, but never more of both than this
 static long workgroups(const FtProduct& p, const FtPlan& pl, bool part) {
   const long tiles = tiles_of(pl, p.M, p.N);
   if (!part) return tiles;
   if (p.Mdyn) return tiles > pl.target ? tiles : pl.target;
-  return tiles * ft_slices(tiles, (long)(p.Ks ? p.Ks : p.K) * p.segs, pl.target, p.nprod);
+  return tiles * ft_parts(p, pl);
 }
 template <class S, int AM, int BMO, int NPROD>
 static int launch(const FtProduct& p, const FtPlan& pl, float* part, bool add, hipStream_t s) {
