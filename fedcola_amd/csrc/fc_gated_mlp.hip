@@ -109,12 +109,13 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int m = m0 + (wm * S::NI + i) * 16 + (lane & 15), f = f0 + wn * J * 16 + 16 * j + 4 * (lane >> 4);
-        const bool in = m < a.T && f < a.ldd;                   // (ldd is F in whole eights, the columns in between are zeros)
+        const bool in = m < a.T && f < a.ldd;                   // (ldd is F in whole eights)
         const float* at = a.dh + (in ? (long)m * a.ldd + f : 0);
         ft_f4 v = *(const ft_f4*)at;
         if (S::TM < 256)                                        // (the large tile's registers are full, and its products are long enough unsliced)
           for (int q = 1; q < a.dh_parts; ++q) v += *(const ft_f4*)(at + (long)q * a.T * a.ldd);
-        d[j] = in ? v : ft_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) d[j][x] = in && f + x < a.F ? v[x] : 0.f;
       }
     }
 #pragma unroll
@@ -184,8 +185,6 @@ template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream
   }
 }
 
-// fp32, few rows: the weights are read where they are, or from a copy in 32 bits (the up rows within a tile load's reach), and split in registers
-static bool gm_b32(int dt, long T, long D, long F) { return ft_b32(dt, T) && (F + 512) * ft_up(D, 64) < (1L << 29); }
 struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan_dh, plan[3]; bool group; };
 // dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
 static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProduct (&p)[3]) {
@@ -220,18 +219,17 @@ static FtProduct gm_y_product(int dt, long T, long D, long F, bool b32) {
   p.M = (int)T; p.N = (int)D; p.K = (int)F;
   return p;
 }
-static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backward) {
+// b32: fp32 weights read where they are; packed: what is not planes anyway is laid out
+static GmSizes gm_sizes(int dt, long T, long D, long F, bool b32, bool packed, bool backward) {
   GmSizes z = {};
   const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6;
-  const bool b32 = gm_b32(dt, T, D, F);
   if (packed || !dt) {
     z.x = ft_up(T * Dp * e, 256);
     z.dy = backward ? z.x : 0;
   }
-  if (packed) {
-    const long we = b32 ? 4 : e;
-    z.w_in = ft_up(2 * F * Dp * we, 256);
-    z.w_out = ft_up(D * Fp * we, 256);
+  if (dt ? packed : !b32) {
+    z.w_in = ft_up(2 * F * Dp * e, 256);
+    z.w_out = ft_up(D * Fp * e, 256);
   }
   z.h = ft_up(T * Fp * e, 256);
   if (!backward) {
@@ -259,19 +257,21 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool packed, bool backwa
 }
 static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.dh + z.part; }
 
-// a matrix as the products take it: where it is, or as one of the packs.  whole: an fp32 one that is not split into planes.
-static bool gm_whole(const void* p, long ld, long R, long C) { return ft_direct32(p, ld, C) && (R + 512) * ld < (1L << 29); }
-static void gm_matrix(int dt, bool whole, bool direct, const void* p, long ld, long R, long C, char*& ws, FtMat& m, FtPacks& l) {
-  const int units = whole ? 2 : 1;
-  if (direct) {
+// a matrix as the products take it: where it is, or as one of the packs
+static void gm_matrix(int dt, bool b32, const void* p, long ld, long R, long C, char*& ws, FtMat& m, FtPacks& l) {
+  if (b32) {
+    m = ft_mat32(p, ld, R, C);
+    return;
+  }
+  if (ft_direct(dt, p, ld, C)) {
     m.p = (const bf16_t*)p;
-    m.ld = units * ld;
+    m.ld = ld;
     return;
   }
   FtPack k;
-  k.src = p; k.lds = ld; k.dt = dt; k.whole = whole; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 64);
-  m.p = k.dst; m.ld = units * k.ldd; m.plane = R * k.ldd;
-  ws += ft_up((dt ? 2 : whole ? 4 : 6) * R * k.ldd, 256);
+  k.src = p; k.lds = ld; k.dt = dt; k.R = R; k.C = C; k.dst = (bf16_t*)ws; k.ldd = ft_up(C, 64);
+  m.p = k.dst; m.ld = k.ldd; m.plane = R * k.ldd;
+  ws += ft_up((dt ? 2 : 6) * R * k.ldd, 256);
   l.add(k);
 }
 struct GmCall { int dt, act; long T, D, F; const void *x, *w_in, *w_out, *dy; long ldx, ld_in, ld_out, lddy; };
@@ -287,40 +287,36 @@ static int gm_check(const char* what, const GmCall& c, const void* ws) {
   FC_REQUIRE(((size_t)ws & 255) == 0, "%s: the workspace is aligned to 256 bytes", what);
   return ft_check_device(c.w_in, what);
 }
-// which of w_in and w_out is read where it is, and whether all operands of the type's are (fp32: the weights alone, x and dy become planes)
-static bool gm_direct(const GmCall& c, bool b32, bool& in, bool& out) {
-  in = b32 ? gm_whole(c.w_in, c.ld_in, c.F, c.D) : ft_direct(c.dt, c.w_in, c.ld_in, c.D);
-  out = b32 ? gm_whole(c.w_out, c.ld_out, 0, c.F) : ft_direct(c.dt, c.w_out, c.ld_out, c.F);
-  return in && out && (!c.dt || (ft_direct(c.dt, c.x, c.ldx, c.D) && (!c.dy || ft_direct(c.dt, c.dy, c.lddy, c.D))));
+static bool gm_direct(const GmCall& c) {
+  return ft_direct(c.dt, c.x, c.ldx, c.D) && ft_direct(c.dt, c.w_in, c.ld_in, c.D) && ft_direct(c.dt, c.w_out, c.ld_out, c.F) &&
+         (!c.dy || ft_direct(c.dt, c.dy, c.lddy, c.D));
+}
+// fp32, few rows: both weights are read where they are, where the up rows are within a tile load's reach
+static bool gm_b32(const GmCall& c) {
+  return ft_b32(c.dt, c.T, c.w_in, c.ld_in) && ft_b32(c.dt, c.T, c.w_out, c.ld_out) && (c.F + 512) * c.ld_in < (1L << 29);
 }
 // the operands as the products take them; what of them cannot be taken as it is goes to the workspace
 static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
-  bool in, out;
-  a.b32 = gm_b32(c.dt, c.T, c.D, c.F);
-  gm_direct(c, a.b32, in, out);
+  a.b32 = gm_b32(c);
   a.T = (int)c.T; a.D = (int)c.D; a.F = (int)c.F; a.act = c.act; a.up = c.F; a.ldh = ft_up(c.F, 64);
   FtPacks l;
-  gm_matrix(c.dt, false, ft_direct(c.dt, c.x, c.ldx, c.D), c.x, c.ldx, c.T, c.D, ws, a.x, l);
-  if (c.dy) gm_matrix(c.dt, false, ft_direct(c.dt, c.dy, c.lddy, c.D), c.dy, c.lddy, c.T, c.D, ws, a.dy, l);
-  gm_matrix(c.dt, a.b32, out, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
-  gm_matrix(c.dt, a.b32, in, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
+  gm_matrix(c.dt, false, c.x, c.ldx, c.T, c.D, ws, a.x, l);
+  if (c.dy) gm_matrix(c.dt, false, c.dy, c.lddy, c.T, c.D, ws, a.dy, l);
+  gm_matrix(c.dt, a.b32, c.w_out, c.ld_out, c.D, c.F, ws, a.w_out, l);
+  gm_matrix(c.dt, a.b32, c.w_in, c.ld_in, 2 * c.F, c.D, ws, a.w_in, l);
   return ft_pack(l, s);
-}
-static GmSizes gm_call_sizes(const GmCall& c, bool backward) {
-  bool in, out;
-  return gm_sizes(c.dt, c.T, c.D, c.F, !gm_direct(c, gm_b32(c.dt, c.T, c.D, c.F), in, out), backward);
 }
 
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
   if (T < 0 || D < 1 || F < 1) return 0;
-  return gm_total(gm_sizes(dt, T, D, F, packed || (!dt && !gm_b32(dt, T, D, F)), backward != 0)) + 256;
+  return gm_total(gm_sizes(dt, T, D, F, !dt && !packed && T <= FT_B32, packed || F % 8 || D % 8, backward != 0)) + 256;
 }
 extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t ldx, const void* w_in, int64_t ld_in, const void* w_out, int64_t ld_out,
                                 int32_t T, int32_t D, int32_t F, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   GmCall c = {dt, act, T, D, F, x, w_in, w_out, nullptr, ldx, ld_in, ld_out, 0};
   FC_TRY(gm_check("fc_gated_mlp_fwd", c, workspace));
   FC_REQUIRE((y || T == 0) && ldy >= D, "fc_gated_mlp_fwd: output missing or its rows %ld apart", (long)ldy);
-  const GmSizes z = gm_call_sizes(c, false);
+  const GmSizes z = gm_sizes(dt, T, D, F, gm_b32(c), !gm_direct(c), false);
   FC_REQUIRE(workspace_bytes >= gm_total(z), "fc_gated_mlp_fwd: workspace too small");
   if (T == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
@@ -343,7 +339,7 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   FC_TRY(gm_check("fc_gated_mlp_bwd", c, workspace));
   FC_REQUIRE((dy || T == 0) && lddy >= D && lddy < (1L << 21) && (!dx || lddx >= D) && (!dw_in || ldd_in >= D) && (!dw_out || ldd_out >= F),
              "fc_gated_mlp_bwd: dy missing, or rows too close");
-  const GmSizes z = gm_call_sizes(c, true);
+  const GmSizes z = gm_sizes(dt, T, D, F, gm_b32(c), !gm_direct(c), true);
   FC_REQUIRE(workspace_bytes >= gm_total(z), "fc_gated_mlp_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;

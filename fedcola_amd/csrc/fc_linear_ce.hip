@@ -110,6 +110,7 @@ template <int NPROD> __device__ __forceinline__ CePart ce_join(CePart a, CePart 
 
 struct CeArgs {
   FtMat x, w;
+  bool b32;                   // fp32: w is the fp32 matrix itself
   int T, V, D, v0, nv;        // this launch's columns [v0, v0 + nv) of the vocabulary
   const int *n, *y, *idx;
   CePart* part;               // [tiles of columns][T]
@@ -300,8 +301,8 @@ typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
 typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> CeRows32;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> CeMid32;
 // 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32, 32 x 64 for the few rows of a scoring call
-static int ce_shape(int dt, long T, long V) {
-  if (ft_few(dt ? 1 : 6, T)) return 2;
+static int ce_shape(int dt, long T, long V, bool b32) {
+  if ((dt || b32) && ft_few(dt ? 1 : 6, T)) return 2;
   return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
@@ -324,7 +325,7 @@ template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, h
 template <bool GRAD> static int ce_run(int dt, int shape, const CeArgs& a, hipStream_t s) {
   if (a.T == 0 || a.nv == 0) return 0;
   if (dt) return shape == 0 ? ce_launch<CeBig, 1, GRAD>(a, s) : shape == 1 ? ce_launch<CeMid, 1, GRAD>(a, s) : ce_launch<CeRow, 1, GRAD>(a, s);
-  return shape != 1 ? ce_launch<CeRows32, 6, GRAD>(a, s) : ft_b32(dt, a.T) ? ce_launch<CeMid32, 6, GRAD>(a, s) : ce_launch<CePlanes, 6, GRAD>(a, s);
+  return shape != 1 ? ce_launch<CeRows32, 6, GRAD>(a, s) : a.b32 ? ce_launch<CeMid32, 6, GRAD>(a, s) : ce_launch<CePlanes, 6, GRAD>(a, s);
 }
 
 // columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
@@ -334,15 +335,16 @@ static long ce_piece(int dt, long T, long V) {
 }
 struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx, dw; bool group; };
 // dx = dL w and dw = dL^T x of nv columns; n: device, the rows that count
-static void ce_products(int dt, long T, long D, long nv, const int* n, FtProduct& x, FtProduct& w) {
-  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.b32 = ft_b32(dt, T); x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
+static void ce_products(int dt, long T, long D, long nv, bool b32, const int* n, FtProduct& x, FtProduct& w) {
+  x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.b32 = b32; x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
   w.am = TR; w.bm = TR; w.nprod = x.nprod; w.M = (int)nv; w.N = (int)D; w.K = (int)T; w.Kdyn = n;
 }
 static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad) {
   CeSizes z = {};
-  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : ft_b32(dt, T) ? 4 : 6) * V * ft_up(D, 64), 256);
+  const bool b32 = !dt && direct_w;
+  z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : 6) * V * ft_up(D, 64), 256);
   if (!grad) {
-    const int tn = ce_tn(ce_shape(dt, T, V));
+    const int tn = ce_tn(ce_shape(dt, T, V, b32));
     z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
     z.rows = (size_t)ft_up(T * 4, 256) * 2;
     return z;
@@ -352,7 +354,7 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
   if (z.piece >= V) {                     // one piece: its two products may run together
     FtProduct p[2];
     FtPlan plan[2];
-    ce_products(dt, T, D, V, nullptr, p[0], p[1]);
+    ce_products(dt, T, D, V, b32, nullptr, p[0], p[1]);
     if (ft_group_plan(p, 2, plan)) {
       z.group = true;
       z.dx = plan[0];
@@ -363,7 +365,7 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
     }
   }
   FtProduct px, pw;
-  ce_products(dt, T, D, z.piece, nullptr, px, pw);
+  ce_products(dt, T, D, z.piece, b32, nullptr, px, pw);
   z.dx = ft_plan(px, true);
   z.dxp = (size_t)ft_up(ft_part_floats(T, D, z.dx) * 4, 256);
   for (long nv : {z.piece < V ? z.piece : V, V % z.piece}) {
@@ -380,19 +382,16 @@ static int ce_args(const char* what, int dt, long T, long V, long D, long ldw, c
   return ft_check_device(w, what);
 }
 // the weight as the products take it: where it is, or laid out in the workspace
-static bool ce_direct(int dt, const void* w, long ldw, long T, long D) { return ft_b32(dt, T) ? ft_direct32(w, ldw, D) : ft_direct(dt, w, ldw, D); }
-static int ce_weight(int dt, const void* w, long ldw, long T, long V, long D, char*& ws, FtMat& m, hipStream_t s) {
-  const bool whole = ft_b32(dt, T);
-  const int units = whole ? 2 : 1;
-  if (ce_direct(dt, w, ldw, T, D)) {
-    m.p = (const bf16_t*)w;
-    m.ld = units * ldw;
+static bool ce_direct(int dt, const void* w, long ldw, long T, long D) { return dt ? ft_direct(dt, w, ldw, D) : ft_b32(dt, T, w, ldw); }
+static int ce_weight(int dt, const void* w, long ldw, bool direct, long V, long D, char*& ws, FtMat& m, hipStream_t s) {
+  if (direct) {
+    if (dt) { m.p = (const bf16_t*)w; m.ld = ldw; } else { m = ft_mat32(w, ldw, V, D); }
     return 0;
   }
   FtPack k;
-  k.src = w; k.lds = ldw; k.dt = dt; k.whole = whole; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64);
-  m.p = k.dst; m.ld = units * k.ldd; m.plane = V * k.ldd;
-  ws += (size_t)ft_up((dt ? 2 : whole ? 4 : 6) * V * k.ldd, 256);
+  k.src = w; k.lds = ldw; k.dt = dt; k.R = V; k.C = D; k.dst = (bf16_t*)ws; k.ldd = ft_up(D, 64);
+  m.p = k.dst; m.ld = k.ldd; m.plane = V * k.ldd;
+  ws += (size_t)ft_up((dt ? 2 : 6) * V * k.ldd, 256);
   FtPacks l;
   l.add(k);
   return ft_pack(l, s);
@@ -401,7 +400,7 @@ static int ce_weight(int dt, const void* w, long ldw, long T, long V, long D, ch
 extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t D) { return T < 0 || D < 1 ? 0 : ce_saved(nullptr, dt, T, D).bytes; }
 extern "C" size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward) {
   if (T < 0 || V < 1 || D < 1) return 0;
-  const CeSizes z = ce_sizes(dt, T, V, D, !packed, backward != 0);
+  const CeSizes z = ce_sizes(dt, T, V, D, !packed && (dt || T <= FT_B32), backward != 0);
   return z.w + z.part + z.rows + z.dl + z.dxp + z.dwp + 256;
 }
 extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
@@ -418,8 +417,9 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   CeArgs a = {};
-  FC_TRY(ce_weight(dt, w, ldw, T, V, D, ws, a.w, s));
+  FC_TRY(ce_weight(dt, w, ldw, direct, V, D, ws, a.w, s));
   a.x = sv.x;
+  a.b32 = !dt && direct;
   a.T = T; a.V = V; a.D = D; a.v0 = 0; a.nv = V;
   a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
   a.part = (CePart*)ws;
@@ -434,7 +434,7 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
     hipLaunchKernelGGL((k_ce_rows<float, 3>), dim3(blocks), dim3(256), 0, s, (const float*)x, (long)ldx, y, (long)T, R, V, ignore_index, D, false, sv);
   }
   FC_LAUNCH_CHECK();
-  const int shape = ce_shape(dt, T, V), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
+  const int shape = ce_shape(dt, T, V, a.b32), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
   FC_TRY(ce_run<false>(dt, shape, a, s));
   if (T) {
     const dim3 gj((unsigned)(T <= 64 ? T : (T + 15) / 16));
@@ -464,8 +464,9 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   CeArgs a = {};
-  FC_TRY(ce_weight(dt, w, ldw, T, V, D, ws, a.w, s));
+  FC_TRY(ce_weight(dt, w, ldw, direct, V, D, ws, a.w, s));
   a.x = sv.x;
+  a.b32 = !dt && direct;
   a.T = T; a.V = V; a.D = D;
   a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
   a.lse = sv.lse; a.g = gloss; a.reduction = reduction;
@@ -476,7 +477,7 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   float* dwp = (float*)(ws + z.dl + z.dxp);
   const int es = dt ? 2 : 4;
   FtProduct px, pw;
-  ce_products(dt, T, D, z.piece, sv.n, px, pw);
+  ce_products(dt, T, D, z.piece, a.b32, sv.n, px, pw);
   px.out = dx; px.ldo = lddx;
   px.a.p = a.dl; px.a.ld = a.ldl; px.a.plane = a.plane;
   pw.a = px.a;
@@ -489,7 +490,7 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   for (long v0 = 0; v0 < V; v0 += z.piece) {
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < z.piece ? V - v0 : z.piece);
-    FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv), a, s));
+    FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv, a.b32), a, s));
     if (z.group) {
       px.K = pw.M = a.nv;
       px.b = a.w;

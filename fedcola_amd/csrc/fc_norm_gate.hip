@@ -7,7 +7,7 @@
 // it holds.  h comes from r before r is rounded.
 // Backward: r and both norms' statistics are formed again from y and x, so nothing is kept and dwn, dwp are those of the unrounded r.
 // Bound: HBM, 4 T D elements forward (y, x in; r, h out), 6 T D backward (y, x, dr, dh in; dy, dx out).
-// A row is held in registers by a wave (D <= 512), 4 waves (<= 2048) or 8 (<= 8192): 8 or 16 values a lane.  A workgroup walks several
+// A row is held in registers by a wave (D <= 1024), 4 waves (<= 2048, backward <= 4096) or 8 (<= 8192): 8 or 16 values a lane.  A workgroup walks several
 // rows with the weight vectors in registers (forward) or LDS (backward): read per row they would be 20 bytes an element from L2 beside the 8
 // from HBM.  The next row is loaded while this one is summed.  Measured at the rate of a large copy (4.9 TB/s) for 65536 x 4096 bf16: 417 us
 // forward (5.1 TB/s), 667 us backward (4.8 TB/s); 12608 x 384: 13 and 27 us, where filling and draining the chip is most of the time.
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(1024) k_ng_sum(const float* part, int D, long 
 
 // ---------------------------------------------------------------- host
 // Waves of a row and values of a lane.  A wave alone needs no barriers for its sums, so one takes a row as long as 16 values a lane are enough
-// (12608 x 768 bf16: 14 and 40 us forward and backward, of four waves of 8 values about 80 and 90); above, backward 16 values leave two workgroups a
+// (12608 x 768 bf16: 19 and 41 us forward and backward, 30 and 67 by four waves of 8 values; 16384 x 1024: 30 and 50, 39 and 82); above, backward 16 values leave two workgroups a
 // CU instead of one of twice the waves (65536 x 4096 bf16: 667 us against 1151), forward 8 are as good.
 static void ng_form(long D, bool bwd, int& W, int& E) {
   W = D <= 1024 ? 1 : D <= 2048 || (bwd && D <= 4096) ? 4 : 8;

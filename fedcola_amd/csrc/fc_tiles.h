@@ -34,6 +34,7 @@ enum { TK = 0, TR = 1 };
 struct FtMat {
   const bf16_t* p = nullptr;
   long ld = 0, plane = 0;
+  const bf16_t* end = nullptr;     // an fp32 matrix read where it is (FtB32): one past its last element
 };
 
 __device__ __forceinline__ int ft_wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
@@ -175,15 +176,30 @@ struct FtRowsA {
   }
 };
 // An fp32 B that is read where it is, in 32 bits, and split when its fragments are formed: its tile is a bf16 stager's with two columns to a
-// value, [rows][64] (TK) or [32][2 columns] (TR).
+// value, [rows][64] (TK) or [32][2 columns] (TR).  Any alignment of a float does: buffer loads of 16 bytes start at any dword and are clipped at the
+// descriptor's size dword by dword.  What a row's last 16 bytes take of the next row is masked (TK) or belongs to columns that are not there (TR).
 template <int MODE, int W, int NW> struct FtB32 : FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, NW> {
   typedef FtStager<MODE, MODE == TK ? W : 2 * W, MODE == TK ? 64 : 32, NW> Base;
+  const bf16_t* end;
   // the matrix' ld counts bf16 units, two to a value
   template <class F> __device__ __forceinline__ void init(const FtMat& m, long base, int K_, int wave, int lane, F map) {
+    end = m.end;
     if (MODE == TK) Base::init(m, base, 2 * K_, wave, lane, map);
     else Base::init(m, base, K_, wave, lane, [&](int r) { const long c = map(r >> 1); return c < 0 ? -1L : 2 * c; });
   }
   __device__ __forceinline__ void seek(long k0) { Base::seek(MODE == TK ? 2 * k0 : k0); }
+  __device__ __forceinline__ int left_at(long k0) const { return (int)((MODE == TK ? this->K / 2 : this->K) - k0); }
+  __device__ __forceinline__ void step() {
+    Base::step();
+    const long rest = (end - this->cur) * 2;
+    this->r = ft_rsrc(this->cur, MODE == TK || rest < this->cur_bytes ? rest : this->cur_bytes);
+  }
+  // a stage with `left` k to come
+  static __device__ __forceinline__ void mask(int left, int g, float (&v)[8]) {
+    if (MODE == TK && left < 32)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 8 * g + i < left ? v[i] : 0.f;
+  }
   // eight k of column r (the lane's)
   static __device__ __forceinline__ void read(const char* t, int r, int g, float (&v)[8]) {
     if (MODE == TK) {
@@ -365,7 +381,11 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
   };
   ft_b8 fa[2][3][NI], fb[2][3][NJ];
   float raw[NJ][8];
-  auto split = [&](int j, int h) { ft_split8(raw[j], fb[h][0][j], fb[h][1][j], fb[h][2][j]); };
+  int left = 0;                                       // k from the stage that is read on (F32)
+  auto split = [&](int j, int h) {
+    if constexpr (S::F32) FtStageB<S, BMO>::mask(left, lane >> 4, raw[j]);
+    ft_split8(raw[j], fb[h][0][j], fb[h][1][j], fb[h][2][j]);
+  };
   auto read = [&](int i, int h, int at) {             // in the order of use: both first planes, then the others
     const char* t = smem + at * S::STAGE;
     if constexpr (S::F32) {
@@ -392,15 +412,18 @@ __device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>&
   ft_barrier();
 #pragma unroll
   for (int i = 0; i < NF; ++i) read(i, 0, 0);
-  if constexpr (S::F32)
+  if constexpr (S::F32) {
+    left = sb.left_at((long)kt0 * 64);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) split(j, 0);
+  }
   constexpr int M0 = NM / 8, RM = (NM - M0) / NF, LATE = 4;
   static_assert(RM >= 1 && (!S::F32 || LATE + 2 * NJ <= NF), "an MFMA to every read, and the splits' places");
   int at = 0;
   auto stage = [&](int h) {
     const int to = at + 1 == S::NS ? 0 : at + 1;
     next();
+    if (S::F32) left -= 32;
 #pragma unroll
     for (int m = 0; m < M0; ++m) mfma(m, h);
     __builtin_amdgcn_sched_barrier(0);
@@ -435,6 +458,7 @@ __device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtB32<BMO, S::TN, S::NW>&
   const unsigned lds0 = ft_lds_addr(smem);
   const int steps = (kt1 - kt0) * 2, g = lane >> 4;
   long k0 = (long)kt0 * 64;
+  int left = sb.left_at(k0);
   sb.seek(k0);
   auto put = [&](int at) {
     const unsigned l = lds0 + at * S::STAGE;
@@ -460,7 +484,8 @@ __device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtB32<BMO, S::TN, S::NW>&
 #pragma unroll
     for (int j = 0; j < S::NJ; ++j) {
       float v[8];
-      FtB32<BMO, S::TN, S::NW>::read(tb, (wn * S::NJ + j) * 16 + (lane & 15), g, v);
+      sb.read(tb, (wn * S::NJ + j) * 16 + (lane & 15), g, v);
+      sb.mask(left, g, v);
       ft_split8(v, fb[j][0], fb[j][1], fb[j][2]);
     }
 #pragma unroll
@@ -470,6 +495,7 @@ __device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtB32<BMO, S::TN, S::NW>&
         constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
         acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j][qb[q]], fa[qa[q]], acc[0][j], 0, 0, 0);
       }
+    left -= 32;
     free_slot = slot;
     slot = slot + 1 == S::NS ? 0 : slot + 1;
   }
@@ -607,7 +633,6 @@ struct FtPack {
   const void* src = nullptr;
   long lds = 0;                   // elements between source rows
   int dt = 1;
-  bool whole = false;             // fp32 kept in 32 bits: dst is fp32, ldd counts values
   long R = 0, C = 0;
   bf16_t* dst = nullptr;
   long ldd = 0;                   // multiple of 64, >= C: the columns in between are written as zeros
@@ -621,10 +646,16 @@ struct FtPacks {                  // up to four of one type in one launch
 int ft_pack(const FtPacks& p, hipStream_t s);
 // rows up to which tiles are 32 rows high
 static inline bool ft_few(int nprod, long T) { return T <= (nprod == 1 ? 64 : 32); }
-// fp32: up to how many rows a weight is not worth laying out in planes, and whether it can be read where it is (or else from a copy)
+// fp32: up to how many rows a weight is not worth laying out in planes, and whether it can be read where it is
 #define FT_B32 512
-static inline bool ft_b32(int dt, long T) { return !dt && T <= FT_B32; }
-static inline bool ft_direct32(const void* p, long ld, long cols) { return ((size_t)p & 15) == 0 && ld % 4 == 0 && cols % 4 == 0 && ld < (1L << 20); }
+static inline bool ft_b32(int dt, long T, const void* p, long ld) { return !dt && T <= FT_B32 && ((size_t)p & 3) == 0 && ld < (1L << 20); }
+static inline FtMat ft_mat32(const void* p, long ld, long R, long C) {
+  FtMat m;
+  m.p = (const bf16_t*)p;
+  m.ld = 2 * ld;
+  m.end = m.p + 2 * ((R - 1) * ld + C);
+  return m;
+}
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
 static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }
 // > 64 KB of LDS for a kernel: asked for once on each device (a static of the launch that needs it)

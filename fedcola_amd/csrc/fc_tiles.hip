@@ -32,12 +32,6 @@ __global__ void __launch_bounds__(256) k_ft_pack(FtPacks l) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
-  if (PL == 3 && a.whole) {
-    ft_f4* d = (ft_f4*)((float*)a.dst + r * a.ldd + c0);
-    d[0] = ft_f4{v[0], v[1], v[2], v[3]};
-    d[1] = ft_f4{v[4], v[5], v[6], v[7]};
-    return;
-  }
   float h[3][8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {

@@ -48,7 +48,7 @@ def as_rows(t):
 def in_place(t, ld, rows):
     """whether the tiled products of `rows` rows read this matrix where it is (include/fedcola_hip.h)"""
     if t.element_size() == 4:
-        return rows <= 512 and ld % 4 == 0 and t.shape[1] % 4 == 0 and t.data_ptr() % 16 == 0 and ld < 1 << 20
+        return rows <= 512 and ld < 1 << 20
     return ld % 8 == 0 and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0
 
 

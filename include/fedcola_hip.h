@@ -114,9 +114,8 @@ int fc_ce_loss_fwd_bwd(const float* logits, const int64_t* y, int32_t B, int32_t
  * A row-major matrix is given by its first element and its row stride in elements (ld*, at least the row's length, below 2^21), any
  * alignment of the element's own type.  bf16 operands whose base is 16-byte aligned and whose stride and row length are multiples of 8
  * are read in place; others are first laid out in the workspace: pass packed = 1 to the workspace functions for them.  fp32 operands are
- * multiplied as three bf16 planes, exact to fp32 (an infinity in one gives NaN), which are laid out in the workspace too; of up to 512 rows (T) the
- * weights stay as they are where the base is 16-byte aligned and stride (below 2^20; times F + 512 below 2^29) and row length are multiples
- * of 4, with packed = 0, or are copied there otherwise, with packed = 1.  Workspaces and `saved` are aligned to 256 bytes; what they hold before does not matter.
+ * multiplied as three bf16 planes, exact to fp32 (an infinity in one gives NaN), which are laid out in the workspace too, but for the weights of
+ * up to 512 rows (T): these are read in place with packed = 0 (strides below 2^20, ld_in * (F + 512) below 2^29).  Workspaces and `saved` are aligned to 256 bytes; what they hold before does not matter.
  * Two calls that may run at once need workspaces of their own.  Results are bitwise reproducible (no atomics). */
 enum { FC_REDUCE_NONE = 0, FC_REDUCE_MEAN = 1, FC_REDUCE_SUM = 2 };
 enum { FC_ACT_SILU = 0, FC_ACT_GELU = 1 };

@@ -37,6 +37,11 @@ def layout(t, how):
         v = b[1:].view(t.shape[0], t.shape[1] + 3)[:, :t.shape[1]]
         v.copy_(t)
         return v
+    if how == "holes":                                    # the same with NaN all around
+        b = torch.full((t.shape[0] * (t.shape[1] + 5) + 3,), math.nan, dtype=t.dtype, device=t.device)
+        v = b[3:].view(t.shape[0], t.shape[1] + 5)[:, :t.shape[1]]
+        v.copy_(t)
+        return v
     if how == "turned":
         return t.t().contiguous().t()
     return t
@@ -53,7 +58,8 @@ def ce_case(T, V, D, dt, ignored, seed):
 
 CE = [(1, 2, 1, 0.0, "", ""), (1, 1003, 384, 0.0, "", ""), (7, 50, 16, 0.0, "wide", ""), (33, 257, 64, 0.5, "", "odd"), (64, 1000, 100, 0.0, "odd", ""),
       (65, 513, 7, 0.3, "turned", "turned"), (300, 999, 72, 0.0, "", "wide"), (200, 4100, 136, 0.85, "", ""), (129, 130, 520, 0.0, "", ""), (1030, 6000, 64, 0.2, "", ""),
-      (31, 700, 332, 0.0, "", "wide"), (17, 9000, 516, 0.2, "", "odd"), (64, 20, 4, 0.0, "", "turned")]
+      (31, 700, 332, 0.0, "", "wide"), (17, 9000, 516, 0.2, "", "odd"), (64, 20, 4, 0.0, "", "turned"), (20, 333, 50, 0.1, "holes", "holes"), (200, 700, 131, 0.1, "", "holes"),
+      (513, 300, 33, 0.0, "holes", "holes")]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
@@ -163,7 +169,8 @@ def test_linear_cross_entropy_module():
 
 # ------------------------------------------------------------------------------------------------ gated feed-forward
 MLP = [(1, 16, 8, "", ""), (1, 384, 1024, "", ""), (5, 7, 3, "", ""), (33, 64, 48, "wide", ""), (64, 1, 5, "", ""), (130, 100, 37, "odd", ""), (257, 192, 515, "", ""),
-       (300, 136, 264, "", "turned"), (1000, 64, 24, "turned", "odd"), (700, 320, 640, "", ""), (40, 172, 300, "", "wide"), (64, 1100, 700, "odd", ""), (9, 260, 1028, "", "odd"), (32, 4, 2052, "", "turned")]
+       (300, 136, 264, "", "turned"), (1000, 64, 24, "turned", "odd"), (700, 320, 640, "", ""), (40, 172, 300, "", "wide"), (64, 1100, 700, "odd", ""), (9, 260, 1028, "", "odd"), (32, 4, 2052, "", "turned"), (20, 37, 70, "holes", "holes"), (130, 101, 35, "", "holes"),
+       (512, 130, 67, "", "holes"), (513, 67, 130, "holes", "holes")]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
