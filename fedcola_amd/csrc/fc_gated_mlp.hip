@@ -49,18 +49,16 @@ template <class S, int NPROD>
 __device__ __forceinline__ void gm_gate_up(const GmArgs& a, char* smem, ft_f4 (&acc)[S::NI][S::NJ], const FtTile& t, int wave, int lane) {
   constexpr int WC = S::NJ * 16, HC = WC / 2;            // columns of a wave: HC gate rows and the HC up rows of the same units
   const int wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, f0 = t.n * (S::TN / 2);
-  FtStageA<S, TK> sa;
-  FtStageB<S, TK> sb;
-  sa.init(a.x, m0, a.D, wave, lane, [&](int r) { return m0 + r < a.T ? (long)m0 + r : -1L; });
-  sb.init(a.w_in, f0, a.D, wave, lane, [&](int r) {
+  FtPipe<S, TK, TK> pipe(smem);
+  pipe.sa.init(a.x, m0, a.D, wave, lane, [&](int r) { return m0 + r < a.T ? (long)m0 + r : -1L; });
+  pipe.sb.init(a.w_in, f0, a.D, wave, lane, [&](int r) {
     const int in = r % WC, f = f0 + (r / WC) * HC + in % HC;
     return f < a.F ? (long)f + (in < HC ? 0 : a.up) : -1L;
   });
-#pragma unroll
-  for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-    for (int j = 0; j < S::NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
-  ft_loop<S, TK, TK, NPROD, S::NJ>(sa, sb, smem, 0, (a.D + 63) / 64, acc, wm, wn, wave, lane);
+  ft_zero(acc);
+  pipe.fill(0);
+  pipe.run(0, (a.D + 63) / 64, acc);
+  pipe.drain();
 }
 
 // one row block of values, J columns of 16, into the planes' LDS images

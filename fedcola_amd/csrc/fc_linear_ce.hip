@@ -121,79 +121,91 @@ struct CeArgs {
   long ldl, plane;
 };
 
-template <class S, int NPROD>
-__device__ __forceinline__ bool ce_product(const CeArgs& a, char* smem, ft_f4 (&acc)[S::NI][S::NJ], FtTile& t, int M, int wave, int lane) {
-  t = ft_tile((M + S::TM - 1) / S::TM, (a.nv + S::TN - 1) / S::TN, 1, blockIdx.x);
-  if (!t.any) return false;
-  const int wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = a.v0 + t.n * S::TN;
-  FtStageA<S, TK> sa;
-  FtStageB<S, TK> sb;
-  sa.init(a.x, m0, a.D, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
-  sb.init(a.w, n0, a.D, wave, lane, [&](int r) { return n0 + r < a.V ? (long)n0 + r : -1L; });
-#pragma unroll
-  for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-    for (int j = 0; j < S::NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
-  ft_loop<S, TK, TK, NPROD, S::NJ>(sa, sb, smem, 0, (a.D + 63) / 64, acc, wm, wn, wave, lane);
-  return true;
+// the tiles of a workgroup: the product's in turn, epilogue(tile, acc, pipe) after each
+template <class S, class F> __device__ __forceinline__ void ce_tiles(const CeArgs& a, char* smem, int M, F epilogue) {
+  const int tm = (M + S::TM - 1) / S::TM, tn = (a.nv + S::TN - 1) / S::TN, nk = (a.D + 63) / 64;
+  int b = blockIdx.x;
+  FtTile t = ft_tile(tm, tn, 1, b);
+  if (!t.any) return;
+  FtPipe<S, TK, TK> pipe(smem);
+  auto go = [&](const FtTile& u) {
+    const int m0 = u.m * S::TM, n0 = a.v0 + u.n * S::TN, lane = ft_fresh(pipe.lane);
+    pipe.sa.init(a.x, m0, a.D, pipe.wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
+    pipe.sb.init(a.w, n0, a.D, pipe.wave, lane, [&](int r) { return n0 + r < a.V ? (long)n0 + r : -1L; });
+  };
+  go(t);
+  pipe.fill(0);
+  for (;;) {
+    ft_f4 acc[S::NI][S::NJ];
+    ft_zero(acc);
+    const FtTile u = ft_tile(tm, tn, 1, b += gridDim.x);
+    pipe.run(0, nk, acc, [&] {
+      if (u.any) { go(u); pipe.seek(0); }
+    });
+    epilogue(t, acc, pipe);
+    if (!u.any) break;
+    t = u;
+  }
+  pipe.drain();
 }
 
+template <class S> constexpr int ce_red_bytes() { return S::WN * S::TM * (int)sizeof(CePart); }
 template <class S, int NPROD>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_stats(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4, M = min(a.T, *a.n);
-  ft_f4 acc[S::NI][S::NJ];
-  FtTile t;
-  if (!ce_product<S, NPROD>(a, smem, acc, t, M, wave, lane)) return;
-  const int m0 = t.m * S::TM, n0 = t.n * S::TN + wn * S::NJ * 16;
-  CePart* red = (CePart*)smem;                           // [WN][TM]
-  const bool edge = n0 + S::NJ * 16 > a.V;
+  const int M = min(a.T, *a.n);
+  CePart* red = (CePart*)(smem + S::LDS);                // [WN][TM]
+  ce_tiles<S>(a, smem, M, [&](const FtTile& t, ft_f4 (&acc)[S::NI][S::NJ], auto& pipe) {
+    const int lane = ft_fresh(pipe.lane), wm = pipe.wm, wn = pipe.wn, g = lane >> 4, m0 = t.m * S::TM, n0 = t.n * S::TN + wn * S::NJ * 16;
+    const bool edge = n0 + S::NJ * 16 > a.V;
 #pragma unroll
-  for (int i = 0; i < S::NI; ++i) {
-    const int r = (wm * S::NI + i) * 16 + (lane & 15), m = m0 + r;
-    if (edge)
+    for (int i = 0; i < S::NI; ++i) {
+      const int r = (wm * S::NI + i) * 16 + (lane & 15), m = m0 + r;
+      if (edge)
 #pragma unroll
-      for (int j = 0; j < S::NJ; ++j)
+        for (int j = 0; j < S::NJ; ++j)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (n0 + 16 * j + 4 * g + x >= a.V) acc[i][j][x] = -__builtin_inff();
-    CePart p;
-    p.m = -__builtin_inff();
-#pragma unroll
-    for (int j = 0; j < S::NJ; ++j)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) p.m = fmaxf(p.m, acc[i][j][x]);
-    p.m = fmaxf(p.m, __shfl_xor(p.m, 16, 64));
-    p.m = fmaxf(p.m, __shfl_xor(p.m, 32, 64));
-    p.s = 0.f;
-    // a maximum of -inf: columns past the vocabulary alone, logits of -inf, or NaN, which fmaxf leaves out and the sum must not
-    const float base = p.m == -__builtin_inff() ? 0.f : p.m;
-#pragma unroll
-    for (int j = 0; j < S::NJ; ++j)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) p.s += ce_exp<NPROD>(acc[i][j][x], base);
-    p.s += __shfl_xor(p.s, 16, 64);
-    p.s += __shfl_xor(p.s, 32, 64);
-    if (g == 0) red[wn * S::TM + r] = p;
-    const int rel = (m < M ? a.y[m] : -1) - n0;          // the target's logit, where this wave holds it
-    if (rel >= 0 && rel < S::NJ * 16 && ((rel >> 2) & 3) == g) {
-      float v = 0.f;
+          for (int x = 0; x < 4; ++x)
+            if (n0 + 16 * j + 4 * g + x >= a.V) acc[i][j][x] = -__builtin_inff();
+      CePart p;
+      p.m = -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < S::NJ; ++j)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (16 * j + x == (rel & ~12)) v = acc[i][j][x];
-      a.tlogit[m] = v;
-    }
-  }
-  ft_barrier();
-  for (int r = threadIdx.x; r < S::TM; r += S::NT)
-    if (m0 + r < M) {
-      CePart p = red[r];
+        for (int x = 0; x < 4; ++x) p.m = fmaxf(p.m, acc[i][j][x]);
+      p.m = fmaxf(p.m, __shfl_xor(p.m, 16, 64));
+      p.m = fmaxf(p.m, __shfl_xor(p.m, 32, 64));
+      p.s = 0.f;
+      // a maximum of -inf: columns past the vocabulary alone, logits of -inf, or NaN, which fmaxf leaves out and the sum must not
+      const float base = p.m == -__builtin_inff() ? 0.f : p.m;
 #pragma unroll
-      for (int q = 1; q < S::WN; ++q) p = ce_join<NPROD>(p, red[q * S::TM + r]);
-      a.part[(long)t.n * a.T + m0 + r] = p;
+      for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p.s += ce_exp<NPROD>(acc[i][j][x], base);
+      p.s += __shfl_xor(p.s, 16, 64);
+      p.s += __shfl_xor(p.s, 32, 64);
+      if (g == 0) red[wn * S::TM + r] = p;
+      const int rel = (m < M ? a.y[m] : -1) - n0;          // the target's logit, where this wave holds it
+      if (rel >= 0 && rel < S::NJ * 16 && ((rel >> 2) & 3) == g) {
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (16 * j + x == (rel & ~12)) v = acc[i][j][x];
+        a.tlogit[m] = v;
+      }
     }
+    ft_barrier();
+    pipe.settle();
+    for (int r = pipe.wave * 64 + lane; r < S::TM; r += S::NT)
+      if (m0 + r < M) {
+        CePart p = red[r];
+#pragma unroll
+        for (int q = 1; q < S::WN; ++q) p = ce_join<NPROD>(p, red[q * S::TM + r]);
+        a.part[(long)t.n * a.T + m0 + r] = p;
+      }
+  });
 }
 
 // joins the tiles' partial sums: ROWS rows a workgroup, 256 / ROWS lanes a row (16: whole lines of neighbouring rows; 1: a scoring call's few rows)
@@ -246,51 +258,49 @@ __global__ void __launch_bounds__(1024) k_ce_loss(const float* rows, long T, con
 
 // dL of the tile's logits, rounded once to the operands' precision.  A factor that all rows share (g, g / count) is applied to the products'
 // results instead: multiplied in here, it gives the targets' entries, which are all close to -1, all the same rounding error.
+template <class S> constexpr int ce_img_bytes() { return 16 * S::NJ * 16 * 2; }         // of a wave: 16 rows
 template <class S, int NPROD>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4, M = min(a.T, *a.n);
-  ft_f4 acc[S::NI][S::NJ];
-  FtTile t;
-  if (!ce_product<S, NPROD>(a, smem, acc, t, M, wave, lane)) return;
-  const int m0 = t.m * S::TM, c0 = wn * S::NJ * 16, n0 = a.v0 + t.n * S::TN + c0;
+  constexpr int W = S::NJ * 16;
+  const int M = min(a.T, *a.n);
+  ce_tiles<S>(a, smem, M, [&](const FtTile& t, ft_f4 (&acc)[S::NI][S::NJ], auto& pipe) {
+    const int lane = ft_fresh(pipe.lane), g = lane >> 4, m0 = t.m * S::TM + pipe.wm * S::NI * 16, c0 = t.n * S::TN + pipe.wn * W, n0 = a.v0 + c0;
+    char* img = smem + S::LDS + pipe.wave * ce_img_bytes<S>();
 #pragma unroll
-  for (int i = 0; i < S::NI; ++i) {
-    const int r = (wm * S::NI + i) * 16 + (lane & 15), m = m0 + r;
-    const bool live = m < M;
-    const float lse = live ? a.lse[m] : 0.f;
-    const int rel = (live ? a.y[m] : -1) - n0 - 4 * g;
-    const float sc = live && a.reduction == FC_REDUCE_NONE ? a.g[a.idx[m]] : 1.f;
+    for (int i = 0; i < S::NI; ++i) {
+      const int m = m0 + i * 16 + (lane & 15);
+      const bool live = m < M;
+      const float lse = live ? a.lse[m] : 0.f;
+      const int rel = (live ? a.y[m] : -1) - n0 - 4 * g;
+      const float sc = live && a.reduction == FC_REDUCE_NONE ? a.g[a.idx[m]] : 1.f;
 #pragma unroll
-    for (int j = 0; j < S::NJ; ++j)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float p = ce_exp<NPROD>(acc[i][j][x], lse);
-        if (rel == 16 * j + x) p -= 1.f;
-        acc[i][j][x] = live && n0 + 16 * j + 4 * g + x < a.V ? p * sc : 0.f;
-      }
-  }
-  const FtRows rows;
-#pragma unroll
-  for (int pl = 0; pl < (NPROD == 1 ? 1 : 3); ++pl) {
-    if (pl) ft_barrier();
-#pragma unroll
-    for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-      for (int j = 0; j < S::NJ; ++j) {
-        float v[4];
+      for (int j = 0; j < S::NJ; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          if (NPROD == 1) { v[x] = acc[i][j][x]; continue; }
-          float h[3];
-          ft_split(acc[i][j][x], h[0], h[1], h[2]);
-          v[x] = h[pl];
+          float p = ce_exp<NPROD>(acc[i][j][x], lse);
+          if (rel == 16 * j + x) p -= 1.f;
+          acc[i][j][x] = live && n0 + 16 * j + 4 * g + x < a.V ? p * sc : 0.f;
         }
-        ft_img_put<S::TN>(smem, (wm * S::NI + i) * 16 + (lane & 15), c0 + 16 * j + 4 * g, v[0], v[1], v[2], v[3]);
+      if (i == 0) pipe.settle();
+#pragma unroll
+      for (int pl = 0; pl < (NPROD == 1 ? 1 : 3); ++pl) {
+#pragma unroll
+        for (int j = 0; j < S::NJ; ++j) {
+          float v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (NPROD == 1) { v[x] = acc[i][j][x]; continue; }
+            float h[3];
+            ft_split(acc[i][j][x], h[0], h[1], h[2]);
+            v[x] = h[pl];
+          }
+          ft_wimg_put<W>(img, lane & 15, 16 * j + 4 * g, v[0], v[1], v[2], v[3]);
+        }
+        ft_wimg_out<W>(img, a.dl + pl * a.plane, a.ldl, m0 + i * 16, c0, M, (int)a.ldl, lane);
       }
-    ft_barrier();
-    ft_img_out<S::TM, S::TN, S::NT>(smem, a.dl + pl * a.plane, a.ldl, m0, t.n * S::TN, M, (int)a.ldl, rows, true);
-  }
+    }
+  });
 }
 
 // ---------------------------------------------------------------- host
@@ -310,14 +320,17 @@ static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
 template <class S, int NPROD, bool GRAD> static int ce_launch(const CeArgs& a, hipStream_t s) {
   const long tiles = (long)((a.T + S::TM - 1) / S::TM) * ((a.nv + S::TN - 1) / S::TN);
   FC_REQUIRE(tiles < (1L << 31), "linear_ce: too many tiles");
+  const dim3 g((unsigned)ft_walkers<S>(tiles, a.D));
   if (GRAD) {
+    constexpr int bytes = S::LDS + S::NW * ce_img_bytes<S>();
     static FtLds lds;
-    FC_TRY(lds.allow((const void*)k_ce_grad<S, NPROD>, S::LDS));
-    hipLaunchKernelGGL((k_ce_grad<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
+    FC_TRY(lds.allow((const void*)k_ce_grad<S, NPROD>, bytes));
+    hipLaunchKernelGGL((k_ce_grad<S, NPROD>), g, dim3(S::NT), bytes, s, a);
   } else {
+    constexpr int bytes = S::LDS + ce_red_bytes<S>();
     static FtLds lds;
-    FC_TRY(lds.allow((const void*)k_ce_stats<S, NPROD>, S::LDS));
-    hipLaunchKernelGGL((k_ce_stats<S, NPROD>), dim3((unsigned)tiles), dim3(S::NT), S::LDS, s, a);
+    FC_TRY(lds.allow((const void*)k_ce_stats<S, NPROD>, bytes));
+    hipLaunchKernelGGL((k_ce_stats<S, NPROD>), g, dim3(S::NT), bytes, s, a);
   }
   FC_LAUNCH_CHECK();
   return 0;

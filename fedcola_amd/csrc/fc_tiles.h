@@ -62,6 +62,9 @@ __device__ __forceinline__ ft_i4 ft_rsrc(const void* p, long bytes) {
   return r;
 }
 
+// the same value, of which nothing is computed ahead of time and kept in registers over a loop that needs them all
+__device__ __forceinline__ int ft_fresh(int v) { asm volatile("" : "+v"(v)); return v; }
+
 // the XOR of a TK row's 16-B chunks: rows that would meet in a bank differ in it
 template <int KS> __device__ __forceinline__ int ft_tk_swz(int row) { return KS == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
@@ -234,282 +237,290 @@ template <int TM_, int TN_, int WM_, int WN_, int NS_, int KS_ = 64, int PL_ = 1
   static constexpr bool F32 = F32_;
   static constexpr int NI = TM / WM / 16, NJ = TN / WN / 16, STAGE = F32 ? TM * KS * 2 * PL + TN * KS * 4 : (TM + TN) * KS * 2 * PL, LDS = NS * STAGE;
 };
-template <class S, int MODE, int NJ, bool F32> struct FtStagers {
+template <class S, int MODE, bool F32> struct FtStagers {
   typedef FtStager<MODE, S::TM, S::KS, S::NW> A;
-  typedef FtStager<MODE, NJ * 16 * S::WN, S::KS, S::NW> B;
+  typedef FtStager<MODE, S::TN, S::KS, S::NW> B;
 };
-template <class S, int MODE, int NJ> struct FtStagers<S, MODE, NJ, true> {
+template <class S, int MODE> struct FtStagers<S, MODE, true> {
   typedef typename std::conditional<S::TM == 32, FtRowsA, FtStager<TK, S::TM < 128 ? 128 : S::TM, S::KS, S::NW>>::type A;
   typedef FtB32<MODE, S::TN, S::NW> B;
 };
-template <class S, int MODE> using FtStageA = typename FtStagers<S, MODE, S::NJ, S::F32>::A;
-template <class S, int MODE, int NJ = S::NJ> using FtStageB = typename FtStagers<S, MODE, NJ, S::F32>::B;
+template <class S, int MODE> using FtStageA = typename FtStagers<S, MODE, S::F32>::A;
+template <class S, int MODE> using FtStageB = typename FtStagers<S, MODE, S::F32>::B;
 
-// acc += the k-steps [kt0, kt1).  On return every wave has left the loop's LDS reads behind and no load into LDS is in flight.
+// The loops over k: acc += the k-steps [kt0, kt1).
 //
-// A step's two halves of 32 k are held in registers in turn: while the MFMAs of one run, the fragments of the next are read, one read to every
-// few MFMAs, so that neither the LDS nor the matrix pipe waits for the other.  The one barrier stands between the halves: there a wave has the
-// step's second half in registers, so its stage is free for the loads of the step NS on, and the next stage, loaded for NS - 1 steps by then, is
-// read from there on.
-template <class S, int AM, int BMO, int NJ>
-__device__ __forceinline__ void ft_halves(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
-                                         ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  constexpr int TNL = NJ * 16 * S::WN;      // columns staged (the shape's TN, or less in a second loop over the same tile)
-  constexpr int PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO, NJ>::NP, NF = S::NI + NJ, NM = S::NI * NJ;
-  const unsigned lds0 = ft_lds_addr(smem);
-  const int steps = kt1 - kt0;
-  sa.seek((long)kt0 * 64);
-  sb.seek((long)kt0 * 64);
-  auto next = [&]() { sa.step(); sb.step(); };   // steps past a slice's end, or the matrices', are loaded and not used: every step issues as many loads
-  auto piece = [&](int i, int at) {
-    if (i < PA) sa.piece(i, lds0 + at * S::STAGE, wave); else sb.piece(i - PA, lds0 + at * S::STAGE + S::TM * 128, wave);
-  };
-  ft_b8 f[2][NF];                           // [half][B fragments, then A fragments]
-  auto read = [&](int i, int ks, int at) {
-    const char* t = smem + at * S::STAGE;
-    f[ks][i] = i < NJ ? ft_frag<BMO, TNL, 64>(t + S::TM * 128, (wn * NJ + i) * 16, ks, lane) : ft_frag<AM, S::TM, 64>(t, (wm * S::NI + i - NJ) * 16, ks, lane);
-  };
-  auto mfma = [&](int m, int ks) {
-    const int i = m / NJ, j = m % NJ;
-    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[ks][j], f[ks][NJ + i], acc[i][j], 0, 0, 0);
-  };
-#pragma unroll
-  for (int st = 0; st < S::NS; ++st) {
-    next();
-#pragma unroll
-    for (int i = 0; i < PA + PB; ++i) piece(i, st);
-  }
-  ft_dma_wait<(S::NS - 1) * (PA + PB)>();
-  ft_barrier();
-#pragma unroll
-  for (int i = 0; i < NF; ++i) read(i, 0, 0);
-  // a half: reads spread over the first three quarters of its MFMAs, so that the last ones cover the last read's way
-  constexpr int RM = NM * 3 / 4 / NF > 0 ? NM * 3 / 4 / NF : 1;
-  auto half = [&](int ks, int at, auto before) {
-#pragma unroll
-    for (int g = 0; g < NF; ++g) {
-      before(g);
-      read(g, ks ^ 1, at);
-#pragma unroll
-      for (int m = g * RM; m < (g + 1 < NF ? (g + 1) * RM : NM); ++m) mfma(m, ks);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  int at = 0;
-  for (int s = 0; s < steps; ++s) {
-    half(0, at, [&](int g) { if (g == 0) next(); });
-    ft_dma_wait<(S::NS - 2) * (PA + PB)>();
-    ft_barrier();
-    const int to = at + 1 == S::NS ? 0 : at + 1;
-    half(1, to, [&](int g) {
-#pragma unroll
-      for (int i = g * (PA + PB) / NF; i < (g + 1) * (PA + PB) / NF; ++i) piece(i, at);
-    });
-    at = to;
-  }
-  ft_dma_wait<0>();
-  ft_barrier();
-}
+// For the large tiles (NS < 4) the loads run on from one tile of a workgroup to its next: fill() loads the first tile's first NS stages, run() takes
+// a tile's steps and, when the last of its loads is issued, calls advance(), which sets the stagers to the next tile; what a tile's last NS steps load
+// is the next one's beginning, which arrives while the epilogue runs.  Steps past the end of the matrices load zeros.  settle() in front of the epilogue's first store keeps
+// the next run from waiting for these stores; drain() in front of LDS reuse and the kernel's end leaves no load in flight.
+//
+// bf16: a step's two halves of 32 k are held in registers in turn: while the MFMAs of one run, the fragments of the next are read, one read to
+// every few MFMAs, so that neither the LDS nor the matrix pipe waits for the other.  The one barrier stands between the halves: there a wave has
+// the step's second half in registers, so its stage is free for the loads of the step NS on, and the next stage, loaded for NS - 1 steps by then,
+// is read from there on.
+// fp32: all three planes of both operands (F32: of A, and B in 32 bits) in a stage of 32 k, six products from one read of each fragment.  (A plane
+// pair a step would load every plane twice and meet six barriers for one here.)  The fragments of the next stage are read under the MFMAs of this
+// one, whose barrier stands under the first of them; B's of F32 are split a few groups of MFMAs later.
+template <class S, int AM, int BMO> struct FtPipe {
+  static constexpr bool ROWS = S::NS >= 4, PLANES = S::PL == 3;
+  static constexpr int NI = S::NI, NJ = S::NJ, PA1 = FtStageA<S, AM>::NP, PB1 = FtStageB<S, BMO>::NP;
+  static constexpr int PA = PA1 * (PLANES && !ROWS ? 3 : 1), PB = PB1 * (PLANES && !S::F32 ? 3 : 1), P = PA + PB;      // loads of a wave a stage
+  static constexpr int TA = S::TM * S::KS * 2, TB = S::TN * S::KS * 2;                                                // bytes of a plane's tile
+  typedef ft_f4 Acc[S::NI][S::NJ];
+  FtStageA<S, AM> sa;
+  FtStageB<S, BMO> sb;
+  char* smem;
+  unsigned lds0;
+  int wave, lane, wm, wn, at = 0;
+  bool landed = false;
 
-// the same without halves, for few rows: a step is short, and its loads' way from memory long
-template <class S, int AM, int BMO, int NJ>
-__device__ __forceinline__ void ft_rows(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
-                                             ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  constexpr int TNL = NJ * 16 * S::WN;
-  constexpr int PA = FtStageA<S, AM>::NP, PB = FtStageB<S, BMO, NJ>::NP;
-  const unsigned lds0 = ft_lds_addr(smem);
-  const int steps = kt1 - kt0;
-  int slot = 0;
-  sa.seek((long)kt0 * 64);
-  sb.seek((long)kt0 * 64);
-  auto put = [&](int at) {
-    sa.step();
-    sb.step();
-#pragma unroll
-    for (int i = 0; i < PA; ++i) sa.piece(i, lds0 + at * S::STAGE, wave);
-#pragma unroll
-    for (int i = 0; i < PB; ++i) sb.piece(i, lds0 + at * S::STAGE + S::TM * 128, wave);
-  };
-#pragma unroll
-  for (int s = 0; s < S::NS - 1; ++s) put(s);
-  int free_slot = S::NS - 1;
-  for (int s = 0; s < steps; ++s) {
-    ft_dma_wait<(S::NS - 2) * (PA + PB)>();
-    ft_barrier();
-    put(free_slot);
-    const char* ta = smem + slot * S::STAGE;
-    const char* tb = ta + S::TM * 128;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      ft_b8 af[S::NI], bf[NJ];
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) bf[j] = ft_frag<BMO, TNL, 64>(tb, (wn * NJ + j) * 16, ks, lane);
-#pragma unroll
-      for (int i = 0; i < S::NI; ++i) af[i] = ft_frag<AM, S::TM, 64>(ta, (wm * S::NI + i) * 16, ks, lane);
-#pragma unroll
-      for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
-    }
-    free_slot = slot;
-    slot = slot + 1 == S::NS ? 0 : slot + 1;
+  __device__ __forceinline__ FtPipe(char* smem_) : smem(smem_), lds0(ft_lds_addr(smem_)), wave(ft_wave()), lane(threadIdx.x & 63) {
+    wm = wave / S::WN;
+    wn = wave % S::WN;
   }
-  ft_dma_wait<0>();
-  ft_barrier();
-}
-// fp32 operands with all three planes of both in a stage of 32 k: six products from one read of each fragment.  (A plane pair a step
-// would load every plane twice and meet six barriers for one here.)  The fragments of the next stage are read under the MFMAs of this one,
-// whose barrier stands under the first of them.
-// F32: B's fragments are read in 32 bits and split a few groups of MFMAs later.
-template <class S, int AM, int BMO>
-__device__ __forceinline__ void ft_planes(FtStageA<S, AM>& sa, FtStageB<S, BMO>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
-                                          int lane) {
-  static_assert(S::KS == 32 && S::PL == 3, "a stage is one fragment deep");
-  constexpr int NI = S::NI, NJ = S::NJ, PA = 3 * FtStageA<S, AM>::NP, PB1 = FtStageB<S, BMO>::NP, PB = S::F32 ? PB1 : 3 * PB1, P = PA + PB, NM = 6 * NI * NJ;
-  constexpr int NF = 3 * NI + (S::F32 ? NJ : 3 * NJ);
-  constexpr int TA = S::TM * 64, TB = S::TN * 64;     // bytes of a plane's tile
-  const unsigned lds0 = ft_lds_addr(smem);
-  const int steps = (kt1 - kt0) * 2;
-  sa.seek((long)kt0 * 64);
-  sb.seek((long)kt0 * 64);
-  auto next = [&]() { sa.step(); sb.step(); };
-  auto piece = [&](int i, int at) {
-    const unsigned l = lds0 + at * S::STAGE;
-    if (i < PA) sa.piece_of(i / (PA / 3), i % (PA / 3), l + i / (PA / 3) * TA, wave);
-    else if (S::F32) sb.piece(i - PA, l + 3 * TA, wave);
-    else sb.piece_of((i - PA) / PB1, (i - PA) % PB1, l + 3 * TA + (i - PA) / PB1 * TB, wave);
-  };
-  ft_b8 fa[2][3][NI], fb[2][3][NJ];
-  float raw[NJ][8];
-  int left = 0;                                       // k from the stage that is read on (F32)
-  auto split = [&](int j, int h) {
-    if constexpr (S::F32) FtStageB<S, BMO>::mask(left, lane >> 4, raw[j]);
-    ft_split8(raw[j], fb[h][0][j], fb[h][1][j], fb[h][2][j]);
-  };
-  auto read = [&](int i, int h, int at) {             // in the order of use: both first planes, then the others
-    const char* t = smem + at * S::STAGE;
-    if constexpr (S::F32) {
-      if (i < NJ) FtStageB<S, BMO>::read(t + 3 * TA, (wn * NJ + i) * 16 + (lane & 15), lane >> 4, raw[i]);
-      else fa[h][(i - NJ) / NI][(i - NJ) % NI] = ft_frag<AM, S::TM, 32>(t + (i - NJ) / NI * TA, (wm * NI + (i - NJ) % NI) * 16, 0, lane);
+  __device__ __forceinline__ void seek(int kt) {
+    if constexpr (!(ROWS && PLANES)) sa.seek((long)kt * 64);
+    sb.seek((long)kt * 64);
+  }
+  __device__ __forceinline__ void next() { sa.step(); sb.step(); }
+  __device__ __forceinline__ void piece(int i, int slot) const {
+    const unsigned l = lds0 + slot * S::STAGE;
+    if constexpr (!PLANES) {
+      if (i < PA) sa.piece(i, l, wave); else sb.piece(i - PA, l + TA, wave);
     } else {
-      const int pl = i / (NI + NJ), k = i % (NI + NJ);
-      if (k < NJ) fb[h][pl][k] = ft_frag<BMO, S::TN, 32>(t + 3 * TA + pl * TB, (wn * NJ + k) * 16, 0, lane);
-      else fa[h][pl][k - NJ] = ft_frag<AM, S::TM, 32>(t + pl * TA, (wm * NI + k - NJ) * 16, 0, lane);
+      if (i < PA) sa.piece_of(i / PA1, i % PA1, l + i / PA1 * TA, wave);
+      else if (S::F32) sb.piece(i - PA, l + 3 * TA, wave);
+      else sb.piece_of((i - PA) / PB1, (i - PA) % PB1, l + 3 * TA + (i - PA) / PB1 * TB, wave);
     }
-  };
-  auto mfma = [&](int m, int h) {
-    constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
-    const int q = m / (NI * NJ), i = m % (NI * NJ) / NJ, j = m % NJ;
-    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[h][qb[q]][j], fa[h][qa[q]][i], acc[i][j], 0, 0, 0);
-  };
-#pragma unroll
-  for (int st = 0; st < S::NS; ++st) {
-    next();
-#pragma unroll
-    for (int i = 0; i < P; ++i) piece(i, st);
   }
-  ft_dma_wait<(S::NS - 1) * P>();
-  ft_barrier();
+  __device__ __forceinline__ void fill(int kt0) {
+    if constexpr (!ROWS) {
+      seek(kt0);
 #pragma unroll
-  for (int i = 0; i < NF; ++i) read(i, 0, 0);
-  if constexpr (S::F32) {
-    left = sb.left_at((long)kt0 * 64);
+      for (int st = 0; st < S::NS; ++st) {
+        next();
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) split(j, 0);
-  }
-  constexpr int M0 = NM / 8, RM = (NM - M0) / NF, LATE = 4;
-  static_assert(RM >= 1 && (!S::F32 || LATE + 2 * NJ <= NF), "an MFMA to every read, and the splits' places");
-  int at = 0;
-  auto stage = [&](int h) {
-    const int to = at + 1 == S::NS ? 0 : at + 1;
-    next();
-    if (S::F32) left -= 32;
-#pragma unroll
-    for (int m = 0; m < M0; ++m) mfma(m, h);
-    __builtin_amdgcn_sched_barrier(0);
-    ft_dma_wait<(S::NS - 2) * P>();
-    ft_barrier();                                     // slot `to` is there, and slot `at` read by everybody
-#pragma unroll
-    for (int g = 0; g < NF; ++g) {
-#pragma unroll
-      for (int i = g * P / NF; i < (g + 1) * P / NF; ++i) piece(i, at);
-      read(g, h ^ 1, to);
-      if constexpr (S::F32)
-        if (g >= LATE && (g - LATE) % 2 == 0 && (g - LATE) / 2 < NJ) split((g - LATE) / 2, h ^ 1);
-#pragma unroll
-      for (int m = M0 + g * RM; m < (g + 1 < NF ? M0 + (g + 1) * RM : NM); ++m) mfma(m, h);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    at = to;
-  };
-  for (int s = 0; s < steps; s += 2) {
-    stage(0);
-    stage(1);
-  }
-  ft_dma_wait<0>();
-  ft_barrier();
-}
-
-template <class S, int BMO>
-__device__ __forceinline__ void ft_rows32(FtRowsA& sa, FtB32<BMO, S::TN, S::NW>& sb, char* smem, int kt0, int kt1, ft_f4 (&acc)[S::NI][S::NJ], int wm, int wn, int wave,
-                                          int lane) {
-  static_assert(S::TM == 32 && S::NW == 4 && S::KS == 32 && S::PL == 3 && S::NI == 1, "two waves by two");
-  constexpr int PB = FtB32<BMO, S::TN, S::NW>::NP, P = 2 + PB, TA = S::TM * 64;
-  const unsigned lds0 = ft_lds_addr(smem);
-  const int steps = (kt1 - kt0) * 2, g = lane >> 4;
-  long k0 = (long)kt0 * 64;
-  int left = sb.left_at(k0);
-  sb.seek(k0);
-  auto put = [&](int at) {
-    const unsigned l = lds0 + at * S::STAGE;
-    sb.step();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) sa.load(i, k0, l, wave);
-#pragma unroll
-    for (int i = 0; i < PB; ++i) sb.piece(i, l + 3 * TA, wave);
-    k0 += 32;
-  };
-#pragma unroll
-  for (int s = 0; s < S::NS - 1; ++s) put(s);
-  int slot = 0, free_slot = S::NS - 1;
-  for (int s = 0; s < steps; ++s) {
-    ft_dma_wait<(S::NS - 2) * P>();
-    ft_barrier();
-    put(free_slot);
-    const char* ta = smem + slot * S::STAGE;
-    const char* tb = ta + 3 * TA;
-    ft_b8 fa[3], fb[S::NJ][3];
-#pragma unroll
-    for (int p = 0; p < 3; ++p) fa[p] = ft_frag<TK, 32, 32>(ta + p * TA, wm * 16, 0, lane);
-#pragma unroll
-    for (int j = 0; j < S::NJ; ++j) {
-      float v[8];
-      sb.read(tb, (wn * S::NJ + j) * 16 + (lane & 15), g, v);
-      sb.mask(left, g, v);
-      ft_split8(v, fb[j][0], fb[j][1], fb[j][2]);
-    }
-#pragma unroll
-    for (int q = 0; q < 6; ++q)
-#pragma unroll
-      for (int j = 0; j < S::NJ; ++j) {
-        constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
-        acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j][qb[q]], fa[qa[q]], acc[0][j], 0, 0, 0);
+        for (int i = 0; i < P; ++i) piece(i, st);
       }
-    left -= 32;
-    free_slot = slot;
-    slot = slot + 1 == S::NS ? 0 : slot + 1;
+      ft_dma_wait<(S::NS - 1) * P>();
+      ft_barrier();
+      at = 0;
+      landed = false;
+    }
   }
-  ft_dma_wait<0>();
-  ft_barrier();
-}
+  __device__ __forceinline__ void settle() {
+    if constexpr (!ROWS) { ft_dma_wait<0>(); landed = true; }
+  }
+  __device__ __forceinline__ void drain() {
+    if constexpr (!ROWS) { ft_dma_wait<0>(); ft_barrier(); }
+  }
+  // (every stage but the one that the next step reads may be on its way; a settled pipe's are all there)
+  __device__ __forceinline__ void await(bool first) const {
+    if (!(first && landed)) ft_dma_wait<(S::NS - 2) * P>();
+    ft_barrier();
+  }
+  __device__ __forceinline__ static int following(int slot) { return slot + 1 == S::NS ? 0 : slot + 1; }
 
-template <class S, int AM, int BMO, int NPROD, int NJ>
-__device__ __forceinline__ void ft_loop(FtStageA<S, AM>& sa, FtStageB<S, BMO, NJ>& sb, char* smem, int kt0, int kt1,
-                                        ft_f4 (&acc)[S::NI][NJ], int wm, int wn, int wave, int lane) {
-  if constexpr (S::F32 && S::TM == 32) ft_rows32<S, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
-  else if constexpr (S::PL == 3) ft_planes<S, AM, BMO>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
-  else if constexpr (S::NS < 4) ft_halves<S, AM, BMO, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
-  else ft_rows<S, AM, BMO, NJ>(sa, sb, smem, kt0, kt1, acc, wm, wn, wave, lane);
+  template <class F> __device__ __forceinline__ void run(int kt0, int kt1, Acc& acc, F advance) {
+    if constexpr (ROWS && S::F32) rows32(kt0, kt1, acc);
+    else if constexpr (ROWS) rows(kt0, kt1, acc);
+    else if constexpr (PLANES) planes(kt0, kt1, acc, advance);
+    else halves(kt0, kt1, acc, advance);
+    landed = false;
+  }
+  __device__ __forceinline__ void run(int kt0, int kt1, Acc& acc) { run(kt0, kt1, acc, [] {}); }
+
+  template <class F> __device__ __forceinline__ void halves(int kt0, int kt1, Acc& acc, F advance) {
+    constexpr int NF = NI + NJ, NM = NI * NJ;
+    const int steps = kt1 - kt0;
+    ft_b8 f[2][NF];                           // [half][B fragments, then A fragments]
+    auto read = [&](int i, int ks, int slot) {
+      const char* t = smem + slot * S::STAGE;
+      f[ks][i] = i < NJ ? ft_frag<BMO, S::TN, 64>(t + TA, (wn * NJ + i) * 16, ks, lane) : ft_frag<AM, S::TM, 64>(t, (wm * NI + i - NJ) * 16, ks, lane);
+    };
+    auto mfma = [&](int m, int ks) {
+      const int i = m / NJ, j = m % NJ;
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[ks][j], f[ks][NJ + i], acc[i][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < NF; ++i) read(i, 0, at);
+    // a half: reads spread over the first three quarters of its MFMAs, so that the last ones cover the last read's way
+    constexpr int RM = NM * 3 / 4 / NF > 0 ? NM * 3 / 4 / NF : 1;
+    auto half = [&](int ks, int slot, auto before) {
+#pragma unroll
+      for (int g = 0; g < NF; ++g) {
+        before(g);
+        read(g, ks ^ 1, slot);
+#pragma unroll
+        for (int m = g * RM; m < (g + 1 < NF ? (g + 1) * RM : NM); ++m) mfma(m, ks);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int s = 0; s < steps; ++s) {
+      if (s == steps - S::NS) advance();
+      half(0, at, [&](int g) { if (g == 0) next(); });
+      await(s == 0);
+      const int to = following(at);
+      half(1, to, [&](int g) {
+#pragma unroll
+        for (int i = g * P / NF; i < (g + 1) * P / NF; ++i) piece(i, at);
+      });
+      at = to;
+    }
+  }
+
+  template <class F> __device__ __forceinline__ void planes(int kt0, int kt1, Acc& acc, F advance) {
+    static_assert(S::KS == 32, "a stage is one fragment deep");
+    constexpr int NM = 6 * NI * NJ, NF = 3 * NI + (S::F32 ? NJ : 3 * NJ);
+    const int steps = (kt1 - kt0) * 2;
+    ft_b8 fa[2][3][NI], fb[2][3][NJ];
+    float raw[NJ][8];
+    int left = 0;                                       // k from the stage that is read on (F32)
+    auto split = [&](int j, int h) {
+      if constexpr (S::F32) FtStageB<S, BMO>::mask(left, lane >> 4, raw[j]);
+      ft_split8(raw[j], fb[h][0][j], fb[h][1][j], fb[h][2][j]);
+    };
+    auto read = [&](int i, int h, int slot) {             // in the order of use: both first planes, then the others
+      const char* t = smem + slot * S::STAGE;
+      if constexpr (S::F32) {
+        if (i < NJ) FtStageB<S, BMO>::read(t + 3 * TA, (wn * NJ + i) * 16 + (lane & 15), lane >> 4, raw[i]);
+        else fa[h][(i - NJ) / NI][(i - NJ) % NI] = ft_frag<AM, S::TM, 32>(t + (i - NJ) / NI * TA, (wm * NI + (i - NJ) % NI) * 16, 0, lane);
+      } else {
+        const int pl = i / (NI + NJ), k = i % (NI + NJ);
+        if (k < NJ) fb[h][pl][k] = ft_frag<BMO, S::TN, 32>(t + 3 * TA + pl * TB, (wn * NJ + k) * 16, 0, lane);
+        else fa[h][pl][k - NJ] = ft_frag<AM, S::TM, 32>(t + pl * TA, (wm * NI + k - NJ) * 16, 0, lane);
+      }
+    };
+    auto mfma = [&](int m, int h) {
+      constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
+      const int q = m / (NI * NJ), i = m % (NI * NJ) / NJ, j = m % NJ;
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[h][qb[q]][j], fa[h][qa[q]][i], acc[i][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < NF; ++i) read(i, 0, at);
+    if constexpr (S::F32) {
+      left = sb.left_at((long)kt0 * 64);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) split(j, 0);
+    }
+    constexpr int M0 = NM / 8, RM = (NM - M0) / NF, LATE = 4;
+    static_assert(RM >= 1 && (!S::F32 || LATE + 2 * NJ <= NF), "an MFMA to every read, and the splits' places");
+    auto stage = [&](int h, bool first) {
+      const int to = following(at);
+      next();
+      if (S::F32) left -= 32;
+#pragma unroll
+      for (int m = 0; m < M0; ++m) mfma(m, h);
+      __builtin_amdgcn_sched_barrier(0);
+      await(first);                                     // slot `to` is there, and slot `at` read by everybody
+#pragma unroll
+      for (int g = 0; g < NF; ++g) {
+#pragma unroll
+        for (int i = g * P / NF; i < (g + 1) * P / NF; ++i) piece(i, at);
+        read(g, h ^ 1, to);
+        if constexpr (S::F32)
+          if (g >= LATE && (g - LATE) % 2 == 0 && (g - LATE) / 2 < NJ) split((g - LATE) / 2, h ^ 1);
+#pragma unroll
+        for (int m = M0 + g * RM; m < (g + 1 < NF ? M0 + (g + 1) * RM : NM); ++m) mfma(m, h);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      at = to;
+    };
+    static_assert(S::NS % 2 == 1, "the last load of a tile is issued in an odd stage");
+    for (int s = 0; s < steps; s += 2) {
+      stage(0, s == 0);
+      if (s + 1 == steps - S::NS) advance();
+      stage(1, false);
+    }
+  }
+
+  // few rows: a step is short, and its loads' way from memory long.  Nothing is in flight before and after.
+  __device__ __forceinline__ void rows(int kt0, int kt1, Acc& acc) {
+    const int steps = kt1 - kt0;
+    int slot = 0, free_slot = S::NS - 1;
+    seek(kt0);
+    auto put = [&](int to) {
+      next();
+#pragma unroll
+      for (int i = 0; i < P; ++i) piece(i, to);
+    };
+#pragma unroll
+    for (int s = 0; s < S::NS - 1; ++s) put(s);
+    for (int s = 0; s < steps; ++s) {
+      await(false);
+      put(free_slot);
+      const char* ta = smem + slot * S::STAGE;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        ft_b8 af[NI], bf[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) bf[j] = ft_frag<BMO, S::TN, 64>(ta + TA, (wn * NJ + j) * 16, ks, lane);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) af[i] = ft_frag<AM, S::TM, 64>(ta, (wm * NI + i) * 16, ks, lane);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
+      }
+      free_slot = slot;
+      slot = following(slot);
+    }
+    ft_dma_wait<0>();
+    ft_barrier();
+  }
+  __device__ __forceinline__ void rows32(int kt0, int kt1, Acc& acc) {
+    static_assert(S::TM == 32 && S::NW == 4 && S::KS == 32 && S::PL == 3 && S::NI == 1, "two waves by two");
+    const int steps = (kt1 - kt0) * 2, g = lane >> 4;
+    int slot = 0, free_slot = S::NS - 1, left = sb.left_at((long)kt0 * 64);
+    long k0 = (long)kt0 * 64;
+    sb.seek(k0);
+    auto put = [&](int to) {
+      const unsigned l = lds0 + to * S::STAGE;
+      sb.step();
+#pragma unroll
+      for (int i = 0; i < PA; ++i) sa.load(i, k0, l, wave);
+#pragma unroll
+      for (int i = 0; i < PB; ++i) sb.piece(i, l + 3 * TA, wave);
+      k0 += 32;
+    };
+#pragma unroll
+    for (int s = 0; s < S::NS - 1; ++s) put(s);
+    for (int s = 0; s < steps; ++s) {
+      await(false);
+      put(free_slot);
+      const char* ta = smem + slot * S::STAGE;
+      const char* tb = ta + 3 * TA;
+      ft_b8 fa[3], fb[NJ][3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) fa[p] = ft_frag<TK, 32, 32>(ta + p * TA, wm * 16, 0, lane);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        float v[8];
+        sb.read(tb, (wn * NJ + j) * 16 + (lane & 15), g, v);
+        sb.mask(left, g, v);
+        ft_split8(v, fb[j][0], fb[j][1], fb[j][2]);
+      }
+#pragma unroll
+      for (int q = 0; q < 6; ++q)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          constexpr int qa[6] = {0, 0, 1, 1, 0, 2}, qb[6] = {0, 1, 0, 1, 2, 0};
+          acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j][qb[q]], fa[qa[q]], acc[0][j], 0, 0, 0);
+        }
+      left -= 32;
+      free_slot = slot;
+      slot = following(slot);
+    }
+    ft_dma_wait<0>();
+    ft_barrier();
+  }
+};
+template <int NI, int NJ> __device__ __forceinline__ void ft_zero(ft_f4 (&acc)[NI][NJ]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
 }
 
 // ---- which tile a workgroup takes.  Consecutive ids share an XCD's L2 (workgroups are dealt to the 8 XCDs in turn), and ids walk the
@@ -566,6 +577,20 @@ __device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld
     }
   }
 }
+// the same for one wave's 16 rows of W columns, in 16 * W * 2 bytes of its own: no barrier
+template <int W> __device__ __forceinline__ int ft_wimg(int row, int chunk) { return row * (W * 2) + ((chunk ^ (W == 64 ? row & 7 : (row >> 1) & 3 & (W / 8 - 1))) << 4); }
+template <int W> __device__ __forceinline__ void ft_wimg_put(char* img, int row, int col, float a, float b, float c, float d) {
+  *(uint2*)(img + ft_wimg<W>(row, col >> 3) + (col & 4) * 2) = make_uint2(f2bf2(a, b), f2bf2(c, d));
+}
+template <int W> __device__ __forceinline__ void ft_wimg_out(const char* img, bf16_t* out, long ld, int m0, int n0, int M, int N, int lane) {
+#pragma unroll
+  for (int q = 0; q < W / 32; ++q) {
+    const int e = q * 64 + lane, r = e / (W / 8), c = e % (W / 8);
+    const uint4 v = *(const uint4*)(img + ft_wimg<W>(r, c));
+    if (m0 + r < M && n0 + c * 8 < N) *(uint4*)(out + (long)(m0 + r) * ld + n0 + c * 8) = v;
+  }
+}
+
 // ---------------------------------------------------------------- host side (fc_tiles.hip)
 // C = A B^T written to `out` (bf16 for nprod 1, fp32 for 6), or as fp32 partial sums for ft_reduce().
 struct FtProduct {
@@ -657,6 +682,10 @@ static inline FtMat ft_mat32(const void* p, long ld, long R, long C) {
   return m;
 }
 static inline bool ft_direct(int dt, const void* p, long ld, long cols) { return dt == 1 && ((size_t)p & 15) == 0 && ld % 8 == 0 && cols % 8 == 0; }
+// workgroups of a kernel whose workgroups walk the tiles: as many as run at once, where the loads of two tiles can follow each other (FtPipe)
+template <class S> static inline long ft_walkers(long tiles, long K) {
+  return S::NT == 512 && (K + 63) / 64 * (S::KS == 32 ? 2 : 1) >= S::NS && tiles > 256 ? 256 : tiles;
+}
 static inline long ft_up(long v, long m) { return (v + m - 1) / m * m; }
 // > 64 KB of LDS for a kernel: asked for once on each device (a static of the launch that needs it)
 struct FtLds {

@@ -67,23 +67,24 @@ __device__ __forceinline__ void ft_product_tile(const FtProduct& p, float* part,
   const int tm = (M + S::TM - 1) / S::TM, tn = (N + S::TN - 1) / S::TN, Ks = (p.Ks ? p.Ks : K) * p.segs, splits = ft_slices((long)tm * tn, Ks, target, NPROD);
   const FtTile t = ft_tile(tm, tn, splits, b);
   if (!t.any) return;
-  const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN, m0 = t.m * S::TM, n0 = t.n * S::TN;
-  FtStageA<S, AM> sa;
-  FtStageB<S, BMO> sb;
-  sa.init(p.a, m0, K, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
-  sb.init(p.b, n0, K, wave, lane, [&](int r) { return n0 + r < N ? (long)n0 + r : -1L; });
+  FtPipe<S, AM, BMO> pipe(smem);
+  const int wave = pipe.wave, lane = pipe.lane, wm = pipe.wm, wn = pipe.wn, m0 = t.m * S::TM, n0 = t.n * S::TN;
+  pipe.sa.init(p.a, m0, K, wave, lane, [&](int r) { return m0 + r < M ? (long)m0 + r : -1L; });
+  pipe.sb.init(p.b, n0, K, wave, lane, [&](int r) { return n0 + r < N ? (long)n0 + r : -1L; });
   ft_f4 acc[S::NI][S::NJ];
-#pragma unroll
-  for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-    for (int j = 0; j < S::NJ; ++j) acc[i][j] = ft_f4{0.f, 0.f, 0.f, 0.f};
+  ft_zero(acc);
   const int nk = (K + 63) / 64, all = nk * p.segs, per = (p.segs == 1 ? (Ks + 63) / 64 + splits - 1 : all + splits - 1) / splits, kt0 = min(all, t.split * per),
             kt1 = min(all, kt0 + per);
-  ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0 < nk ? kt0 : nk, kt1 < nk ? kt1 : nk, acc, wm, wn, wave, lane);
+  auto part_of = [&](int k0, int k1) {
+    pipe.fill(k0);
+    pipe.run(k0, k1, acc);
+    pipe.drain();
+  };
+  part_of(kt0 < nk ? kt0 : nk, kt1 < nk ? kt1 : nk);
   if (kt1 > nk) {
-    sa.p += p.a2;
-    sb.p += p.b2;
-    ft_loop<S, AM, BMO, NPROD, S::NJ>(sa, sb, smem, kt0 > nk ? kt0 - nk : 0, kt1 - nk, acc, wm, wn, wave, lane);
+    pipe.sa.p += p.a2;
+    pipe.sb.p += p.b2;
+    part_of(kt0 > nk ? kt0 - nk : 0, kt1 - nk);
   }
   const int mr = wm * S::NI * 16 + (lane & 15), nc = wn * S::NJ * 16 + 4 * (lane >> 4);
   if (part) {
