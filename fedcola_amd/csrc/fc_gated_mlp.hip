@@ -61,6 +61,9 @@ __device__ __forceinline__ void gm_gate_up(const GmArgs& a, char* smem, ft_f4 (&
   pipe.drain();
 }
 
+// Planes of h, dg and du: fp32's three; bf16's one, each rounded once; two (16 bits of mantissa) in the tiles of few rows, whose
+// products read the weights once all the same, and whose few results would show how one rounding more is distributed.
+template <class S, int NPROD> constexpr int gm_planes() { return NPROD == 6 ? 3 : S::TM == 32 ? 2 : 1; }
 // one row block of values, J columns of 16, into the planes' LDS images
 template <class S, int NPROD>
 __device__ __forceinline__ void gm_put(char* img, int i, const ft_f4 (&v)[S::NJ / 2], int wm, int wn, int lane) {
@@ -68,14 +71,15 @@ __device__ __forceinline__ void gm_put(char* img, int i, const ft_f4 (&v)[S::NJ 
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int r = (wm * S::NI + i) * 16 + (lane & 15), c = wn * J * 16 + 16 * j + 4 * (lane >> 4);
-    if (NPROD == 1) {
+    constexpr int PL = gm_planes<S, NPROD>();
+    if (PL == 1) {
       ft_img_put<FC>(img, r, c, v[j][0], v[j][1], v[j][2], v[j][3]);
     } else {
       float h[3][4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) ft_split(v[j][x], h[0][x], h[1][x], h[2][x]);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) ft_img_put<FC>(img + p * IMG, r, c, h[p][0], h[p][1], h[p][2], h[p][3]);
+      for (int p = 0; p < PL; ++p) ft_img_put<FC>(img + p * IMG, r, c, h[p][0], h[p][1], h[p][2], h[p][3]);
     }
   }
 }
@@ -84,14 +88,14 @@ template <class S, int NPROD> __device__ __forceinline__ void gm_out(const char*
   constexpr int FC = S::TN / 2, IMG = S::TM * FC * 2;
   const FtRows rows;
 #pragma unroll
-  for (int p = 0; p < (NPROD == 1 ? 1 : 3); ++p) ft_img_out<S::TM, FC, S::NT>(img + p * IMG, out + p * plane, ld, m0, f0, a.T, (int)a.ldh, rows, true);
+  for (int p = 0; p < gm_planes<S, NPROD>(); ++p) ft_img_out<S::TM, FC, S::NT>(img + p * IMG, out + p * plane, ld, m0, f0, a.T, (int)a.ldh, rows, true);
 }
 
 // GRAD: the backward's pass over the same product
 template <class S, int NPROD, bool GRAD>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int J = S::NJ / 2, FC = S::TN / 2, SET = (NPROD == 1 ? 1 : 3) * S::TM * FC * 2;     // bytes of an output's images
+  constexpr int J = S::NJ / 2, FC = S::TN / 2, SET = gm_planes<S, NPROD>() * S::TM * FC * 2;     // bytes of an output's images
   constexpr bool TURN = 2 * SET <= S::LDS;                                                      // room for two outputs' in turn
   static_assert(SET <= S::LDS, "an output's images fit");
   const int wave = ft_wave(), lane = threadIdx.x & 63, wm = wave / S::WN, wn = wave % S::WN;
@@ -184,6 +188,8 @@ template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream
 }
 
 struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan_dh, plan[3]; bool group; };
+// bf16, few rows: h, dg and du are two planes, which are rows behind each other, of the result (y, dx) or of the reduction (dw_in, dw_out: one k-step)
+static bool gm_two(int dt, long T) { return dt && T <= 32; }
 // dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
 static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProduct (&p)[3]) {
   p[0].b32 = a.b32;
@@ -202,6 +208,12 @@ static void gm_products(int dt, long T, long D, long F, const GmArgs& a, FtProdu
   p[2].M = (int)D; p[2].N = (int)F;
   p[2].a = a.dy;
   p[2].b.p = a.h; p[2].b.ld = Fp; p[2].b.plane = T * Fp;
+  if (gm_two(dt, T)) {
+    p[0].M = (int)(2 * T);
+    p[0].fold = (int)T;
+    p[1].K = p[2].K = (int)(2 * T);
+    p[1].b.wrap = p[2].a.wrap = (int)T;
+  }
 }
 // dh = dy w_out, whose slices' sums the activation's pass adds up
 static FtProduct gm_dh_product(int dt, long T, long D, long F, bool b32) {
@@ -215,12 +227,16 @@ static FtProduct gm_y_product(int dt, long T, long D, long F, bool b32) {
   p.nprod = dt ? 1 : 6;
   p.b32 = b32;
   p.M = (int)T; p.N = (int)D; p.K = (int)F;
+  if (gm_two(dt, T)) {
+    p.M = (int)(2 * T);
+    p.fold = (int)T;
+  }
   return p;
 }
 // b32: fp32 weights read where they are; packed: what is not planes anyway is laid out
 static GmSizes gm_sizes(int dt, long T, long D, long F, bool b32, bool packed, bool backward) {
   GmSizes z = {};
-  const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6;
+  const long Dp = ft_up(D, 64), Fp = ft_up(F, 64), e = dt ? 2 : 6, eh = dt && ft_few(1, T) ? 4 : e;
   if (packed || !dt) {
     z.x = ft_up(T * Dp * e, 256);
     z.dy = backward ? z.x : 0;
@@ -229,12 +245,12 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool b32, bool packed, b
     z.w_in = ft_up(2 * F * Dp * e, 256);
     z.w_out = ft_up(D * Fp * e, 256);
   }
-  z.h = ft_up(T * Fp * e, 256);
+  z.h = ft_up(T * Fp * eh, 256);
   if (!backward) {
     z.part = ft_product_part_floats(gm_y_product(dt, T, D, F, b32)) * 4;
     return z;
   }
-  z.dgu = ft_up(T * 2 * Fp * e, 256);
+  z.dgu = ft_up(T * 2 * Fp * eh, 256);
   z.plan_dh = ft_plan(gm_dh_product(dt, T, D, F, b32), false);
   if (gm_big(dt, T, D, F, true)) z.plan_dh.target = 0;
   z.dh = ft_up(ft_part_floats(T, F, z.plan_dh) * 4, 256);
@@ -377,7 +393,7 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
     plan[n] = z.plan[i];
     at[n] = z.plan[i].target ? (float*)part : nullptr;
     if (at[n]) {
-      sums.add(q[n], plan[n], at[n], nullptr, q[n].M);
+      sums.add(q[n], plan[n], at[n], nullptr, q[n].fold ? q[n].fold : q[n].M);
       part += ft_up(ft_part_floats(q[n].M, q[n].N, plan[n]) * 4, 256);
     }
     ++n;

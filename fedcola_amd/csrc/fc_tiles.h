@@ -34,6 +34,7 @@ enum { TK = 0, TR = 1 };
 struct FtMat {
   const bf16_t* p = nullptr;
   long ld = 0, plane = 0;
+  int wrap = 0;                    // TR, > 0: rows k from there on are rows k - wrap again (up to 2 wrap, at most 64: one k-step)
   const bf16_t* end = nullptr;     // an fp32 matrix read where it is (FtB32): one past its last element
 };
 
@@ -98,11 +99,11 @@ template <int MODE, int W, int KS, int NW> struct FtStager {
         const long row = map(t);
         voff[i] = row >= 0 ? (unsigned)(((row - base) * ld + (lane % CR ^ ft_tk_swz<KS>(t)) * 8) * 2) : FT_OOB;
       } else {
-        const int k = piece * (512 / W) + lane * 8 / W, pc = lane % (W / 8);
+        const int k = piece * (512 / W) + lane * 8 / W, pc = lane % (W / 8), kr = m.wrap && k >= m.wrap ? k - m.wrap : k;
         const int s = (((k >> 3) & 1) << 2) | (k & 3);
         const int c = (((pc >> 1) ^ s) << 1) | (pc & 1);
         const long col = map(c * 8);
-        voff[i] = col >= 0 ? (unsigned)(((long)k * ld + col) * 2) : FT_OOB;
+        voff[i] = col >= 0 && (!m.wrap || kr < m.wrap) ? (unsigned)(((long)kr * ld + col) * 2) : FT_OOB;
       }
     }
   }
@@ -601,6 +602,7 @@ struct FtProduct {
   int Ks = 0;                     // > 0: the length that the slices are cut from, >= K (products added onto each other's partial sums)
   const int* Mdyn = nullptr;      // device: the rows (M) / reduction length (K) really there, at most M / K
   const int* Kdyn = nullptr;
+  int fold = 0;                   // > 0: A's rows are two terms of each of `fold` rows, first terms first, and the result is their sum
   int segs = 1;                   // 2: the reduction is two pieces of length K, the second a2 / b2 elements on in A / B
   long a2 = 0, b2 = 0;
   const float* alpha = nullptr;   // device: factor of the result (null: 1), over *alpha_over where that is given
@@ -647,7 +649,7 @@ int ft_reduce(const FtSums& l, hipStream_t s);
 // whether they are better run as a group, and how; part[i] null: straight into out
 bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan);
 int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, hipStream_t s);
-// out = the sum over the slices, in their order, of ft_product's partial sums; with `pos`: out[r] = row pos[r] of the sums, 0 where pos[r] < 0, for R rows
+// out = the sum over the slices, in one order, of ft_product's partial sums; with `pos`: out[r] = row pos[r] of the sums, 0 where pos[r] < 0, for R rows
 int ft_reduce(const FtProduct& p, const FtPlan& plan, const float* part, const int* pos, long R, hipStream_t s);
 // the product into p.out, by way of partial sums in `part` where the plan slices the reduction
 int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s);

@@ -109,6 +109,22 @@ __device__ __forceinline__ void ft_product_tile(const FtProduct& p, float* part,
   for (int i = 0; i < S::NI; ++i)
 #pragma unroll
     for (int j = 0; j < S::NJ; ++j) acc[i][j] *= al;
+  if constexpr (NPROD == 1 && S::TM == 32) {
+    if (p.fold) {                                         // both terms of every row are in this tile
+      constexpr int LD = S::TN + 4;
+      float* sum = (float*)smem;
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NJ; ++j) *(ft_f4*)(sum + (mr + 16 * i) * LD + nc + 16 * j) = acc[i][j];
+      ft_barrier();
+      for (int e = threadIdx.x; e < p.fold * S::TN; e += S::NT) {
+        const int r = e / S::TN, c = e % S::TN;
+        if (n0 + c < N) ((bf16_t*)p.out)[r * p.ldo + n0 + c] = f2bf(sum[r * LD + c] + sum[(r + p.fold) * LD + c]);
+      }
+      return;
+    }
+  }
   if (NPROD == 1) {
 #pragma unroll
     for (int i = 0; i < S::NI; ++i)
@@ -162,6 +178,7 @@ struct FtCost { double step, fixed; int slots; };   // us a k-step with the chip
 static const FtCost kCost[6] = {{1.6, 7.0, 256}, {1.15, 5.0, 512}, {0.45, 4.0, 512}, {2.6, 6.0, 256}, {1.0, 5.0, 512}, {2.8, 6.0, 256}};
 static const int kTM[6] = {256, 128, 32, 128, 32, 128}, kTN[6] = {256, 128, 64, 128, 64, 128};
 
+static long tiles_of(const FtPlan& pl, long M, long N) { return ((M + kTM[pl.shape] - 1) / kTM[pl.shape]) * ((N + kTN[pl.shape] - 1) / kTN[pl.shape]); }
 // The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
 // step + time of a tile's start and end), plus the partial sums' way to memory and back.  The constants are measured: 256 x 256 tiles run
 // a k-step in 1.6 us on all CUs (1.3 PFLOP/s), 128 x 128 ones in 1.15 us, two a CU (0.93), and where they leave half of the chip idle, 0.8.
@@ -188,9 +205,9 @@ FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
       if (sp < want) break;
     }
   }
+  if (p.fold && !best.target && !(best.shape == 2 && M <= kTM[2])) best.target = (int)tiles_of(best, M, N);
   return best;
 }
-static long tiles_of(const FtPlan& pl, long M, long N) { return ((M + kTM[pl.shape] - 1) / kTM[pl.shape]) * ((N + kTN[pl.shape] - 1) / kTN[pl.shape]); }
 // slices x tiles stays under max(target, tiles), and rows x columns under tiles x a tile
 size_t ft_part_floats(long M, long N, const FtPlan& pl) {
   const long tiles = tiles_of(pl, M, N), wg = tiles > pl.target ? tiles : pl.target;
@@ -242,9 +259,13 @@ int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hi
 }
 
 // ---------------------------------------------------------------- sums of the slices
-template <typename T>
+// L lanes share a group of eight columns, each with every L-th slice: one where there are many groups, eight where few rows leave the chip
+// waiting for one lane's loads (one row of 4096 columns, 32 slices of
+// two terms: 15 us with one, 5 with eight), and for rows of two terms
+template <typename T, int L>
 __global__ void __launch_bounds__(256) k_ft_reduce(FtSums l) {
-  const long e0 = (long)blockIdx.x * 256 + threadIdx.x;
+  const long e0 = ((long)blockIdx.x * 256 + threadIdx.x) / L;
+  const int q0 = threadIdx.x % L;
   if (e0 >= l.first[l.n]) return;
   const int w = e0 < l.first[1] ? 0 : e0 < l.first[2] ? 1 : 2;
   const long e = e0 - l.first[w];
@@ -253,6 +274,7 @@ __global__ void __launch_bounds__(256) k_ft_reduce(FtSums l) {
   const long ldp = ft_part_ld(N), cw = ldp / 8;
   const int splits = ft_slices((long)((M + TM - 1) / TM) * ((N + TN - 1) / TN), (long)(p.Ks ? p.Ks : K) * p.segs, l.target[w], p.nprod);
   const int* pos = l.pos[w];
+  const int two = L > 1 && p.fold ? 1 : 0;
   const long m = e / cw;
   const int n = (int)(e - m * cw) * 8;
   const long src = pos ? pos[m] : m, row = pos ? m : p.rows.at((int)m);
@@ -260,11 +282,18 @@ __global__ void __launch_bounds__(256) k_ft_reduce(FtSums l) {
   ft_f4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   if (src >= 0 && src < M)
 #pragma unroll 4
-    for (int q = 0; q < splits; ++q) {
-      const ft_f4* a = (const ft_f4*)(l.part[w] + ((long)q * M + src) * ldp + n);
+    for (int q = q0; q < splits << two; q += L) {
+      const ft_f4* a = (const ft_f4*)(l.part[w] + ((long)(q >> two) * M + src + (q & two) * p.fold) * ldp + n);
       v[0] += a[0];
       v[1] += a[1];
     }
+  if (L > 1) {
+#pragma unroll
+    for (int o = 1; o < L; o *= 2)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x >> 2][x & 3] += __shfl_xor(v[x >> 2][x & 3], o, 64);
+    if (q0) return;
+  }
   const float al = p.factor();
   v[0] *= al;
   v[1] *= al;
@@ -285,9 +314,12 @@ void FtSums::add(const FtProduct& q, const FtPlan& plan, const float* partial, c
 int ft_reduce(const FtSums& l, hipStream_t s) {
   const long n = l.first[l.n];
   if (n == 0) return 0;
-  const dim3 g((unsigned)((n + 255) / 256));
-  if (l.p[0].nprod == 1) hipLaunchKernelGGL(k_ft_reduce<bf16_t>, g, dim3(256), 0, s, l);
-  else hipLaunchKernelGGL(k_ft_reduce<float>, g, dim3(256), 0, s, l);
+  const int L = n <= 16384 || l.p[0].fold || l.p[1].fold || l.p[2].fold ? 8 : 1;
+  const dim3 g((unsigned)((n * L + 255) / 256));
+  if (l.p[0].nprod == 1 && L == 1) hipLaunchKernelGGL((k_ft_reduce<bf16_t, 1>), g, dim3(256), 0, s, l);
+  else if (l.p[0].nprod == 1) hipLaunchKernelGGL((k_ft_reduce<bf16_t, 8>), g, dim3(256), 0, s, l);
+  else if (L == 1) hipLaunchKernelGGL((k_ft_reduce<float, 1>), g, dim3(256), 0, s, l);
+  else hipLaunchKernelGGL((k_ft_reduce<float, 8>), g, dim3(256), 0, s, l);
   FC_LAUNCH_CHECK();
   return 0;
 }
@@ -315,6 +347,7 @@ bool ft_group_plan(const FtProduct* p, int n, FtPlan* plan) {
     plan[i].shape = sh;
     plan[i].target = want > 1 ? (int)(tiles * want < (1 << 20) ? tiles * want : 0) : 0;
     if (p[i].Mdyn && plan[i].target < slots) plan[i].target = slots;
+    if (p[i].fold && !plan[i].target) plan[i].target = (int)tiles;
   }
   return true;
 }
@@ -352,5 +385,5 @@ int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStrea
   if (!plan.target) return ft_product(p, plan, nullptr, false, s);
   FC_REQUIRE(part && part_floats >= ft_part_floats(p.M, p.N, plan), "workspace too small for the partial sums");
   FC_TRY(ft_product(p, plan, part, false, s));
-  return ft_reduce(p, plan, part, nullptr, p.M, s);
+  return ft_reduce(p, plan, part, nullptr, p.fold ? p.fold : p.M, s);
 }
