@@ -170,7 +170,8 @@ def test_linear_cross_entropy_module():
 # ------------------------------------------------------------------------------------------------ gated feed-forward
 MLP = [(1, 16, 8, "", ""), (1, 384, 1024, "", ""), (5, 7, 3, "", ""), (33, 64, 48, "wide", ""), (64, 1, 5, "", ""), (130, 100, 37, "odd", ""), (257, 192, 515, "", ""),
        (300, 136, 264, "", "turned"), (1000, 64, 24, "turned", "odd"), (700, 320, 640, "", ""), (40, 172, 300, "", "wide"), (64, 1100, 700, "odd", ""), (9, 260, 1028, "", "odd"), (32, 4, 2052, "", "turned"), (20, 37, 70, "holes", "holes"), (130, 101, 35, "", "holes"),
-       (512, 130, 67, "", "holes"), (513, 67, 130, "holes", "holes")]
+       (512, 130, 67, "", "holes"), (513, 67, 130, "holes", "holes"), (16, 200, 312, "", ""), (17, 200, 312, "", ""),
+       (32, 520, 1032, "", ""), (2, 2056, 24, "", "")]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
