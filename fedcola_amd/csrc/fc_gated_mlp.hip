@@ -156,6 +156,66 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a
   }
 }
 
+// The same from partial sums of [g | u] (few tiles and a long reduction, which then runs in slices): eight lanes share eight units of a row,
+// each with every eighth slice.  PL: planes of h, dg and du.
+struct GmJoin {
+  GmArgs a;
+  const float* gu;
+  long ldp;
+  int parts;
+};
+__device__ __forceinline__ void gm_sum8(const float* p, long step, int parts, int q0, int cols, float (&v)[8]) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) v[x] = 0.f;
+#pragma unroll 2
+  for (int q = q0; q < parts; q += 8)
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (x < cols) v[x] += p[q * step + x];
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] += __shfl_xor(v[x], o, 64);
+}
+template <int PL> __device__ __forceinline__ void gm_store8(bf16_t* o, long plane, const float (&v)[8]) {
+  float h[3][8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    if (PL == 1) h[0][x] = v[x]; else ft_split(v[x], h[0][x], h[1][x], h[2][x]);
+  }
+#pragma unroll
+  for (int p = 0; p < PL; ++p) *(uint4*)(o + p * plane) = make_uint4(f2bf2(h[p][0], h[p][1]), f2bf2(h[p][2], h[p][3]), f2bf2(h[p][4], h[p][5]), f2bf2(h[p][6], h[p][7]));
+}
+template <int PL, bool GRAD> __global__ void __launch_bounds__(256) k_gm_join(GmJoin j) {
+  const GmArgs& a = j.a;
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) / 8, cw = a.ldh / 8, m = e / cw;
+  const int q0 = threadIdx.x & 7, f = (int)(e - m * cw) * 8, cols = a.F - f;
+  if (m >= a.T) return;
+  float g[8], u[8], d[8];
+  const float* at = j.gu + m * j.ldp + f;
+  gm_sum8(at, a.T * j.ldp, j.parts, q0, cols, g);
+  gm_sum8(at + a.F, a.T * j.ldp, j.parts, q0, cols, u);
+  if (GRAD) gm_sum8(a.dh + m * a.ldd + f, a.T * a.ldd, a.dh_parts, q0, cols, d);
+  if (q0) return;
+  float h[8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    float v, dv;
+    gm_act<PL != 3>(a.act, g[x], v, dv);
+    h[x] = v * u[x];
+    if (GRAD) {
+      g[x] = d[x] * u[x] * dv;
+      u[x] = d[x] * v;
+    }
+  }
+  gm_store8<PL>(a.h + m * a.ldh + f, a.T * a.ldh, h);
+  if (GRAD) {
+    bf16_t* o = a.dgu + m * 2 * a.ldh + f;
+    gm_store8<PL>(o, a.T * 2 * a.ldh, g);
+    gm_store8<PL>(o + a.ldh, a.T * 2 * a.ldh, u);
+  }
+}
+
 // ---------------------------------------------------------------- host
 typedef FtShape<256, 256, 2, 4, 2> GmBig;
 typedef FtShape<128, 128, 2, 2, 2> GmMid;
@@ -187,7 +247,31 @@ template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream
   }
 }
 
-struct GmSizes { size_t x, w_in, w_out, dy, h, dgu, dh, part; FtPlan plan_dh, plan[3]; bool group; };
+struct GmSizes { size_t x, w_in, w_out, dy, h, gu, dgu, dh, part; FtPlan plan_gu, plan_dh, plan[3]; bool group; };
+// [g | u] in slices, where that is much faster by the model of the products' time
+static FtProduct gm_gu_product(int dt, long T, long D, long F, bool b32) {
+  FtProduct p;
+  p.nprod = dt ? 1 : 6;
+  p.b32 = b32;
+  p.M = (int)T; p.N = (int)(2 * F); p.K = (int)D;
+  return p;
+}
+template <bool GRAD> static int gm_act_any(const GmArgs& a, int dt, const FtPlan& gu, float* part, hipStream_t s) {
+  if (!gu.target) return dt ? gm_act_run<1, GRAD>(a, s) : gm_act_run<6, GRAD>(a, s);
+  FtProduct p = gm_gu_product(dt, a.T, a.D, a.F, a.b32);
+  p.a = a.x;
+  p.b = a.w_in;
+  FC_TRY(ft_product(p, gu, part, false, s));
+  GmJoin j;
+  j.a = a; j.gu = part; j.ldp = ft_part_ld(p.N); j.parts = ft_parts(p, gu);
+  const dim3 g((unsigned)((a.T * a.ldh + 255) / 256));
+  if (!dt) hipLaunchKernelGGL((k_gm_join<3, GRAD>), g, dim3(256), 0, s, j);
+  else if (a.T <= 32) hipLaunchKernelGGL((k_gm_join<2, GRAD>), g, dim3(256), 0, s, j);
+  else hipLaunchKernelGGL((k_gm_join<1, GRAD>), g, dim3(256), 0, s, j);
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+
 // bf16, few rows: h, dg and du are two planes, which are rows behind each other, of the result (y, dx) or of the reduction (dw_in, dw_out: one k-step)
 static bool gm_two(int dt, long T) { return dt && T <= 32; }
 // dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h
@@ -246,13 +330,16 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool b32, bool packed, b
     z.w_out = ft_up(D * Fp * e, 256);
   }
   z.h = ft_up(T * Fp * eh, 256);
+  z.plan_gu = ft_plan(gm_gu_product(dt, T, D, F, b32), false);
+  if (z.plan_gu.gain < 1.3) z.plan_gu.target = 0;
+  z.gu = z.plan_gu.target ? ft_up(ft_part_floats(T, 2 * F, z.plan_gu) * 4, 256) : 0;
   if (!backward) {
     z.part = ft_product_part_floats(gm_y_product(dt, T, D, F, b32)) * 4;
     return z;
   }
   z.dgu = ft_up(T * 2 * Fp * eh, 256);
   z.plan_dh = ft_plan(gm_dh_product(dt, T, D, F, b32), false);
-  if (gm_big(dt, T, D, F, true)) z.plan_dh.target = 0;
+  if (gm_big(dt, T, D, F, true) && !z.plan_gu.target) z.plan_dh.target = 0;
   z.dh = ft_up(ft_part_floats(T, F, z.plan_dh) * 4, 256);
   FtProduct p[3];
   GmArgs a = {};
@@ -269,7 +356,7 @@ static GmSizes gm_sizes(int dt, long T, long D, long F, bool b32, bool packed, b
   }
   return z;
 }
-static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.dgu + z.dh + z.part; }
+static size_t gm_total(const GmSizes& z) { return z.x + z.w_in + z.w_out + z.dy + z.h + z.gu + z.dgu + z.dh + z.part; }
 
 // a matrix as the products take it: where it is, or as one of the packs
 static void gm_matrix(int dt, bool b32, const void* p, long ld, long R, long C, char*& ws, FtMat& m, FtPacks& l) {
@@ -339,7 +426,8 @@ extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t 
   FC_TRY(gm_operands(c, ws, a, s));
   a.h = (bf16_t*)ws;
   ws += z.h;
-  FC_TRY(dt ? (gm_act_run<1, false>(a, s)) : (gm_act_run<6, false>(a, s)));
+  FC_TRY(gm_act_any<false>(a, dt, z.plan_gu, (float*)ws, s));
+  ws += z.gu;
   FtProduct p = gm_y_product(dt, T, D, F, a.b32);
   p.a.p = a.h; p.a.ld = a.ldh; p.a.plane = (long)T * a.ldh;
   p.b = a.w_out;
@@ -361,6 +449,8 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
   FC_TRY(gm_operands(c, ws, a, s));
   a.h = (bf16_t*)ws;
   ws += z.h;
+  float* gu = (float*)ws;
+  ws += z.gu;
   a.dgu = (bf16_t*)ws;
   ws += z.dgu;
   char* part = ws + z.dh;
@@ -372,7 +462,7 @@ extern "C" int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t
     a.dh_parts = ft_parts(p, z.plan_dh);
     a.dh = (const float*)ws;
     a.ldd = ft_part_ld(F);
-    FC_TRY(dt ? (gm_act_run<1, true>(a, s)) : (gm_act_run<6, true>(a, s)));
+    FC_TRY(gm_act_any<true>(a, dt, z.plan_gu, gu, s));
   }
   FtProduct p[3], q[3];
   FtPlan plan[3];

@@ -615,8 +615,11 @@ struct FtProduct {
     return alpha_over ? (*alpha_over > 0 ? *alpha / (float)*alpha_over : 0.f) : *alpha;
   }
 };
-// shape: index of the tile shape; target: workgroups wanted, by which the reduction is sliced (0: it is not)
-struct FtPlan { int shape = 0, target = 0; };
+// shape: index of the tile shape (TM x TN); target: workgroups wanted, by which the reduction is sliced (0: it is not)
+struct FtPlan {
+  int shape = 0, target = 0, TM = 0, TN = 0;
+  double gain = 1;      // time of the best unsliced form over this one's, by the model
+};
 FtPlan ft_plan(const FtProduct& p, bool dynamic_rows);
 __host__ __device__ static inline long ft_part_ld(long N) { return (N + 7) / 8 * 8; }
 // slices of a reduction of length K for `tiles` output tiles: as many as the target asks for, none under four k-steps (one of fp32's six products)

@@ -186,7 +186,7 @@ FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
   const long M = p.M, N = p.N, K = (long)p.K * p.segs;
   const int nprod = p.nprod;
   FtPlan best;
-  double least = 1e30;
+  double least = 1e30, whole = 1e30;
   for (int sh = 0; sh < 6; ++sh) {
     if (nprod == 6 ? sh != (!p.b32 ? 3 : ft_few(6, M) ? 4 : 5) : sh > 2 || (sh == 2 && (p.am != TK || p.bm != TK || !ft_few(1, M)))) continue;
     const long tiles = ((M + kTM[sh] - 1) / kTM[sh]) * ((N + kTN[sh] - 1) / kTN[sh]), nk = (K + 63) / 64;
@@ -196,6 +196,7 @@ FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
       const double rounds = wg <= 4 * slots ? (double)((wg + slots - 1) / slots) : (double)wg / slots + 0.5;
       double t = rounds * ((double)per * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
       if (sp > 1) t += 4.0 + (double)sp * M * N * 8.0 / 4e6;
+      else if (t < whole) whole = t;
       if (t < least) {
         least = t;
         best.shape = sh;
@@ -206,6 +207,9 @@ FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
     }
   }
   if (p.fold && !best.target && !(best.shape == 2 && M <= kTM[2])) best.target = (int)tiles_of(best, M, N);
+  best.TM = kTM[best.shape];
+  best.TN = kTN[best.shape];
+  best.gain = whole / least;
   return best;
 }
 // slices x tiles stays under max(target, tiles), and rows x columns under tiles x a tile
