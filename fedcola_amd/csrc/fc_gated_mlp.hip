@@ -248,7 +248,8 @@ template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream
 }
 
 struct GmSizes { size_t x, w_in, w_out, dy, h, gu, dgu, dh, part; FtPlan plan_gu, plan_dh, plan[3]; bool group; };
-// [g | u] in slices, where that is much faster by the model of the products' time
+// [g | u] in slices, where that is much faster by the model of the products' time (fp32, 45 x 3200 x 448: 42 us forward, 149 by whole tiles;
+// bf16, 256 x 4096 x 1024: 39 and 57)
 static FtProduct gm_gu_product(int dt, long T, long D, long F, bool b32) {
   FtProduct p;
   p.nprod = dt ? 1 : 6;

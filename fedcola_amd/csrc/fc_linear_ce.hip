@@ -303,6 +303,79 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_grad(CeArgs 
   });
 }
 
+// ---- few tiles and a long reduction: the logits come as fp32 partial sums of slices of it, for the rows really there
+struct CeSlices {
+  const float* part;            // [slices][M][ldp]
+  long ldp, K;
+  int target, TM, TN, nprod;
+  __device__ __forceinline__ int count(int M, int V) const { return ft_slices((long)((M + TM - 1) / TM) * ((V + TN - 1) / TN), K, target, nprod); }
+  __device__ __forceinline__ ft_f4 at(long row, int col, int M, int slices) const {
+    const float* p = part + row * ldp + col;
+    ft_f4 v = *(const ft_f4*)p;
+#pragma unroll 4
+    for (int q = 1; q < slices; ++q) v += *(const ft_f4*)(p + (long)q * M * ldp);
+    return v;
+  }
+};
+// a workgroup a row: log-sum-exp and loss
+template <int NPROD>
+__global__ void __launch_bounds__(256) k_ce_row(CeSlices l, int V, CeSaved s, float* rows) {
+  __shared__ CePart red[4];
+  __shared__ float target;
+  const long t = blockIdx.x;
+  const int at = s.pos[t], tid = threadIdx.x, M = *s.n;
+  if (at < 0) {
+    if (tid == 0) rows[t] = 0.f;
+    return;
+  }
+  const int y = s.y[at], slices = l.count(M, V);
+  if (tid == 0) target = __builtin_nanf("");             // a target outside of the vocabulary: NaN, in the loss and in the gradients
+  __syncthreads();
+  CePart p = {-__builtin_inff(), 0.f};
+  for (int c = tid * 4; c < V; c += 1024) {
+    const ft_f4 v = l.at(at, c, M, slices);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (c + x < V) {
+        p = ce_join<NPROD>(p, CePart{v[x], 1.f});
+        if (c + x == y) target = v[x];
+      }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) p = ce_join<NPROD>(p, CePart{__shfl_xor(p.m, o, 64), __shfl_xor(p.s, o, 64)});
+  if ((tid & 63) == 0) red[tid >> 6] = p;
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 1; i < 4; ++i) p = ce_join<NPROD>(p, red[i]);
+    const float lse = y >= 0 ? p.m + logf(p.s) : target;
+    s.lse[at] = lse;
+    rows[t] = lse - target;
+  }
+}
+// dL, eight columns a lane
+template <int NPROD> __global__ void __launch_bounds__(256) k_ce_dl(CeSlices l, CeArgs a) {
+  const int M = min(a.T, *a.n), cw = (a.V + 7) / 8;
+  const long e = (long)blockIdx.x * 256 + threadIdx.x, m = e / cw;
+  const int c0 = (int)(e - m * cw) * 8;
+  if (m >= M) return;
+  const int slices = l.count(M, a.V);
+  const ft_f4 v[2] = {l.at(m, c0, M, slices), l.at(m, c0 + 4, M, slices)};
+  const float lse = a.lse[m], sc = a.reduction == FC_REDUCE_NONE ? a.g[a.idx[m]] : 1.f;
+  const int y = a.y[m];
+  float h[3][8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    float p = ce_exp<NPROD>(v[x >> 2][x & 3], lse);
+    if (c0 + x == y) p -= 1.f;
+    p = c0 + x < a.V ? p * sc : 0.f;
+    if (NPROD == 1) h[0][x] = p; else ft_split(p, h[0][x], h[1][x], h[2][x]);
+  }
+#pragma unroll
+  for (int q = 0; q < (NPROD == 1 ? 1 : 3); ++q)
+    *(uint4*)(a.dl + q * a.plane + m * a.ldl + c0) = make_uint4(f2bf2(h[q][0], h[q][1]), f2bf2(h[q][2], h[q][3]), f2bf2(h[q][4], h[q][5]), f2bf2(h[q][6], h[q][7]));
+}
+
 // ---------------------------------------------------------------- host
 typedef FtShape<256, 256, 2, 4, 2> CeBig;
 typedef FtShape<128, 128, 2, 2, 2> CeMid;
@@ -341,12 +414,24 @@ template <bool GRAD> static int ce_run(int dt, int shape, const CeArgs& a, hipSt
   return shape != 1 ? ce_launch<CeRows32, 6, GRAD>(a, s) : a.b32 ? ce_launch<CeMid32, 6, GRAD>(a, s) : ce_launch<CePlanes, 6, GRAD>(a, s);
 }
 
+static FtProduct ce_logits(int dt, long T, long V, long D, bool b32, const int* n) {
+  FtProduct p;
+  p.nprod = dt ? 1 : 6;
+  p.b32 = b32;
+  p.M = (int)T; p.N = (int)V; p.K = (int)D; p.Mdyn = n;
+  return p;
+}
+static CeSlices ce_slices(const FtProduct& p, const FtPlan& plan, const float* part) {
+  CeSlices l;
+  l.part = part; l.ldp = ft_part_ld(p.N); l.K = p.K; l.target = plan.target; l.TM = plan.TM; l.TN = plan.TN; l.nprod = p.nprod;
+  return l;
+}
 // columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
 static long ce_piece(int dt, long T, long V) {
   const long most = (192L << 20) / ((T ? T : 1) * (dt ? 2 : 6)) / 256 * 256, all = ft_up(V, 256);
   return most < 256 ? 256 : most < all ? most : all;
 }
-struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan dx, dw; bool group; };
+struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan logits, dx, dw; bool group; };
 // dx = dL w and dw = dL^T x of nv columns; n: device, the rows that count
 static void ce_products(int dt, long T, long D, long nv, bool b32, const int* n, FtProduct& x, FtProduct& w) {
   x.am = TK; x.bm = TR; x.nprod = dt ? 1 : 6; x.b32 = b32; x.M = (int)T; x.N = (int)D; x.K = (int)nv; x.Mdyn = n;
@@ -356,13 +441,18 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
   CeSizes z = {};
   const bool b32 = !dt && direct_w;
   z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : 6) * V * ft_up(D, 64), 256);
+  // slices pay where the model of the products' time says so by much (122 x 2263 x 326 fp32: 39 us forward, 125 by whole tiles; 64 x 4096 x 1000
+  // bf16: 23 and 31), and where the logits are one piece
+  z.piece = ce_piece(dt, T, V);
+  z.logits = ft_plan(ce_logits(dt, T, V, D, b32, nullptr), false);
+  if (z.logits.gain < 1.3 || z.piece < V) z.logits.target = 0;
+  if (z.logits.target) z.part = (size_t)ft_up(ft_part_floats(T, V, z.logits) * 4, 256);
   if (!grad) {
     const int tn = ce_tn(ce_shape(dt, T, V, b32));
-    z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
+    if (!z.logits.target) z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
     z.rows = (size_t)ft_up(T * 4, 256) * 2;
     return z;
   }
-  z.piece = ce_piece(dt, T, V);
   z.dl = (size_t)ft_up((dt ? 1 : 3) * T * z.piece * 2, 256);
   if (z.piece >= V) {                     // one piece: its two products may run together
     FtProduct p[2];
@@ -447,15 +537,26 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
     hipLaunchKernelGGL((k_ce_rows<float, 3>), dim3(blocks), dim3(256), 0, s, (const float*)x, (long)ldx, y, (long)T, R, V, ignore_index, D, false, sv);
   }
   FC_LAUNCH_CHECK();
-  const int shape = ce_shape(dt, T, V, a.b32), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
-  FC_TRY(ce_run<false>(dt, shape, a, s));
-  if (T) {
-    const dim3 gj((unsigned)(T <= 64 ? T : (T + 15) / 16));
-    if (dt && T <= 64) hipLaunchKernelGGL((k_ce_join<1, 1>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
-    else if (dt) hipLaunchKernelGGL((k_ce_join<1, 16>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
-    else if (T <= 64) hipLaunchKernelGGL((k_ce_join<6, 1>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
-    else hipLaunchKernelGGL((k_ce_join<6, 16>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+  if (z.logits.target) {
+    FtProduct p = ce_logits(dt, T, V, D, a.b32, sv.n);
+    p.a = a.x;
+    p.b = a.w;
+    FC_TRY(ft_product(p, z.logits, (float*)ws, false, s));
+    const CeSlices l = ce_slices(p, z.logits, (const float*)ws);
+    if (dt) hipLaunchKernelGGL(k_ce_row<1>, dim3(T), dim3(256), 0, s, l, V, sv, rows);
+    else hipLaunchKernelGGL(k_ce_row<6>, dim3(T), dim3(256), 0, s, l, V, sv, rows);
     FC_LAUNCH_CHECK();
+  } else {
+    const int shape = ce_shape(dt, T, V, a.b32), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
+    FC_TRY(ce_run<false>(dt, shape, a, s));
+    if (T) {
+      const dim3 gj((unsigned)(T <= 64 ? T : (T + 15) / 16));
+      if (dt && T <= 64) hipLaunchKernelGGL((k_ce_join<1, 1>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+      else if (dt) hipLaunchKernelGGL((k_ce_join<1, 16>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+      else if (T <= 64) hipLaunchKernelGGL((k_ce_join<6, 1>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+      else hipLaunchKernelGGL((k_ce_join<6, 16>), gj, dim3(256), 0, s, a.part, tiles, a.tlogit, sv, rows, (long)T);
+      FC_LAUNCH_CHECK();
+    }
   }
   if (reduction != FC_REDUCE_NONE) {
     hipLaunchKernelGGL(k_ce_loss, dim3(1), dim3(1024), 0, s, rows, (long)T, sv.n, reduction, loss);
@@ -473,7 +574,7 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   const CeSaved sv = ce_saved((void*)saved, dt, T, D);
   const bool direct = ce_direct(dt, w, ldw, T, D);
   const CeSizes z = ce_sizes(dt, T, V, D, direct, true);
-  FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.dl + z.dxp + z.dwp, "fc_linear_ce_bwd: saved or workspace too small");
+  FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.part + z.dl + z.dxp + z.dwp, "fc_linear_ce_bwd: saved or workspace too small");
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   CeArgs a = {};
@@ -483,6 +584,8 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   a.T = T; a.V = V; a.D = D;
   a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
   a.lse = sv.lse; a.g = gloss; a.reduction = reduction;
+  float* part = (float*)ws;
+  ws += z.part;
   a.dl = (bf16_t*)ws;
   a.ldl = z.piece;
   a.plane = (long)T * z.piece;
@@ -503,7 +606,19 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   for (long v0 = 0; v0 < V; v0 += z.piece) {
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < z.piece ? V - v0 : z.piece);
-    FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv, a.b32), a, s));
+    if (z.logits.target) {
+      FtProduct p = ce_logits(dt, T, V, D, a.b32, sv.n);
+      p.a = a.x;
+      p.b = a.w;
+      FC_TRY(ft_product(p, z.logits, part, false, s));
+      const CeSlices l = ce_slices(p, z.logits, part);
+      const dim3 g((unsigned)(((long)T * ((V + 7) / 8) + 255) / 256));
+      if (dt) hipLaunchKernelGGL(k_ce_dl<1>, g, dim3(256), 0, s, l, a);
+      else hipLaunchKernelGGL(k_ce_dl<6>, g, dim3(256), 0, s, l, a);
+      FC_LAUNCH_CHECK();
+    } else {
+      FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv, a.b32), a, s));
+    }
     if (z.group) {
       px.K = pw.M = a.nv;
       px.b = a.w;

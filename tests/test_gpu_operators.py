@@ -59,7 +59,7 @@ def ce_case(T, V, D, dt, ignored, seed):
 CE = [(1, 2, 1, 0.0, "", ""), (1, 1003, 384, 0.0, "", ""), (7, 50, 16, 0.0, "wide", ""), (33, 257, 64, 0.5, "", "odd"), (64, 1000, 100, 0.0, "odd", ""),
       (65, 513, 7, 0.3, "turned", "turned"), (300, 999, 72, 0.0, "", "wide"), (200, 4100, 136, 0.85, "", ""), (129, 130, 520, 0.0, "", ""), (1030, 6000, 64, 0.2, "", ""),
       (31, 700, 332, 0.0, "", "wide"), (17, 9000, 516, 0.2, "", "odd"), (64, 20, 4, 0.0, "", "turned"), (20, 333, 50, 0.1, "holes", "holes"), (200, 700, 131, 0.1, "", "holes"),
-      (513, 300, 33, 0.0, "holes", "holes")]
+      (513, 300, 33, 0.0, "holes", "holes"), (1, 7, 4000, 0.0, "", ""), (90, 130, 2100, 0.5, "", ""), (300, 45, 1500, 0.9, "odd", "wide"), (40, 1030, 1290, 0.0, "", "")]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
@@ -171,7 +171,7 @@ def test_linear_cross_entropy_module():
 MLP = [(1, 16, 8, "", ""), (1, 384, 1024, "", ""), (5, 7, 3, "", ""), (33, 64, 48, "wide", ""), (64, 1, 5, "", ""), (130, 100, 37, "odd", ""), (257, 192, 515, "", ""),
        (300, 136, 264, "", "turned"), (1000, 64, 24, "turned", "odd"), (700, 320, 640, "", ""), (40, 172, 300, "", "wide"), (64, 1100, 700, "odd", ""), (9, 260, 1028, "", "odd"), (32, 4, 2052, "", "turned"), (20, 37, 70, "holes", "holes"), (130, 101, 35, "", "holes"),
        (512, 130, 67, "", "holes"), (513, 67, 130, "holes", "holes"), (16, 200, 312, "", ""), (17, 200, 312, "", ""),
-       (32, 520, 1032, "", ""), (2, 2056, 24, "", "")]
+       (32, 520, 1032, "", ""), (2, 2056, 24, "", ""), (45, 3200, 130, "", ""), (150, 2051, 77, "", "holes"), (600, 1500, 45, "odd", "")]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
