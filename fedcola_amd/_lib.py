@@ -61,7 +61,7 @@ SIGNATURES = {
     "fc_contrastive_loss_fwd_bwd": (C.c_int, [_P, _P, _I, _I, _F, _P, _Z, _P, _P, _P, _P]),
     "fc_contrastive_scratch_floats": (_Z, [_I]),
     "fc_ce_loss_fwd_bwd": (C.c_int, [_P, _P, _I, _I, _P, _P, _P]),
-    "fc_linear_ce_saved_bytes": (_Z, [_I, _I, _I]),
+    "fc_linear_ce_saved_bytes": (_Z, [_I, _I, _I, _I]),
     "fc_linear_ce_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
     "fc_linear_ce_fwd": (C.c_int, [_I, _P, _L, _P, _L, _P, _I, _I, _I, _L, _I, _P, _P, _Z, _P, _Z, _P]),
     "fc_linear_ce_bwd": (C.c_int, [_I, _P, _L, _I, _I, _I, _I, _P, _P, _Z, _P, _L, _P, _L, _P, _Z, _P]),

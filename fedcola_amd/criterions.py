@@ -96,7 +96,7 @@ def linear_cross_entropy_forward(hidden, weight, targets, ignore_index=-100, red
     T, (V, D), L, red = x.shape[0], w.shape, _lib.lib(), _REDUCTIONS[reduction]
     loss = torch.empty(targets.shape if red == 0 else (), device=dev)
     with on_device(dev) as stream:
-        saved = torch.empty(L.fc_linear_ce_saved_bytes(code, T, D), dtype=torch.uint8, device=dev)
+        saved = torch.empty(L.fc_linear_ce_saved_bytes(code, T, V, D), dtype=torch.uint8, device=dev)
         ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw, T), 0), dtype=torch.uint8, device=dev)
         check(L.fc_linear_ce_fwd(code, x.data_ptr(), ldx, w.data_ptr(), ldw, y.data_ptr(), T, V, D, ignore_index, red, loss.data_ptr(), saved.data_ptr(),
                                  saved.numel(), ws.data_ptr(), ws.numel(), stream))

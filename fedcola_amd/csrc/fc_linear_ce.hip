@@ -1,4 +1,4 @@
-// Softmax cross entropy of a linear layer over a large vocabulary, the logits never kept.
+// Softmax cross entropy of a linear layer over a large vocabulary, the logits not kept (but for a few rows, whose logits are little).
 //
 //   L[t, v] = x[t] . w[v];   lse[t] = log sum_v exp L[t, v];   row[t] = lse[t] - L[t, y[t]]      (0 where y[t] is the ignored index)
 //   dL[t, v] = (exp(L[t, v] - lse[t]) - [v = y[t]]) g[t];      dx = dL w;   dw = dL^T x
@@ -23,9 +23,19 @@ struct CeSaved {
   int *pos, *idx, *y;   // row -> place among them or -1; place -> row; place -> target, -1 for one outside of the vocabulary
   float* lse;      // [place]
   FtMat x;         // gathered rows
+  float* logits;   // [place][ldg] where they are kept, else null
+  long ldg;
   size_t bytes;
 };
-static CeSaved ce_saved(void* base, int dt, long T, long D) {
+// columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
+static long ce_piece(int dt, long T, long V) {
+  const long most = (192L << 20) / ((T ? T : 1) * (dt ? 2 : 6)) / 256 * 256, all = ft_up(V, 256);
+  return most < 256 ? 256 : most < all ? most : all;
+}
+// The logits of a few rows are little beside the weight, which forming them again would read once more (1 x 3648 x 59042 fp32 with gradients: 666 us,
+// 1090 without this and the outer product of fc_tiles.hip; k_ce_grad took 217 of them).
+static bool ce_keep(int dt, long T, long V) { return T > 0 && T <= 32 && T * ft_up(V, 8) <= (1L << 25) && ce_piece(dt, T, V) >= V; }
+static CeSaved ce_saved(void* base, int dt, long T, long V, long D) {
   CeSaved s;
   char* p = (char*)base;
   const long ld = ft_up(D, 64), t4 = ft_up(T * 4, 256);
@@ -37,7 +47,11 @@ static CeSaved ce_saved(void* base, int dt, long T, long D) {
   s.x.p = (bf16_t*)(p + 256 + 4 * t4);
   s.x.ld = ld;
   s.x.plane = T * ld;
-  s.bytes = 256 + 4 * t4 + (size_t)(dt ? 1 : 3) * T * ld * 2;
+  s.bytes = 256 + 4 * t4 + ft_up((dt ? 1 : 3) * T * ld * 2, 256);
+  const bool keep = ce_keep(dt, T, V);
+  s.ldg = ft_up(V, 8);
+  s.logits = keep ? (float*)(p + s.bytes) : nullptr;
+  s.bytes += keep ? T * s.ldg * 4 : 0;
   return s;
 }
 
@@ -115,6 +129,8 @@ struct CeArgs {
   const int *n, *y, *idx;
   CePart* part;               // [tiles of columns][T]
   float* tlogit;              // [T]
+  float* logits;              // [T][ldg], where they are kept
+  long ldg;
   const float *lse, *g;
   int reduction;
   bf16_t* dl;                 // planes of [T][ldl]
@@ -167,6 +183,11 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_stats(CeArgs
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             if (n0 + 16 * j + 4 * g + x >= a.V) acc[i][j][x] = -__builtin_inff();
+      if constexpr (S::TM == 32 || (S::PL == 3 && !S::F32))                     // the tiles of few rows
+        if (a.logits && m < M)
+#pragma unroll
+          for (int j = 0; j < S::NJ; ++j)
+            if (n0 + 16 * j + 4 * g < a.ldg) *(ft_f4*)(a.logits + m * a.ldg + n0 + 16 * j + 4 * g) = acc[i][j];
       CePart p;
       p.m = -__builtin_inff();
 #pragma unroll
@@ -334,6 +355,7 @@ __global__ void __launch_bounds__(256) k_ce_row(CeSlices l, int V, CeSaved s, fl
   CePart p = {-__builtin_inff(), 0.f};
   for (int c = tid * 4; c < V; c += 1024) {
     const ft_f4 v = l.at(at, c, M, slices);
+    if (s.logits) *(ft_f4*)(s.logits + at * s.ldg + c) = v;
 #pragma unroll
     for (int x = 0; x < 4; ++x)
       if (c + x < V) {
@@ -426,11 +448,6 @@ static CeSlices ce_slices(const FtProduct& p, const FtPlan& plan, const float* p
   l.part = part; l.ldp = ft_part_ld(p.N); l.K = p.K; l.target = plan.target; l.TM = plan.TM; l.TN = plan.TN; l.nprod = p.nprod;
   return l;
 }
-// columns of the vocabulary in a piece: what dL of T rows takes stays under 192 MB, in whole 256-column tiles
-static long ce_piece(int dt, long T, long V) {
-  const long most = (192L << 20) / ((T ? T : 1) * (dt ? 2 : 6)) / 256 * 256, all = ft_up(V, 256);
-  return most < 256 ? 256 : most < all ? most : all;
-}
 struct CeSizes { size_t w, part, rows, dl, dxp, dwp; long piece; FtPlan logits, dx, dw; bool group; };
 // dx = dL w and dw = dL^T x of nv columns; n: device, the rows that count
 static void ce_products(int dt, long T, long D, long nv, bool b32, const int* n, FtProduct& x, FtProduct& w) {
@@ -445,7 +462,7 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
   // bf16: 23 and 31), and where the logits are one piece
   z.piece = ce_piece(dt, T, V);
   z.logits = ft_plan(ce_logits(dt, T, V, D, b32, nullptr), false);
-  if (z.logits.gain < 1.3 || z.piece < V) z.logits.target = 0;
+  if (z.logits.gain < 1.3 || z.piece < V || (grad && ce_keep(dt, T, V))) z.logits.target = 0;
   if (z.logits.target) z.part = (size_t)ft_up(ft_part_floats(T, V, z.logits) * 4, 256);
   if (!grad) {
     const int tn = ce_tn(ce_shape(dt, T, V, b32));
@@ -500,7 +517,9 @@ static int ce_weight(int dt, const void* w, long ldw, bool direct, long V, long 
   return ft_pack(l, s);
 }
 
-extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t D) { return T < 0 || D < 1 ? 0 : ce_saved(nullptr, dt, T, D).bytes; }
+extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t V, int32_t D) {
+  return T < 0 || V < 1 || D < 1 ? 0 : ce_saved(nullptr, dt, T, V, D).bytes;
+}
 extern "C" size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward) {
   if (T < 0 || V < 1 || D < 1) return 0;
   const CeSizes z = ce_sizes(dt, T, V, D, !packed && (dt || T <= FT_B32), backward != 0);
@@ -513,7 +532,7 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
   FC_REQUIRE(loss && saved && workspace && ((x && y && ldx >= D) || T == 0), "fc_linear_ce_fwd: null pointer, or rows %ld apart", (long)ldx);
   FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_fwd: reduction %d", reduction);
   FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_fwd: saved and workspace are aligned to 256 bytes");
-  const CeSaved sv = ce_saved(saved, dt, T, D);
+  const CeSaved sv = ce_saved(saved, dt, T, V, D);
   const bool direct = ce_direct(dt, w, ldw, T, D);
   const CeSizes z = ce_sizes(dt, T, V, D, direct, false);
   FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.part + z.rows, "fc_linear_ce_fwd: saved or workspace too small");
@@ -525,6 +544,7 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
   a.b32 = !dt && direct;
   a.T = T; a.V = V; a.D = D; a.v0 = 0; a.nv = V;
   a.n = sv.n; a.y = sv.y; a.idx = sv.idx;
+  a.logits = sv.logits; a.ldg = sv.ldg;
   a.part = (CePart*)ws;
   a.tlogit = (float*)(ws + z.part);
   float* rows = reduction == FC_REDUCE_NONE ? loss : (float*)(ws + z.part + z.rows / 2);
@@ -571,7 +591,7 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   FC_REQUIRE((gloss || T == 0) && saved && workspace && (!dx || lddx >= D) && (!dw || lddw >= D), "fc_linear_ce_bwd: null pointer, or an output's rows too close");
   FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_bwd: reduction %d", reduction);
   FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_bwd: saved and workspace are aligned to 256 bytes");
-  const CeSaved sv = ce_saved((void*)saved, dt, T, D);
+  const CeSaved sv = ce_saved((void*)saved, dt, T, V, D);
   const bool direct = ce_direct(dt, w, ldw, T, D);
   const CeSizes z = ce_sizes(dt, T, V, D, direct, true);
   FC_REQUIRE(saved_bytes >= sv.bytes && workspace_bytes >= z.w + z.part + z.dl + z.dxp + z.dwp, "fc_linear_ce_bwd: saved or workspace too small");
@@ -606,12 +626,12 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
   for (long v0 = 0; v0 < V; v0 += z.piece) {
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < z.piece ? V - v0 : z.piece);
-    if (z.logits.target) {
+    if (z.logits.target || sv.logits) {
       FtProduct p = ce_logits(dt, T, V, D, a.b32, sv.n);
       p.a = a.x;
       p.b = a.w;
-      FC_TRY(ft_product(p, z.logits, part, false, s));
-      const CeSlices l = ce_slices(p, z.logits, part);
+      if (!sv.logits) FC_TRY(ft_product(p, z.logits, part, false, s));
+      const CeSlices l = ce_slices(p, z.logits, sv.logits ? sv.logits : part);
       const dim3 g((unsigned)(((long)T * ((V + 7) / 8) + 255) / 256));
       if (dt) hipLaunchKernelGGL(k_ce_dl<1>, g, dim3(256), 0, s, l, a);
       else hipLaunchKernelGGL(k_ce_dl<6>, g, dim3(256), 0, s, l, a);

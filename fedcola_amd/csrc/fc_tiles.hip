@@ -380,11 +380,82 @@ int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, 
   return 0;
 }
 
+// ---------------------------------------------------------------- fp32, a reduction over few rows: C[m, n] = sum_k A[k, m] B[k, n], k < 32
+// All that costs time is the writing of C, of which the tiles, one workgroup of eight waves a CU, reach half the rate (38227 x 2816, 11 rows: 178 us;
+// here 72, 6 TB/s).  A wave's lanes hold four columns each of all rows of B; the values of A, of `per` rows of C, come from LDS.
+// Where C is small and the rows are not the fewest, the tiles' start is the shorter one (gated block with gradients, 768 x 2048, 32 rows: 104 us with
+// tiles, 126 here; 4096 x 11008: 779 and 748; 4 rows: 104 and 100, 752 and 627).
+template <int KM>
+__global__ void __launch_bounds__(256) k_ft_outer(FtProduct p, int per, int cols) {      // cols: waves of a workgroup side by side
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* sa = (float*)smem;                                                            // [per][KM]
+  const int K = p.Kdyn ? min(p.K, *p.Kdyn) : p.K, wave = ft_wave(), lane = threadIdx.x & 63;
+  const long m0 = (long)blockIdx.x * per;
+  const int rows = (int)min((long)per, p.M - m0), n = (blockIdx.y * cols + wave % cols) * 256 + lane * 4;
+  auto whole = [](const FtMat& a, long at) {          // four values (the rows of planes are whole groups of 64, zeros behind the last value)
+    ft_f4 v[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      const uint2 u = *(const uint2*)(a.p + q * a.plane + at);
+      v[q] = ft_f4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
+    }
+    return v[0] + (v[1] + v[2]);
+  };
+  for (int e = threadIdx.x; e < KM * (per / 4); e += 256) {
+    const int k = e / (per / 4), r = (e - k * (per / 4)) * 4;
+    const ft_f4 v = k < K && r < rows ? whole(p.a, k * p.a.ld + m0 + r) : ft_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) sa[(r + x) * KM + k] = v[x];
+  }
+  ft_f4 b[KM];
+#pragma unroll
+  for (int k = 0; k < KM; ++k) b[k] = k < K && n < p.N ? whole(p.b, k * p.b.ld + n) : ft_f4{0.f, 0.f, 0.f, 0.f};
+  __syncthreads();
+  if (n >= p.N) return;
+  const float al = p.factor();
+  const bool vec = p.ldo % 4 == 0 && ((size_t)p.out & 15) == 0 && n + 4 <= p.N;
+  for (int r = wave / cols; r < rows; r += 4 / cols) {
+    ft_f4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KM; k += 4) {
+      const ft_f4 v = *(const ft_f4*)(sa + r * KM + k);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) c += v[x] * b[k + x];
+    }
+    const long row = p.rows.at((int)(m0 + r));
+    if (row < 0) continue;
+    c *= al;
+    float* o = (float*)p.out + row * p.ldo + n;
+    if (vec) {
+      *(ft_f4*)o = c;
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (n + x < p.N) o[x] = c[x];
+    }
+  }
+}
+static bool ft_is_outer(const FtProduct& p) { return p.nprod == 6 && p.am == TR && p.bm == TR && p.segs == 1 && p.K <= 32 && (p.K <= 8 || (long)p.M * p.N >= (1L << 24)); }
+static int ft_outer(const FtProduct& p, hipStream_t s) {
+  if (p.M == 0 || p.N == 0) return 0;
+  const int waves = (p.N + 255) / 256, cols = waves >= 3 ? 4 : waves, by = (waves + cols - 1) / cols;
+  int per = 128;
+  while (per > 16 && (long)by * ((p.M + per - 1) / per) < 1024) per /= 2;
+  const dim3 g((unsigned)((p.M + per - 1) / per), (unsigned)by);
+  if (p.K <= 8) hipLaunchKernelGGL(k_ft_outer<8>, g, dim3(256), per * 8 * 4, s, p, per, cols);
+  else if (p.K <= 16) hipLaunchKernelGGL(k_ft_outer<16>, g, dim3(256), per * 16 * 4, s, p, per, cols);
+  else hipLaunchKernelGGL(k_ft_outer<32>, g, dim3(256), per * 32 * 4, s, p, per, cols);
+  FC_LAUNCH_CHECK();
+  return 0;
+}
+
 size_t ft_product_part_floats(const FtProduct& p) {
+  if (ft_is_outer(p)) return 0;
   const FtPlan plan = ft_plan(p, false);
   return plan.target ? ft_part_floats(p.M, p.N, plan) : 0;
 }
 int ft_product_out(const FtProduct& p, float* part, size_t part_floats, hipStream_t s) {
+  if (ft_is_outer(p)) return ft_outer(p, s);
   const FtPlan plan = ft_plan(p, false);
   if (!plan.target) return ft_product(p, plan, nullptr, false, s);
   FC_REQUIRE(part && part_floats >= ft_part_floats(p.M, p.N, plan), "workspace too small for the partial sums");

@@ -43,7 +43,10 @@ def test_c_entries_refuse_bad_arguments():
 
 def test_sizes_of_workspaces():
     L = lib()
-    assert L.fc_linear_ce_saved_bytes(1, 0, 16) > 0 and L.fc_linear_ce_saved_bytes(1, -1, 16) == 0
+    assert L.fc_linear_ce_saved_bytes(1, 0, 9, 16) > 0 and L.fc_linear_ce_saved_bytes(1, -1, 9, 16) == L.fc_linear_ce_saved_bytes(1, 4, 0, 16) == 0
+    # the logits of up to 32 rows are kept, and not of more than 128 MB
+    assert L.fc_linear_ce_saved_bytes(1, 32, 1 << 20, 64) > 32 << 22 > L.fc_linear_ce_saved_bytes(1, 33, 1 << 20, 64)
+    assert L.fc_linear_ce_saved_bytes(0, 32, (1 << 20) + 1, 64) < 32 << 20
     for backward in (0, 1):
         small, packed = (L.fc_linear_ce_workspace_bytes(1, 100, 1000, 64, p, backward) for p in (0, 1))
         assert 0 < small and packed >= small + 1000 * 64 * 2
