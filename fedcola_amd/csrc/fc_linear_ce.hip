@@ -92,11 +92,11 @@ __global__ void __launch_bounds__(256) k_ce_rows(const T* x, long ldx, const int
         *(uint4*)d = *(const uint4*)p;
         continue;
       }
-      float h[3][8];
+      float v[8], h[3][8];
+      ft_row8(p, D - c0, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float v = c0 + j < D ? Io<T>::ld(p, j) : 0.f;
-        if (PL == 1) h[0][j] = v; else ft_split(v, h[0][j], h[1][j], h[2][j]);
+        if (PL == 1) h[0][j] = v[j]; else ft_split(v[j], h[0][j], h[1][j], h[2][j]);
       }
 #pragma unroll
       for (int q = 0; q < PL; ++q)

@@ -560,6 +560,16 @@ template <int IW> __device__ __forceinline__ void ft_img_put(char* img, int row,
 // image -> global: rows m0 + r < M, columns n0 + c < N of a row-major bf16 matrix
 template <int IR, int IW, int NT>
 __device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld, int m0, int n0, int M, int N, const FtRows& rows, bool vec) {
+  if (!vec) {                             // rows at any element: a wave's lanes write neighbouring ones
+#pragma unroll 4
+    for (int e = threadIdx.x; e < IR * IW; e += NT) {
+      const int r = e / IW, c = e % IW, m = m0 + r, n = n0 + c;
+      if (m >= M || n >= N) continue;
+      const long row = rows.at(m);
+      if (row >= 0) out[row * ld + n] = *(const bf16_t*)(img + ft_img<IW>(r, c >> 3) + (c & 7) * 2);
+    }
+    return;
+  }
 #pragma unroll 4
   for (int e = threadIdx.x; e < IR * (IW / 8); e += NT) {
     const int r = e / (IW / 8), c = e % (IW / 8), m = m0 + r, n = n0 + c * 8;
@@ -568,7 +578,7 @@ __device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld
     if (row < 0) continue;
     const uint4 v = *(const uint4*)(img + ft_img<IW>(r, c));
     bf16_t* o = out + row * ld + n;
-    if (vec && n + 8 <= N) {
+    if (n + 8 <= N) {
       *(uint4*)o = v;
     } else {
       const unsigned w[4] = {v.x, v.y, v.z, v.w};
@@ -578,6 +588,7 @@ __device__ __forceinline__ void ft_img_out(const char* img, bf16_t* out, long ld
     }
   }
 }
+
 // the same for one wave's 16 rows of W columns, in 16 * W * 2 bytes of its own: no barrier
 template <int W> __device__ __forceinline__ int ft_wimg(int row, int chunk) { return row * (W * 2) + ((chunk ^ (W == 64 ? row & 7 : (row >> 1) & 3 & (W / 8 - 1))) << 4); }
 template <int W> __device__ __forceinline__ void ft_wimg_put(char* img, int row, int col, float a, float b, float c, float d) {
@@ -590,6 +601,30 @@ template <int W> __device__ __forceinline__ void ft_wimg_out(const char* img, bf
     const uint4 v = *(const uint4*)(img + ft_wimg<W>(r, c));
     if (m0 + r < M && n0 + c * 8 < N) *(uint4*)(out + (long)(m0 + r) * ld + n0 + c * 8) = v;
   }
+}
+
+// eight values of a row, fewer where it ends, 0 behind its end.  bf16 rows may start at any element: whole dwords are read, from the one that
+// holds the first value to the one that holds the last, and shifted.
+template <typename T> __device__ __forceinline__ void ft_row8(const T* p, int cols, float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    if (cols >= 8) {
+      const bool odd = ((size_t)p & 2) != 0;
+      const unsigned* q = (const unsigned*)((size_t)p & ~(size_t)3);
+      unsigned w[5];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = q[j];
+      w[4] = odd ? q[4] : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned u = odd ? w[j] >> 16 | w[j + 1] << 16 : w[j];
+        v[2 * j] = __uint_as_float(u << 16);
+        v[2 * j + 1] = __uint_as_float(u & 0xffff0000u);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < cols ? Io<T>::ld(p, j) : 0.f;
 }
 
 // ---------------------------------------------------------------- host side (fc_tiles.hip)

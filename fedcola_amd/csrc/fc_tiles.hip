@@ -30,8 +30,7 @@ __global__ void __launch_bounds__(256) k_ft_pack(FtPacks l) {
   const long cw = a.ldd / 8, r = (e - e0) / cw;
   const int c0 = (int)(e - e0 - r * cw) * 8;
   float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = c0 + j < a.C ? Io<T>::ld((const T*)a.src, (size_t)(r * a.lds + c0 + j)) : 0.f;
+  ft_row8((const T*)a.src + r * a.lds + c0, (int)(a.C - c0), v);
   float h[3][8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
