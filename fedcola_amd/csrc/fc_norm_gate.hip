@@ -7,7 +7,8 @@
 // it holds.  h comes from r before r is rounded.
 // Backward: r and both norms' statistics are formed again from y and x, so nothing is kept and dwn, dwp are those of the unrounded r.
 // Bound: HBM, 4 T D elements forward (y, x in; r, h out), 6 T D backward (y, x, dr, dh in; dy, dx out).
-// A row is held in registers by a wave (D <= 1024), 4 waves (<= 2048, backward <= 4096) or 8 (<= 8192): 8 or 16 values a lane.  A workgroup walks several
+// A row is held in registers by 8, 16 or 32 lanes (D <= 64, 128, 256), a wave (<= 1024), 4 waves (<= 2048, backward <= 4096) or 8 (<= 8192): 8 or 16
+// values a lane.  A workgroup walks several
 // rows with the weight vectors in registers (forward) or LDS (backward): read per row they would be 20 bytes an element from L2 beside the 8
 // from HBM.  The next row is loaded while this one is summed.  Measured at the rate of a large copy (4.9 TB/s) for 65536 x 4096 bf16: 417 us
 // forward (5.1 TB/s), 667 us backward (4.8 TB/s); 12608 x 384: 13 and 27 us, where filling and draining the chip is most of the time.
@@ -98,29 +99,31 @@ template <typename T, int VEC, int NTH, int E> struct NgRaw {
     }
   }
 };
-// a wave's sum in every lane, by DPP: pairs, quads, eights, sixteens, then the four rows of sixteen (shuffles through LDS cost six round trips
-// instead; the rows' sums stand in the way of every row's loads)
-__device__ __forceinline__ float ng_wave_sum(float v) {
+// the sum of each G lanes of a wave in all of them, by DPP: pairs, quads, eights, sixteens, then the rows of sixteen (shuffles through LDS cost six
+// round trips instead; the rows' sums stand in the way of every row's loads)
+template <int G> __device__ __forceinline__ float ng_lane_sum(float v) {
 #define NG_DPP(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, false))
   NG_DPP(0xb1);     // quad_perm 1 0 3 2
   NG_DPP(0x4e);     // quad_perm 2 3 0 1
   NG_DPP(0x141);    // row_half_mirror
-  NG_DPP(0x140);    // row_mirror
+  if (G > 8) NG_DPP(0x140);    // row_mirror
 #undef NG_DPP
+  if (G <= 16) return v;
+  if (G == 32) return v + __shfl_xor(v, 16, 64);
   const int i = __float_as_int(v);
   return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
          (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
 }
 // sums over a row's lanes.  W waves: through LDS, one barrier, two buffers in turn (a wave is never two sums ahead of another)
-template <int W> struct NgSum {
+template <int W, int G> struct NgSum {
   float2* red;     // [2][W]
   int turn = 0;
   __device__ __forceinline__ float2 operator()(float a, float b) {
-    a = ng_wave_sum(a);
-    b = ng_wave_sum(b);
+    a = ng_lane_sum<G>(a);
+    b = ng_lane_sum<G>(b);
     return join(a, b);
   }
-  __device__ __forceinline__ float operator()(float a) { return join(ng_wave_sum(a), 0.f).x; }
+  __device__ __forceinline__ float operator()(float a) { return join(ng_lane_sum<G>(a), 0.f).x; }
   __device__ __forceinline__ float2 join(float a, float b) {
     if (W == 1) return make_float2(a, b);
     float2* q = red + turn * W;
@@ -172,12 +175,12 @@ struct NgSample {
   }
 };
 
-template <typename T, int VEC, int W, int E>
+template <typename T, int VEC, int W, int E, int G>
 __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
-  constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;       // rows at once
+  constexpr int NTH = W == 1 ? G : W * 64, RB = W == 1 ? 256 / G : 1;       // lanes of a row, rows at once
   __shared__ float2 red[2 * W];
-  NgSum<W> sum{red};
-  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D;
+  NgSum<W, G> sum{red};
+  const int l = W == 1 ? threadIdx.x % G : threadIdx.x, sub = W > 1 ? 0 : G == 64 ? ft_wave() : threadIdx.x / G, D = a.D;
   const unsigned grp = blockIdx.x / (unsigned)a.blocks;
   const long b0 = (long)(blockIdx.x - grp * (unsigned)a.blocks) * a.per, first = (long)grp * a.gate_rows + b0, left = a.gate_rows - b0;
   const int n = (int)(left < a.per ? left : a.per);
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
   for (int i = sub; i < n; i += RB) {
     const long row = first + i;
     float y[E], x[E];
-    s = ng_uniform(snext);
+    s = G == 64 ? ng_uniform(snext) : snext;
     ry.get(y, l, D, s != 0.f);
     rx.get(x, l, D, true);
     fetch(i + RB);
@@ -223,13 +226,13 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
 
 // The weight vectors stand in LDS here: with the five running sums and the next row's loads they do not fit the registers.
 enum { NG_WP = 0, NG_BP, NG_GT, NG_WN, NG_VECS };
-template <typename T, int VEC, int W, int E>
-__global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 && VEC == 8 ? 4 : 3) : 2) k_ng_bwd(NgArgs a) {
-  constexpr int NTH = W * 64, RB = W == 1 ? 4 : 1;
+template <typename T, int VEC, int W, int E, int G>
+__global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 && VEC == 8 && G == 64 ? 4 : 3) : 2) k_ng_bwd(NgArgs a) {
+  constexpr int NTH = W == 1 ? G : W * 64, RB = W == 1 ? 256 / G : 1;
   extern __shared__ __attribute__((aligned(16))) float vec[];   // [NG_VECS][Dp], then for W = 1 [4][NG_SUMS][Dp] over them
   __shared__ float2 red[2 * W];
-  NgSum<W> sum{red};
-  const int l = W == 1 ? threadIdx.x & 63 : threadIdx.x, sub = W == 1 ? ft_wave() : 0, D = a.D, Dp = (D + 7) & ~7;
+  NgSum<W, G> sum{red};
+  const int l = W == 1 ? threadIdx.x % G : threadIdx.x, sub = W > 1 ? 0 : G == 64 ? ft_wave() : threadIdx.x / G, D = a.D, Dp = (D + 7) & ~7;
   const float inv = 1.f / (float)D;
   const unsigned grp = blockIdx.x / (unsigned)a.blocks;
   const long b0 = (long)(blockIdx.x - grp * (unsigned)a.blocks) * a.per, first = (long)grp * a.gate_rows + b0, left = a.gate_rows - b0;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 &
   for (int i = sub; i < n; i += RB) {
     const long row = first + i;
     float y[E], x[E], d[E], dn[E], w[E], v[E];
-    s = ng_uniform(snext);
+    s = G == 64 ? ng_uniform(snext) : snext;
     ry.get(y, l, D, s != 0.f);
     rx.get(x, l, D, true);
     rr.get(d, l, D, a.dr != nullptr);
@@ -338,9 +341,16 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 &
   if (!a.part) return;
   float* o = a.part + (long)blockIdx.x * NG_SUMS * D;
   if (W == 1) {
-    __syncthreads();
 #pragma unroll
-    for (int q = 0; q < NG_SUMS; ++q) ng_store<float, VEC, NTH, E>(vec + (sub * NG_SUMS + q) * Dp, l, D, sums[q]);
+    for (int o = G; o < 64; o *= 2)                       // the wave's other rows
+#pragma unroll
+      for (int q = 0; q < NG_SUMS; ++q)
+#pragma unroll
+        for (int k = 0; k < E; ++k) sums[q][k] += __shfl_xor(sums[q][k], o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) < G)
+#pragma unroll
+      for (int q = 0; q < NG_SUMS; ++q) ng_store<float, VEC, NTH, E>(vec + (ft_wave() * NG_SUMS + q) * Dp, l, D, sums[q]);
     __syncthreads();
     const int st = NG_SUMS * Dp;
     for (int c = threadIdx.x; c < NG_SUMS * D; c += 256) {
@@ -379,27 +389,29 @@ __global__ void __launch_bounds__(1024) k_ng_sum(const float* part, int D, long 
 }
 
 // ---------------------------------------------------------------- host
-// Waves of a row and values of a lane.  A wave alone needs no barriers for its sums, so one takes a row as long as 16 values a lane are enough
+// Waves of a row, values of a lane, and lanes of a row that is shorter than a wave (262144 x 64 bf16: 24 and 49 us forward and backward, 112 and 252 with
+// a wave a row; 131072 x 256: 49 and 95, 62 and 141).  A wave alone needs no barriers for its sums, so one takes a row as long as 16 values a lane are enough
 // (12608 x 768 bf16: 19 and 41 us forward and backward, 30 and 67 by four waves of 8 values; 16384 x 1024: 30 and 50, 39 and 82); above, backward 16 values leave two workgroups a
 // CU instead of one of twice the waves (65536 x 4096 bf16: 667 us against 1151), forward 8 are as good.
-static void ng_form(long D, bool bwd, int& W, int& E) {
+static void ng_form(long D, bool bwd, int& W, int& E, int& G) {
+  G = D <= 64 ? 8 : D <= 128 ? 16 : D <= 256 ? 32 : 64;
   W = D <= 1024 ? 1 : D <= 2048 || (bwd && D <= 4096) ? 4 : 8;
   E = D <= 512 || (D > 1024 && D <= 2048) || (!bwd && D <= 4096 && D > 2048) ? 8 : 16;
 }
 // workgroups of a gate vector's rows: in all as many as the chip holds at once, each wave with the same number of rows.  deep: waves a SIMD that
 // the registers allow
 static void ng_split(long T, long gate_rows, long D, bool bwd, int deep, long& per, long& blocks) {
-  int W, E;
-  ng_form(D, bwd, W, E);
-  const long groups = T / gate_rows, at_once = W == 1 ? 4 : 1, waves = 4 * 256 * deep, want = waves / (W == 1 ? 4 : W);
+  int W, E, G;
+  ng_form(D, bwd, W, E, G);
+  const long groups = T / gate_rows, at_once = W == 1 ? 256 / G : 1, waves = 4 * 256 * deep, want = waves / (W == 1 ? 4 : W);
   const long b = (want + groups - 1) / groups;
   per = ft_up((gate_rows + b - 1) / b, at_once);
   blocks = (gate_rows + per - 1) / per;
 }
 static int ng_deep(long D, bool bwd, int dt) {
-  int W, E;
-  ng_form(D, bwd, W, E);
-  if (bwd) return E == 16 ? 2 : dt ? 4 : 3;
+  int W, E, G;
+  ng_form(D, bwd, W, E, G);
+  if (bwd) return E == 16 ? 2 : dt && G == 64 ? 4 : 3;
   return W == 8 ? (E == 16 ? 2 : 4) : E == 16 ? 3 : 5;
 }
 static bool ng_aligned(const NgArgs& a, int dt) {
@@ -411,26 +423,29 @@ static bool ng_aligned(const NgArgs& a, int dt) {
 template <typename T, bool BWD> static int ng_launch(const NgArgs& a, int dt, hipStream_t s) {
   const dim3 g((unsigned)(a.T / a.gate_rows * a.blocks));
   const bool v = ng_aligned(a, dt);
-#define NG_RUN(VEC, W, E)                                                                                             \
+#define NG_RUN(VEC, W, E, G)                                                                                           \
   do {                                                                                                                \
     if constexpr (BWD) {                                                                                              \
       static FtLds allowed;                                                                                           \
       constexpr int rows = W == 1 ? 4 * NG_SUMS : NG_VECS;                                                            \
-      FC_TRY(allowed.allow((const void*)k_ng_bwd<T, VEC, W, E>, rows * W * 64 * E * 4));                              \
-      hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), rows * ((a.D + 7) & ~7) * 4, s, a);   \
+      FC_TRY(allowed.allow((const void*)k_ng_bwd<T, VEC, W, E, G>, rows * W * 64 * E * 4));                              \
+      hipLaunchKernelGGL((k_ng_bwd<T, VEC, W, E, G>), g, dim3(W == 8 ? 512 : 256), rows * ((a.D + 7) & ~7) * 4, s, a);   \
     } else {                                                                                                          \
-      hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                             \
+      hipLaunchKernelGGL((k_ng_fwd<T, VEC, W, E, G>), g, dim3(W == 8 ? 512 : 256), 0, s, a);                             \
     }                                                                                                                 \
   } while (0)
-#define NG_PICK(W, E) do { if (v) NG_RUN(8, W, E); else NG_RUN(1, W, E); } while (0)
-  int W, E;
-  ng_form(a.D, BWD, W, E);
-  if (W == 1 && E == 8) NG_PICK(1, 8);
-  else if (W == 1) NG_PICK(1, 16);
-  else if (W == 4 && E == 8) NG_PICK(4, 8);
-  else if (W == 4) { if constexpr (BWD) NG_PICK(4, 16); }
-  else if (E == 8) { if constexpr (!BWD) NG_PICK(8, 8); }
-  else NG_PICK(8, 16);
+#define NG_PICK(W, E, G) do { if (v) NG_RUN(8, W, E, G); else NG_RUN(1, W, E, G); } while (0)
+  int W, E, G;
+  ng_form(a.D, BWD, W, E, G);
+  if (G == 8) NG_PICK(1, 8, 8);
+  else if (G == 16) NG_PICK(1, 8, 16);
+  else if (G == 32) NG_PICK(1, 8, 32);
+  else if (W == 1 && E == 8) NG_PICK(1, 8, 64);
+  else if (W == 1) NG_PICK(1, 16, 64);
+  else if (W == 4 && E == 8) NG_PICK(4, 8, 64);
+  else if (W == 4) { if constexpr (BWD) NG_PICK(4, 16, 64); }
+  else if (E == 8) { if constexpr (!BWD) NG_PICK(8, 8, 64); }
+  else NG_PICK(8, 16, 64);
 #undef NG_PICK
 #undef NG_RUN
   FC_LAUNCH_CHECK();

@@ -242,7 +242,9 @@ NORM = [(1, 1, 384, "layer", 1, 1, "sample", 0), (3, 5, 1, "layer", 1, 1, "all",
         (4, 197, 384, "layer", 1, 1, "sample", 1), (5, 40, 511, "layer", 1, 1, "all", 0), (2, 33, 512, "rms", 0, 1, "sample", 1), (3, 9, 513, "layer", 1, 0, "sample", 1),
         (2, 50, 1000, "layer", 0, 1, "", 0), (7, 3, 2048, "rms", 1, 1, "all", 1), (2, 6, 2051, "layer", 1, 1, "sample", 0), (1, 300, 4096, "rms", 1, 1, "all", 0),
         (2, 5, 4100, "layer", 1, 1, "all", 1), (3, 4, 5001, "rms", 1, 1, "sample", 0), (2, 3, 8192, "layer", 1, 1, "sample", 1), (2, 3, 64, "layer", 0, 0, "sample", 1),
-        (1500, 2, 64, "layer", 1, 1, "sample", 1)]
+        (1500, 2, 64, "layer", 1, 1, "sample", 1), (3, 70, 8, "layer", 1, 1, "sample", 1), (2, 333, 61, "layer", 1, 1, "sample", 1), (5, 33, 65, "rms", 1, 1, "all", 1),
+        (2, 130, 128, "layer", 1, 1, "", 1), (37, 3, 129, "layer", 1, 1, "sample", 1), (3, 100, 256, "layer", 0, 1, "sample", 0), (2, 41, 257, "rms", 1, 1, "sample", 1),
+        (1, 5000, 24, "layer", 1, 0, "all", 0)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
