@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(256) k_txt_embed_bwd_v(const T* __restrict__ d
       // same wave, same row group: the LDS write above is visible to the reads below once lgkmcnt drains (no barrier needed)
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (live && id != 0) {
+      if (live && id != 0 && dword) {
         float* wrow = dword + (size_t)id * D + 128 * t;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -498,9 +498,100 @@ __global__ void __launch_bounds__(256) k_txt_embed_bwd_v(const T* __restrict__ d
   for (int i = threadIdx.x; i < D; i += 256) {
     const float de = red_dyn[(0 * 3 + 0) * D + i] + red_dyn[(1 * 3 + 0) * D + i] + red_dyn[(2 * 3 + 0) * D + i] + red_dyn[(3 * 3 + 0) * D + i];
     atomicAdd(dpos + (size_t)n * D + i, de);
+    if (!dtype) continue;
     atomicAdd(dtype + i, de);
     atomicAdd(dg + i, red_dyn[(0 * 3 + 1) * D + i] + red_dyn[(1 * 3 + 1) * D + i] + red_dyn[(2 * 3 + 1) * D + i] + red_dyn[(3 * 3 + 1) * D + i]);
     atomicAdd(db + i, red_dyn[(0 * 3 + 2) * D + i] + red_dyn[(1 * 3 + 2) * D + i] + red_dyn[(2 * 3 + 2) * D + i] + red_dyn[(3 * 3 + 2) * D + i]);
+  }
+}
+// The gradients of few tokens without atomics, so that two runs give the same bits.  Word table: a wave a token; the wave of an id's first token adds up all of
+// its tokens, in their order.  (The order of the atomics above moved the word table by 6e-7 in a step, and through rounding to bf16 whatever follows it.)
+#define TXT_ORDERED 256
+template <typename T>
+__global__ void __launch_bounds__(64) k_txt_word_grad(const T* __restrict__ dy, const int64_t* __restrict__ ids, const float* __restrict__ word,
+                                                      const float* __restrict__ pos, const float* __restrict__ type, const float* __restrict__ mean,
+                                                      const float* __restrict__ rstd, const float* __restrict__ g, float* dword, int rows, int N, int D, int vocab) {
+  const int first = blockIdx.x, lane = threadIdx.x;
+  const long id = clamp_id(ids[first], vocab);
+  if (id == 0) return;
+  const float* w = word + (size_t)id * D;
+  float sum[TEB_MAXV];
+#pragma unroll
+  for (int t = 0; t < TEB_MAXV; ++t) sum[t] = 0.f;
+  for (int r0 = 0; r0 < rows; r0 += 64) {
+    const int r = r0 + lane;
+    unsigned long long same = __ballot(r < rows && clamp_id(ids[r < rows ? r : 0], vocab) == id);
+    if (r0 <= first && (same & (first - r0 < 64 ? (1ull << (first - r0)) - 1 : ~0ull))) return;      // an earlier token has the id
+    for (; same; same &= same - 1) {
+      const int row = r0 + __ffsll((long long)same) - 1;
+      const float* pp = pos + (size_t)(row % N) * D;
+      const T* dyr = dy + (size_t)row * D;
+      const float mu = mean[row], rs = rstd[row];
+      float d[TEB_MAXV], xh[TEB_MAXV], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int t = 0; t < TEB_MAXV; ++t) {
+        const int i = lane + 64 * t;
+        d[t] = i < D ? Io<T>::ld(dyr, i) * g[i] : 0.f;
+        xh[t] = i < D ? (w[i] + type[i] + pp[i] - mu) * rs : 0.f;
+        s1 += d[t]; s2 += d[t] * xh[t];
+      }
+      s1 = wave_sum(s1) / (float)D;
+      s2 = wave_sum(s2) / (float)D;
+#pragma unroll
+      for (int t = 0; t < TEB_MAXV; ++t) sum[t] += rs * (d[t] - s1 - xh[t] * s2);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TEB_MAXV; ++t)
+    if (lane + 64 * t < D) atomicAdd(dword + (size_t)id * D + lane + 64 * t, sum[t]);
+}
+// dtype, dgamma and dbeta: 16 waves of one workgroup walk the tokens; their sums are added in the waves' order
+template <typename T>
+__global__ void __launch_bounds__(1024) k_txt_embed_sums(const T* __restrict__ dy, const int64_t* __restrict__ ids, const float* __restrict__ word,
+                                                         const float* __restrict__ pos, const float* __restrict__ type, const float* __restrict__ mean,
+                                                         const float* __restrict__ rstd, const float* __restrict__ g, float* dtype, float* dg, float* db, int rows,
+                                                         int N, int D, int vocab) {
+  extern __shared__ float red_sum[];                  // [16][D]
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float ade[TEB_MAXV], agm[TEB_MAXV], abt[TEB_MAXV];
+#pragma unroll
+  for (int t = 0; t < TEB_MAXV; ++t) { ade[t] = 0.f; agm[t] = 0.f; abt[t] = 0.f; }
+  for (int row = wave; row < rows; row += 16) {
+    const float* w = word + (size_t)clamp_id(ids[row], vocab) * D;
+    const float* pp = pos + (size_t)(row % N) * D;
+    const T* dyr = dy + (size_t)row * D;
+    const float mu = mean[row], rs = rstd[row];
+    float d[TEB_MAXV], xh[TEB_MAXV], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int t = 0; t < TEB_MAXV; ++t) {
+      const int i = lane + 64 * t;
+      d[t] = i < D ? Io<T>::ld(dyr, i) : 0.f;
+      xh[t] = i < D ? (w[i] + type[i] + pp[i] - mu) * rs : 0.f;
+      const float dgm = i < D ? d[t] * g[i] : 0.f;
+      s1 += dgm; s2 += dgm * xh[t];
+    }
+    s1 = wave_sum(s1) / (float)D;
+    s2 = wave_sum(s2) / (float)D;
+#pragma unroll
+    for (int t = 0; t < TEB_MAXV; ++t) {
+      const int i = lane + 64 * t;
+      if (i < D) ade[t] += rs * (d[t] * g[i] - s1 - xh[t] * s2);
+      agm[t] += d[t] * xh[t];
+      abt[t] += d[t];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+#pragma unroll
+    for (int t = 0; t < TEB_MAXV; ++t)
+      if (lane + 64 * t < D) red_sum[wave * D + lane + 64 * t] = q == 0 ? ade[t] : q == 1 ? agm[t] : abt[t];
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += 1024) {
+      float v = 0.f;
+      for (int k = 0; k < 16; ++k) v += red_sum[k * D + i];
+      atomicAdd((q == 0 ? dtype : q == 1 ? dg : db) + i, v);
+    }
+    __syncthreads();
   }
 }
 int fc_txt_embed_bwd(int dt, const void* dy, const int64_t* ids, const float* word, const float* pos, const float* type, const float* mean,
@@ -509,6 +600,13 @@ int fc_txt_embed_bwd(int dt, const void* dy, const int64_t* ids, const float* wo
   if ((D & 7) == 0 && D <= 1024 && !(((uintptr_t)dy | (uintptr_t)word | (uintptr_t)pos | (uintptr_t)type | (uintptr_t)g) & 15)) {
     const int ch = fc_cdiv(D / 8, 16);
     const size_t lds = sizeof(float) * (12 * D + 16 * 144);
+    if (B * N <= TXT_ORDERED) {
+      DISPATCH_DT(dt, hipLaunchKernelGGL(k_txt_word_grad<T>, dim3(B * N), dim3(64), 0, s, (const T*)dy, ids, word, pos, type, mean, rstd, g, dword, B * N, N, D, vocab));
+      DISPATCH_DT(dt, hipLaunchKernelGGL(k_txt_embed_sums<T>, dim3(1), dim3(1024), 16 * D * 4, s, (const T*)dy, ids, word, pos, type, mean, rstd, g, dtype, dg, db,
+                                         B * N, N, D, vocab));
+      FC_LAUNCH_CHECK();
+      dword = dtype = dg = db = nullptr;
+    }
 #define GO(CHN) DISPATCH_DT(dt, hipLaunchKernelGGL((k_txt_embed_bwd_v<T, CHN>), dim3(N, fc_cdiv(B, 16)), dim3(256), lds, s, (const T*)dy, ids, word, pos, type, \
                                                    mean, rstd, g, dword, dpos, dtype, dg, db, B, N, D, vocab))
     switch (ch) {
@@ -631,12 +729,54 @@ __global__ void __launch_bounds__(256) k_head_bwd(const float* __restrict__ din,
     float df = normalize ? (dr[i] - out[(size_t)bi * D + i] * dot) * inv : dr[i];
     float xh = (Io<T>::ld(xr, i) - mu) * rs;
     Io<T>::st(dxr, i, rs * (df * g[i] - s1 - xh * s2));
+    if (!dg) continue;
     atomicAdd(dg + i, df * xh);
     atomicAdd(db + i, df);
   }
 }
+// dgamma and dbeta of few rows without atomics: a wave a row, added in the rows' order
+#define HEAD_ORDERED 16
+template <typename T>
+__global__ void __launch_bounds__(1024) k_head_sums(const float* __restrict__ din, const float* __restrict__ out, const float* __restrict__ nrm, int normalize,
+                                                    const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd, float* dg, float* db,
+                                                    int B, int N, int D) {
+  extern __shared__ float red_sum[];                  // [16][D]
+  const int bi = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float dot = 0.f, inv = 1.f, mu = 0.f, rs = 0.f;
+  const float* dr = din + (size_t)(bi < B ? bi : 0) * D;
+  const float* o = normalize ? out + (size_t)(bi < B ? bi : 0) * D : dr;
+  const T* xr = x + (size_t)(bi < B ? bi : 0) * N * D;
+  if (bi < B) {
+    if (normalize) {
+      for (int i = lane; i < D; i += 64) dot += o[i] * dr[i];
+      dot = wave_sum(dot);
+      inv = 1.0f / nrm[bi];
+    }
+    mu = mean[bi];
+    rs = rstd[bi];
+  }
+  for (int q = 0; q < 2; ++q) {
+    if (bi < B)
+      for (int i = lane; i < D; i += 64) {
+        const float df = normalize ? (dr[i] - o[i] * dot) * inv : dr[i];
+        red_sum[bi * D + i] = q ? df : df * ((Io<T>::ld(xr, i) - mu) * rs);
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += 1024) {
+      float v = 0.f;
+      for (int k = 0; k < B; ++k) v += red_sum[k * D + i];
+      atomicAdd((q ? db : dg) + i, v);          // (other towers' and chains' heads add to the same norm)
+    }
+    __syncthreads();
+  }
+}
 int fc_head_bwd(int dt, const float* din, const float* out, const float* nrm, int normalize, const void* x, const float* mean,
                 const float* rstd, const float* g, void* dx, float* dg, float* db, int B, int N, int D, hipStream_t s) {
+  if (B <= HEAD_ORDERED && D <= 1024) {
+    DISPATCH_DT(dt, hipLaunchKernelGGL(k_head_sums<T>, dim3(1), dim3(1024), 16 * D * 4, s, din, out, nrm, normalize, (const T*)x, mean, rstd, dg, db, B, N, D));
+    FC_LAUNCH_CHECK();
+    dg = db = nullptr;
+  }
   DISPATCH_DT(dt, hipLaunchKernelGGL(k_head_bwd<T>, dim3(fc_cdiv((long)B * N, 4)), dim3(256), 0, s, din, out, nrm, normalize, (const T*)x,
                                      mean, rstd, g, (T*)dx, dg, db, B, N, D));
   FC_LAUNCH_CHECK();
