@@ -411,7 +411,11 @@ static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
 
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
   if (T < 0 || D < 1 || F < 1) return 0;
-  return gm_total(gm_sizes(dt, T, D, F, !dt && !packed && T <= FT_B32, packed || F % 8 || D % 8, backward != 0)) + 256;
+  const bool few = !dt && T <= FT_B32;
+  const size_t n = gm_total(gm_sizes(dt, T, D, F, few, packed || F % 8 || D % 8, backward != 0)) + 256;
+  if (!few || !packed) return n;
+  const size_t planes = gm_total(gm_sizes(dt, T, D, F, false, true, backward != 0)) + 256;      // (weights said to be packed may still be read in place)
+  return n > planes ? n : planes;
 }
 extern "C" int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t ldx, const void* w_in, int64_t ld_in, const void* w_out, int64_t ld_out,
                                 int32_t T, int32_t D, int32_t F, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {

@@ -522,8 +522,15 @@ extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t V, int
 }
 extern "C" size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward) {
   if (T < 0 || V < 1 || D < 1) return 0;
-  const CeSizes z = ce_sizes(dt, T, V, D, !packed && (dt || T <= FT_B32), backward != 0);
-  return z.w + z.part + z.rows + z.dl + z.dxp + z.dwp + 256;
+  size_t most = 0;
+  for (bool direct : {false, true}) {                 // (a weight said to be packed may still be read in place)
+    if (!packed && !direct && (dt || T <= FT_B32)) continue;
+    if (direct && !dt && T > FT_B32) continue;
+    const CeSizes z = ce_sizes(dt, T, V, D, direct, backward != 0);
+    const size_t n = z.w + z.part + z.rows + z.dl + z.dxp + z.dwp + 256;
+    most = most > n ? most : n;
+  }
+  return most;
 }
 extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
                                 int64_t ignore_index, int32_t reduction, float* loss, void* saved, size_t saved_bytes, void* workspace,

@@ -96,6 +96,36 @@ def test_linear_cross_entropy_in_pieces(dt, T):
     within(dw, want["dw"], bound["dw"], "dw")
 
 
+@pytest.mark.parametrize("layout_", ["", "holes"])
+def test_linear_cross_entropy_in_pieces_of_a_weight_in_place(layout_):
+    """fp32 rows few enough that the weight stays where it is, and many enough that the vocabulary comes in two pieces (65536 columns); backward twice"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(512, 70003, 13, "fp32", 0.3, 12)
+    y[:2] = torch.tensor([70002, 65536], device="cuda")
+    g = torch.tensor(1.3, device="cuda")
+    want, bound = O.linear_ce(x, w, y, g, -100, "mean", DT["fp32"])
+    loss, saved = linear_cross_entropy_forward(x, layout(w, layout_), y)
+    first = linear_cross_entropy_backward(g, saved, layout(w, layout_))
+    dx, dw = linear_cross_entropy_backward(g, saved, layout(w, layout_))
+    within(loss, want["loss"], bound["loss"], "loss")
+    within(dx, want["dx"], bound["dx"], "dx")
+    within(dw, want["dw"], bound["dw"], "dw")
+    assert torch.equal(dx, first[0]) and torch.equal(dw, first[1])
+
+
+@pytest.mark.parametrize("T", [1, 32, 33])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_linear_cross_entropy_no_row_counts(dt, T):
+    """every row ignored, with logits kept and not: no loss, zero gradients, nothing read of what the rows hold"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(T, 700, 72, dt, 0.0, 5)
+    x.fill_(math.nan)
+    y.fill_(-100)
+    loss, saved = linear_cross_entropy_forward(x, w, y, reduction="sum")
+    dx, dw = linear_cross_entropy_backward(torch.tensor(2.0, device="cuda"), saved, w)
+    assert loss.item() == 0 and not dx.any() and not dw.any()
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 def test_linear_cross_entropy_masked_rows_hold_anything(dt):
     from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward

@@ -55,6 +55,10 @@ def test_sizes_of_workspaces():
         few = [L.fc_gated_mlp_workspace_bytes(0, 512, 64, 128, p, backward) for p in (0, 1)]
         assert few[1] >= few[0] + 2 * 64 * 128 * 6
         assert L.fc_gated_mlp_workspace_bytes(0, 513, 64, 128, 0, backward) == L.fc_gated_mlp_workspace_bytes(0, 513, 64, 128, 1, backward) > few[1]
+        # a workspace for packed operands is enough for ones in place
+        for T, D, F in ((20, 4096, 64), (512, 2048, 64), (300, 64, 4096)):
+            assert L.fc_gated_mlp_workspace_bytes(0, T, D, F, 1, backward) >= L.fc_gated_mlp_workspace_bytes(0, T, D, F, 0, backward)
+            assert L.fc_linear_ce_workspace_bytes(0, T, 2 * F, D, 1, backward) >= L.fc_linear_ce_workspace_bytes(0, T, 2 * F, D, 0, backward)
         few = [L.fc_linear_ce_workspace_bytes(0, 512, 1000, 64, p, backward) for p in (0, 1)]
         assert few[1] >= few[0] + 1000 * 64 * 6 - 512
 
