@@ -402,9 +402,10 @@ def test_operators_together(dt):
         assert (a.double() - b).norm() <= tol * b.norm(), (k, float((a.double() - b).norm() / b.norm()))
 
 
-def test_operators_captured_into_a_graph():
+@pytest.mark.parametrize("dt,sizes", [("bf16", {}), ("fp32", {}), ("bf16", dict(B=1, N=12, D=1200)), ("fp32", dict(B=1, N=12, D=1200, V=301)), ("fp32", dict(B=1, N=200, D=1201))])
+def test_operators_captured_into_a_graph(dt, sizes):
     """forward and backward of the tower captured once and replayed on new inputs, eager work in between: the eager results, to the bit"""
-    x, y, P, s = tower_case(torch.bfloat16)
+    x, y, P, s = tower_case(DT[dt], **sizes)
     st = torch.cuda.Stream()
     names = ["x", *P]
     sx, sy = x.clone(), y.clone()
@@ -423,7 +424,7 @@ def test_operators_captured_into_a_graph():
     with torch.cuda.graph(graph):
         out = step(sx, sy)
     for k in range(4):
-        x2, y2, _, _ = tower_case(torch.bfloat16, seed=20 + k)
+        x2, y2, _, _ = tower_case(DT[dt], seed=20 + k, **sizes)
         eager = step(x2, y2)
         sx.copy_(x2)
         sy.copy_(y2)
