@@ -405,10 +405,11 @@ typedef FtShape<32, 64, 2, 2, 6> CeRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
 typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> CeRows32;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> CeMid32;
-// 256 x 256 tiles once they fill the chip, 128 x 128 below and for fp32, 32 x 64 for the few rows of a scoring call
+// 256 x 256 tiles where there are enough for three quarters of the chip, 128 x 128 below and for fp32, 32 x 64 (ft_few) for the few rows of a scoring
+// call.  Forward, 768 wide: 512 x 32768 (256 large tiles) 36 us, 42 with 128 x 128; 256 x 32768 (128 tiles) 32 and 27.5.
 static int ce_shape(int dt, long T, long V, bool b32) {
   if ((dt || b32) && ft_few(dt ? 1 : 6, T)) return 2;
-  return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 128 ? 0 : 1;
+  return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 192 ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
 

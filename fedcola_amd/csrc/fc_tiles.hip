@@ -180,7 +180,8 @@ static const int kTM[6] = {256, 128, 32, 128, 32, 128}, kTN[6] = {256, 128, 64, 
 static long tiles_of(const FtPlan& pl, long M, long N) { return ((M + kTM[pl.shape] - 1) / kTM[pl.shape]) * ((N + kTN[pl.shape] - 1) / kTN[pl.shape]); }
 // The cheaper of the shapes and slice counts by a model of the time: rounds of tiles over the chip times (k-steps of a slice x time of a
 // step + time of a tile's start and end), plus the partial sums' way to memory and back.  The constants are measured: 256 x 256 tiles run
-// a k-step in 1.6 us on all CUs (1.3 PFLOP/s), 128 x 128 ones in 1.15 us, two a CU (0.93), and where they leave half of the chip idle, 0.8.
+// a k-step in 1.6 us on all CUs (1.3 PFLOP/s), 128 x 128 ones in 1.15 us, two a CU (0.93), and where they leave half of the chip idle, 0.8; 32 x 64 ones in 0.45.
+// fp32, in 64 k: 2.6 us from planes, 2.8 with B split on the way, 1.0 for 32 rows.
 FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
   const long M = p.M, N = p.N, K = (long)p.K * p.segs;
   const int nprod = p.nprod;
