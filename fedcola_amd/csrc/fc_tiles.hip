@@ -264,8 +264,8 @@ int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hi
 
 // ---------------------------------------------------------------- sums of the slices
 // L lanes share a group of eight columns, each with every L-th slice: one where there are many groups, eight where few rows leave the chip
-// waiting for one lane's loads (one row of 4096 columns, 32 slices of
-// two terms: 15 us with one, 5 with eight), and for rows of two terms
+// waiting for one lane's loads (512 groups, 32 slices of two terms: 15 us
+// with one, 5 with eight; 122880 groups of 4 slices: 8 and 15), and for rows of two terms
 template <typename T, int L>
 __global__ void __launch_bounds__(256) k_ft_reduce(FtSums l) {
   const long e0 = ((long)blockIdx.x * 256 + threadIdx.x) / L;
