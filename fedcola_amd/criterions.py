@@ -139,7 +139,7 @@ class _LinearCEFn(torch.autograd.Function):
 
 class LinearCrossEntropyLoss(nn.Module):
     """``CrossEntropyLoss`` of a linear layer over a large vocabulary: ``loss(hidden, weight, targets)`` = cross entropy of
-    ``hidden @ weight.T``, whose logits [rows, V] are not kept, but for up to 32 rows (``linear_cross_entropy_forward``)."""
+    ``hidden @ weight.T``, whose logits [rows, V] are not kept, but for a few rows (``linear_cross_entropy_forward``)."""
 
     def __init__(self, ignore_index=-100, reduction="mean"):
         super().__init__()

@@ -233,11 +233,11 @@ template <class S, int NPROD, bool GRAD> static int gm_act_launch(const GmArgs& 
   FC_LAUNCH_CHECK();
   return 0;
 }
-// 256 x 256 tiles where there are enough for three quarters of the chip, 128 x 128 below, 32 x 64 (ft_few) for a few rows (forward, 12608 x 384 x 1024, 400
+// 256 x 256 or 128 x 128 tiles by the model of the time, 32 x 64 (ft_few) for a few rows (forward, 12608 x 384 x 1024, 400
 // large tiles: 55 us, 59 with 128 x 128; 2048 x 768 x 2048, 128 tiles: 46 and 42).  Backward: 256 x 256 only where the product is long; the epilogue
 // (8 bytes a unit in, 6 out) stands still while it runs, and two 128 x 128 workgroups a CU cover each other's (12608 x 384 x 1024: 52 us against 70;
 // 8192 x 4096 x 11000 the other way, 1571 against 1310)
-static bool gm_big(int dt, long T, long D, long F, bool grad) { return dt && ((T + 255) / 256) * ((F + 127) / 128) >= 192 && (!grad || D >= 1024); }
+static bool gm_big(int dt, long T, long D, long F, bool grad) { return dt && (!grad || D >= 1024) && ft_large(T, 2 * F, D); }
 template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream_t s) {
   if constexpr (NPROD == 6) {
     return !a.b32 ? gm_act_launch<GmPlanes, NPROD, GRAD>(a, s) : ft_few(6, a.T) ? gm_act_launch<GmRows32, NPROD, GRAD>(a, s) : gm_act_launch<GmMid32, NPROD, GRAD>(a, s);

@@ -33,8 +33,10 @@ static long ce_piece(int dt, long T, long V) {
   return most < 256 ? 256 : most < all ? most : all;
 }
 // The logits of a few rows are little beside the weight, which forming them again would read once more (1 x 3648 x 59042 fp32 with gradients: 666 us,
-// 1090 without this and the outer product of fc_tiles.hip; k_ce_grad took 217 of them).
-static bool ce_keep(int dt, long T, long V) { return T > 0 && T <= 32 && T * ft_up(V, 8) <= (1L << 25) && ce_piece(dt, T, V) >= V; }
+// 1090 without this and the outer product of fc_tiles.hip; k_ce_grad took 217 of them): up to 32 rows, and up to 128 while they are an eighth of it.
+static bool ce_keep(int dt, long T, long V, long D) {
+  return T > 0 && (T <= 32 || (T <= 128 && T * 32 <= D * (dt ? 2 : 4))) && T * ft_up(V, 8) <= (1L << 25) && ce_piece(dt, T, V) >= V;
+}
 static CeSaved ce_saved(void* base, int dt, long T, long V, long D) {
   CeSaved s;
   char* p = (char*)base;
@@ -48,7 +50,7 @@ static CeSaved ce_saved(void* base, int dt, long T, long V, long D) {
   s.x.ld = ld;
   s.x.plane = T * ld;
   s.bytes = 256 + 4 * t4 + ft_up((dt ? 1 : 3) * T * ld * 2, 256);
-  const bool keep = ce_keep(dt, T, V);
+  const bool keep = ce_keep(dt, T, V, D);
   s.ldg = ft_up(V, 8);
   s.logits = keep ? (float*)(p + s.bytes) : nullptr;
   s.bytes += keep ? T * s.ldg * 4 : 0;
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_ce_stats(CeArgs
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             if (n0 + 16 * j + 4 * g + x >= a.V) acc[i][j][x] = -__builtin_inff();
-      if constexpr (S::TM == 32 || (S::PL == 3 && !S::F32))                     // the tiles of few rows
+      if constexpr (S::TM < 256)                                                // (the few rows whose logits are kept never take the large tiles)
         if (a.logits && m < M)
 #pragma unroll
           for (int j = 0; j < S::NJ; ++j)
@@ -405,11 +407,11 @@ typedef FtShape<32, 64, 2, 2, 6> CeRow;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
 typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> CeRows32;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> CeMid32;
-// 256 x 256 tiles where there are enough for three quarters of the chip, 128 x 128 below and for fp32, 32 x 64 (ft_few) for the few rows of a scoring
-// call.  Forward, 768 wide: 512 x 32768 (256 large tiles) 36 us, 42 with 128 x 128; 256 x 32768 (128 tiles) 32 and 27.5.
-static int ce_shape(int dt, long T, long V, bool b32) {
+// 256 x 256 or 128 x 128 tiles by the model of the time (forward, 768 wide: 512 x 32768 36 us, 42 with 128 x 128; 256 x 32768 32 and 27.5; of 13 sizes
+// around the border it takes the faster every time), 128 x 128 for fp32, 32 x 64 (ft_few) for the few rows of a scoring call
+static int ce_shape(int dt, long T, long V, long D, bool b32) {
   if ((dt || b32) && ft_few(dt ? 1 : 6, T)) return 2;
-  return dt && ((T + 255) / 256) * ((V + 255) / 256) >= 192 ? 0 : 1;
+  return dt && ft_large(T, V, D) ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
 
@@ -463,10 +465,10 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
   // bf16: 23 and 31), and where the logits are one piece
   z.piece = ce_piece(dt, T, V);
   z.logits = ft_plan(ce_logits(dt, T, V, D, b32, nullptr), false);
-  if (z.logits.gain < 1.3 || z.piece < V || (grad && ce_keep(dt, T, V))) z.logits.target = 0;
+  if (z.logits.gain < 1.3 || z.piece < V || (grad && ce_keep(dt, T, V, D))) z.logits.target = 0;
   if (z.logits.target) z.part = (size_t)ft_up(ft_part_floats(T, V, z.logits) * 4, 256);
   if (!grad) {
-    const int tn = ce_tn(ce_shape(dt, T, V, b32));
+    const int tn = ce_tn(ce_shape(dt, T, V, D, b32));
     if (!z.logits.target) z.part = (size_t)ft_up((V + tn - 1) / tn * T * (long)sizeof(CePart), 256);
     z.rows = (size_t)ft_up(T * 4, 256) * 2;
     return z;
@@ -575,7 +577,7 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
     else hipLaunchKernelGGL(k_ce_row<6>, dim3(T), dim3(256), 0, s, l, V, sv, rows);
     FC_LAUNCH_CHECK();
   } else {
-    const int shape = ce_shape(dt, T, V, a.b32), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
+    const int shape = ce_shape(dt, T, V, D, a.b32), tn = ce_tn(shape), tiles = (V + tn - 1) / tn;
     FC_TRY(ce_run<false>(dt, shape, a, s));
     if (T) {
       const dim3 gj((unsigned)(T <= 64 ? T : (T + 15) / 16));
@@ -645,7 +647,7 @@ extern "C" int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t 
       else hipLaunchKernelGGL(k_ce_dl<6>, g, dim3(256), 0, s, l, a);
       FC_LAUNCH_CHECK();
     } else {
-      FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv, a.b32), a, s));
+      FC_TRY(ce_run<true>(dt, ce_shape(dt, T, a.nv, D, a.b32), a, s));
     }
     if (z.group) {
       px.K = pw.M = a.nv;

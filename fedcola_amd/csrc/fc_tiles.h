@@ -656,6 +656,8 @@ struct FtPlan {
   double gain = 1;      // time of the best unsliced form over this one's, by the model
 };
 FtPlan ft_plan(const FtProduct& p, bool dynamic_rows);
+// whether a bf16 product that cannot be sliced is faster in tiles of 256 x 256 than of 128 x 128, by the same model
+bool ft_large(long M, long N, long K);
 __host__ __device__ static inline long ft_part_ld(long N) { return (N + 7) / 8 * 8; }
 // slices of a reduction of length K for `tiles` output tiles: as many as the target asks for, none under four k-steps (one of fp32's six products)
 __host__ __device__ static inline int ft_slices(long tiles, long K, int target, int nprod) {

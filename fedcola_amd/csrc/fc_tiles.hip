@@ -182,6 +182,15 @@ static long tiles_of(const FtPlan& pl, long M, long N) { return ((M + kTM[pl.sha
 // step + time of a tile's start and end), plus the partial sums' way to memory and back.  The constants are measured: 256 x 256 tiles run
 // a k-step in 1.6 us on all CUs (1.3 PFLOP/s), 128 x 128 ones in 1.15 us, two a CU (0.93), and where they leave half of the chip idle, 0.8; 32 x 64 ones in 0.45.
 // fp32, in 64 k: 2.6 us from planes, 2.8 with B split on the way, 1.0 for 32 rows.
+static double rounds_of(long wg, int slots) { return wg <= 4 * slots ? (double)((wg + slots - 1) / slots) : (double)wg / slots + 0.5; }
+bool ft_large(long M, long N, long K) {
+  double t[2];
+  for (int sh = 0; sh < 2; ++sh) {
+    const long tiles = tiles_of(FtPlan{sh, 0}, M, N);
+    t[sh] = rounds_of(tiles, kCost[sh].slots) * ((double)((K + 63) / 64) * kCost[sh].step * (sh && 2 * tiles <= kCost[sh].slots ? 0.7 : 1.0) + kCost[sh].fixed);
+  }
+  return t[0] < t[1];
+}
 FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
   const long M = p.M, N = p.N, K = (long)p.K * p.segs;
   const int nprod = p.nprod;
@@ -193,8 +202,7 @@ FtPlan ft_plan(const FtProduct& p, bool dynamic_rows) {
     for (int want = 1; want <= 32; ++want) {
       const int sp = ft_slices(tiles, K, (int)(tiles * want > (1 << 20) ? 0 : tiles * want), nprod);
       const long per = (nk + sp - 1) / sp, wg = tiles * sp, slots = kCost[sh].slots;
-      const double rounds = wg <= 4 * slots ? (double)((wg + slots - 1) / slots) : (double)wg / slots + 0.5;
-      double t = rounds * ((double)per * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
+      double t = rounds_of(wg, slots) * ((double)per * kCost[sh].step * (2 * wg <= slots && sh ? 0.7 : 1.0) + kCost[sh].fixed);
       if (sp > 1) t += 4.0 + (double)sp * M * N * 8.0 / 4e6;
       else if (t < whole) whole = t;
       if (t < least) {
@@ -264,8 +272,8 @@ int ft_product(const FtProduct& p, const FtPlan& plan, float* part, bool add, hi
 
 // ---------------------------------------------------------------- sums of the slices
 // L lanes share a group of eight columns, each with every L-th slice: one where there are many groups, eight where few rows leave the chip
-// waiting for one lane's loads (512 groups, 32 slices of two terms: 15 us
-// with one, 5 with eight; 122880 groups of 4 slices: 8 and 15), and for rows of two terms
+// waiting for one lane's loads (512 groups, 32 slices of two terms: 15 us with one, 5 with eight; 122880 groups of 4 slices: 8 and 15), and for
+// rows of two terms
 template <typename T, int L>
 __global__ void __launch_bounds__(256) k_ft_reduce(FtSums l) {
   const long e0 = ((long)blockIdx.x * 256 + threadIdx.x) / L;

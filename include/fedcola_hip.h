@@ -121,7 +121,8 @@ enum { FC_REDUCE_NONE = 0, FC_REDUCE_MEAN = 1, FC_REDUCE_SUM = 2 };
 enum { FC_ACT_SILU = 0, FC_ACT_GELU = 1 };
 enum { FC_NORM_LAYER = 0, FC_NORM_RMS = 1 };
 
-/* softmax cross entropy of logits x w^T, x [T, D], w [V, D], which are not kept (but for up to 32 rows): loss (fp32: one value, or T with FC_REDUCE_NONE).  Rows with
+/* softmax cross entropy of logits x w^T, x [T, D], w [V, D], which are not kept (but for up to 32 rows, and up to 128
+ * while they are an eighth of w): loss (fp32: one value, or T with FC_REDUCE_NONE).  Rows with
  * y = ignore_index have loss 0, cost nothing, and what they hold reaches no output; MEAN divides by the rows that count (none: NaN).  A target
  * outside of [0, V) makes its row's loss and the gradients NaN.  `saved` (fc_linear_ce_saved_bytes) is what fc_linear_ce_bwd reads in x's place. */
 size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t V, int32_t D);

@@ -59,7 +59,7 @@ def ce_case(T, V, D, dt, ignored, seed):
 CE = [(1, 2, 1, 0.0, "", ""), (1, 1003, 384, 0.0, "", ""), (7, 50, 16, 0.0, "wide", ""), (33, 257, 64, 0.5, "", "odd"), (64, 1000, 100, 0.0, "odd", ""),
       (65, 513, 7, 0.3, "turned", "turned"), (300, 999, 72, 0.0, "", "wide"), (200, 4100, 136, 0.85, "", ""), (129, 130, 520, 0.0, "", ""), (1030, 6000, 64, 0.2, "", ""),
       (31, 700, 332, 0.0, "", "wide"), (17, 9000, 516, 0.2, "", "odd"), (64, 20, 4, 0.0, "", "turned"), (20, 333, 50, 0.1, "holes", "holes"), (200, 700, 131, 0.1, "", "holes"),
-      (513, 300, 33, 0.0, "holes", "holes"), (1, 7, 4000, 0.0, "", ""), (90, 130, 2100, 0.5, "", ""), (300, 45, 1500, 0.9, "odd", "wide"), (40, 1030, 1290, 0.0, "", "")]
+      (513, 300, 33, 0.0, "holes", "holes"), (1, 7, 4000, 0.0, "", ""), (90, 130, 2100, 0.5, "", ""), (300, 45, 1500, 0.9, "odd", "wide"), (40, 1030, 1290, 0.0, "", ""), (100, 9000, 1608, 0.2, "", "")]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])

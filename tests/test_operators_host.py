@@ -44,7 +44,8 @@ def test_c_entries_refuse_bad_arguments():
 def test_sizes_of_workspaces():
     L = lib()
     assert L.fc_linear_ce_saved_bytes(1, 0, 9, 16) > 0 and L.fc_linear_ce_saved_bytes(1, -1, 9, 16) == L.fc_linear_ce_saved_bytes(1, 4, 0, 16) == 0
-    # the logits of up to 32 rows are kept, and not of more than 128 MB
+    # the logits of up to 32 rows are kept, of 128 beside a wide enough weight, and not of more than 128 MB
+    assert L.fc_linear_ce_saved_bytes(1, 128, 1000, 2048) > 128 * 4000 + 128 * 4096 > L.fc_linear_ce_saved_bytes(1, 128, 1000, 2047)
     assert L.fc_linear_ce_saved_bytes(1, 32, 1 << 20, 64) > 32 << 22 > L.fc_linear_ce_saved_bytes(1, 33, 1 << 20, 64)
     assert L.fc_linear_ce_saved_bytes(0, 32, (1 << 20) + 1, 64) < 32 << 20
     for backward in (0, 1):
