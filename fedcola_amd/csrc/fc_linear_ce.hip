@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(256) k_ce_rows(const T* x, long ldx, const int
       const int i = e / cw, c0 = (e - i * cw) * 8;
       const T* p = x + (b + src[i]) * ldx + c0;
       bf16_t* d = (bf16_t*)s.x.p + (long)(at + i) * s.x.ld + c0;
-      if (PL == 1 && vec) {
-        *(uint4*)d = *(const uint4*)p;
+      if (PL == 1 && vec) {                                    // (D in whole chunks; the row's padding is zeros, and nothing behind its D values is read)
+        *(uint4*)d = c0 < D ? *(const uint4*)p : make_uint4(0, 0, 0, 0);
         continue;
       }
       float v[8], h[3][8];

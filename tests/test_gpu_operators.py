@@ -126,6 +126,26 @@ def test_linear_cross_entropy_no_row_counts(dt, T):
     assert loss.item() == 0 and not dx.any() and not dw.any()
 
 
+@pytest.mark.parametrize("D", [8, 64, 72, 96, 120, 136])
+def test_linear_cross_entropy_gathers_a_rows_own_values(D):
+    """aligned rows that are no whole 64 values wide, with NaN behind them: of what is gathered for the products, the padding is zeros"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    T, V = 70, 130
+    x, w, y = ce_case(T, V, D, "bf16", 0.3, D)
+    wide = torch.full((T, D + 128), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:, :D] = x
+    loss, saved = linear_cross_entropy_forward(wide[:, :D], w, y, reduction="sum")
+    n, ld, t4 = int((y != -100).sum()), (D + 63) // 64 * 64, (T * 4 + 255) // 256 * 256
+    at = 256 + 4 * t4                                                   # behind the count and the four tables
+    rows = saved[0][at:at + T * ld * 2].view(torch.bfloat16).view(T, ld)[:n]
+    assert torch.equal(rows[:, :D], x[y != -100]) and not rows[:, D:].any()
+    want, bound = O.linear_ce(x, w, y, torch.tensor(1.0, device="cuda"), -100, "sum", DT["bf16"])
+    dx, dw = linear_cross_entropy_backward(torch.tensor(1.0, device="cuda"), saved, w)
+    within(loss, want["loss"], bound["loss"], "loss")
+    within(dx, want["dx"], bound["dx"], "dx")
+    within(dw, want["dw"], bound["dw"], "dw")
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 def test_linear_cross_entropy_masked_rows_hold_anything(dt):
     from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
