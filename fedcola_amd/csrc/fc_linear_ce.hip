@@ -539,8 +539,8 @@ extern "C" int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const vo
                                 int64_t ignore_index, int32_t reduction, float* loss, void* saved, size_t saved_bytes, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   FC_TRY(ce_args("fc_linear_ce_fwd", dt, T, V, D, ldw, w));
-  FC_REQUIRE(loss && saved && workspace && ((x && y && ldx >= D) || T == 0), "fc_linear_ce_fwd: null pointer, or rows %ld apart", (long)ldx);
   FC_REQUIRE(reduction >= FC_REDUCE_NONE && reduction <= FC_REDUCE_SUM, "fc_linear_ce_fwd: reduction %d", reduction);
+  FC_REQUIRE((loss || (T == 0 && reduction == FC_REDUCE_NONE)) && saved && workspace && ((x && y && ldx >= D) || T == 0), "fc_linear_ce_fwd: null pointer, or rows %ld apart", (long)ldx);
   FC_REQUIRE((((size_t)saved | (size_t)workspace) & 255) == 0, "fc_linear_ce_fwd: saved and workspace are aligned to 256 bytes");
   const CeSaved sv = ce_saved(saved, dt, T, V, D);
   const bool direct = ce_direct(dt, w, ldw, T, D);

@@ -171,6 +171,18 @@ def test_linear_cross_entropy_masked_rows_hold_anything(dt):
         assert float(loss) == 0.0
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_linear_cross_entropy_of_no_rows_each(dt):
+    """no rows and a loss for each: an empty loss, an empty gradient of the rows, zeros for the weight"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(4, 30, 24, dt, 0.0, 0)
+    for shape in ((0,), (3, 0)):
+        loss, saved = linear_cross_entropy_forward(x.new_empty(*shape, 24), w, y.new_empty(shape), reduction="none")
+        assert loss.shape == shape and loss.dtype == torch.float32
+        dx, dw = linear_cross_entropy_backward(torch.empty(shape, device="cuda"), saved, w)
+        assert dx.shape == (*shape, 24) and dw.shape == w.shape and not dw.any()
+
+
 def test_linear_cross_entropy_extreme_values():
     from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
     w = torch.zeros(300, 64, device="cuda")
