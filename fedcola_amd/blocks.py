@@ -185,6 +185,8 @@ def norm_gate_residual_backward(d_residual, d_normed, branch, residual, *, post_
     dx = torch.empty(branch.shape, dtype=branch.dtype, device=dev)
     grads = [torch.empty(t.shape, device=dev) if t is not None and weight_grads and i != 3 else None for i, t in enumerate(v)]
     pw, pb, g, s, nw, _ = map(address, v)
+    if not T and grads[2] is not None:
+        grads[2].zero_()                                  # no rows: the library does not see how many gates there are
     gpw, gpb, gg, _, gnw, gnb = map(address, grads)
     L, ws, n = _lib.lib(), None, 0
     with on_device(dev) as stream:

@@ -500,7 +500,7 @@ extern "C" int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_
   a.scale_rows = row_scale && scale_rows ? scale_rows : T ? T : 1;
   FC_TRY(ng_check("fc_norm_gate_bwd", dt, kind, a, dy));
   FC_REQUIRE((dx || T == 0) && (!dr || lddr >= D) && (!dh || lddh >= D) && (!dh || pre_w), "fc_norm_gate_bwd: null pointer, rows too close, or a gradient without its norm");
-  const long groups = T ? T / a.gate_rows : 0;
+  const long groups = T ? T / a.gate_rows : gate_rows ? 0 : 1;      // (no rows: the one vector's gradient is zeros; how many others there are is not known)
   NgOut out = {{d_post_w, d_post_b, d_pre_w, d_pre_b, gate ? d_gate : nullptr}};
   const bool sums = out.p[0] || out.p[1] || out.p[2] || out.p[3] || out.p[4];
   hipStream_t s = (hipStream_t)stream;

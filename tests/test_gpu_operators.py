@@ -363,6 +363,24 @@ def test_norm_gate_residual_dropped_branch_holds_anything(dt):
     assert not g["branch"][1:3].any() and g["branch"][0].any() and not g["gate"][1:3].any()
 
 
+@pytest.mark.parametrize("gate", ["all", "sample"])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_norm_gate_residual_of_no_rows(dt, gate):
+    """no rows: empty results, and zeros for every gradient of a vector, the gate's among them"""
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    S, D = 3, 200
+    _, _, _, _, v = norm_case(S, 1, D, dt, "layer", 1, 1, gate, 1, 4)
+    empty = torch.empty(S, 0, D, dtype=DT[dt], device="cuda")
+    r, h = norm_gate_residual_forward(empty, empty, **v)
+    assert r.shape == h.shape == empty.shape
+    used = [torch.full(s, math.nan, device="cuda") for s in ((S, D), (D,)) for _ in range(32)]      # what new buffers are likely to hold
+    del used
+    got = norm_gate_residual_backward(empty, empty, empty, empty, **v)
+    assert got["branch"].shape == got["residual"].shape == empty.shape
+    for k in ("post_weight", "post_bias", "gate", "pre_weight", "pre_bias"):
+        assert got[k].shape == v[k].shape and not got[k].any(), k
+
+
 def test_norm_gate_residual_module():
     from fedcola_amd.blocks import NormGateResidual
     for kind in ("layer", "rms"):
