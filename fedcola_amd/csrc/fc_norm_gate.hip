@@ -368,23 +368,28 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 &
   }
 }
 
-// out[c] = sum over workgroups of their partial sums: 64 columns by 16 slices of the workgroups
+// out[c] = sum over workgroups of their partial sums: 64 columns by 16 slices of the workgroups.  blockIdx.y: 0 to 3 the four weights, from 4 on gate
+// vectors, each workgroup every (gridDim.y - 4)th of them (there may be more than a launch has workgroups in y)
 struct NgOut { float* p[NG_SUMS]; };
 __global__ void __launch_bounds__(1024) k_ng_sum(const float* part, int D, long blocks, long groups, NgOut out) {
   __shared__ double red[16][64];
   const int q = blockIdx.y < 4 ? blockIdx.y : NG_DGATE, c = blockIdx.x * 64 + (threadIdx.x & 63), sl = threadIdx.x >> 6;
-  const long g = blockIdx.y < 4 ? 0 : blockIdx.y - 4, b0 = g * blocks, b1 = q == NG_DGATE ? b0 + blocks : groups * blocks;
   if (!out.p[q]) return;
-  double v = 0;
-  if (c < D)
+  for (long g = blockIdx.y < 4 ? 0 : blockIdx.y - 4; g < (q == NG_DGATE ? groups : 1); g += gridDim.y - 4) {
+    const long b0 = g * blocks, b1 = q == NG_DGATE ? b0 + blocks : groups * blocks;
+    double v = 0;
+    if (c < D)
 #pragma unroll 4
-    for (long b = b0 + sl; b < b1; b += 16) v += (double)part[(b * NG_SUMS + q) * D + c];
-  red[sl][threadIdx.x & 63] = v;
-  __syncthreads();
-  if (sl == 0 && c < D) {
+      for (long b = b0 + sl; b < b1; b += 16) v += (double)part[(b * NG_SUMS + q) * D + c];
+    __syncthreads();                                   // the vector before has been read
+    red[sl][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (sl == 0 && c < D) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += red[i][threadIdx.x & 63];
-    out.p[q][g * D + c] = (float)v;
+      for (int i = 1; i < 16; ++i) v += red[i][threadIdx.x & 63];
+      out.p[q][g * D + c] = (float)v;
+    }
+    if (q != NG_DGATE) return;
   }
 }
 
@@ -451,6 +456,13 @@ template <typename T, bool BWD> static int ng_launch(const NgArgs& a, int dt, hi
   FC_LAUNCH_CHECK();
   return 0;
 }
+// a launch has fewer than 2^32 threads in a dimension; the backward has no more workgroups than the forward, nor larger ones
+static int ng_grid(const char* what, const NgArgs& a, bool bwd) {
+  int W, E, G;
+  ng_form(a.D, bwd, W, E, G);
+  FC_REQUIRE(a.T / a.gate_rows * a.blocks * (W == 8 ? 512 : 256) < (1L << 32), "%s: too many samples (%ld gate vectors)", what, a.T / a.gate_rows);
+  return 0;
+}
 static int ng_check(const char* what, int dt, int kind, const NgArgs& a, const void* out) {
   FC_REQUIRE(dt == FC_PREC_FP32 || dt == FC_PREC_BF16, "%s: dt %d", what, dt);
   FC_REQUIRE(kind == FC_NORM_LAYER || kind == FC_NORM_RMS, "%s: norm %d", what, kind);
@@ -485,7 +497,7 @@ extern "C" int fc_norm_gate_fwd(int32_t dt, int32_t kind, const void* y, int64_t
   FC_REQUIRE(!a.pre || h || T == 0, "fc_norm_gate_fwd: no place for the second norm's output");
   if (T == 0) return 0;
   ng_split(T, a.gate_rows, D, false, ng_deep(D, false, dt), a.per, a.blocks);
-  FC_REQUIRE(T / a.gate_rows * a.blocks < (1L << 31), "fc_norm_gate_fwd: too many samples");
+  FC_TRY(ng_grid("fc_norm_gate_fwd", a, false));
   return dt ? ng_launch<bf16_t, false>(a, dt, (hipStream_t)stream) : ng_launch<float, false>(a, dt, (hipStream_t)stream);
 }
 extern "C" int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_t lddr, const void* dh, int64_t lddh, const void* y, int64_t ldy, const void* x,
@@ -506,7 +518,7 @@ extern "C" int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_
   hipStream_t s = (hipStream_t)stream;
   if (T) {
     ng_split(T, a.gate_rows, D, true, ng_deep(D, true, dt), a.per, a.blocks);
-    FC_REQUIRE(groups * a.blocks < (1L << 31) && groups < 65000, "fc_norm_gate_bwd: too many samples");
+    FC_TRY(ng_grid("fc_norm_gate_bwd", a, true));
     if (sums) {
       FC_REQUIRE(workspace && ((size_t)workspace & 255) == 0 && workspace_bytes >= (size_t)groups * a.blocks * NG_SUMS * D * sizeof(float), "fc_norm_gate_bwd: workspace too small or not aligned to 256 bytes");
       a.part = (float*)workspace;
@@ -514,7 +526,7 @@ extern "C" int fc_norm_gate_bwd(int32_t dt, int32_t kind, const void* dr, int64_
     FC_TRY(dt ? (ng_launch<bf16_t, true>(a, dt, s)) : (ng_launch<float, true>(a, dt, s)));
   }
   if (sums) {
-    hipLaunchKernelGGL(k_ng_sum, dim3((D + 63) / 64, (unsigned)(4 + (out.p[NG_DGATE] ? groups : 0))), dim3(1024), 0, s, a.part, D, a.blocks, groups, out);
+    hipLaunchKernelGGL(k_ng_sum, dim3((D + 63) / 64, (unsigned)(4 + (!out.p[NG_DGATE] ? 0 : groups < 60000 ? groups : 60000))), dim3(1024), 0, s, a.part, D, a.blocks, groups, out);
     FC_LAUNCH_CHECK();
   }
   return 0;

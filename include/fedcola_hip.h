@@ -145,7 +145,7 @@ int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t lddy, cons
                      int64_t ldd_in, void* dw_out, int64_t ldd_out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* between two branches: n = norm(y) post_w + post_b; r = alpha x + row_scale[t / scale_rows] gate[t / gate_rows] n; h = norm(r) pre_w + pre_b, for y the
- * branch's output and x the residual stream [T, D], D <= 8192; r and h are contiguous.  post_w NULL: n = y; pre_w NULL: no h; gate / row_scale NULL:
+ * branch's output and x the residual stream [T, D], D <= 8192, fewer than 2^23 gate vectors (T / gate_rows; one for each row, say); r and h are contiguous.  post_w NULL: n = y; pre_w NULL: no h; gate / row_scale NULL:
  * 1; gate_rows / scale_rows 0: one vector / value for all rows.  Weights, gate and row_scale are fp32.  A row_scale of 0 drops the branch: its rows
  * of y are not read and their gradient is 0.  The backward takes dr and / or dh (the other NULL) and reads y and x again; the five weight gradients
  * (fp32; d_gate one row for each gate vector) are NULL where not wanted.  T = 0: they are zeros, d_gate with gate_rows 0 alone (else it is not written). */

@@ -333,6 +333,23 @@ def test_norm_gate_residual(S, N, D, kind, post, pre, gate, scale, dt):
             within(t, want[k], bound[k], f"{mode} {k}")
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,D", [(64_999, 8), (65_001, 8), (140_003, 3)])
+def test_norm_gate_residual_a_gate_for_each_row(T, D, dt):
+    """as many gate vectors as rows, more of them than a launch has workgroups in its second dimension"""
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    b, r, dr, dh, v = norm_case(T, 1, D, dt, "layer", 1, 1, "sample", 1, 3)
+    want, bound = O.norm_gate(b, r, DT[dt], **v, d_residual=dr, d_normed=dh)
+    gr, gh = norm_gate_residual_forward(b, r, **v)
+    within(gr, want["r"], bound["r"], "r")
+    within(gh, want["h"], bound["h"], "h")
+    got = norm_gate_residual_backward(dr, dh, b, r, **v)
+    for k, t in got.items():
+        within(t, want[k], bound[k], k)
+    some = norm_gate_residual_backward(dr, dh, b, r, weight_grads=False, **v)
+    assert set(some) == {"branch", "residual"} and all(torch.equal(t, got[k]) for k, t in some.items())
+
+
 def test_norm_gate_residual_layouts():
     """rows of wider buffers, odd strides, unaligned vectors: the same bits as contiguous operands where the values a lane holds are the same"""
     from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
