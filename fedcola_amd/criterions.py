@@ -100,16 +100,18 @@ def linear_cross_entropy_forward(hidden, weight, targets, ignore_index=-100, red
         ws = torch.empty(L.fc_linear_ce_workspace_bytes(code, T, V, D, not in_place(w, ldw, T), 0), dtype=torch.uint8, device=dev)
         check(L.fc_linear_ce_fwd(code, x.data_ptr(), ldx, w.data_ptr(), ldw, y.data_ptr(), T, V, D, ignore_index, red, loss.data_ptr(), saved.data_ptr(),
                                  saved.numel(), ws.data_ptr(), ws.numel(), stream))
-    return loss, (saved, hidden.shape, red)
+    return loss, (saved, hidden.shape, red, (V, code))
 
 
 def linear_cross_entropy_backward(gloss, saved, weight, need_hidden=True, need_weight=True):
-    """Gradients ``(dhidden, dweight)`` for the gradient ``gloss`` of the loss (fp32, of its shape); None where not needed."""
-    saved, shape, red = saved
+    """Gradients ``(dhidden, dweight)`` for the gradient ``gloss`` of the loss (fp32, of its shape); None where not needed.  weight: the forward's."""
+    saved, shape, red, (V, saved_code) = saved
     code, dev = operand_type("linear_cross_entropy", weight)
+    T, D, L = math.prod(shape[:-1]), shape[-1], _lib.lib()
+    if weight.shape != (V, D) or code != saved_code or saved.device != dev:
+        raise ValueError(f"linear_cross_entropy: weight {tuple(weight.shape)} of {weight.dtype} on {weight.device} is not of the size, type and device of the forward's")
     w, ldw = as_rows(weight)
-    T, (V, D), L = math.prod(shape[:-1]), w.shape, _lib.lib()
-    if gloss.shape != (shape[:-1] if red == 0 else ()) or gloss.device != dev or shape[-1] != D:
+    if gloss.shape != (shape[:-1] if red == 0 else ()) or gloss.device != dev:
         raise ValueError(f"linear_cross_entropy: a gradient of shape {tuple(gloss.shape)} on {gloss.device} is not that of the loss")
     g = gloss.float().contiguous()
     dx = torch.empty(shape, dtype=weight.dtype, device=dev) if need_hidden else None
@@ -124,9 +126,9 @@ def linear_cross_entropy_backward(gloss, saved, weight, need_hidden=True, need_w
 class _LinearCEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        loss, (saved, shape, red) = linear_cross_entropy_forward(hidden, weight, targets, ignore_index, reduction)
+        loss, (saved, *how) = linear_cross_entropy_forward(hidden, weight, targets, ignore_index, reduction)
         ctx.save_for_backward(saved, weight)
-        ctx.how = shape, red
+        ctx.how = how
         return loss
 
     @staticmethod

@@ -130,7 +130,8 @@ size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D,
 int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
                      int64_t ignore_index, int32_t reduction, float* loss, void* saved, size_t saved_bytes, void* workspace,
                      size_t workspace_bytes, void* stream);
-/* gloss: device gradient of the loss (one value, or T with FC_REDUCE_NONE); dx [T, D] (0 in ignored rows), dw [V, D]: either may be NULL */
+/* dt, w's values, T, V, D and reduction: those of the forward that filled `saved`, which does not hold them.  gloss: device gradient of the loss (one value, or
+ * T with FC_REDUCE_NONE); dx [T, D] (0 in ignored rows), dw [V, D]: either may be NULL */
 int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t T, int32_t V, int32_t D, int32_t reduction, const float* gloss,
                      const void* saved, size_t saved_bytes, void* dx, int64_t lddx, void* dw, int64_t lddw, void* workspace,
                      size_t workspace_bytes, void* stream);

@@ -183,6 +183,19 @@ def test_linear_cross_entropy_of_no_rows_each(dt):
         assert dx.shape == (*shape, 24) and dw.shape == w.shape and not dw.any()
 
 
+def test_linear_cross_entropy_backward_takes_the_forwards_weight():
+    """what a forward saved belongs to a weight of its type and size: another one is refused"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    g = torch.tensor(1.0, device="cuda")
+    for dt, other in (("fp32", torch.bfloat16), ("bf16", torch.float32)):
+        x, w, y = ce_case(40, 300, 24, dt, 0.0, 2)
+        _, saved = linear_cross_entropy_forward(x, w, y)
+        for bad in (w.to(other), w[:299], torch.cat([w, w]), w[:, :16], w[0]):
+            with pytest.raises(ValueError):
+                linear_cross_entropy_backward(g, saved, bad)
+        linear_cross_entropy_backward(g, saved, w.clone())
+
+
 def test_linear_cross_entropy_extreme_values():
     from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
     w = torch.zeros(300, 64, device="cuda")
