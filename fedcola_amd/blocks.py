@@ -15,7 +15,7 @@ import torch.nn as nn
 
 from . import _lib
 from ._lib import check
-from .operands import address, as_rows, in_place, on_device, operand_type
+from .operands import address, as_rows, check_sizes, in_place, on_device, operand_type
 
 _ACTS = {"silu": 0, "gelu": 1}
 _NORMS = {"layer": 0, "rms": 1}
@@ -29,6 +29,7 @@ def _mlp_operands(x, w_in, w_out, act):
     if w_in.dim() != 2 or w_out.dim() != 2 or x.dim() < 1 or x.shape[-1] != w_in.shape[1] or w_out.shape != (w_in.shape[1], w_in.shape[0] // 2) or \
             w_in.shape[0] % 2 or w_in.numel() == 0:
         raise ValueError(f"gated_mlp: x [..., D], w_in [2F, D], w_out [D, F] are expected, not {tuple(x.shape)}, {tuple(w_in.shape)}, {tuple(w_out.shape)}")
+    check_sizes("gated_mlp", x.numel() // x.shape[-1], w_out.shape[0], 1 << 18, w_out.shape[1], 1 << 20)
     return code, dev, as_rows(x), as_rows(w_in), as_rows(w_out)
 
 

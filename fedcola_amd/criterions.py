@@ -14,7 +14,7 @@ import torch.nn as nn
 
 from . import _lib
 from ._lib import check, ptr
-from .operands import address, as_rows, in_place, on_device, operand_type
+from .operands import address, as_rows, check_sizes, in_place, on_device, operand_type
 
 
 def contrastive_tau() -> float:
@@ -90,6 +90,7 @@ def linear_cross_entropy_forward(hidden, weight, targets, ignore_index=-100, red
         raise ValueError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
     if targets.shape != hidden.shape[:-1] or targets.dtype != torch.int64 or targets.device != dev:
         raise ValueError(f"linear_cross_entropy: targets are int64 of shape {tuple(hidden.shape[:-1])} on {dev}, not {targets.dtype} {tuple(targets.shape)} on {targets.device}")
+    check_sizes("linear_cross_entropy", targets.numel(), weight.shape[1], 1 << 20, weight.shape[0], 1 << 30)
     x, ldx = as_rows(hidden)
     w, ldw = as_rows(weight)
     y = targets.contiguous()

@@ -45,6 +45,12 @@ def as_rows(t):
     return t, ld
 
 
+def check_sizes(what, rows, D, most_D, N, most_N):
+    """refuses sizes past the library's: its arguments are 32 bits wide, and a larger number would arrive as another one"""
+    if rows > 1 << 28 or D > most_D or N > most_N:
+        raise ValueError(f"{what}: {rows} rows, width {D}, {N} classes or hidden units: at most {1 << 28}, {most_D} and {most_N}")
+
+
 def in_place(t, ld, rows):
     """whether the tiled products of `rows` rows read this matrix where it is (include/fedcola_hip.h)"""
     if t.element_size() == 4:

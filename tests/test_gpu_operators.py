@@ -550,6 +550,25 @@ def test_operator_refusals_on_the_device():
             bad()
 
 
+@pytest.mark.parametrize("n", [(1 << 28) + 1, (1 << 32) + 5, 1 << 33])
+def test_sizes_past_the_librarys_are_refused(n):
+    """row counts, vocabularies and widths that 32 bits do not hold, or that a kernel's offsets do not: refused before anything is laid out (the
+    operands are one element, expanded)"""
+    from fedcola_amd import blocks, criterions
+    one = torch.zeros((), dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros((), dtype=torch.int64, device="cuda")
+    many = max(n, (1 << 30) + 1)
+    for bad in (lambda: criterions.linear_cross_entropy_forward(one.expand(n, 1), one.expand(7, 1), y.expand(n)),
+                lambda: criterions.linear_cross_entropy_forward(one.expand(2, 1), one.expand(many, 1), y.expand(2)),
+                lambda: criterions.linear_cross_entropy_forward(one.expand(2, n), one.expand(3, n), y.expand(2)),
+                lambda: blocks.gated_mlp_forward(one.expand(n, 1), one.expand(4, 1), one.expand(1, 2)),
+                lambda: blocks.gated_mlp_forward(one.expand(2, n), one.expand(4, n), one.expand(n, 2)),
+                lambda: blocks.gated_mlp_forward(one.expand(2, 1), one.expand(2 * n, 1), one.expand(1, n)),
+                lambda: blocks.gated_mlp_backward(one.expand(n, 1), one.expand(n, 1), one.expand(4, 1), one.expand(1, 2))):
+        with pytest.raises(ValueError, match="at most"):
+            bad()
+
+
 # ------------------------------------------------------------------------------------------------ offsets past 32 bits
 def test_offsets_past_32_bits_in_the_vocabulary():
     """a weight of 4.9 GB, zeros but for three rows: everything has a closed form"""

@@ -92,6 +92,14 @@ def test_rows_of_a_tensor():
             assert (v.data_ptr() != t.data_ptr()) == copied
 
 
+def test_sizes_that_32_bits_do_not_hold():
+    from fedcola_amd.operands import check_sizes
+    check_sizes("op", 1 << 28, 8, 8, 1 << 30, 1 << 30)
+    for rows, v, d in (((1 << 28) + 1, 4, 4), ((1 << 32) + 5, 4, 4), (4, (1 << 30) + 1, 4), (4, 4, 9)):
+        with pytest.raises(ValueError, match="at most"):
+            check_sizes("op", rows, d, 8, v, 1 << 30)
+
+
 # ---- the oracle itself: its values against torch's functions and autograd in float64
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_oracle_linear_ce(reduction):
