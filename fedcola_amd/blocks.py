@@ -152,7 +152,7 @@ def norm_gate_residual_forward(branch, residual, *, post_weight=None, post_bias=
 
     branch, residual [..., D] in one type, bf16 or fp32; the vectors fp32.  post_weight / post_bias [D]: the norm after the branch (None: no
     norm).  gate [D] for all rows or [S, D], one for each of S (fewer than 2^23) samples of equally many consecutive rows.  row_scale [S]: a sample's drop-path
-    multiplier; 0 drops the branch, whatever it holds.  pre_weight / pre_bias [D]: the norm in front of the next branch.  norm: "layer" or
+    multiplier; 0 drops the branch, whatever it and its gate hold.  pre_weight / pre_bias [D]: the norm in front of the next branch.  norm: "layer" or
     "rms" (which has no bias)."""
     code, dev, T, D, gate_rows, scale_rows, v = _norm_operands(branch, residual, norm, eps, (post_weight, post_bias, gate, row_scale, pre_weight, pre_bias))
     y, ldy = as_rows(branch)

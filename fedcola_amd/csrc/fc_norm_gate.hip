@@ -3,8 +3,8 @@
 //   n = norm(y) wp + bp;   r = alpha x + s_b gate n;   h = norm(r) wn + bn
 //
 // y the branch's output, x the residual stream, gate one vector for all rows or one for each sample, s_b a sample's drop-path multiplier;
-// norm: LayerNorm or RMSNorm.  Each part may be absent.  A multiplier of 0 drops the branch: y is not used and its gradient is 0, whatever
-// it holds.  h comes from r before r is rounded.
+// norm: LayerNorm or RMSNorm.  Each part may be absent.  A multiplier of 0 drops the branch: y and the gate are not used and their gradients are 0,
+// whatever they hold (the loads are in range all the same).  h comes from r before r is rounded.
 // Backward: r and both norms' statistics are formed again from y and x, so nothing is kept and dwn, dwp are those of the unrounded r.
 // Bound: HBM, 4 T D elements forward (y, x in; r, h out), 6 T D backward (y, x, dr, dh in; dy, dx out).
 // A row is held in registers by 8, 16 or 32 lanes (D <= 64, 128, 256), a wave (<= 1024), 4 waves (<= 2048, backward <= 4096) or 8 (<= 8192): 8 or 16
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256) k_ng_fwd(NgArgs a) {
       for (int k = 0; k < E; ++k) y[k] = y[k] * wp[k] + bp[k];
     }
 #pragma unroll
-    for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + s * (a.gate ? gt[k] * y[k] : y[k]);
+    for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + (s != 0.f ? s * (a.gate ? gt[k] * y[k] : y[k]) : 0.f);      // (a dropped sample's gate may hold anything)
     ng_store<T, VEC, NTH, E>((T*)a.r + row * D, l, D, x);
     if (a.pre) {
       ng_norm<VEC, NTH, E>(x, l, D, a.rms, a.eps, sum);
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 &
       branch(v);
       get(NG_GT, w);
 #pragma unroll
-      for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + s * (w[k] * v[k]);
+      for (int k = 0; k < E; ++k) x[k] = a.alpha * x[k] + (s != 0.f ? s * (w[k] * v[k]) : 0.f);
       const float rs2 = ng_norm<VEC, NTH, E>(x, l, D, a.rms, a.eps, sum);
       get(NG_WN, w);
       float s1 = 0.f, s2 = 0.f;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(W == 8 ? 512 : 256, E == 8 ? (sizeof(T) == 2 &
     for (int k = 0; k < E; ++k) {
       const float dp = s == 0.f ? 0.f : d[k] * s;
       sums[NG_DGATE][k] += dp * v[k];
-      d[k] = dp * w[k];
+      d[k] = s == 0.f ? 0.f : dp * w[k];
     }
     if (a.post) {
       float s1 = 0.f, s2 = 0.f;

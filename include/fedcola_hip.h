@@ -148,8 +148,8 @@ int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t lddy, cons
 
 /* between two branches: n = norm(y) post_w + post_b; r = alpha x + row_scale[t / scale_rows] gate[t / gate_rows] n; h = norm(r) pre_w + pre_b, for y the
  * branch's output and x the residual stream [T, D], D <= 8192, fewer than 2^23 gate vectors (T / gate_rows; one for each row, say); r and h are contiguous.  post_w NULL: n = y; pre_w NULL: no h; gate / row_scale NULL:
- * 1; gate_rows / scale_rows 0: one vector / value for all rows.  Weights, gate and row_scale are fp32.  A row_scale of 0 drops the branch: its rows
- * of y are not read and their gradient is 0.  The backward takes dr and / or dh (the other NULL) and reads y and x again; the five weight gradients
+ * 1; gate_rows / scale_rows 0: one vector / value for all rows.  Weights, gate and row_scale are fp32.  A row_scale of 0 drops the branch: what
+ * its rows of y and their gate hold is not used (the memory has to be readable) and their gradients are 0.  The backward takes dr and / or dh (the other NULL) and reads y and x again; the five weight gradients
  * (fp32; d_gate one row for each gate vector) are NULL where not wanted.  T = 0: they are zeros, d_gate with gate_rows 0 alone (else it is not written). */
 size_t fc_norm_gate_workspace_bytes(int64_t T, int32_t D, int64_t gate_rows);
 int fc_norm_gate_fwd(int32_t dt, int32_t kind, const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t T, int32_t D, const float* post_w,

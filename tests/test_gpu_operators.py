@@ -393,6 +393,26 @@ def test_norm_gate_residual_dropped_branch_holds_anything(dt):
     assert not g["branch"][1:3].any() and g["branch"][0].any() and not g["gate"][1:3].any()
 
 
+@pytest.mark.parametrize("post", [0, 1])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("D", [40, 200, 1001, 3000])
+def test_norm_gate_residual_dropped_samples_gate_holds_anything(D, dt, kind, post):
+    """a row_scale of 0 drops the branch and its gate with it: no infinity or NaN of either reaches a result"""
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    b, r, dr, dh, v = norm_case(4, 6, D, dt, kind, post, 1, "sample", 1, 8)
+    v["row_scale"] = torch.tensor([1.5, 0.0, 0.0, 1.0], device="cuda")
+    dirty, gate = b.clone(), v["gate"].clone()
+    dirty[1], gate[1], gate[2] = math.nan, math.inf, math.nan
+    out = []
+    for t, g in ((b, v["gate"]), (dirty, gate)):
+        d = norm_gate_residual_backward(dr, dh, t, r, **{**v, "gate": g})
+        out.append((*norm_gate_residual_forward(t, r, **{**v, "gate": g}), *d.values()))
+    for x, y in zip(*out):
+        assert torch.isfinite(y).all() and torch.equal(x, y)
+    assert not d["branch"][1:3].any() and not d["gate"][1:3].any()
+
+
 @pytest.mark.parametrize("gate", ["all", "sample"])
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 def test_norm_gate_residual_of_no_rows(dt, gate):
