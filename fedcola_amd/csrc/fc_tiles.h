@@ -145,13 +145,14 @@ template <int MODE, int W, int KS> __device__ __forceinline__ ft_b8 ft_frag(cons
   return ft_b8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// the three planes of an fp32 value.  A value that is no number or infinite is its first plane alone.
+// the three planes of an fp32 value, exact for every finite one: above bf16's largest (3.3895e38) the first plane is that, not infinity.  An infinity
+// or no number gives planes with no number among them, and so does every product with it.
 __device__ __forceinline__ void ft_split(float x, float& hi, float& mid, float& lo) {
-  hi = bf2f(f2bf(x));
+  constexpr float top = 3.38953138925153547590470800371487867e38f;       // 0x7f7f0000
+  hi = __builtin_amdgcn_fmed3f(bf2f(f2bf(x)), -top, top);
   const float r = x - hi;
-  const bool fin = __builtin_fabsf(hi) < __builtin_inff();
-  mid = fin ? bf2f(f2bf(r)) : 0.f;
-  lo = fin ? r - mid : 0.f;
+  mid = bf2f(f2bf(r));
+  lo = r - mid;
 }
 
 // fp32 tiles of 32 rows (a scoring call's): 32 rows of A's three planes, 32 k deep, are six pieces by four waves, the last two of them moved

@@ -9,6 +9,7 @@ from oracle import blocks_oracle as O
 pytestmark = pytest.mark.gpu
 DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
 TINY = 1e-30
+LOWEST = torch.finfo(torch.float32).min
 
 
 def rnd(gen, *shape, scale=1.0, dtype=torch.float32):
@@ -587,6 +588,34 @@ def test_sizes_past_the_librarys_are_refused(n):
                 lambda: blocks.gated_mlp_backward(one.expand(n, 1), one.expand(n, 1), one.expand(4, 1), one.expand(1, 2))):
         with pytest.raises(ValueError, match="at most"):
             bad()
+
+
+@pytest.mark.parametrize("T", [5, 40, 520])
+def test_fp32_values_next_to_the_largest(T):
+    """fp32 values above bf16's largest are finite: where they meet zeros they are not there, where they meet small values they count"""
+    from fedcola_amd.blocks import gated_mlp_backward, gated_mlp_forward
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    one = torch.tensor(1.0, device="cuda")
+    x, w, y = ce_case(T, 300, 40, "fp32", 0.1, 7)
+    x[:, 3], w[:, 3], w[5, 3] = 0.0, LOWEST, -LOWEST
+    x[:, 4], w[:, 4] = -LOWEST, 0.0
+    want, bound = O.linear_ce(x, w, y, one, -100, "sum", torch.float32)
+    loss, saved = linear_cross_entropy_forward(x, w, y, reduction="sum")
+    dx, dw = linear_cross_entropy_backward(one, saved, w)
+    within(loss, want["loss"], bound["loss"], "loss")
+    keep = [i for i in range(40) if i not in (3, 4)]                       # (the two columns' own gradients are sums of such values, past fp32's range)
+    within(dx[:, keep], want["dx"][:, keep], bound["dx"][:, keep], "dx")
+    within(dw[:, keep], want["dw"][:, keep], bound["dw"][:, keep], "dw")
+    g = gen(T)
+    D, F = 24, 36
+    x, wi, wo, dy = rnd(g, T, D), rnd(g, 2 * F, D, scale=1 / math.sqrt(D)), rnd(g, D, F, scale=1 / math.sqrt(F)), rnd(g, T, D, scale=1e-6)
+    x[:, 2], wi[:, 2] = LOWEST, 0.0
+    x[0, 5], wi[:F, 5], wi[F:, 5] = LOWEST, 0.0, 2.0 ** -125          # an up projection of about -8 from one such value
+    want, bound = O.gated_mlp(x, wi, wo, dy, "silu", torch.float32)
+    within(gated_mlp_forward(x, wi, wo), want["y"], bound["y"], "y")
+    for k, t in zip(("dx", "dw_in", "dw_out"), gated_mlp_backward(dy, x, wi, wo)):
+        assert torch.isfinite(t).all()
+        within(t, want[k], bound[k], k)
 
 
 # ------------------------------------------------------------------------------------------------ offsets past 32 bits
