@@ -17,6 +17,7 @@ elif os.environ.get("FC_PROBES_LIB"):      # tools only: the -DFC_PROBES build w
 FC_PREC_FP32, FC_PREC_BF16 = 0, 1
 FC_TASK_NONE, FC_TASK_CLS, FC_TASK_RTV = 0, 1, 2
 FC_OPT_MLP_FUSED, FC_OPT_STEP_GRAPH, FC_OPT_GEMM_FORM = 1, 2, 3
+FORM_WALK, FORM_SLICED, FORM_KEPT, FORM_PIECES, FORM_GROUP = (1 << b for b in range(16, 21))
 
 
 class FcModelCfg(C.Structure):
@@ -68,6 +69,8 @@ SIGNATURES = {
     "fc_gated_mlp_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
     "fc_gated_mlp_fwd": (C.c_int, [_I, _I, _P, _L, _P, _L, _P, _L, _I, _I, _I, _P, _L, _P, _Z, _P]),
     "fc_gated_mlp_bwd": (C.c_int, [_I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _Z, _P]),
+    "fc_linear_ce_form": (_I, [_I, _I, _I, _I, _I, _I]),
+    "fc_gated_mlp_form": (_I, [_I, _I, _I, _I, _I, _I]),
     "fc_norm_gate_workspace_bytes": (_Z, [_L, _I, _L]),
     "fc_norm_gate_fwd": (C.c_int, [_I, _I, _P, _L, _P, _L, _L, _I, _P, _P, _P, _L, _P, _L, _F, _P, _P, _F, _P, _P, _P]),
     "fc_norm_gate_bwd": (C.c_int, [_I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _L, _I, _P, _P, _P, _L, _P, _L, _F, _P, _F, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),

@@ -410,6 +410,15 @@ static int gm_operands(const GmCall& c, char*& ws, GmArgs& a, hipStream_t s) {
   return ft_pack(l, s);
 }
 
+extern "C" int32_t fc_gated_mlp_form(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
+  if (T < 1 || D < 1 || F < 1) return 0;
+  const bool b32 = !dt && !packed && T <= FT_B32;
+  const GmSizes z = gm_sizes(dt, T, D, F, b32, packed || F % 8 || D % 8, backward != 0);
+  const int group = z.group ? FC_FORM_GROUP : 0;
+  if (z.plan_gu.target) return z.plan_gu.TM | FC_FORM_SLICED | group;
+  if (dt ? ft_few(1, T) : b32 && ft_few(6, T)) return 32 | group;
+  return (gm_big(dt, T, D, F, backward != 0) ? 256 : 128) | group;
+}
 extern "C" size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward) {
   if (T < 0 || D < 1 || F < 1) return 0;
   const bool few = !dt && T <= FT_B32;

@@ -408,10 +408,11 @@ typedef FtShape<128, 128, 2, 4, 3, 32, 3> CePlanes;
 typedef FtShape<32, 64, 2, 2, 5, 32, 3, true> CeRows32;
 typedef FtShape<128, 128, 2, 4, 3, 32, 3, true> CeMid32;
 // 256 x 256 or 128 x 128 tiles by the model of the time (forward, 768 wide: 512 x 32768 36 us, 42 with 128 x 128; 256 x 32768 32 and 27.5; of 13 sizes
-// around the border it takes the faster every time), 128 x 128 for fp32, 32 x 64 (ft_few) for the few rows of a scoring call
+// around the border it takes the faster every time), 128 x 128 for fp32, 32 x 64 (ft_few) for the few rows of a scoring call.  Kept logits are
+// written by tiles of up to 128 rows alone, whatever the model says of the large ones.
 static int ce_shape(int dt, long T, long V, long D, bool b32) {
   if ((dt || b32) && ft_few(dt ? 1 : 6, T)) return 2;
-  return dt && ft_large(T, V, D) ? 0 : 1;
+  return dt && !ce_keep(dt, T, V, D) && ft_large(T, V, D) ? 0 : 1;
 }
 static int ce_tn(int shape) { return shape == 0 ? 256 : shape == 1 ? 128 : 64; }
 
@@ -520,6 +521,21 @@ static int ce_weight(int dt, const void* w, long ldw, bool direct, long V, long 
   return ft_pack(l, s);
 }
 
+template <class S> static bool ce_walks(long T, long nv, long D) {
+  const long tiles = ((T + S::TM - 1) / S::TM) * ((nv + S::TN - 1) / S::TN);
+  return ft_walkers<S>(tiles, D) < tiles;
+}
+extern "C" int32_t fc_linear_ce_form(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward) {
+  if (T < 1 || V < 1 || D < 1) return 0;
+  if (backward && ce_keep(dt, T, V, D)) return FC_FORM_KEPT;
+  const bool direct = !packed && (dt || T <= FT_B32), b32 = !dt && direct;
+  const CeSizes z = ce_sizes(dt, T, V, D, direct, backward != 0);
+  if (z.logits.target) return z.logits.TM | FC_FORM_SLICED;
+  const long nv = backward && z.piece < V ? z.piece : V;
+  const int shape = ce_shape(dt, T, nv, D, b32);
+  const bool walk = shape == 0 ? ce_walks<CeBig>(T, nv, D) : shape == 2 ? false : dt ? ce_walks<CeMid>(T, nv, D) : b32 ? ce_walks<CeMid32>(T, nv, D) : ce_walks<CePlanes>(T, nv, D);
+  return (shape == 0 ? 256 : shape == 1 ? 128 : 32) | (walk ? FC_FORM_WALK : 0) | (nv < V ? FC_FORM_PIECES : 0);
+}
 extern "C" size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t V, int32_t D) {
   return T < 0 || V < 1 || D < 1 ? 0 : ce_saved(nullptr, dt, T, V, D).bytes;
 }

@@ -146,6 +146,14 @@ int fc_gated_mlp_bwd(int32_t dt, int32_t act, const void* dy, int64_t lddy, cons
                      const void* w_out, int64_t ld_out, int32_t T, int32_t D, int32_t F, void* dx, int64_t lddx, void* dw_in,
                      int64_t ldd_in, void* dw_out, int64_t ldd_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* the form that the first product of a call of these sizes takes, for tests and tuning: rows of an output tile, and flags.  The choice follows a
+ * model of the time, and may change between builds. */
+enum { FC_FORM_ROWS = 0xffff, FC_FORM_WALK = 1 << 16 /* workgroups compute several tiles */, FC_FORM_SLICED = 1 << 17 /* the reduction is cut */,
+       FC_FORM_KEPT = 1 << 18 /* no product: the logits that the forward kept */, FC_FORM_PIECES = 1 << 19 /* the vocabulary is cut */,
+       FC_FORM_GROUP = 1 << 20 /* the gradients' products share a launch */ };
+int32_t fc_linear_ce_form(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward);
+int32_t fc_gated_mlp_form(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward);
+
 /* between two branches: n = norm(y) post_w + post_b; r = alpha x + row_scale[t / scale_rows] gate[t / gate_rows] n; h = norm(r) pre_w + pre_b, for y the
  * branch's output and x the residual stream [T, D], D <= 8192, fewer than 2^23 gate vectors (T / gate_rows; one for each row, say); r and h are contiguous.  post_w NULL: n = y; pre_w NULL: no h; gate / row_scale NULL:
  * 1; gate_rows / scale_rows 0: one vector / value for all rows.  Weights, gate and row_scale are fp32.  A row_scale of 0 drops the branch: what

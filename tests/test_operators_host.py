@@ -64,6 +64,19 @@ def test_sizes_of_workspaces():
         assert few[1] >= few[0] + 1000 * 64 * 6 - 512
 
 
+def test_kept_logits_are_never_of_the_large_tiles():
+    """the large tiles do not write them: wherever the backward reads kept logits, the forward takes another form"""
+    import random
+    from fedcola_amd import _lib
+    L, r, kept = lib(), random.Random(0), 0
+    for _ in range(20000):
+        c = (r.randint(0, 1), r.randint(1, 130), int(2 ** r.uniform(1, 22)), int(2 ** r.uniform(0, 15)), r.randint(0, 1))
+        if L.fc_linear_ce_form(*c, 1) & _lib.FORM_KEPT:
+            kept += 1
+            assert L.fc_linear_ce_form(*c, 0) & 0xffff < 256, c
+    assert kept > 5000
+
+
 def test_python_refuses_host_tensors_and_bad_choices():
     from fedcola_amd import blocks, criterions
     from fedcola_amd._lib import FedcolaHipError
