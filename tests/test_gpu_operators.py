@@ -127,6 +127,38 @@ def test_linear_cross_entropy_no_row_counts(dt, T):
     assert loss.item() == 0 and not dx.any() and not dw.any()
 
 
+# sizes whose workgroups walk several tiles, the next one's loads under this one's epilogue: two to nine k-steps, ragged last tiles of rows, columns and k,
+# rows that do not count (so that some workgroups find no second tile, or none at all), one piece of the vocabulary and two; type, T, V, D, ignored,
+# weight's layout, pieces backward
+WALKS = [("bf16", 1030, 20011, 128, 0.0, "", 0), ("bf16", 2560, 30522, 136, 0.85, "", 0), ("bf16", 1100, 30522, 520, 0.3, "wide", 0), ("bf16", 700, 30001, 130, 0.1, "odd", 0),
+         ("bf16", 4000, 30522, 136, 0.2, "", 1), ("fp32", 600, 30000, 130, 0.0, "", 0), ("fp32", 1100, 30522, 72, 0.3, "", 1), ("fp32", 700, 20011, 200, 0.6, "holes", 0),
+         ("fp32", 200, 30000, 130, 0.0, "", 0), ("fp32", 500, 20011, 66, 0.4, "holes", 0), ("fp32", 512, 70003, 130, 0.1, "", 1)]
+
+
+@pytest.mark.parametrize("dt,T,V,D,ignored,wl,pieces", WALKS)
+def test_linear_cross_entropy_workgroups_of_several_tiles(dt, T, V, D, ignored, wl, pieces):
+    from fedcola_amd import _lib
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    for backward in (0, 1):
+        form = _lib.lib().fc_linear_ce_form(dt == "bf16", T, V, D, dt == "bf16" and wl in ("odd", "holes"), backward)
+        assert form & 0xffff == (256 if dt == "bf16" else 128) and form & _lib.FORM_WALK and bool(form & _lib.FORM_PIECES) == bool(pieces and backward)
+    x, w, y = ce_case(T, V, D, dt, ignored, T + V + D)
+    y[:3] = torch.tensor([V - 1, 0, V - 1 - V % 256], device="cuda")
+    g = torch.tensor(1.3, device="cuda")
+    want, bound = O.linear_ce(x, w, y, g, -100, "mean", DT[dt])
+    loss, saved = linear_cross_entropy_forward(x, layout(w, wl), y)
+    dx, dw = linear_cross_entropy_backward(g, saved, layout(w, wl))
+    u, n = O.half_step(DT[dt]), int((y != -100).sum())
+    for got, k, terms in ((loss, "loss", 1), (dx, "dx", V), (dw, "dw", n)):
+        within(got, want[k], bound[k], k)
+        # The elementwise bound of a long sum is wide beside its value.  In norm: bf16's two stored roundings of u each; 6 / 32 additions a product, each
+        # off by 2^-24 of a running sum of independent terms, whose largest is at most twice the last in the mean square; logit and exponential 2^-18.
+        tol = (2 * u if dt == "bf16" else u) + 2 * 6 / 32 * terms * O.F24 + 2.0 ** -18
+        assert (got.double() - want[k]).norm() <= tol * want[k].norm(), (k, float((got.double() - want[k]).norm() / want[k].norm()), tol)
+    again = linear_cross_entropy_backward(g, saved, layout(w, wl))
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
 @pytest.mark.parametrize("D", [8, 64, 72, 96, 120, 136])
 def test_linear_cross_entropy_gathers_a_rows_own_values(D):
     """aligned rows that are no whole 64 values wide, with NaN behind them: of what is gathered for the products, the padding is zeros"""
@@ -264,6 +296,32 @@ def test_gated_mlp(T, D, F, xl, wl, dt):
         for k in want:
             assert got[k].dtype == DT[dt]
             within(got[k], want[k], bound[k], f"{act} {k}")
+
+
+# sizes of the 256 x 256 tile: T, D, F, weights' layout, whether the gradients' products share a launch
+LARGE = [(2100, 1032, 4104, "", 1), (4096, 1536, 4096, "", 0), (3001, 1100, 4100, "odd", 1), (4500, 2056, 3001, "holes", 0)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("T,D,F,wl,group", LARGE)
+def test_gated_mlp_large_tiles(T, D, F, wl, group, act):
+    """the large tile, forward and backward, whole and ragged in rows, units and k; the gradients' products in one launch and in three"""
+    from fedcola_amd import _lib
+    from fedcola_amd.blocks import gated_mlp_backward, gated_mlp_forward
+    for backward in (0, 1):
+        form = _lib.lib().fc_gated_mlp_form(1, T, D, F, wl in ("odd", "holes"), backward)
+        assert form & 0xffff == 256 and not form & _lib.FORM_SLICED and bool(form & _lib.FORM_GROUP) == bool(group and backward)
+    g = gen(T + D + F)
+    dt = torch.bfloat16
+    x, wi, wo, dy = rnd(g, T, D, dtype=dt), rnd(g, 2 * F, D, scale=1 / math.sqrt(D), dtype=dt), rnd(g, D, F, scale=1 / math.sqrt(F), dtype=dt), rnd(g, T, D, dtype=dt)
+    want, bound = O.gated_mlp(x, wi, wo, dy, act, dt)
+    a = layout(x, wl), layout(wi, wl), layout(wo, wl)
+    got = dict(y=gated_mlp_forward(*a, act=act))
+    got["dx"], got["dw_in"], got["dw_out"] = gated_mlp_backward(layout(dy, wl), *a, act=act)
+    for k in want:
+        within(got[k], want[k], bound[k], k)
+        # in norm, where the roundings of one result's terms are independent: u for the stored hidden values, u for the result, u for everything in 32 bits
+        assert (got[k].double() - want[k]).norm() <= 3 * O.half_step(dt) * want[k].norm(), (k, float((got[k].double() - want[k]).norm() / want[k].norm()))
 
 
 def test_gated_mlp_extreme_values():

@@ -64,6 +64,22 @@ def test_sizes_of_workspaces():
         assert few[1] >= few[0] + 1000 * 64 * 6 - 512
 
 
+def test_forms_of_the_tested_sizes():
+    """the GPU tests' sizes reach the forms that they are there for, whatever becomes of the model of the time"""
+    from fedcola_amd import _lib
+    from test_gpu_operators import LARGE, WALKS
+    L = lib()
+    for dt, T, V, D, _, wl, pieces in WALKS:
+        packed = dt == "bf16" and wl in ("odd", "holes")
+        for backward in (0, 1):
+            form = L.fc_linear_ce_form(dt == "bf16", T, V, D, packed, backward)
+            assert form & 0xffff == (256 if dt == "bf16" else 128) and form & _lib.FORM_WALK and bool(form & _lib.FORM_PIECES) == bool(pieces and backward)
+    for T, D, F, wl, group in LARGE:
+        assert L.fc_gated_mlp_form(1, T, D, F, wl in ("odd", "holes"), 0) == 256
+        assert L.fc_gated_mlp_form(1, T, D, F, wl in ("odd", "holes"), 1) == 256 | (group and _lib.FORM_GROUP)
+    assert L.fc_linear_ce_form(1, 0, 4, 4, 0, 0) == L.fc_gated_mlp_form(1, 4, 4, 0, 0, 0) == 0
+
+
 def test_kept_logits_are_never_of_the_large_tiles():
     """the large tiles do not write them: wherever the backward reads kept logits, the forward takes another form"""
     import random
