@@ -545,18 +545,19 @@ __global__ void __launch_bounds__(64) k_txt_word_grad(const T* __restrict__ dy, 
   for (int t = 0; t < TEB_MAXV; ++t)
     if (lane + 64 * t < D) atomicAdd(dword + (size_t)id * D + lane + 64 * t, sum[t]);
 }
-// dtype, dgamma and dbeta: 16 waves of one workgroup walk the tokens; their sums are added in the waves' order
+// dtype, dgamma and dbeta: 16 waves of workgroup 0 walk the tokens; their sums are added in the waves' order.  Workgroup n + 1, where there are such:
+// the same for dpos of position n over its texts (more than 16, which k_txt_embed_bwd_v would add up from several workgroups).
 template <typename T>
 __global__ void __launch_bounds__(1024) k_txt_embed_sums(const T* __restrict__ dy, const int64_t* __restrict__ ids, const float* __restrict__ word,
                                                          const float* __restrict__ pos, const float* __restrict__ type, const float* __restrict__ mean,
-                                                         const float* __restrict__ rstd, const float* __restrict__ g, float* dtype, float* dg, float* db, int rows,
-                                                         int N, int D, int vocab) {
+                                                         const float* __restrict__ rstd, const float* __restrict__ g, float* dpos, float* dtype, float* dg, float* db,
+                                                         int rows, int N, int D, int vocab) {
   extern __shared__ float red_sum[];                  // [16][D]
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = (int)blockIdx.x - 1, step = n < 0 ? 1 : N;
   float ade[TEB_MAXV], agm[TEB_MAXV], abt[TEB_MAXV];
 #pragma unroll
   for (int t = 0; t < TEB_MAXV; ++t) { ade[t] = 0.f; agm[t] = 0.f; abt[t] = 0.f; }
-  for (int row = wave; row < rows; row += 16) {
+  for (int row = n < 0 ? wave : wave * N + n; row < rows; row += 16 * step) {
     const float* w = word + (size_t)clamp_id(ids[row], vocab) * D;
     const float* pp = pos + (size_t)(row % N) * D;
     const T* dyr = dy + (size_t)row * D;
@@ -582,6 +583,7 @@ __global__ void __launch_bounds__(1024) k_txt_embed_sums(const T* __restrict__ d
   }
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
+    if (q && n >= 0) return;
 #pragma unroll
     for (int t = 0; t < TEB_MAXV; ++t)
       if (lane + 64 * t < D) red_sum[wave * D + lane + 64 * t] = q == 0 ? ade[t] : q == 1 ? agm[t] : abt[t];
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(1024) k_txt_embed_sums(const T* __restrict__ d
     for (int i = threadIdx.x; i < D; i += 1024) {
       float v = 0.f;
       for (int k = 0; k < 16; ++k) v += red_sum[k * D + i];
-      atomicAdd((q == 0 ? dtype : q == 1 ? dg : db) + i, v);
+      atomicAdd((q == 0 ? (n < 0 ? dtype : dpos + (size_t)n * D) : q == 1 ? dg : db) + i, v);
     }
     __syncthreads();
   }
@@ -602,9 +604,10 @@ int fc_txt_embed_bwd(int dt, const void* dy, const int64_t* ids, const float* wo
     const size_t lds = sizeof(float) * (12 * D + 16 * 144);
     if (B * N <= TXT_ORDERED) {
       DISPATCH_DT(dt, hipLaunchKernelGGL(k_txt_word_grad<T>, dim3(B * N), dim3(64), 0, s, (const T*)dy, ids, word, pos, type, mean, rstd, g, dword, B * N, N, D, vocab));
-      DISPATCH_DT(dt, hipLaunchKernelGGL(k_txt_embed_sums<T>, dim3(1), dim3(1024), 16 * D * 4, s, (const T*)dy, ids, word, pos, type, mean, rstd, g, dtype, dg, db,
-                                         B * N, N, D, vocab));
+      DISPATCH_DT(dt, hipLaunchKernelGGL(k_txt_embed_sums<T>, dim3(B > 16 ? 1 + N : 1), dim3(1024), 16 * D * 4, s, (const T*)dy, ids, word, pos, type, mean, rstd, g,
+                                         dpos, dtype, dg, db, B * N, N, D, vocab));
       FC_LAUNCH_CHECK();
+      if (B > 16) return 0;
       dword = dtype = dg = db = nullptr;
     }
 #define GO(CHN) DISPATCH_DT(dt, hipLaunchKernelGGL((k_txt_embed_bwd_v<T, CHN>), dim3(N, fc_cdiv(B, 16)), dim3(256), lds, s, (const T*)dy, ids, word, pos, type, \

@@ -229,6 +229,30 @@ def test_device_table_cache_survives_starting_over(tmp_path):
         assert abs(x - y) <= 2e-2 * max(1.0, abs(y))
 
 
+@pytest.mark.parametrize("B,N", [(16, 16), (50, 5), (120, 2), (256, 1)])
+@pytest.mark.parametrize("prec", ["fp32", "bf16"])
+def test_small_batches_text_embedding_gradients_have_one_order(prec, B, N):
+    """up to 256 tokens the text embedding's gradients are the same bits in every run, however many texts there are, and in fp32 the oracle's"""
+    rec = G.load("model_txtcls_aux.json")
+    g = torch.Generator().manual_seed(B)
+    ids, y = torch.randint(0, 64, (B, N), generator=g), torch.randint(0, 4, (B,), generator=g)
+    w0 = G.case_weights("txtcls_aux")
+    model = PU.build_product(rec["mk"], prec, w0)
+    runs = []
+    for _ in range(12):
+        model.load_state_dict(w0, strict=True)
+        runs.append(PU.product_step(model, "txt", None, ids, y, 1e-3)[1])
+    names = [k for k in runs[0] if "text_embeddings" in k]
+    assert len(names) == 5
+    for k in names:
+        assert all(torch.equal(runs[0][k], r[k]) for r in runs[1:]), k
+    if prec == "fp32":
+        cfg = cfg_from_mk(rec["mk"])
+        _, _, grads = O.client_step(O.resolve_colearn({k: v.clone() for k, v in w0.items()}, cfg), cfg, ("txt", ids, y), dict(step=0, m={}, v={}), lr=1e-3)
+        for k in names:
+            assert float((runs[0][k] - grads[k]).abs().max()) <= grad_tol(k, grads[k], grads, w0, 1e-4, 1e-7), k
+
+
 @pytest.mark.parametrize("B", [8, 32])
 def test_colearn_attn_d384_bf16_shared_attention_gradients(B):
     """colearn_param == 'attn' at the ViT-S width in the timed mode: the text tower's weight gradients of the shared qkv / proj go
