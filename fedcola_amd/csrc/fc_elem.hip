@@ -755,12 +755,54 @@ int fc_head_fwd(int dt, const void* x, const float* g, const float* b, float* f,
   return 0;
 }
 
+// dgamma and dbeta of up to 16 samples by 16 waves, a sample each, added in the samples' order
 template <typename T>
-__global__ void __launch_bounds__(256) k_head_bwd(const float* __restrict__ din, const float* __restrict__ out, const float* __restrict__ nrm,
+__device__ __forceinline__ void head_sums(const float* __restrict__ din, const float* __restrict__ out, const float* __restrict__ nrm, int normalize,
+                                          const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd, float* dg, float* db, int B, int N,
+                                          int D) {
+  extern __shared__ float red_sum[];                  // [B][D]
+  const int bi = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float dot = 0.f, inv = 1.f, mu = 0.f, rs = 0.f;
+  const float* dr = din + (size_t)(bi < B ? bi : 0) * D;
+  const float* o = normalize ? out + (size_t)(bi < B ? bi : 0) * D : dr;
+  const T* xr = x + (size_t)(bi < B ? bi : 0) * N * D;
+  if (bi < B) {
+    if (normalize) {
+      for (int i = lane; i < D; i += 64) dot += o[i] * dr[i];
+      dot = wave_sum(dot);
+      inv = 1.0f / nrm[bi];
+    }
+    mu = mean[bi];
+    rs = rstd[bi];
+  }
+  for (int q = 0; q < 2; ++q) {
+    if (bi < B)
+      for (int i = lane; i < D; i += 64) {
+        const float df = normalize ? (dr[i] - o[i] * dot) * inv : dr[i];
+        red_sum[bi * D + i] = q ? df : df * ((Io<T>::ld(xr, i) - mu) * rs);
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += 1024) {
+      float v = 0.f;
+      for (int k = 0; k < B; ++k) v += red_sum[k * D + i];
+      atomicAdd((q ? db : dg) + i, v);          // (other towers' and chains' heads add to the same norm)
+    }
+    __syncthreads();
+  }
+}
+// ORDERED: dgamma and dbeta of up to 16 samples come from the first workgroup, added in the samples' order, the rows from the others; else by atomics.
+// (A launch of its own for the sums took 9 us of a step.)
+#define HEAD_ORDERED 16
+template <typename T, bool ORDERED>
+__global__ void __launch_bounds__(ORDERED ? 1024 : 256) k_head_bwd(const float* __restrict__ din, const float* __restrict__ out, const float* __restrict__ nrm,
                                                   int normalize, const T* __restrict__ x, const float* __restrict__ mean,
                                                   const float* __restrict__ rstd, const float* __restrict__ g, T* __restrict__ dx, float* dg,
                                                   float* db, int B, int N, int D) {
-  int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (ORDERED && blockIdx.x == 0) {
+    head_sums<T>(din, out, nrm, normalize, x, mean, rstd, dg, db, B, N, D);
+    return;
+  }
+  int row = ORDERED ? (blockIdx.x - 1) * 16 + (threadIdx.x >> 6) : blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= B * N) return;
   T* dxr = dx + (size_t)row * D;
   if (row % N != 0) {                                   // no gradient reaches the non-cls rows through the head: zero rows, 16 bytes per lane
@@ -795,56 +837,20 @@ __global__ void __launch_bounds__(256) k_head_bwd(const float* __restrict__ din,
     float df = normalize ? (dr[i] - out[(size_t)bi * D + i] * dot) * inv : dr[i];
     float xh = (Io<T>::ld(xr, i) - mu) * rs;
     Io<T>::st(dxr, i, rs * (df * g[i] - s1 - xh * s2));
-    if (!dg) continue;
+    if (ORDERED) continue;
     atomicAdd(dg + i, df * xh);
     atomicAdd(db + i, df);
-  }
-}
-// dgamma and dbeta of few rows without atomics: a wave a row, added in the rows' order
-#define HEAD_ORDERED 16
-template <typename T>
-__global__ void __launch_bounds__(1024) k_head_sums(const float* __restrict__ din, const float* __restrict__ out, const float* __restrict__ nrm, int normalize,
-                                                    const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd, float* dg, float* db,
-                                                    int B, int N, int D) {
-  extern __shared__ float red_sum[];                  // [16][D]
-  const int bi = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float dot = 0.f, inv = 1.f, mu = 0.f, rs = 0.f;
-  const float* dr = din + (size_t)(bi < B ? bi : 0) * D;
-  const float* o = normalize ? out + (size_t)(bi < B ? bi : 0) * D : dr;
-  const T* xr = x + (size_t)(bi < B ? bi : 0) * N * D;
-  if (bi < B) {
-    if (normalize) {
-      for (int i = lane; i < D; i += 64) dot += o[i] * dr[i];
-      dot = wave_sum(dot);
-      inv = 1.0f / nrm[bi];
-    }
-    mu = mean[bi];
-    rs = rstd[bi];
-  }
-  for (int q = 0; q < 2; ++q) {
-    if (bi < B)
-      for (int i = lane; i < D; i += 64) {
-        const float df = normalize ? (dr[i] - o[i] * dot) * inv : dr[i];
-        red_sum[bi * D + i] = q ? df : df * ((Io<T>::ld(xr, i) - mu) * rs);
-      }
-    __syncthreads();
-    for (int i = threadIdx.x; i < D; i += 1024) {
-      float v = 0.f;
-      for (int k = 0; k < B; ++k) v += red_sum[k * D + i];
-      atomicAdd((q ? db : dg) + i, v);          // (other towers' and chains' heads add to the same norm)
-    }
-    __syncthreads();
   }
 }
 int fc_head_bwd(int dt, const float* din, const float* out, const float* nrm, int normalize, const void* x, const float* mean,
                 const float* rstd, const float* g, void* dx, float* dg, float* db, int B, int N, int D, hipStream_t s) {
   if (B <= HEAD_ORDERED && D <= 1024) {
-    DISPATCH_DT(dt, hipLaunchKernelGGL(k_head_sums<T>, dim3(1), dim3(1024), 16 * D * 4, s, din, out, nrm, normalize, (const T*)x, mean, rstd, dg, db, B, N, D));
-    FC_LAUNCH_CHECK();
-    dg = db = nullptr;
+    DISPATCH_DT(dt, hipLaunchKernelGGL((k_head_bwd<T, true>), dim3(1 + fc_cdiv((long)B * N, 16)), dim3(1024), B * D * 4, s, din, out, nrm, normalize, (const T*)x,
+                                       mean, rstd, g, (T*)dx, dg, db, B, N, D));
+  } else {
+    DISPATCH_DT(dt, hipLaunchKernelGGL((k_head_bwd<T, false>), dim3(fc_cdiv((long)B * N, 4)), dim3(256), 0, s, din, out, nrm, normalize, (const T*)x, mean, rstd, g,
+                                       (T*)dx, dg, db, B, N, D));
   }
-  DISPATCH_DT(dt, hipLaunchKernelGGL(k_head_bwd<T>, dim3(fc_cdiv((long)B * N, 4)), dim3(256), 0, s, din, out, nrm, normalize, (const T*)x,
-                                     mean, rstd, g, (T*)dx, dg, db, B, N, D));
   FC_LAUNCH_CHECK();
   return 0;
 }
