@@ -504,171 +504,124 @@ __global__ void __launch_bounds__(256) k_txt_embed_bwd_v(const T* __restrict__ d
     atomicAdd(db + i, red_dyn[(0 * 3 + 2) * D + i] + red_dyn[(1 * 3 + 2) * D + i] + red_dyn[(2 * 3 + 2) * D + i] + red_dyn[(3 * 3 + 2) * D + i]);
   }
 }
-// The gradients of few tokens in a fixed order, so that two runs give the same bits, in one launch.  (The order of the atomics above moved the word table by
-// 6e-7 in a step, and through rounding to bf16 whatever follows it.)  Workgroups of 16 waves: the first adds up dtype over all tokens; above 16 texts
-// (which k_txt_embed_bwd_v would add from several workgroups) N more the same for dpos of a position; ceil(D / 64) more dgamma and dbeta, which need no
-// sum over a row, a lane a column; the others the word table.  A wave takes every 16th token; the waves' sums are added in order.
-// Bound: latency, of a wave's tokens one after the other.  V: values of a lane (D <= 64 V), U: tokens whose loads are in flight together.  Loads are made
-// from inside the row by every lane: in a branch each of them would be waited for alone.
+// The gradients of few tokens in a fixed order, so that two runs give the same bits.  (The order of the atomics above moved the word table by 6e-7 in a step,
+// and through rounding to bf16 whatever follows it.)  Two launches: a wave a token takes the row's two sums, leaves them in `sums` and adds to the word
+// table -- the wave of an id's first token for all of its tokens; then a lane a column adds up dtype, dgamma and dbeta over the tokens and, above 16 texts
+// (which k_txt_embed_bwd_v would add from several workgroups), dpos of each position over its texts: 16 waves, every 16th token each, added in order.
+// Bound: latency (bf16, 8 x 32 tokens: 7 and 12 us at D = 384 and at 768; one workgroup that took the rows' sums and added them up too: 132 and 244 us).
+// Loads are made from inside the row by every lane, none in a branch, where each would be waited for alone.  V: values of a lane (D <= 64 V).
 #define TXT_ORDERED 256
-template <typename T, int V> struct TxtRow {            // dy, and the embedding's sum as it was normalised
-  float d[V], x[V], mu, rs;
-  __device__ __forceinline__ void load(const T* __restrict__ dy, const float* __restrict__ w, const float* __restrict__ pos, const float (&ty)[V],
-                                       const float* __restrict__ mean, const float* __restrict__ rstd, int row, int N, int D, int lane) {
+template <typename T, int V>
+__global__ void __launch_bounds__(64) k_txt_word_grad(const T* __restrict__ dy, const int64_t* __restrict__ ids, const float* __restrict__ word,
+                                                      const float* __restrict__ pos, const float* __restrict__ type, const float* __restrict__ mean,
+                                                      const float* __restrict__ rstd, const float* __restrict__ g, float* dword, float2* sums, int rows, int N, int D,
+                                                      int vocab) {
+  const int first = blockIdx.x, lane = threadIdx.x;
+  const long id = clamp_id(ids[first], vocab);
+  const float* w = word + (size_t)id * D;
+  float gg[V], wt[V], de[V], sum[V], rs;
+#pragma unroll
+  for (int t = 0; t < V; ++t) {
+    const int i = min(lane + 64 * t, D - 1);
+    gg[t] = g[i];
+    wt[t] = w[i] + type[i];
+    sum[t] = 0.f;
+  }
+  auto token = [&](int row) {                           // rs de: the gradient of the row's embedding
     const T* dyr = dy + (size_t)row * D;
     const float* pp = pos + (size_t)(row % N) * D;
-    mu = mean[row]; rs = rstd[row];
+    const float mu = mean[row];
+    float d[V], xh[V], s1 = 0.f, s2 = 0.f;
+    rs = rstd[row];
 #pragma unroll
     for (int t = 0; t < V; ++t) {
       const int i = min(lane + 64 * t, D - 1);
       d[t] = Io<T>::ld(dyr, i);
-      x[t] = w[i] + ty[t] + pp[i];
-    }
-  }
-};
-template <int V> __device__ __forceinline__ void txt_vec(const float* __restrict__ p, int D, int lane, float (&v)[V]) {
-#pragma unroll
-  for (int t = 0; t < V; ++t) v[t] = p[min(lane + 64 * t, D - 1)];
-}
-template <typename T, int V, int U>
-__global__ void __launch_bounds__(1024) k_txt_ordered(const T* __restrict__ dy, const int64_t* __restrict__ ids, const float* __restrict__ word,
-                                                      const float* __restrict__ pos, const float* __restrict__ type, const float* __restrict__ mean,
-                                                      const float* __restrict__ rstd, const float* __restrict__ g, float* dword, float* dpos, float* dtype, float* dg,
-                                                      float* db, int rows, int positions, int N, int D, int vocab) {
-  extern __shared__ float red_sum[];                  // [16][D]
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, columns = (D + 63) / 64;
-  int b = blockIdx.x;
-  if (b <= positions) {                                 // dtype; dpos of position b - 1
-    const int first = b ? wave * N + b - 1 : wave, step = b ? 16 * N : 16;
-    float gg[V], ty[V], ade[V];
-    txt_vec<V>(g, D, lane, gg);
-    txt_vec<V>(type, D, lane, ty);
-#pragma unroll
-    for (int t = 0; t < V; ++t) ade[t] = 0.f;
-    for (int r0 = first; r0 < rows; r0 += U * step) {
-      TxtRow<T, V> r[U];
-      long id[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) id[u] = clamp_id(ids[r0 + u * step < rows ? r0 + u * step : r0], vocab);
-#pragma unroll
-      for (int u = 0; u < U; ++u) r[u].load(dy, word + (size_t)id[u] * D, pos, ty, mean, rstd, r0 + u * step < rows ? r0 + u * step : r0, N, D, lane);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r0 + u * step >= rows) break;
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int t = 0; t < V; ++t) {
-          const bool in = lane + 64 * t < D;
-          r[u].x[t] = in ? (r[u].x[t] - r[u].mu) * r[u].rs : 0.f;
-          const float dgm = in ? r[u].d[t] * gg[t] : 0.f;
-          s1 += dgm; s2 += dgm * r[u].x[t];
-        }
-        s1 = wave_sum(s1) / (float)D;
-        s2 = wave_sum(s2) / (float)D;
-#pragma unroll
-        for (int t = 0; t < V; ++t) ade[t] += r[u].rs * (r[u].d[t] * gg[t] - s1 - r[u].x[t] * s2);
-      }
+      xh[t] = pp[i];
     }
 #pragma unroll
-    for (int t = 0; t < V; ++t)
-      if (lane + 64 * t < D) red_sum[wave * D + lane + 64 * t] = ade[t];
-    __syncthreads();
-    float* o = b ? dpos + (size_t)(b - 1) * D : dtype;
-    for (int i = threadIdx.x; i < D; i += 1024) {
-      float v = 0.f;
-      for (int k = 0; k < 16; ++k) v += red_sum[k * D + i];
-      atomicAdd(o + i, v);                              // (alone: other towers' and chains' heads add to the same norm, in launches of their own)
+    for (int t = 0; t < V; ++t) {
+      const bool in = lane + 64 * t < D;
+      d[t] = in ? d[t] * gg[t] : 0.f;
+      xh[t] = in ? (wt[t] + xh[t] - mu) * rs : 0.f;
+      s1 += d[t]; s2 += d[t] * xh[t];
     }
-    return;
-  }
-  b -= positions + 1;
-  if (b < columns) {
-    const int c = b * 64 + lane, i = min(c, D - 1);
-    const float ty = type[i];
-    float agm = 0.f, abt = 0.f;
-    for (int r0 = wave; r0 < rows; r0 += 64) {
-      float d[4], x[4], mu[4], rs[4];
-      long id[4];
+    s1 = wave_sum(s1) / (float)D;
+    s2 = wave_sum(s2) / (float)D;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) id[u] = clamp_id(ids[r0 + 16 * u < rows ? r0 + 16 * u : r0], vocab);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int row = r0 + 16 * u < rows ? r0 + 16 * u : r0;
-        d[u] = Io<T>::ld(dy, (size_t)row * D + i);
-        x[u] = word[(size_t)id[u] * D + i] + ty + pos[(size_t)(row % N) * D + i];
-        mu[u] = mean[row]; rs[u] = rstd[row];
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (r0 + 16 * u >= rows) break;
-        agm += d[u] * ((x[u] - mu[u]) * rs[u]);
-        abt += d[u];
-      }
-    }
-    red_sum[wave * 64 + lane] = agm;                    // (2048 floats: the launch asks for no less)
-    red_sum[1024 + wave * 64 + lane] = abt;
-    __syncthreads();
-    if (wave < 2 && c < D) {
-      float v = 0.f;
-      for (int k = 0; k < 16; ++k) v += red_sum[wave * 1024 + k * 64 + lane];
-      atomicAdd((wave ? db : dg) + c, v);
-    }
-    return;
-  }
-  b -= columns;
-  // word table: a wave a token; the wave of an id's first token adds up all of its tokens
-  const int first = b * 16 + wave;
-  if (first >= rows) return;
-  const long id = clamp_id(ids[first], vocab);
+    for (int t = 0; t < V; ++t) de[t] = d[t] - s1 - xh[t] * s2;
+    return make_float2(s1, s2);
+  };
+  const float2 own = token(first);
+  if (lane == 0) sums[first] = own;
   if (id == 0) return;
-  const float* w = word + (size_t)id * D;
-  float gg[V], ty[V], sum[V];
-  txt_vec<V>(g, D, lane, gg);
-  txt_vec<V>(type, D, lane, ty);
-#pragma unroll
-  for (int t = 0; t < V; ++t) sum[t] = 0.f;
   for (int r0 = 0; r0 < rows; r0 += 64) {
-    const int q = r0 + lane;
-    unsigned long long same = __ballot(q < rows && clamp_id(ids[q < rows ? q : 0], vocab) == id);
+    const int r = r0 + lane;
+    unsigned long long same = __ballot(r < rows && clamp_id(ids[r < rows ? r : 0], vocab) == id);
     if (r0 <= first && (same & (first - r0 < 64 ? (1ull << (first - r0)) - 1 : ~0ull))) return;      // an earlier token has the id
     for (; same; same &= same - 1) {
-      TxtRow<T, V> r;
-      r.load(dy, w, pos, ty, mean, rstd, r0 + __ffsll((long long)same) - 1, N, D, lane);
-      float s1 = 0.f, s2 = 0.f;
+      const int row = r0 + __ffsll((long long)same) - 1;
+      if (row != first) token(row);
 #pragma unroll
-      for (int t = 0; t < V; ++t) {
-        const bool in = lane + 64 * t < D;
-        r.d[t] = in ? r.d[t] * gg[t] : 0.f;
-        r.x[t] = in ? (r.x[t] - r.mu) * r.rs : 0.f;
-        s1 += r.d[t]; s2 += r.d[t] * r.x[t];
-      }
-      s1 = wave_sum(s1) / (float)D;
-      s2 = wave_sum(s2) / (float)D;
-#pragma unroll
-      for (int t = 0; t < V; ++t) sum[t] += r.rs * (r.d[t] - s1 - r.x[t] * s2);
+      for (int t = 0; t < V; ++t) sum[t] += rs * de[t];
     }
   }
 #pragma unroll
   for (int t = 0; t < V; ++t)
     if (lane + 64 * t < D) atomicAdd(dword + (size_t)id * D + lane + 64 * t, sum[t]);
 }
-template <typename T, int V, int U>
-static void txt_ordered(const T* dy, const int64_t* ids, const float* word, const float* pos, const float* type, const float* mean, const float* rstd, const float* g,
-                        float* dword, float* dpos, float* dtype, float* dg, float* db, int B, int N, int D, int vocab, hipStream_t s) {
-  const int positions = B > 16 ? N : 0, blocks = 1 + positions + fc_cdiv(D, 64) + fc_cdiv(B * N, 16);
-  hipLaunchKernelGGL((k_txt_ordered<T, V, U>), dim3(blocks), dim3(1024), (D < 128 ? 2048 : 16 * D) * 4, s, dy, ids, word, pos, type, mean, rstd, g, dword, dpos, dtype,
-                     dg, db, B * N, positions, N, D, vocab);
+template <typename T>
+__global__ void __launch_bounds__(1024) k_txt_columns(const T* __restrict__ dy, const int64_t* __restrict__ ids, const float* __restrict__ word,
+                                                      const float* __restrict__ pos, const float* __restrict__ type, const float* __restrict__ mean,
+                                                      const float* __restrict__ rstd, const float* __restrict__ g, const float2* __restrict__ sums, float* dpos,
+                                                      float* dtype, float* dg, float* db, int rows, int N, int D, int vocab) {
+  __shared__ float red[3][16][64];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = blockIdx.x * 64 + lane, i = min(c, D - 1);
+  const int n = (int)blockIdx.y - 1, step = n < 0 ? 16 : 16 * N;       // n: the position whose dpos is added up, -1: the sums over all tokens
+  const float ty = type[i], gi = g[i];
+  float ade = 0.f, agm = 0.f, abt = 0.f;
+  for (int r0 = n < 0 ? wave : wave * N + n; r0 < rows; r0 += 4 * step) {
+    float d[4], x[4], mu[4], rs[4];
+    float2 s[4];
+    long id[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) id[u] = clamp_id(ids[r0 + u * step < rows ? r0 + u * step : r0], vocab);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int row = r0 + u * step < rows ? r0 + u * step : r0;
+      d[u] = Io<T>::ld(dy, (size_t)row * D + i);
+      x[u] = word[(size_t)id[u] * D + i] + ty + pos[(size_t)(row % N) * D + i];
+      mu[u] = mean[row]; rs[u] = rstd[row]; s[u] = sums[row];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (r0 + u * step >= rows) break;
+      const float xh = (x[u] - mu[u]) * rs[u];
+      ade += rs[u] * (d[u] * gi - s[u].x - xh * s[u].y);
+      agm += d[u] * xh;
+      abt += d[u];
+    }
+  }
+  red[0][wave][lane] = ade; red[1][wave][lane] = agm; red[2][wave][lane] = abt;
+  __syncthreads();
+  if (wave >= (n < 0 ? 3 : 1) || c >= D) return;
+  float v = 0.f;
+  for (int k = 0; k < 16; ++k) v += red[wave][k][lane];
+  atomicAdd((wave == 0 ? (n < 0 ? dtype : dpos + (size_t)n * D) : wave == 1 ? dg : db) + c, v);
 }
 int fc_txt_embed_bwd(int dt, const void* dy, const int64_t* ids, const float* word, const float* pos, const float* type, const float* mean,
-                     const float* rstd, const float* g, float* dword, float* dpos, float* dtype, float* dg, float* db, int B, int N, int D,
+                     const float* rstd, const float* g, float* dword, float* dpos, float* dtype, float* dg, float* db, float* sums, int B, int N, int D,
                      int vocab, hipStream_t s) {
   if ((D & 7) == 0 && D <= 1024 && !(((uintptr_t)dy | (uintptr_t)word | (uintptr_t)pos | (uintptr_t)type | (uintptr_t)g) & 15)) {
     const int ch = fc_cdiv(D / 8, 16);
     const size_t lds = sizeof(float) * (12 * D + 16 * 144);
     if (B * N <= TXT_ORDERED) {
-#define GO(V, U) DISPATCH_DT(dt, (txt_ordered<T, V, U>)((const T*)dy, ids, word, pos, type, mean, rstd, g, dword, dpos, dtype, dg, db, B, N, D, vocab, s))
-      if (D <= 128) { GO(2, 4); } else if (D <= 384) { GO(6, 4); } else if (D <= 768) { GO(12, 2); } else { GO(16, 1); }
+#define GO(V) DISPATCH_DT(dt, hipLaunchKernelGGL((k_txt_word_grad<T, V>), dim3(B * N), dim3(64), 0, s, (const T*)dy, ids, word, pos, type, mean, rstd, g, dword, \
+                                                 (float2*)sums, B * N, N, D, vocab))
+      if (D <= 128) { GO(2); } else if (D <= 384) { GO(6); } else if (D <= 768) { GO(12); } else { GO(16); }
 #undef GO
+      DISPATCH_DT(dt, hipLaunchKernelGGL(k_txt_columns<T>, dim3(fc_cdiv(D, 64), B > 16 ? 1 + N : 1), dim3(1024), 0, s, (const T*)dy, ids, word, pos, type, mean, rstd,
+                                         g, (const float2*)sums, dpos, dtype, dg, db, B * N, N, D, vocab));
       FC_LAUNCH_CHECK();
       if (B > 16) return 0;
       dword = dtype = dg = db = nullptr;

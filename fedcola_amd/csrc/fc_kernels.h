@@ -66,7 +66,7 @@ int fc_txt_embed_fwd(int dt, const int64_t* ids, const float* word, const float*
                      const float* b, void* y, float* mean, float* rstd, int B, int N, int D, int vocab, float eps, hipStream_t s);
 int fc_txt_embed_bwd(int dt, const void* dy, const int64_t* ids, const float* word, const float* pos, const float* type,
                      const float* mean, const float* rstd, const float* g, float* dword, float* dpos, float* dtype,
-                     float* dg, float* db, int B, int N, int D, int vocab, hipStream_t s);
+                     float* dg, float* db, float* sums, int B, int N, int D, int vocab, hipStream_t s);      // sums: scratch, two floats a token
 
 // ---- final LN on cls rows + (optional) L2 normalise (K10)
 int fc_head_fwd(int dt, const void* x, const float* g, const float* b, float* f, float* mean, float* rstd, float* nrm,

@@ -318,7 +318,7 @@ struct TowerWs {
   int dp_off = 0;          // first sample of this (micro-batch) view in the drop-path table
   size_t ln_stride = 0;    // elements between the partial sets of consecutive LayerNorm instances (sized for the full batch)
   void *patches = nullptr, *dtok = nullptr;
-  float *emb_mean = nullptr, *emb_rstd = nullptr;
+  float *emb_mean = nullptr, *emb_rstd = nullptr, *emb_sums = nullptr;
   std::vector<void*> x;
   std::vector<void*> gx;   // gradient w.r.t. x[l]
   std::vector<LayerWs> L;
@@ -375,6 +375,7 @@ static void carve(const fc_model* m, int B, int n_txt, void* base, Ws& w) {
     } else {
       t.emb_mean = (float*)bp.take(sizeof(float) * t.M);
       t.emb_rstd = (float*)bp.take(sizeof(float) * t.M);
+      t.emb_sums = (float*)bp.take(sizeof(float) * 2 * t.M);
     }
     t.x.resize(c.depth + 1);
     t.gx.resize(c.depth + 1);
@@ -448,6 +449,7 @@ static Ws slice_ws(const fc_model* m, const Ws& w, int i, int b0, int bn, int mb
   } else {
     t.emb_mean = f.emb_mean + r0;
     t.emb_rstd = f.emb_rstd + r0;
+    t.emb_sums = f.emb_sums + 2 * r0;
   }
   for (size_t l = 0; l < f.x.size(); ++l) { t.x[l] = adv(f.x[l], D * es); t.gx[l] = adv(f.gx[l], D * es); }
   for (size_t l = 0; l < f.L.size(); ++l) {
@@ -1487,7 +1489,7 @@ static int tower_backward(const Ctx& c, Ws& w, int i, const float* d_out, float*
     FC_TRY(weight_grad(c, t.dtok, t.patches, B * np, D, kp, grads + tp.pw, grads + tp.pb));
   } else {
     FC_TRY(fc_txt_embed_bwd(c.dt, dx, w.ids, P + tp.word, P + tp.tpos, P + tp.ttype, t.emb_mean, t.emb_rstd, P + tp.lnw, grads + tp.word,
-                            grads + tp.tpos, grads + tp.ttype, grads + tp.lnw, grads + tp.lnb, B, N, D, cf.vocab, c.s));
+                            grads + tp.tpos, grads + tp.ttype, grads + tp.lnw, grads + tp.lnb, t.emb_sums, B, N, D, cf.vocab, c.s));
   }
   if (phase == PH_ALL) FC_TRY(flush_dw(c));
   return 0;
