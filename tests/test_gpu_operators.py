@@ -229,6 +229,22 @@ def test_linear_cross_entropy_backward_takes_the_forwards_weight():
         linear_cross_entropy_backward(g, saved, w.clone())
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,V,ignore", [(45, 300, 0), (300, 40, 39), (45, 300, -(1 << 40)), (20, 7, 1 << 33)])
+def test_linear_cross_entropy_any_index_may_be_the_ignored_one(T, V, ignore, dt):
+    """a class of the vocabulary (a padding token), and numbers that 32 bits do not hold"""
+    from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
+    x, w, y = ce_case(T, V, 48, dt, 0.0, T + V)
+    y[torch.arange(T, device="cuda") % 3 == 1] = ignore
+    g = torch.tensor(0.9, device="cuda")
+    want, bound = O.linear_ce(x, w, y, g, ignore, "mean", DT[dt])
+    loss, saved = linear_cross_entropy_forward(x, w, y, ignore_index=ignore)
+    dx, dw = linear_cross_entropy_backward(g, saved, w)
+    within(loss, want["loss"], bound["loss"], "loss")
+    within(dx, want["dx"], bound["dx"], "dx")
+    within(dw, want["dw"], bound["dw"], "dw")
+
+
 def test_linear_cross_entropy_extreme_values():
     from fedcola_amd.criterions import linear_cross_entropy_backward, linear_cross_entropy_forward
     w = torch.zeros(300, 64, device="cuda")
@@ -488,6 +504,22 @@ def test_norm_gate_residual_of_no_rows(dt, gate):
     assert got["branch"].shape == got["residual"].shape == empty.shape
     for k in ("post_weight", "post_bias", "gate", "pre_weight", "pre_bias"):
         assert got[k].shape == v[k].shape and not got[k].any(), k
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("S,gates,N,D", [(6, 3, 5, 72), (12, 1, 9, 384), (8, 4, 33, 1100)])
+def test_norm_gate_residual_gates_of_several_samples(S, gates, N, D, dt):
+    """a gate for several samples' rows, each sample with a multiplier of its own; the branch without a norm, r and h of one gradient"""
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    for post in (0, 1):
+        b, r, dr, _, v = norm_case(S, N, D, dt, "rms", post, 1, "sample", 1, S + D)
+        v["gate"] = v["gate"][:gates]
+        want, bound = O.norm_gate(b, r, DT[dt], **v, d_residual=dr, d_normed=dr)
+        gr, gh = norm_gate_residual_forward(b, r, **v)
+        within(gr, want["r"], bound["r"], "r")
+        within(gh, want["h"], bound["h"], "h")
+        for k, t in norm_gate_residual_backward(dr, dr, b, r, **v).items():
+            within(t, want[k], bound[k], k)
 
 
 def test_norm_gate_residual_module():
