@@ -40,7 +40,9 @@ def _packed(T, F, w_in, w_out, *rows):
 
 
 def gated_mlp_forward(x, w_in, w_out, act="silu"):
-    """y = (act(x wg^T) * (x wu^T)) w_out^T.  x [..., D]; w_in [2F, D]: wg over wu; w_out [D, F]; one type, bf16 or fp32.  act: "silu", "gelu" (erf)."""
+    """y = (act(x wg^T) * (x wu^T)) w_out^T.  x [..., D]; w_in [2F, D]: wg over wu; w_out [D, F]; one type, bf16 or fp32.  act: "silu", "gelu" (erf).
+    bf16: the hidden values are rounded to bf16 once between the products, for up to 32 rows to 16 bits of mantissa.  Up to 2^28 rows, D 2^18, F 2^20,
+    and (F + 512) (D + 64) below 2^30."""
     code, dev, (x2, ldx), (wi, ldi), (wo, ldo) = _mlp_operands(x, w_in, w_out, act)
     T, D, F, L = x2.shape[0], wi.shape[1], wo.shape[1], _lib.lib()
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)

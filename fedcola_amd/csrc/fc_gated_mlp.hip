@@ -7,7 +7,9 @@
 // epilogue, which has g and u in 32 bits, reads dh and writes
 //   h = act(g) u,   dg = dh u act'(g),   du = dh act(g)
 // each rounded once; then dx = [dg | du] w_in, dw_in = [dg | du]^T x, dw_out = dy^T h.  That is 16 T D F operations for the 12 of a backward
-// pass that reads g and u back; these would have to be stored in 32 bits too, or rounded once more than here.  (dh on the same tile as g and
+// pass that reads g and u back.  Kept in 32 bits (in 16 they would be rounded once more than here) these are 8 T F bytes, four times h, for as long as the
+// layers above run, and 16 T F of traffic: at the rate of a copy 292 us for 8192 x 4096 x 11000, where the product takes 1100; at widths of about 1050 both
+// cost the same.  What is saved here is that memory.  (dh on the same tile as g and
 // u, without its 8 bytes a unit through memory, leaves registers for 128 x 256 tiles only: 2300 us for 8192 x 4096 x 11000, 2000 in two kernels;
 // 70 against 74 for 12608 x 384 x 1024.)
 #include <math.h>
@@ -27,7 +29,8 @@ struct GmArgs {
   int dh_parts;
 };
 
-// act(g) and act'(g); FAST: through v_exp_f32 and v_rcp_f32, for bf16 operands
+// act(g) and act'(g); FAST, for bf16 operands: through v_exp_f32 and v_rcp_f32 (an ulp each), gelu's erf by a polynomial that is off by up to 1.5e-7: gates
+// under about -5, where gelu is smaller than that, keep its size and not its digits
 template <bool FAST> __device__ __forceinline__ void gm_act(int act, float g, float& a, float& da) {
   if (act == FC_ACT_SILU) {
     const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f)) : 1.f / (1.f + expf(-g));
@@ -61,8 +64,8 @@ __device__ __forceinline__ void gm_gate_up(const GmArgs& a, char* smem, ft_f4 (&
   pipe.drain();
 }
 
-// Planes of h, dg and du: fp32's three; bf16's one, each rounded once; two (16 bits of mantissa) in the tiles of few rows, whose
-// products read the weights once all the same, and whose few results would show how one rounding more is distributed.
+// Planes of h, dg and du: fp32's three; bf16's one, each value rounded once to bf16, which is half of a result's error (2.35e-3 in norm, 1.66e-3 without);
+// two (16 bits of mantissa) for up to 32 rows, whose products read the weights once all the same: there the second plane costs no time.
 template <class S, int NPROD> constexpr int gm_planes() { return NPROD == 6 ? 3 : S::TM == 32 ? 2 : 1; }
 // one row block of values, J columns of 16, into the planes' LDS images
 template <class S, int NPROD>
@@ -91,7 +94,8 @@ template <class S, int NPROD> __device__ __forceinline__ void gm_out(const char*
   for (int p = 0; p < gm_planes<S, NPROD>(); ++p) ft_img_out<S::TM, FC, S::NT>(img + p * IMG, out + p * plane, ld, m0, f0, a.T, (int)a.ldh, rows, true);
 }
 
-// GRAD: the backward's pass over the same product
+// GRAD: the backward's pass over the same product.  (The large tile with its 128 accumulators, dh and the activation's values takes all 256 registers and
+// spills 144 bytes a lane: 1307 us of the 6600 of 8192 x 4096 x 11000.)
 template <class S, int NPROD, bool GRAD>
 __global__ void __launch_bounds__(S::NT, S::NT == 512 ? 2 : 1) k_gm_act(GmArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -249,7 +253,7 @@ template <int NPROD, bool GRAD> static int gm_act_run(const GmArgs& a, hipStream
 }
 
 struct GmSizes { size_t x, w_in, w_out, dy, h, gu, dgu, dh, part; FtPlan plan_gu, plan_dh, plan[3]; bool group; };
-// [g | u] in slices, where that is much faster by the model of the products' time (fp32, 45 x 3200 x 448: 42 us forward, 149 by whole tiles;
+// [g | u] in slices, where that is much faster by the model of the products' time (fp32, 45 x 3200 x 448: 41 us forward, 134 by whole tiles;
 // bf16, 256 x 4096 x 1024: 39 and 57)
 static FtProduct gm_gu_product(int dt, long T, long D, long F, bool b32) {
   FtProduct p;

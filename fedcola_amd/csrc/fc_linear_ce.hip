@@ -32,8 +32,8 @@ static long ce_piece(int dt, long T, long V) {
   const long most = (192L << 20) / ((T ? T : 1) * (dt ? 2 : 6)) / 256 * 256, all = ft_up(V, 256);
   return most < 256 ? 256 : most < all ? most : all;
 }
-// The logits of a few rows are little beside the weight, which forming them again would read once more (1 x 3648 x 59042 fp32 with gradients: 666 us,
-// 1090 without this and the outer product of fc_tiles.hip; k_ce_grad took 217 of them): up to 32 rows, and up to 128 while they are an eighth of it.
+// The logits of a few rows are little beside the weight, which forming them again would read once more (1 x 3648 x 59042 fp32 with gradients: 625 us,
+// 1017 without this and the outer product of fc_tiles.hip): up to 32 rows, and up to 128 while they are an eighth of it.
 static bool ce_keep(int dt, long T, long V, long D) {
   return T > 0 && (T <= 32 || (T <= 128 && T * 32 <= D * (dt ? 2 : 4))) && T * ft_up(V, 8) <= (1L << 25) && ce_piece(dt, T, V) >= V;
 }
@@ -462,7 +462,7 @@ static CeSizes ce_sizes(int dt, long T, long V, long D, bool direct_w, bool grad
   CeSizes z = {};
   const bool b32 = !dt && direct_w;
   z.w = direct_w ? 0 : (size_t)ft_up((dt ? 2 : 6) * V * ft_up(D, 64), 256);
-  // slices pay where the model of the products' time says so by much (122 x 2263 x 326 fp32: 39 us forward, 125 by whole tiles; 64 x 4096 x 1000
+  // slices pay where the model of the products' time says so by much (122 x 2263 x 326 fp32: 38 us forward, 115 by whole tiles; 64 x 4096 x 1000
   // bf16: 23 and 31), and where the logits are one piece
   z.piece = ce_piece(dt, T, V);
   z.logits = ft_plan(ce_logits(dt, T, V, D, b32, nullptr), false);

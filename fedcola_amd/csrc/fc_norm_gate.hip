@@ -11,7 +11,9 @@
 // values a lane.  A workgroup walks several
 // rows with the weight vectors in registers (forward) or LDS (backward): read per row they would be 20 bytes an element from L2 beside the 8
 // from HBM.  The next row is loaded while this one is summed.  Measured at the rate of a large copy (4.9 TB/s) for 65536 x 4096 bf16: 417 us
-// forward (5.1 TB/s), 667 us backward (4.8 TB/s); 12608 x 384: 13 and 27 us, where filling and draining the chip is most of the time.
+// forward (5.1 TB/s), 667 us backward (4.8 TB/s); fp32, 32768 x 4096: 418 (5.1) and 662 (4.9), 65536 x 1024: 223 and 328; 12608 x 384: 13 and 27 us, where
+// filling and draining the chip is most of the time.  Rows that are no whole eights wide are read value by value, and above 512 values a lane's
+// 16 of them spill in the backward (144 to 240 bytes; fp32 of whole eights above 2048, 16): 65536 x 1001 bf16 133 and 592 us, 65536 x 1024 112 and 181.
 // dwp, dbp, dwn, dbn, dgate: each workgroup's sums over its rows (fp32) are one row of partial sums, added in fp64 in a fixed order by a
 // second launch.  A workgroup's rows share one gate vector.
 #include "../../include/fedcola_hip.h"
@@ -404,7 +406,9 @@ static void ng_form(long D, bool bwd, int& W, int& E, int& G) {
   E = D <= 512 || (D > 1024 && D <= 2048) || (!bwd && D <= 4096 && D > 2048) ? 8 : 16;
 }
 // workgroups of a gate vector's rows: in all as many as the chip holds at once, each wave with the same number of rows.  deep: waves a SIMD that
-// the registers allow
+// the registers of the form in most use allow.  (By the compiler's report others hold one fewer, so that their last workgroups start when the
+// first end: forward, rows no whole eights wide up to 256, from 513 to 1024 and from 4097 on, and fp32 up to 256; backward, bf16 rows no whole eights wide
+// from 257 to 512.)
 static void ng_split(long T, long gate_rows, long D, bool bwd, int deep, long& per, long& blocks) {
   int W, E, G;
   ng_form(D, bwd, W, E, G);

@@ -714,10 +714,10 @@ struct FtPacks {                  // up to four of one type in one launch
 };
 int ft_pack(const FtPacks& p, hipStream_t s);
 // rows up to which tiles are 32 rows high: their reading of B is what counts (bf16, 64 rows of 4096 x 11008: 77 us forward, 88 with 128 x 128 tiles;
-// fp32, where every 32 rows split B's fragments once more, 64 rows: 302 us, 251 with 128 x 128)
+// fp32, where every 32 rows split B's fragments once more, 64 rows: 271 us, 222 with 128 x 128)
 static inline bool ft_few(int nprod, long T) { return T <= (nprod == 1 ? 64 : 32); }
-// fp32: up to how many rows a weight is not worth laying out in planes (gated block forward, 4096 x 11008: 96 rows 258 us, 576 with planes; 512 rows 845
-// and 1027; with gradients, 384 x 1024, 1000 rows: 155 and 138), and whether it can be read where it is
+// fp32: up to how many rows a weight is not worth laying out in planes (gated block forward, 4096 x 11008: 96 rows 229 us, 564 with planes; 512 rows 767
+// and 997; with gradients, 384 x 1024, 1000 rows: 147 and 136), and whether it can be read where it is
 #define FT_B32 512
 static inline bool ft_b32(int dt, long T, const void* p, long ld) { return !dt && T <= FT_B32 && ((size_t)p & 3) == 0 && ld < (1L << 20); }
 static inline FtMat ft_mat32(const void* p, long ld, long R, long C) {

@@ -391,8 +391,8 @@ int ft_group(const FtProduct* p, const FtPlan* plan, int n, float* const* part, 
 // ---------------------------------------------------------------- fp32, a reduction over few rows: C[m, n] = sum_k A[k, m] B[k, n], k < 32
 // All that costs time is the writing of C, of which the tiles, one workgroup of eight waves a CU, reach half the rate (38227 x 2816, 11 rows: 178 us;
 // here 72, 6 TB/s).  A wave's lanes hold four columns each of all rows of B; the values of A, of `per` rows of C, come from LDS.
-// Where C is small and the rows are not the fewest, the tiles' start is the shorter one (gated block with gradients, 768 x 2048, 32 rows: 104 us with
-// tiles, 126 here; 4096 x 11008: 779 and 748; 4 rows: 104 and 100, 752 and 627).
+// Where C is small and the rows are not the fewest, the tiles' start is the shorter one (gated block with gradients, 768 x 2048, 32 rows: 99 us with
+// tiles, 120 here; 4096 x 11008: 731 and 700; 4 rows: 98 and 95, 701 and 585).
 template <int KM>
 __global__ void __launch_bounds__(256) k_ft_outer(FtProduct p, int per, int cols) {      // cols: waves of a workgroup side by side
   extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -124,7 +124,8 @@ enum { FC_NORM_LAYER = 0, FC_NORM_RMS = 1 };
 /* softmax cross entropy of logits x w^T, x [T, D], w [V, D] (T up to 2^28, V 2^30, D 2^20), which are not kept (but for up to 32 rows, and up to 128
  * while they are an eighth of w): loss (fp32: one value, or T with FC_REDUCE_NONE).  Rows with
  * y = ignore_index have loss 0, cost nothing, and what they hold reaches no output; MEAN divides by the rows that count (none: NaN).  A target
- * outside of [0, V) makes its row's loss and the gradients NaN.  `saved` (fc_linear_ce_saved_bytes) is what fc_linear_ce_bwd reads in x's place. */
+ * outside of [0, V) makes its row's loss and the gradients NaN.  Logits, sums and losses are held in 32 bits; bf16's dL is rounded to bf16 once, before the
+ * factor that all rows share.  `saved` (fc_linear_ce_saved_bytes) is what fc_linear_ce_bwd reads in x's place. */
 size_t fc_linear_ce_saved_bytes(int32_t dt, int32_t T, int32_t V, int32_t D);
 size_t fc_linear_ce_workspace_bytes(int32_t dt, int32_t T, int32_t V, int32_t D, int32_t packed, int32_t backward);
 int fc_linear_ce_fwd(int32_t dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* y, int32_t T, int32_t V, int32_t D,
@@ -138,7 +139,9 @@ int fc_linear_ce_bwd(int32_t dt, const void* w, int64_t ldw, int32_t T, int32_t 
 
 /* gated feed-forward block: y = (act(x wg^T) * (x wu^T)) w_out^T, w_in [2F, D] = wg over wu, w_out [D, F], x and y [T, D], T up to 2^28, D 2^18, F
  * 2^20, and (F + 512) times the larger of ld_in and D + 64 below 2^30 (a tile reaches the up rows from the gate rows).  The backward forms the
- * hidden units again from x (nothing is kept); dx, dw_in, dw_out: any may be NULL */
+ * hidden units again from x (nothing is kept); dx, dw_in, dw_out: any may be NULL.  bf16: the hidden values, and dg and du backward, are rounded to bf16
+ * once between the products; for T up to 32 they keep 16 bits of mantissa, so a row's result may differ in its last bits with the rows beside it.  gelu's erf
+ * is off by up to 1.5e-7 for bf16. */
 size_t fc_gated_mlp_workspace_bytes(int32_t dt, int32_t T, int32_t D, int32_t F, int32_t packed, int32_t backward);
 int fc_gated_mlp_fwd(int32_t dt, int32_t act, const void* x, int64_t ldx, const void* w_in, int64_t ld_in, const void* w_out, int64_t ld_out,
                      int32_t T, int32_t D, int32_t F, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
