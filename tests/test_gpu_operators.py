@@ -506,6 +506,25 @@ def test_norm_gate_residual_of_no_rows(dt, gate):
         assert got[k].shape == v[k].shape and not got[k].any(), k
 
 
+def test_norm_gate_residual_the_most_gates():
+    """one gate fewer than the limit, a row each: the first, the last and some in between, and the weights' gradients in norm"""
+    from fedcola_amd.blocks import norm_gate_residual_backward, norm_gate_residual_forward
+    T, D = (1 << 23) - 1, 8
+    b, r, dr, dh, v = norm_case(T, 1, D, "bf16", "rms", 1, 1, "sample", 0, 1)
+    gr, gh = norm_gate_residual_forward(b, r, **v)
+    got = norm_gate_residual_backward(dr, dh, b, r, **v)
+    some = torch.tensor([0, 1, 59_999, 60_000, 65_535, 65_536, 4_194_304, T - 2, T - 1], device="cuda")
+    want, bound = O.norm_gate(b[some], r[some], DT["bf16"], **{**v, "gate": v["gate"][some]}, d_residual=dr[some], d_normed=dh[some])
+    for k, t in (("r", gr), ("h", gh), ("branch", got["branch"]), ("residual", got["residual"]), ("gate", got["gate"])):
+        within(t[some], want[k], bound[k], k)
+    hat = lambda t: t / (t.square().mean(-1, keepdim=True) + 1e-5).sqrt()  # noqa: E731
+    dn = dh.double()[:, 0]
+    res = 0.9 * r.double()[:, 0] + v["gate"].double() * (hat(b.double()[:, 0]) * v["post_weight"].double())
+    want = (dn * hat(res)).sum(0)
+    # a row's term is off by at most 40 roundings of 2^-24 (two norms, the residual, the product); the sum over the rows is in 64 bits
+    assert ((got["pre_weight"].double() - want).abs() <= 40 * O.F24 * (dn * hat(res)).abs().sum(0)).all()
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 @pytest.mark.parametrize("S,gates,N,D", [(6, 3, 5, 72), (12, 1, 9, 384), (8, 4, 33, 1100)])
 def test_norm_gate_residual_gates_of_several_samples(S, gates, N, D, dt):
